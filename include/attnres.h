@@ -446,6 +446,123 @@ int attnres_merge_bwd(const void* partial, int64_t num_tokens, int hidden, int p
                       const void* grad_out, void* grad_partial, void* grad_inter, float* grad_inter_lse,
                       void* workspace, int64_t workspace_bytes, void* grad_query, void* stream);
 
+/*
+ * ---- Language-model operators -------------------------------------------
+ *
+ * The dense sublayers around the routing points (llama.py:155-192, 300-346).
+ * Element strides are given per tensor as an array of three, (batch, head,
+ * token) for (batch, heads, tokens, head_dim) tensors whose last dimension is
+ * contiguous; any order of the others, 0 for a broadcast dimension.
+ */
+
+/* Widths of the whole numbers in index arrays. */
+#define ATTNRES_INDEX_I32 0
+#define ATTNRES_INDEX_I64 1
+
+/* attnres_attention_*: query 0 of each sequence is at kv_len - q_len (the last query at the last key). */
+#define ATTNRES_START_FROM_END INT64_MIN
+
+/*
+ * Attention of `heads` query heads over `kv_heads` key/value heads (heads a
+ * multiple of kv_heads; query head h reads key head h / (heads / kv_heads)):
+ *   s_ij = scale q_i . k_j over the keys j that query i sees
+ *   out_i = sum_j softmax_j(s_ij) v_j,   lse_i = log sum_j exp(s_ij)
+ * kv_slots keys are stored per sequence; kv_lens ((batch,) index_dtype, or NULL
+ * for kv_slots) says how many of them exist (values are taken into [0,
+ * kv_slots]).  What the others hold is not used.  Query i of sequence b is at
+ * position start_b + i, start_b = q_start[b] ((batch,) index_dtype) or, with
+ * q_start NULL, q_start_value, or ATTNRES_START_FROM_END.  causal: it sees the
+ * keys 0 .. position if 0 <= position < kv_len, and none otherwise; else every
+ * key that exists.  A query that sees no key gets out = 0, lse = -inf and a
+ * zero gradient.  A NaN or infinity in a key or value that exists may reach
+ * every query of its sequence.
+ *
+ * dtype: bf16 or fp32 (all of q, k, v, out); head_dim a multiple of 8 up to
+ * 128; 16-byte aligned pointers and strides.  lse ((batch, heads, q_len) fp32)
+ * may be NULL.  Scores and sums are fp32; the probabilities are rounded to the
+ * dtype for the product with v, the result once.  workspace: device memory of
+ * attnres_attention_workspace_size bytes (backward 0 or 1).
+ */
+int attnres_attention_workspace_size(int batch, int heads, int kv_heads, int64_t q_len, int64_t kv_slots, int head_dim,
+                                     int dtype, int backward, int64_t* bytes);
+int attnres_attention_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                          const void* v, const int64_t* v_strides, int batch, int heads, int kv_heads, int64_t q_len,
+                          int64_t kv_slots, int head_dim, int dtype, int causal, float scale, const void* kv_lens,
+                          const void* q_start, int index_dtype, int64_t q_start_value, void* out,
+                          const int64_t* out_strides, float* lse, void* workspace, int64_t workspace_bytes,
+                          void* stream);
+
+/*
+ * Its backward: the gradients of q, k and v from dL/dout and dL/dlse (or
+ * NULL), the probabilities recomputed from q, k and the forward's lse.  Every
+ * row of grad_q, grad_k and grad_v is written (zeros where nothing is seen);
+ * no atomics, so results repeat bit for bit.
+ */
+int attnres_attention_bwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                          const void* v, const int64_t* v_strides, const void* out, const int64_t* out_strides,
+                          const void* grad_out, const int64_t* grad_out_strides, const float* lse,
+                          const float* grad_lse, int batch, int heads, int kv_heads, int64_t q_len, int64_t kv_slots,
+                          int head_dim, int dtype, int causal, float scale, const void* kv_lens, const void* q_start,
+                          int index_dtype, int64_t q_start_value, void* grad_q, const int64_t* grad_q_strides,
+                          void* grad_k, const int64_t* grad_k_strides, void* grad_v, const int64_t* grad_v_strides,
+                          void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * RMSNorm of every query and key head (llama.py:300-346 with qk_norm) and the
+ * rotation of its two halves (llama.py:155-192) in one pass:
+ *   n = x * rsqrt(mean(x^2) + eps) * weight,  y = n cos_p + rot(n) sin_p,
+ *   rot(n) = (-n[dim/2:], n[:dim/2])
+ * q (batch, q_heads, tokens, head_dim), k likewise with k_heads (either count
+ * may be 0).  cos and sin: (table_rows, head_dim), table_dtype dtype or fp32,
+ * row strides cos_ld and sin_ld.  Token (b, t) uses table row
+ * positions[b * pos_batch_stride + t * pos_token_stride] (index_dtype), or t
+ * with positions NULL; a row outside the tables makes the token's results NaN.
+ * head_dim even, up to 256.
+ */
+int attnres_qk_norm_rope_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                             int batch, int q_heads, int k_heads, int64_t tokens, int head_dim, int dtype,
+                             const void* q_weight, const void* k_weight, const void* cos, int64_t cos_ld,
+                             const void* sin, int64_t sin_ld, int64_t table_rows, int table_dtype,
+                             const void* positions, int index_dtype, int64_t pos_batch_stride,
+                             int64_t pos_token_stride, float eps, void* q_out, const int64_t* q_out_strides,
+                             void* k_out, const int64_t* k_out_strides, void* stream);
+
+/*
+ * Its backward: gradients of q and k (any strides) and of the two weights
+ * ((head_dim,), NULL to skip; summed in a fixed order).  workspace: device
+ * memory of attnres_qk_norm_rope_workspace_size bytes.
+ */
+int attnres_qk_norm_rope_workspace_size(int head_dim, int64_t* bytes);
+int attnres_qk_norm_rope_bwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                             const void* grad_q_out, const int64_t* grad_q_out_strides, const void* grad_k_out,
+                             const int64_t* grad_k_out_strides, int batch, int q_heads, int k_heads, int64_t tokens,
+                             int head_dim, int dtype, const void* q_weight, const void* k_weight, const void* cos,
+                             int64_t cos_ld, const void* sin, int64_t sin_ld, int64_t table_rows, int table_dtype,
+                             const void* positions, int index_dtype, int64_t pos_batch_stride,
+                             int64_t pos_token_stride, float eps, void* grad_q, const int64_t* grad_q_strides,
+                             void* grad_k, const int64_t* grad_k_strides, void* grad_q_weight, void* grad_k_weight,
+                             void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Embedding lookup: out[n] = scale * weight[ids[n]] for num_ids contiguous ids
+ * (index_dtype); weight (rows, hidden), rows weight_ld apart; out contiguous.
+ * An id outside the table gives a row of NaN.
+ */
+int attnres_embedding_fwd(const void* ids, int index_dtype, int64_t num_ids, const void* weight, int64_t weight_ld,
+                          int64_t rows, int hidden, int dtype, float scale, void* out, void* stream);
+
+/*
+ * Its backward: grad_weight[r] = scale * sum of grad_out[n] over the n with
+ * ids[n] == r, every row of the contiguous (rows, hidden) grad_weight written.
+ * Tokens are sorted by row, stably, and each row's sum is taken in a fixed
+ * order in fp32.  Ids equal to padding_idx (-1: none) or outside the table
+ * have no gradient.  num_ids and rows up to 2^31 - 1.
+ */
+int attnres_embedding_workspace_size(int64_t num_ids, int64_t rows, int hidden, int64_t* bytes);
+int attnres_embedding_bwd(const void* ids, int index_dtype, int64_t num_ids, const void* grad_out, int64_t grad_out_ld,
+                          int64_t rows, int hidden, int dtype, float scale, int64_t padding_idx, void* grad_weight,
+                          void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

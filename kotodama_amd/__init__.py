@@ -10,6 +10,9 @@ Hand-written HIP kernels behind a C ABI (``include/attnres.h``,
   ``phase_2_online_softmax_merge_triton_op``
 * :func:`kotodama_amd.engine.forward_attn_res` / ``forward_attn_res_cached`` —
   the prefill / KV-cache caller loops over a preallocated block arena
+* :func:`kotodama_amd.attention`, :func:`kotodama_amd.qk_norm_rope`,
+  :func:`kotodama_amd.embedding` — the language model's own operators around
+  the routing, forward and backward (:mod:`kotodama_amd.lmops`)
 * :mod:`kotodama_amd.checkpoint` — routing weights from trained checkpoints
   (safe loading only)
 """
@@ -17,6 +20,7 @@ Hand-written HIP kernels behind a C ABI (``include/attnres.h``,
 from . import ops  # noqa: F401  (registers the attnres_hip ops)
 from .checkpoint import RoutingWeights, load_checkpoint_registry, load_routing_weights
 from .engine import AttnResRouter, BlockArena, forward_attn_res, forward_attn_res_cached
+from .lmops import attention, embedding, qk_norm_rope
 from .routing import block_attn_res_from_list, route_static, route_weights
 from .schedule import AttnResSchedule
 
@@ -25,11 +29,14 @@ __all__ = [
     "AttnResSchedule",
     "BlockArena",
     "RoutingWeights",
+    "attention",
     "block_attn_res_from_list",
+    "embedding",
     "forward_attn_res",
     "forward_attn_res_cached",
     "load_checkpoint_registry",
     "load_routing_weights",
+    "qk_norm_rope",
     "route_static",
     "route_weights",
 ]

@@ -28,6 +28,10 @@ ERR_HIP = -4
 
 MAX_SOURCES = 16
 
+INDEX_I32 = 0
+INDEX_I64 = 1
+START_FROM_END = -(1 << 63)  # ATTNRES_START_FROM_END
+
 POLICY_AUTO = 0
 POLICY_WORKGROUP = 1
 POLICY_STREAM = 2
@@ -64,6 +68,15 @@ EXPORTS = (
     "attnres_route_bwd_queries",
     "attnres_route_bwd_queries_kernel_name",
     "attnres_merge_bwd",
+    "attnres_attention_workspace_size",
+    "attnres_attention_fwd",
+    "attnres_attention_bwd",
+    "attnres_qk_norm_rope_fwd",
+    "attnres_qk_norm_rope_workspace_size",
+    "attnres_qk_norm_rope_bwd",
+    "attnres_embedding_fwd",
+    "attnres_embedding_workspace_size",
+    "attnres_embedding_bwd",
 )
 
 _c_vp = ctypes.c_void_p
@@ -383,6 +396,214 @@ _SIGNATURES = {
         ],
         _c_int,
     ),
+    "attnres_attention_workspace_size": (
+        [
+            _c_int,  # batch
+            _c_int,  # heads
+            _c_int,  # kv_heads
+            _c_i64,  # q_len
+            _c_i64,  # kv_slots
+            _c_int,  # head_dim
+            _c_int,  # dtype
+            _c_int,  # backward
+            ctypes.POINTER(_c_i64),  # bytes
+        ],
+        _c_int,
+    ),
+    "attnres_attention_fwd": (
+        [
+            _c_vp,  # q
+            ctypes.POINTER(_c_i64),  # q_strides
+            _c_vp,  # k
+            ctypes.POINTER(_c_i64),  # k_strides
+            _c_vp,  # v
+            ctypes.POINTER(_c_i64),  # v_strides
+            _c_int,  # batch
+            _c_int,  # heads
+            _c_int,  # kv_heads
+            _c_i64,  # q_len
+            _c_i64,  # kv_slots
+            _c_int,  # head_dim
+            _c_int,  # dtype
+            _c_int,  # causal
+            _c_float,  # scale
+            _c_vp,  # kv_lens
+            _c_vp,  # q_start
+            _c_int,  # index_dtype
+            _c_i64,  # q_start_value
+            _c_vp,  # out
+            ctypes.POINTER(_c_i64),  # out_strides
+            _c_vp,  # lse
+            _c_vp,  # workspace
+            _c_i64,  # workspace_bytes
+            _c_vp,  # stream
+        ],
+        _c_int,
+    ),
+    "attnres_attention_bwd": (
+        [
+            _c_vp,  # q
+            ctypes.POINTER(_c_i64),  # q_strides
+            _c_vp,  # k
+            ctypes.POINTER(_c_i64),  # k_strides
+            _c_vp,  # v
+            ctypes.POINTER(_c_i64),  # v_strides
+            _c_vp,  # out
+            ctypes.POINTER(_c_i64),  # out_strides
+            _c_vp,  # grad_out
+            ctypes.POINTER(_c_i64),  # grad_out_strides
+            _c_vp,  # lse
+            _c_vp,  # grad_lse
+            _c_int,  # batch
+            _c_int,  # heads
+            _c_int,  # kv_heads
+            _c_i64,  # q_len
+            _c_i64,  # kv_slots
+            _c_int,  # head_dim
+            _c_int,  # dtype
+            _c_int,  # causal
+            _c_float,  # scale
+            _c_vp,  # kv_lens
+            _c_vp,  # q_start
+            _c_int,  # index_dtype
+            _c_i64,  # q_start_value
+            _c_vp,  # grad_q
+            ctypes.POINTER(_c_i64),  # grad_q_strides
+            _c_vp,  # grad_k
+            ctypes.POINTER(_c_i64),  # grad_k_strides
+            _c_vp,  # grad_v
+            ctypes.POINTER(_c_i64),  # grad_v_strides
+            _c_vp,  # workspace
+            _c_i64,  # workspace_bytes
+            _c_vp,  # stream
+        ],
+        _c_int,
+    ),
+    "attnres_qk_norm_rope_fwd": (
+        [
+            _c_vp,  # q
+            ctypes.POINTER(_c_i64),  # q_strides
+            _c_vp,  # k
+            ctypes.POINTER(_c_i64),  # k_strides
+            _c_int,  # batch
+            _c_int,  # q_heads
+            _c_int,  # k_heads
+            _c_i64,  # tokens
+            _c_int,  # head_dim
+            _c_int,  # dtype
+            _c_vp,  # q_weight
+            _c_vp,  # k_weight
+            _c_vp,  # cos
+            _c_i64,  # cos_ld
+            _c_vp,  # sin
+            _c_i64,  # sin_ld
+            _c_i64,  # table_rows
+            _c_int,  # table_dtype
+            _c_vp,  # positions
+            _c_int,  # index_dtype
+            _c_i64,  # pos_batch_stride
+            _c_i64,  # pos_token_stride
+            _c_float,  # eps
+            _c_vp,  # q_out
+            ctypes.POINTER(_c_i64),  # q_out_strides
+            _c_vp,  # k_out
+            ctypes.POINTER(_c_i64),  # k_out_strides
+            _c_vp,  # stream
+        ],
+        _c_int,
+    ),
+    "attnres_qk_norm_rope_workspace_size": (
+        [
+            _c_int,  # head_dim
+            ctypes.POINTER(_c_i64),  # bytes
+        ],
+        _c_int,
+    ),
+    "attnres_qk_norm_rope_bwd": (
+        [
+            _c_vp,  # q
+            ctypes.POINTER(_c_i64),  # q_strides
+            _c_vp,  # k
+            ctypes.POINTER(_c_i64),  # k_strides
+            _c_vp,  # grad_q_out
+            ctypes.POINTER(_c_i64),  # grad_q_out_strides
+            _c_vp,  # grad_k_out
+            ctypes.POINTER(_c_i64),  # grad_k_out_strides
+            _c_int,  # batch
+            _c_int,  # q_heads
+            _c_int,  # k_heads
+            _c_i64,  # tokens
+            _c_int,  # head_dim
+            _c_int,  # dtype
+            _c_vp,  # q_weight
+            _c_vp,  # k_weight
+            _c_vp,  # cos
+            _c_i64,  # cos_ld
+            _c_vp,  # sin
+            _c_i64,  # sin_ld
+            _c_i64,  # table_rows
+            _c_int,  # table_dtype
+            _c_vp,  # positions
+            _c_int,  # index_dtype
+            _c_i64,  # pos_batch_stride
+            _c_i64,  # pos_token_stride
+            _c_float,  # eps
+            _c_vp,  # grad_q
+            ctypes.POINTER(_c_i64),  # grad_q_strides
+            _c_vp,  # grad_k
+            ctypes.POINTER(_c_i64),  # grad_k_strides
+            _c_vp,  # grad_q_weight
+            _c_vp,  # grad_k_weight
+            _c_vp,  # workspace
+            _c_i64,  # workspace_bytes
+            _c_vp,  # stream
+        ],
+        _c_int,
+    ),
+    "attnres_embedding_fwd": (
+        [
+            _c_vp,  # ids
+            _c_int,  # index_dtype
+            _c_i64,  # num_ids
+            _c_vp,  # weight
+            _c_i64,  # weight_ld
+            _c_i64,  # rows
+            _c_int,  # hidden
+            _c_int,  # dtype
+            _c_float,  # scale
+            _c_vp,  # out
+            _c_vp,  # stream
+        ],
+        _c_int,
+    ),
+    "attnres_embedding_workspace_size": (
+        [
+            _c_i64,  # num_ids
+            _c_i64,  # rows
+            _c_int,  # hidden
+            ctypes.POINTER(_c_i64),  # bytes
+        ],
+        _c_int,
+    ),
+    "attnres_embedding_bwd": (
+        [
+            _c_vp,  # ids
+            _c_int,  # index_dtype
+            _c_i64,  # num_ids
+            _c_vp,  # grad_out
+            _c_i64,  # grad_out_ld
+            _c_i64,  # rows
+            _c_int,  # hidden
+            _c_int,  # dtype
+            _c_float,  # scale
+            _c_i64,  # padding_idx
+            _c_vp,  # grad_weight
+            _c_vp,  # workspace
+            _c_i64,  # workspace_bytes
+            _c_vp,  # stream
+        ],
+        _c_int,
+    ),
 }
 
 _lock = threading.Lock()
@@ -516,6 +737,52 @@ def route_bwd_queries(*args) -> int:
 
 def merge_bwd(*args) -> None:
     check("attnres_merge_bwd", lib().attnres_merge_bwd(*args))
+
+
+def attention_workspace_size(*args) -> int:
+    """Bytes of workspace :func:`attention_fwd` / :func:`attention_bwd` need (the last argument says which)."""
+    out = _c_i64(0)
+    check("attnres_attention_workspace_size", lib().attnres_attention_workspace_size(*args, ctypes.byref(out)))
+    return out.value
+
+
+def attention_fwd(*args) -> None:
+    check("attnres_attention_fwd", lib().attnres_attention_fwd(*args))
+
+
+def attention_bwd(*args) -> None:
+    check("attnres_attention_bwd", lib().attnres_attention_bwd(*args))
+
+
+def qk_norm_rope_workspace_size(head_dim: int) -> int:
+    """Bytes of workspace :func:`qk_norm_rope_bwd` needs on the current device."""
+    out = _c_i64(0)
+    check("attnres_qk_norm_rope_workspace_size", lib().attnres_qk_norm_rope_workspace_size(head_dim, ctypes.byref(out)))
+    return out.value
+
+
+def qk_norm_rope_fwd(*args) -> None:
+    check("attnres_qk_norm_rope_fwd", lib().attnres_qk_norm_rope_fwd(*args))
+
+
+def qk_norm_rope_bwd(*args) -> None:
+    check("attnres_qk_norm_rope_bwd", lib().attnres_qk_norm_rope_bwd(*args))
+
+
+def embedding_fwd(*args) -> None:
+    check("attnres_embedding_fwd", lib().attnres_embedding_fwd(*args))
+
+
+def embedding_workspace_size(num_ids: int, rows: int, hidden: int) -> int:
+    """Bytes of workspace :func:`embedding_bwd` needs."""
+    out = _c_i64(0)
+    check("attnres_embedding_workspace_size",
+          lib().attnres_embedding_workspace_size(num_ids, rows, hidden, ctypes.byref(out)))
+    return out.value
+
+
+def embedding_bwd(*args) -> None:
+    check("attnres_embedding_bwd", lib().attnres_embedding_bwd(*args))
 
 
 def set_kernel_policy(policy: int) -> int:

@@ -3,11 +3,13 @@
 Steps (all outputs under ``kotodama_amd/lib/``):
 
 1. ``hipcc --genco --offload-arch=gfx950`` compiles ``csrc/attnres_kernels.hip``
-   once per code-object part (``-DATTNRES_PART=0..11``, in parallel).
+   once per code-object part (``-DATTNRES_PART=0..11``, in parallel), and
+   ``csrc/lm_kernels.hip`` and ``csrc/attention_kernels.hip`` into the parts
+   after those (``-DLM_PART``).
 2. ``gcc`` assembles ``csrc/attnres_blob.S``, which ``.incbin``s the parts.
 3. ``hipcc -c -fPIC`` compiles ``csrc/attnres_noalloc.hip`` (the no-alloc
    entry point; its device array needs HIP device code of its own).
-4. ``g++`` links ``csrc/attnres_capi.cpp``, the blob and that object into the
+4. ``g++`` links ``csrc/attnres_capi.cpp``, ``csrc/lm_capi.cpp``, the blob and that object into the
    shared library, linked against ROCm's ``libamdhip64.so.7``.  Loaded after ``import torch``,
    the dynamic linker binds that soname to the HIP runtime torch already
    loaded, so streams and device memory are shared with torch.
@@ -37,7 +39,8 @@ LIB_NAME = "libattnres_hip.so"
 NATIVE_NAME = "_attnres_torch" + EXTENSION_SUFFIXES[0]  # as _native.py looks it up
 ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 ARCH = "gfx950"
-NUM_PARTS = 12
+NUM_PARTS = 12  # of attnres_kernels.hip
+LM_PARTS = {12: "lm_kernels.hip", 13: "attention_kernels.hip", 14: "attention_kernels.hip"}
 
 # Packed-fp32 VALU ops are disabled for every HIP compile (the kernels are
 # written with scalar fp32 arithmetic).
@@ -105,10 +108,11 @@ def build(verbose: bool = False, out_dir: Path | None = None, defines: tuple = (
         if torch is not None:
             native = _native_cmd(torch, native_o)
             native_proc = subprocess.Popen(native, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True)
-        for part in range(NUM_PARTS):
+        parts = [(part, "attnres_kernels.hip", f"-DATTNRES_PART={part}") for part in range(NUM_PARTS)]
+        parts += [(part, src, f"-DLM_PART={part}") for part, src in LM_PARTS.items()]
+        for part, src, select in parts:
             out = tmpd / f"attnres_gfx950_part{part}.hsaco"
-            cmd = [hipcc, *HIP_FLAGS, *extra, f"-DATTNRES_PART={part}", f"-I{CSRC}", str(CSRC / "attnres_kernels.hip"),
-                   "-o", str(out)]
+            cmd = [hipcc, *HIP_FLAGS, *extra, select, f"-I{CSRC}", str(CSRC / src), "-o", str(out)]
             if verbose:
                 print(" ".join(cmd), flush=True)
             procs.append((cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True)))
@@ -137,6 +141,7 @@ def build(verbose: bool = False, out_dir: Path | None = None, defines: tuple = (
                 f"-I{CSRC}",
                 f"-I{ROCM / 'include'}",
                 str(CSRC / "attnres_capi.cpp"),
+                str(CSRC / "lm_capi.cpp"),
                 str(blob_o),
                 str(noalloc_o),
                 f"-L{ROCM / 'lib'}",

@@ -1,4 +1,4 @@
-/* The twelve gfx950 code-object parts, linked into libattnres_hip.so as bytes
+/* The gfx950 code-object parts, linked into libattnres_hip.so as bytes
  * and loaded with hipModuleLoadData.  The build passes -I<dir of the .hsaco>. */
     .section .rodata
     .balign 4096
@@ -49,4 +49,16 @@ attnres_hsaco_part10:
     .global attnres_hsaco_part11
 attnres_hsaco_part11:
     .incbin "attnres_gfx950_part11.hsaco"
+    .balign 4096
+    .global attnres_hsaco_part12
+attnres_hsaco_part12:
+    .incbin "attnres_gfx950_part12.hsaco"
+    .balign 4096
+    .global attnres_hsaco_part13
+attnres_hsaco_part13:
+    .incbin "attnres_gfx950_part13.hsaco"
+    .balign 4096
+    .global attnres_hsaco_part14
+attnres_hsaco_part14:
+    .incbin "attnres_gfx950_part14.hsaco"
     .section .note.GNU-stack,"",@progbits

@@ -20,6 +20,7 @@
 #include <string>
 
 #include "attnres.h"
+#include "attnres_internal.h"
 #include "attnres_params.h"
 
 // Code-object parts (attnres_blob.S).
@@ -35,10 +36,13 @@ extern "C" const unsigned char attnres_hsaco_part8[];
 extern "C" const unsigned char attnres_hsaco_part9[];
 extern "C" const unsigned char attnres_hsaco_part10[];
 extern "C" const unsigned char attnres_hsaco_part11[];
+extern "C" const unsigned char attnres_hsaco_part12[];
+extern "C" const unsigned char attnres_hsaco_part13[];
+extern "C" const unsigned char attnres_hsaco_part14[];
 
 namespace {
 
-constexpr int kParts = 12;
+constexpr int kParts = 15;  // 12..14: the language-model operators (lm_capi.cpp)
 constexpr int kMaxDevices = 64;
 constexpr int kMaxThreads = 512;  // __launch_bounds__ of every kernel
 
@@ -123,6 +127,7 @@ struct DeviceState {
   KernelSlot bwd_mqg[2 * 9];     // batched-query backward on the matrix cores: query groups x S
   KernelSlot bwd_defer[4 * 10];  // row-per-wave backward with deferred block gradients: row width x S
   KernelSlot gather_seg[4 * ATTNRES_SEG_MAX_BLOCKS];  // segment sums: row width x blocks
+  KernelSlot lm[ATTNRES_INTERNAL_SLOTS];  // the language-model operators, numbered by lm_capi.cpp
 };
 
 DeviceState g_dev[kMaxDevices];
@@ -209,7 +214,8 @@ int ensure_loaded(DeviceState** out) {
       const unsigned char* blobs[kParts] = {attnres_hsaco_part0, attnres_hsaco_part1, attnres_hsaco_part2,
                                             attnres_hsaco_part3, attnres_hsaco_part4, attnres_hsaco_part5,
                                             attnres_hsaco_part6, attnres_hsaco_part7, attnres_hsaco_part8,
-                                            attnres_hsaco_part9, attnres_hsaco_part10, attnres_hsaco_part11};
+                                            attnres_hsaco_part9, attnres_hsaco_part10, attnres_hsaco_part11,
+                                            attnres_hsaco_part12, attnres_hsaco_part13, attnres_hsaco_part14};
       // On a failure nothing stays half-loaded: the next call starts over.
       auto unload = [&st](int n) {
         for (int j = 0; j < n; ++j) {
@@ -1080,6 +1086,21 @@ extern "C" {
 // Sets attnres_last_error() for attnres_noalloc.hip; returns `code`.
 __attribute__((visibility("hidden"))) int attnres_internal_fail(int code, const char* msg) {
   return fail(code, "%s", msg);
+}
+
+int attnres_internal_kernel(int slot, int part, const char* name, hipFunction_t* f, int* num_cus) {
+  DeviceState* st = nullptr;
+  int rc = ensure_loaded(&st);
+  if (rc != ATTNRES_OK) return rc;
+  *num_cus = st->num_cus;
+  return slot_function(*st, st->lm[slot], part, name, f);
+}
+
+int attnres_internal_num_cus(int* num_cus) {
+  DeviceState* st = nullptr;
+  int rc = ensure_loaded(&st);
+  if (rc == ATTNRES_OK) *num_cus = st->num_cus;
+  return rc;
 }
 
 int attnres_version(void) { return 10000; }

@@ -1,0 +1,613 @@
+// Memory-bound language-model operators for gfx950: per-head RMSNorm with the
+// position rotation of queries and keys, and the embedding lookup with its
+// gradient by sorted tokens.  Sums and statistics are fp32; results are
+// rounded once.
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "lm_params.h"
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+namespace {
+
+constexpr float kNan = __builtin_nanf("");
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  bf16x2 r = {(__bf16)lo, (__bf16)hi};
+  return __builtin_bit_cast(uint32_t, r);
+}
+
+// V consecutive elements of type T (V = 1, or a 16-byte chunk) as fp32.
+struct Bf16 {
+  typedef uint16_t raw;
+  static constexpr int kVec = 8;
+  static __device__ __forceinline__ float one(uint16_t r) { return __builtin_bit_cast(float, (uint32_t)r << 16); }
+  static __device__ __forceinline__ void chunk(const u32x4& w, float* v) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t u = w[i];
+      v[2 * i] = __builtin_bit_cast(float, u << 16);
+      v[2 * i + 1] = __builtin_bit_cast(float, u & 0xffff0000u);
+    }
+  }
+  static __device__ __forceinline__ u32x4 unchunk(const float* v) {
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+    return w;
+  }
+  static __device__ __forceinline__ uint16_t from(float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }
+};
+struct F32 {
+  typedef float raw;
+  static constexpr int kVec = 4;
+  static __device__ __forceinline__ float one(float r) { return r; }
+  static __device__ __forceinline__ void chunk(const u32x4& w, float* v) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t u = w[i];
+      v[i] = __builtin_bit_cast(float, u);
+    }
+  }
+  static __device__ __forceinline__ u32x4 unchunk(const float* v) {
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __builtin_bit_cast(uint32_t, v[i]);
+    return w;
+  }
+  static __device__ __forceinline__ float from(float v) { return v; }
+};
+
+template <typename T, int V>
+__device__ __forceinline__ void load(const void* base, int64_t at, float* v) {
+  const typename T::raw* p = (const typename T::raw*)base + at;
+  if constexpr (V == 1) {
+    v[0] = T::one(*p);
+  } else {
+    T::chunk(*(const u32x4*)p, v);
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ void store(void* base, int64_t at, const float* v) {
+  typename T::raw* p = (typename T::raw*)base + at;
+  if constexpr (V == 1) {
+    *p = T::from(v[0]);
+  } else {
+    *(u32x4*)p = T::unchunk(v);
+  }
+}
+
+__device__ __forceinline__ int64_t index_at(const void* p, int64_t i, int is64) {
+  return is64 ? ((const int64_t*)p)[i] : (int64_t)((const int32_t*)p)[i];
+}
+
+// Sum over the G lanes of a row's group (G a power of two).
+__device__ __forceinline__ float group_sum(float v, int g) {
+  for (int m = 1; m < g; m <<= 1) v += __shfl_xor(v, m);
+  return v;
+}
+
+// ---------------------------------------------------------- qk_norm_rope --
+//
+//   n = x r w,  r = rsqrt(mean x^2 + eps)
+//   y_i = n_i cos_i - n_{i+h} sin_i,  y_{i+h} = n_{i+h} cos_{i+h} + n_i sin_{i+h}   (i < h = dim / 2)
+// and backward, from g = dL/dy:
+//   dn_i = g_i cos_i + g_{i+h} sin_{i+h},  dn_{i+h} = g_{i+h} cos_{i+h} - g_i sin_i
+//   dx = r (w dn - x r^2 mean(w dn x)),   dw = sum over rows of dn x r
+//
+// A group of G lanes holds one head row, a lane the V elements from V l of
+// each half, so the rotation needs nothing from other lanes and the mean is a
+// sum over the group.  Bound by memory: one read and one write of a row.
+
+template <typename T, int V, int C>
+struct Rope {
+  float clo[C][V], chi[C][V], slo[C][V], shi[C][V];
+};
+
+template <typename T, int V, int C>
+__device__ __forceinline__ void load_table(const lm_rope_params& P, int64_t pos, int l, int g, Rope<T, V, C>& R) {
+  const int half = P.dim >> 1;
+  const bool ok = pos >= 0 && pos < P.table_rows;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int d = (c * g + l) * V;
+    const bool in = ok && d < half;
+#pragma unroll
+    for (int j = 0; j < V; ++j) R.clo[c][j] = R.chi[c][j] = R.slo[c][j] = R.shi[c][j] = kNan;
+    if (in) {
+      const int64_t ac = pos * P.cos_ld + d, as = pos * P.sin_ld + d;
+      if (P.table_f32) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          R.clo[c][j] = ((const float*)P.cos)[ac + j];
+          R.chi[c][j] = ((const float*)P.cos)[ac + half + j];
+          R.slo[c][j] = ((const float*)P.sin)[as + j];
+          R.shi[c][j] = ((const float*)P.sin)[as + half + j];
+        }
+      } else {
+        load<T, V>(P.cos, ac, R.clo[c]);
+        load<T, V>(P.cos, ac + half, R.chi[c]);
+        load<T, V>(P.sin, as, R.slo[c]);
+        load<T, V>(P.sin, as + half, R.shi[c]);
+      }
+    }
+  }
+}
+
+template <typename T, int V, int C>
+__device__ __forceinline__ void load_halves(const void* base, int64_t at, int half, int l, int g, bool live,
+                                            float (&lo)[C][V], float (&hi)[C][V]) {
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int d = (c * g + l) * V;
+#pragma unroll
+    for (int j = 0; j < V; ++j) lo[c][j] = hi[c][j] = 0.f;
+    if (live && d < half) {
+      load<T, V>(base, at + d, lo[c]);
+      load<T, V>(base, at + half + d, hi[c]);
+    }
+  }
+}
+
+__device__ __forceinline__ int64_t token_position(const lm_rope_params& P, int64_t b, int64_t t) {
+  return P.positions == nullptr ? t : index_at(P.positions, b * P.pos_b + t * P.pos_t, P.pos64);
+}
+
+// HPG heads of one token per lane group.
+template <typename T, int V, int C, int HPG>
+__device__ __forceinline__ void qk_norm_rope_fwd(const lm_rope_params& P) {
+  const int g = P.lanes, l = threadIdx.x & (g - 1);
+  const int64_t item = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / g;
+  const int qc = (P.heads[0] + HPG - 1) / HPG, kc = (P.heads[1] + HPG - 1) / HPG;
+  if (item >= (int64_t)P.batch * P.tokens * (qc + kc)) return;
+  const int64_t n = item / (qc + kc);
+  const int part = (int)(item - n * (qc + kc));
+  const int x = part < qc ? 0 : 1;
+  const int h0 = (x ? part - qc : part) * HPG;
+  const int64_t b = n / P.tokens, t = n - b * P.tokens;
+  const int half = P.dim >> 1;
+  const void* src = x ? P.x[1] : P.x[0];
+  void* dst = x ? P.y[1] : P.y[0];
+  const void* wp = x ? P.w[1] : P.w[0];
+  const lm_strides sx = x ? P.sx[1] : P.sx[0], sy = x ? P.sy[1] : P.sy[0];
+  const int heads = x ? P.heads[1] : P.heads[0];
+
+  float lo[HPG][C][V], hi[HPG][C][V];
+#pragma unroll
+  for (int i = 0; i < HPG; ++i)
+    load_halves<T, V, C>(src, b * sx.b + (int64_t)(h0 + i) * sx.h + t * sx.t, half, l, g, h0 + i < heads, lo[i], hi[i]);
+  float wlo[C][V], whi[C][V];
+  load_halves<T, V, C>(wp, 0, half, l, g, true, wlo, whi);
+  Rope<T, V, C> R;
+  load_table<T, V, C>(P, token_position(P, b, t), l, g, R);
+#pragma unroll
+  for (int i = 0; i < HPG; ++i) {
+    float ss = 0.f;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        ss = __builtin_fmaf(lo[i][c][j], lo[i][c][j], ss);
+        ss = __builtin_fmaf(hi[i][c][j], hi[i][c][j], ss);
+      }
+    const float r = __builtin_amdgcn_rsqf(group_sum(ss, g) * P.inv_dim + P.eps);
+    if (h0 + i >= heads) continue;
+    const int64_t at = b * sy.b + (int64_t)(h0 + i) * sy.h + t * sy.t;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int d = (c * g + l) * V;
+      if (d >= half) continue;
+      float ylo[V], yhi[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float a = lo[i][c][j] * r * wlo[c][j], e = hi[i][c][j] * r * whi[c][j];
+        ylo[j] = a * R.clo[c][j] - e * R.slo[c][j];
+        yhi[j] = e * R.chi[c][j] + a * R.shi[c][j];
+      }
+      store<T, V>(dst, at + d, ylo);
+      store<T, V>(dst, at + half + d, yhi);
+    }
+  }
+}
+
+// blockIdx.y: queries or keys.  The lane groups of the grid walk over (token,
+// HPG heads) items; each lane keeps its columns' weight gradient, the
+// workgroup adds its groups' in a fixed order and writes one row of partials.
+template <typename T, int V, int C, int HPG>
+__device__ __forceinline__ void qk_norm_rope_bwd(const lm_rope_params& P, float* red) {
+  const int g = P.lanes, l = threadIdx.x & (g - 1);
+  const int x = blockIdx.y;
+  const int half = P.dim >> 1;
+  const void* src = x ? P.x[1] : P.x[0];
+  const void* gsrc = x ? P.g[1] : P.g[0];
+  void* dst = x ? P.y[1] : P.y[0];
+  const void* wp = x ? P.w[1] : P.w[0];
+  const lm_strides sx = x ? P.sx[1] : P.sx[0], sy = x ? P.sy[1] : P.sy[0], sg = x ? P.sg[1] : P.sg[0];
+  const int heads = x ? P.heads[1] : P.heads[0];
+  const int hc = (heads + HPG - 1) / HPG;
+  const int64_t items = (int64_t)P.batch * P.tokens * hc;
+  const int groups = blockDim.x / g, grp = threadIdx.x / g;
+  float wlo[C][V], whi[C][V], dwlo[C][V], dwhi[C][V];
+  load_halves<T, V, C>(wp, 0, half, l, g, true, wlo, whi);
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+#pragma unroll
+    for (int j = 0; j < V; ++j) dwlo[c][j] = dwhi[c][j] = 0.f;
+  for (int64_t item = (int64_t)blockIdx.x * groups + grp; item < items; item += (int64_t)gridDim.x * groups) {
+    const int64_t n = item / hc;
+    const int h0 = (int)(item - n * hc) * HPG;
+    const int64_t b = n / P.tokens, t = n - b * P.tokens;
+    float lo[HPG][C][V], hi[HPG][C][V], glo[HPG][C][V], ghi[HPG][C][V];
+#pragma unroll
+    for (int i = 0; i < HPG; ++i) {
+      const bool live = h0 + i < heads;
+      load_halves<T, V, C>(src, b * sx.b + (int64_t)(h0 + i) * sx.h + t * sx.t, half, l, g, live, lo[i], hi[i]);
+      load_halves<T, V, C>(gsrc, b * sg.b + (int64_t)(h0 + i) * sg.h + t * sg.t, half, l, g, live, glo[i], ghi[i]);
+    }
+    Rope<T, V, C> R;
+    load_table<T, V, C>(P, token_position(P, b, t), l, g, R);
+#pragma unroll
+    for (int i = 0; i < HPG; ++i) {
+      float ss = 0.f, mx = 0.f;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const bool in = (c * g + l) * V < half;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float a = lo[i][c][j], e = hi[i][c][j];
+          ss = __builtin_fmaf(a, a, ss);
+          ss = __builtin_fmaf(e, e, ss);
+          const float da = in ? glo[i][c][j] * R.clo[c][j] + ghi[i][c][j] * R.shi[c][j] : 0.f;
+          const float de = in ? ghi[i][c][j] * R.chi[c][j] - glo[i][c][j] * R.slo[c][j] : 0.f;
+          glo[i][c][j] = da;
+          ghi[i][c][j] = de;
+          mx = __builtin_fmaf(da * wlo[c][j], a, mx);
+          mx = __builtin_fmaf(de * whi[c][j], e, mx);
+        }
+      }
+      ss = group_sum(ss, g);
+      mx = group_sum(mx, g);
+      const float r = __builtin_amdgcn_rsqf(ss * P.inv_dim + P.eps);
+      const float k = r * r * mx * P.inv_dim;
+      if (h0 + i >= heads) continue;
+      const int64_t at = b * sy.b + (int64_t)(h0 + i) * sy.h + t * sy.t;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int d = (c * g + l) * V;
+        if (d >= half) continue;
+        float olo[V], ohi[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float a = lo[i][c][j], e = hi[i][c][j], da = glo[i][c][j], de = ghi[i][c][j];
+          olo[j] = r * (wlo[c][j] * da - a * k);
+          ohi[j] = r * (whi[c][j] * de - e * k);
+          dwlo[c][j] = __builtin_fmaf(da * a, r, dwlo[c][j]);
+          dwhi[c][j] = __builtin_fmaf(de * e, r, dwhi[c][j]);
+        }
+        store<T, V>(dst, at + d, olo);
+        store<T, V>(dst, at + half + d, ohi);
+      }
+    }
+  }
+  // the workgroup's weight gradient, one column after another, groups in order
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int d = (c * g + l) * V;
+    if (d < half) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        red[grp * P.dim + d + j] = dwlo[c][j];
+        red[grp * P.dim + half + d + j] = dwhi[c][j];
+      }
+    }
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < P.dim; d += blockDim.x) {
+    float s = 0.f;
+    for (int i = 0; i < groups; ++i) s += red[i * P.dim + d];
+    P.dw_part[((int64_t)x * gridDim.x + blockIdx.x) * P.dim + d] = s;
+  }
+}
+
+// Sums the partial rows: workgroup (column block, queries or keys) of 32
+// columns x 8 row strides, added in a fixed order.
+template <typename T>
+__device__ __forceinline__ void rope_dw_sum(const lm_rope_params& P, float* red) {
+  const int x = blockIdx.y, col = threadIdx.x & 31, str = threadIdx.x >> 5;
+  const int d = blockIdx.x * 32 + col;
+  float s = 0.f;
+  if (d < P.dim) {
+    const float* p = P.dw_part + (int64_t)x * P.parts * P.dim + d;
+#pragma unroll 4
+    for (int i = str; i < P.parts; i += 32) s += p[(int64_t)i * P.dim];
+  }
+  red[str * 33 + col] = s;
+  __syncthreads();
+  if (threadIdx.x < 32 && d < P.dim) {
+    float tot = 0.f;
+    for (int i = 0; i < 32; ++i) tot += red[i * 33 + col];
+    void* dw = x ? P.dw[1] : P.dw[0];
+    if (dw != nullptr) store<T, 1>(dw, d, &tot);
+  }
+}
+
+// ------------------------------------------------------------- embedding --
+//
+//   out_n = scale w[id_n]          dw_r = scale sum over {n: id_n = r} of g_n
+//
+// The gradient sorts the tokens by row, stably, so that every row's sum has a
+// fixed order whatever the launch.  Three launches:
+//   sort   one workgroup per range of table rows.  Each scans all ids (they
+//          stay in L2): its 16 waves, each a stretch of the tokens in order,
+//          count their tokens per row in LDS; a scan over rows and waves
+//          gives every (row, wave) its place, and ids below the range the
+//          range's own; a second walk places the tokens.  Rows without tokens
+//          are zeroed here.
+//   sum    one workgroup per stretch of `seg` sorted tokens and column slice:
+//          runs of one row are added in order and written; a run that crosses
+//          the stretch's ends is left as an fp32 partial row.
+//   join   the crossing runs' partial rows are added in order.
+
+template <typename T, int V>
+__device__ __forceinline__ void embedding_fwd(const lm_embed_params& P) {
+  const int tpr = P.threads_per_row;
+  const int64_t n = (int64_t)blockIdx.x * (blockDim.x / tpr) + threadIdx.x / tpr;
+  if (n >= P.n) return;
+  const int64_t id = index_at(P.ids, n, P.ids64);
+  const bool ok = id >= 0 && id < P.rows;
+  for (int c = threadIdx.x & (tpr - 1); c * V < P.dim; c += tpr) {
+    float v[V];
+    if (ok) {
+      load<T, V>(P.w, id * P.w_ld + c * V, v);
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] *= P.scale;
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = kNan;
+    }
+    store<T, V>(P.out, n * P.dim + c * V, v);
+  }
+}
+
+// cnt: LM_EMBED_WAVES x range counters; scan: one word per wave
+template <typename T, int V>
+__device__ __forceinline__ void embedding_sort(const lm_embed_params& P, int* cnt, int* scan) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int range = P.range;
+  const int64_t lo = (int64_t)blockIdx.x * range;
+  const int64_t hi = lo + range < P.rows ? lo + range : P.rows;
+  int* mine = cnt + wave * range;
+  for (int i = threadIdx.x; i < range * LM_EMBED_WAVES; i += blockDim.x) cnt[i] = 0;
+  __syncthreads();
+  const int64_t per = ((P.n + LM_EMBED_WAVES - 1) / LM_EMBED_WAVES + 63) / 64 * 64;
+  const int64_t t0 = per * wave, t1 = t0 + per < P.n ? t0 + per : P.n;
+  int below = 0;
+#pragma unroll 4
+  for (int64_t t = t0 + lane; t < t1; t += 64) {
+    const int64_t id = index_at(P.ids, t, P.ids64);
+    if (id == P.padding) continue;
+    if (id >= lo && id < hi) atomicAdd(&mine[id - lo], 1);
+    else if (id >= 0 && id < lo) ++below;
+  }
+  for (int m = 1; m < 64; m <<= 1) below += __shfl_xor(below, m);
+  if (lane == 0) scan[wave] = below;
+  __syncthreads();
+  int base = 0;
+  for (int i = 0; i < LM_EMBED_WAVES; ++i) base += scan[i];
+  __syncthreads();
+  // thread r: row lo + r
+  const int r = threadIdx.x;
+  int total = 0;
+  if (r < range)
+    for (int i = 0; i < LM_EMBED_WAVES; ++i) total += cnt[i * range + r];
+  int incl = total;
+  for (int m = 1; m < 64; m <<= 1) {
+    const int o = __shfl_up(incl, m);
+    if (lane >= m) incl += o;
+  }
+  if (lane == 63) scan[wave] = incl;
+  __syncthreads();
+  int at = base + incl - total;
+  for (int i = 0; i < wave; ++i) at += scan[i];
+  if (r < range) {
+    if (lo + r < P.rows) P.row_count[lo + r] = total;
+    for (int i = 0; i < LM_EMBED_WAVES; ++i) {
+      const int c = cnt[i * range + r];
+      cnt[i * range + r] = at;
+      at += c;
+    }
+  }
+  if (blockIdx.x == gridDim.x - 1 && r == range - 1) P.counts[0] = at;  // tokens in all
+  __syncthreads();
+  for (int64_t tb = t0; tb < t1; tb += 64) {
+    const int64_t t = tb + lane;
+    int64_t id = -1;
+    if (t < t1) id = index_at(P.ids, t, P.ids64);
+    const bool in = id >= lo && id < hi && id != P.padding;
+    const int row = (int)(id - lo);
+    uint64_t left = __ballot(in);
+    while (left != 0) {
+      const int lead = __builtin_ctzll(left);
+      const int rr = __builtin_amdgcn_readlane(row, lead);
+      const uint64_t same = __ballot(in && row == rr);
+      const int from = *(volatile int*)&mine[rr];
+      if (in && row == rr) {
+        const int p = from + __popcll(same & (((uint64_t)1 << lane) - 1));
+        P.sorted_token[p] = (int32_t)t;
+        P.sorted_row[p] = (int32_t)id;
+      }
+      if (lane == lead) *(volatile int*)&mine[rr] = from + __popcll(same);
+      left &= ~same;
+    }
+  }
+}
+
+// Rows without tokens get a zero gradient: a wave per row.
+template <typename T, int V>
+__device__ __forceinline__ void embedding_zero(const lm_embed_params& P) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6);
+  if (row >= P.rows || P.row_count[row] != 0) return;
+  float z[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) z[j] = 0.f;
+  for (int c = lane; c * V < P.dim; c += 64) store<T, V>(P.dw, row * P.dim + c * V, z);
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void embedding_sum(const lm_embed_params& P) {
+  const int count = P.counts[0];
+  const int s0 = blockIdx.x * P.seg;
+  if (s0 >= count) return;
+  const int s1 = s0 + P.seg < count ? s0 + P.seg : count;
+  const int c = blockIdx.y * blockDim.x + threadIdx.x;
+  if (c * V >= P.dim) return;
+  const int before = s0 > 0 ? P.sorted_row[s0 - 1] : -1;
+  const int after = s1 < count ? P.sorted_row[s1] : -1;
+  float acc[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) acc[j] = 0.f;
+  int row = P.sorted_row[s0];
+  auto flush = [&](bool end) {
+    // crossing the start: partial 0; crossing the end only: partial 1
+    const bool head = row == before, tail = end && row == after;
+    if (head || tail) {
+      float* p = P.part + ((int64_t)blockIdx.x * 2 + (head ? 0 : 1)) * P.dim + c * V;
+#pragma unroll
+      for (int j = 0; j < V; ++j) p[j] = acc[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) acc[j] *= P.scale;
+      store<T, V>(P.dw, (int64_t)row * P.dim + c * V, acc);
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) acc[j] = 0.f;
+  };
+  constexpr int U = 4;
+  for (int i = s0; i < s1; i += U) {
+    float v[U][V];
+    int rows[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = i + u < s1 ? i + u : s1 - 1;
+      rows[u] = P.sorted_row[k];
+      load<T, V>(P.g, (int64_t)P.sorted_token[k] * P.g_ld + c * V, v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (i + u < s1) {
+        if (rows[u] != row) {
+          flush(false);
+          row = rows[u];
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) acc[j] += v[u][j];
+      }
+    }
+  }
+  flush(true);
+}
+
+// Workgroup (16 stretches, 64 columns): for each run that starts in one of the
+// stretches and leaves it, the 16 waves add every 16th partial row and then
+// each other's sums in order.
+template <typename T>
+__device__ __forceinline__ void embedding_join(const lm_embed_params& P, float* red) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int count = P.counts[0];
+  const int stretches = (count + P.seg - 1) / P.seg;
+  const int d = blockIdx.y * 64 + lane;
+  for (int i = 0; i < LM_EMBED_JOIN; ++i) {
+    const int s = blockIdx.x * LM_EMBED_JOIN + i;
+    if (s + 1 >= stretches) return;
+    const int s0 = s * P.seg, s1 = s0 + P.seg;
+    const int row = P.sorted_row[s1];
+    if (P.sorted_row[s1 - 1] != row) continue;                                             // no run crosses this end
+    if (P.sorted_row[s0] == row && s0 > 0 && P.sorted_row[s0 - 1] == row) continue;      // it started earlier
+    // stretches s+1 .. e hold the rest of the run: the first whose first row is another ends it
+    int e = s + 1;
+    {
+      int lo = s + 1, hi = stretches - 1;  // the last stretch that begins with this row
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (P.sorted_row[mid * P.seg] == row) lo = mid;
+        else hi = mid - 1;
+      }
+      e = lo;
+    }
+    float sum = 0.f;
+    if (d < P.dim) {
+#pragma unroll 4
+      for (int k = s + wave; k <= e; k += LM_EMBED_WAVES)
+        sum += P.part[((int64_t)k * 2 + (k == s ? 1 : 0)) * P.dim + d];
+    }
+    red[wave * 64 + lane] = sum;
+    __syncthreads();
+    if (wave == 0 && d < P.dim) {
+      float tot = 0.f;
+      for (int w = 0; w < LM_EMBED_WAVES; ++w) tot += red[w * 64 + lane];
+      tot *= P.scale;
+      store<T, 1>(P.dw, (int64_t)row * P.dim + d, &tot);
+    }
+    __syncthreads();
+  }
+}
+
+}  // namespace
+
+// C: chunks of a half row per lane; one except for scalar rows wider than 128.
+#define LM_ROPE(NAME, T, V, C)                                                                      \
+  extern "C" __global__ void __launch_bounds__(256) attnres_qk_norm_rope_##NAME##_h1(lm_rope_params P) { \
+    qk_norm_rope_fwd<T, V, C, 1>(P);                                                                \
+  }                                                                                                 \
+  extern "C" __global__ void __launch_bounds__(256) attnres_qk_norm_rope_##NAME##_h4(lm_rope_params P) { \
+    qk_norm_rope_fwd<T, V, C, 4>(P);                                                                \
+  }                                                                                                 \
+  extern "C" __global__ void __launch_bounds__(256) attnres_qk_norm_rope_bwd_##NAME(lm_rope_params P) { \
+    extern __shared__ float lm_red[];                                                               \
+    qk_norm_rope_bwd<T, V, C, 2>(P, lm_red);                                                        \
+  }
+LM_ROPE(bf16_v8, Bf16, 8, 1)
+LM_ROPE(bf16_v1, Bf16, 1, 2)
+LM_ROPE(f32_v4, F32, 4, 1)
+LM_ROPE(f32_v1, F32, 1, 2)
+
+#define LM_ROPE_SUM(NAME, T)                                                                          \
+  extern "C" __global__ void __launch_bounds__(1024) attnres_qk_norm_rope_dw_##NAME(lm_rope_params P) { \
+    __shared__ float red[32 * 33];                                                                    \
+    rope_dw_sum<T>(P, red);                                                                           \
+  }
+LM_ROPE_SUM(bf16, Bf16)
+LM_ROPE_SUM(f32, F32)
+
+#define LM_EMBED(NAME, T, V)                                                                              \
+  extern "C" __global__ void __launch_bounds__(256) attnres_embedding_fwd_##NAME(lm_embed_params P) {     \
+    embedding_fwd<T, V>(P);                                                                               \
+  }                                                                                                       \
+  extern "C" __global__ void __launch_bounds__(256) attnres_embedding_zero_##NAME(lm_embed_params P) {    \
+    embedding_zero<T, V>(P);                                                                              \
+  }                                                                                                       \
+  extern "C" __global__ void __launch_bounds__(512) attnres_embedding_sum_##NAME(lm_embed_params P) {     \
+    embedding_sum<T, V>(P);                                                                               \
+  }
+LM_EMBED(bf16_v8, Bf16, 8)
+LM_EMBED(bf16_v1, Bf16, 1)
+LM_EMBED(f32_v4, F32, 4)
+LM_EMBED(f32_v1, F32, 1)
+
+extern "C" __global__ void __launch_bounds__(64 * LM_EMBED_WAVES) attnres_embedding_sort(lm_embed_params P) {
+  __shared__ int cnt[LM_EMBED_WAVES * LM_EMBED_MAX_RANGE];
+  __shared__ int scan[LM_EMBED_WAVES];
+  embedding_sort<F32, 1>(P, cnt, scan);
+}
+#define LM_EMBED_JOIN_K(NAME, T)                                                                                  \
+  extern "C" __global__ void __launch_bounds__(64 * LM_EMBED_WAVES) attnres_embedding_join_##NAME(lm_embed_params P) { \
+    __shared__ float red[64 * LM_EMBED_WAVES];                                                                    \
+    embedding_join<T>(P, red);                                                                                    \
+  }
+LM_EMBED_JOIN_K(bf16, Bf16)
+LM_EMBED_JOIN_K(f32, F32)
