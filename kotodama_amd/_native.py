@@ -1,7 +1,8 @@
 """The native call path of the eager torch layer (``csrc/attnres_torch.cpp``).
 
 ``native.route`` / ``route_list`` / ``merge`` / ``block_step`` and the training
-points' ``step`` / ``bwd_rows`` / ``bwd_defer`` / ``gather_seg`` launch one
+points' ``step`` / ``bwd_rows`` / ``bwd_defer`` / ``gather_seg``, and the
+language-model operators' ``attention`` / ``qk_norm_rope`` / ``embedding`` launch one
 plain call and return its result, or return None with nothing done for any
 call that is not plain (the caller then takes it through Python).  Loaded on
 first use.  Without the built extension every function returns None and the
@@ -20,7 +21,8 @@ from pathlib import Path
 # named for this interpreter: one built for another Python is not found
 NAME = "_attnres_torch" + importlib.machinery.EXTENSION_SUFFIXES[0]
 PATH = Path(__file__).resolve().parent / "lib" / NAME
-FUNCTIONS = ("route", "route_list", "merge", "block_step", "step", "bwd_rows", "bwd_defer", "gather_seg")
+FUNCTIONS = ("route", "route_list", "merge", "block_step", "step", "bwd_rows", "bwd_defer", "gather_seg", "attention",
+             "qk_norm_rope", "embedding")
 
 _lock = threading.Lock()
 

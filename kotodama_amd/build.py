@@ -14,7 +14,7 @@ Steps (all outputs under ``kotodama_amd/lib/``):
    the dynamic linker binds that soname to the HIP runtime torch already
    loaded, so streams and device memory are shared with torch.
 5. Where a ROCm torch is importable, ``g++`` compiles ``csrc/attnres_torch.cpp``
-   against its headers into ``_attnres_torch`` (with this Python's extension
+   and ``csrc/lm_torch.cpp`` against its headers into ``_attnres_torch`` (with this Python's extension
    suffix), the CPython extension through which the eager torch layer calls
    that library.  The library needs no torch and is in place before this step
    can fail; an extension of an earlier build does not stay beside it.
@@ -37,6 +37,7 @@ LIBDIR = PKG / "lib"
 INCLUDE = PKG.parent / "include"
 LIB_NAME = "libattnres_hip.so"
 NATIVE_NAME = "_attnres_torch" + EXTENSION_SUFFIXES[0]  # as _native.py looks it up
+NATIVE_SOURCES = ("attnres_torch.cpp", "lm_torch.cpp")
 ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 ARCH = "gfx950"
 NUM_PARTS = 12  # of attnres_kernels.hip
@@ -65,8 +66,8 @@ def _rocm_torch():
     return torch if torch.version.hip is not None else None
 
 
-def _native_cmd(torch, out: Path) -> list[str]:
-    """Compile the torch layer's extension to an object file (the link follows the C-ABI library's)."""
+def _native_cmd(torch, src: str, out: Path) -> list[str]:
+    """Compile one source of the torch layer's extension to an object file (the link follows the C-ABI library's)."""
     import sysconfig
 
     from torch.utils.cpp_extension import include_paths
@@ -75,7 +76,7 @@ def _native_cmd(torch, out: Path) -> list[str]:
     return ["g++", "-c", "-fPIC", "-O2", "-std=c++17", "-Wall", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__",
             "-DUSE_ROCM", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
             f'-DATTNRES_TORCH_VERSION="{torch.__version__}"', f"-I{INCLUDE}", f"-I{CSRC}", *incs,
-            str(CSRC / "attnres_torch.cpp"), "-o", str(out)]
+            str(CSRC / src), "-o", str(out)]
 
 
 def _run(cmd: list[str], cwd: Path | None = None) -> None:
@@ -103,11 +104,12 @@ def build(verbose: bool = False, out_dir: Path | None = None, defines: tuple = (
     with tempfile.TemporaryDirectory(prefix="attnres_build_", dir=libdir) as tmp:
         tmpd = Path(tmp)
         procs = []
-        native_o = tmpd / "attnres_torch.o"
         torch = _rocm_torch()
-        if torch is not None:
-            native = _native_cmd(torch, native_o)
-            native_proc = subprocess.Popen(native, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True)
+        native, native_o = [], []
+        for src in NATIVE_SOURCES if torch is not None else ():
+            native_o.append(tmpd / f"{Path(src).stem}.o")
+            cmd = _native_cmd(torch, src, native_o[-1])
+            native.append((cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True)))
         parts = [(part, "attnres_kernels.hip", f"-DATTNRES_PART={part}") for part in range(NUM_PARTS)]
         parts += [(part, src, f"-DLM_PART={part}") for part, src in LM_PARTS.items()]
         for part, src, select in parts:
@@ -156,10 +158,11 @@ def build(verbose: bool = False, out_dir: Path | None = None, defines: tuple = (
         for old in libdir.glob("_attnres_torch*.so"):
             old.unlink()  # made for the library that was here before
         if torch is not None:
-            _wait(native, native_proc)
+            for cmd, p in native:
+                _wait(cmd, p)
             torch_lib = Path(torch.__file__).parent / "lib"
             native_tmp = tmpd / NATIVE_NAME
-            _run(["g++", "-shared", str(native_o), f"-L{libdir}", "-lattnres_hip", f"-L{torch_lib}", "-ltorch_python",
+            _run(["g++", "-shared", *map(str, native_o), f"-L{libdir}", "-lattnres_hip", f"-L{torch_lib}", "-ltorch_python",
                   "-ltorch_cpu", "-ltorch_hip", "-lc10_hip", "-lc10", "-Wl,-rpath,$ORIGIN",
                   f"-Wl,-rpath,{torch_lib}", "-o", str(native_tmp)])
             os.replace(native_tmp, libdir / NATIVE_NAME)

@@ -26,8 +26,7 @@ enum Slot {
   kRopeBwd = kRopeFwd + 8,     // + 2 * (fp32) + (scalar)
   kRopeDw = kRopeBwd + 4,      // + (fp32)
   kEmbedFwd = kRopeDw + 2,     // + 2 * (fp32) + (scalar)
-  kEmbedZero = kEmbedFwd + 4,
-  kEmbedSum = kEmbedZero + 4,
+  kEmbedSum = kEmbedFwd + 4,
   kEmbedJoin = kEmbedSum + 4,  // + (fp32)
   kEmbedSort = kEmbedJoin + 2,
   kSlots
@@ -232,7 +231,7 @@ const char* rope_kind(bool f32, bool vec) { return f32 ? (vec ? "f32_v4" : "f32_
 struct EmbedPlan {
   int range, ranges, seg;
   int64_t stretches;
-  int64_t at_rows, at_token, at_row, at_part, bytes;
+  int64_t at_rows, at_start, at_token, at_row, at_part, bytes;
 };
 
 int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
@@ -245,11 +244,12 @@ EmbedPlan embed_plan(int64_t n, int64_t rows, int hidden) {
   p.range = (int)range;
   p.ranges = (int)((rows + range - 1) / range);
   int64_t seg = 8;
-  while (seg < 64 && seg * 1024 < n) seg <<= 1;
+  while (seg < LM_EMBED_MAX_SEG && seg * 1024 < n) seg <<= 1;
   p.seg = (int)seg;
   p.stretches = (n + seg - 1) / seg;
   p.at_rows = 256;
-  p.at_token = p.at_rows + round256(rows * 4);
+  p.at_start = p.at_rows + round256(rows * 4);
+  p.at_token = p.at_start + round256(rows * 4);
   p.at_row = p.at_token + round256(n * 4);
   p.at_part = p.at_row + round256(n * 4);
   p.bytes = p.at_part + p.stretches * 2 * hidden * 4;
@@ -568,31 +568,30 @@ int attnres_embedding_bwd(const void* ids, int index_dtype, int64_t num_ids, con
   P.dw = grad_weight;
   P.counts = reinterpret_cast<int32_t*>(ws);
   P.row_count = reinterpret_cast<int32_t*>(ws + plan.at_rows);
+  P.row_start = reinterpret_cast<int32_t*>(ws + plan.at_start);
   P.sorted_token = reinterpret_cast<int32_t*>(ws + plan.at_token);
   P.sorted_row = reinterpret_cast<int32_t*>(ws + plan.at_row);
   P.part = reinterpret_cast<float*>(ws + plan.at_part);
   P.range = plan.range;
   P.seg = plan.seg;
+  P.stretches = (int32_t)plan.stretches;
   rc = launch(kEmbedSort, kLmPart, "attnres_embedding_sort", (unsigned)plan.ranges, 1, 64 * LM_EMBED_WAVES, 0, P,
               stream);
   if (rc != ATTNRES_OK) return rc;
   const char* kind = embed_kind(f32, vec);
   const int idx = (f32 ? 2 : 0) + (vec ? 0 : 1);
   char name[64];
-  snprintf(name, sizeof(name), "attnres_embedding_zero_%s", kind);
-  rc = launch(kEmbedZero + idx, kLmPart, name, (unsigned)((rows + 3) / 4), 1, 256, 0, P, stream);
-  if (rc != ATTNRES_OK || num_ids == 0) return rc;
   const int chunks = vec ? hidden / v : hidden;
   const int block = chunks >= 512 ? 512 : (chunks + 63) / 64 * 64;
   const int64_t slices = (chunks + block - 1) / block;
   snprintf(name, sizeof(name), "attnres_embedding_sum_%s", kind);
-  rc = launch(kEmbedSum + idx, kLmPart, name, (unsigned)plan.stretches, (unsigned)slices, (unsigned)block, 0, P,
+  rc = launch(kEmbedSum + idx, kLmPart, name, (unsigned)(plan.stretches + (rows + LM_EMBED_ZERO - 1) / LM_EMBED_ZERO),
+              (unsigned)slices, (unsigned)block, 0, P,
               stream);
   if (rc != ATTNRES_OK || plan.stretches < 2) return rc;
   snprintf(name, sizeof(name), "attnres_embedding_join_%s", f32 ? "f32" : "bf16");
-  return launch(kEmbedJoin + (f32 ? 1 : 0), kLmPart, name,
-                (unsigned)((plan.stretches + LM_EMBED_JOIN - 1) / LM_EMBED_JOIN), (unsigned)((hidden + 63) / 64),
-                64 * LM_EMBED_WAVES, 0, P, stream);
+  return launch(kEmbedJoin + (f32 ? 1 : 0), kLmPart, name, (unsigned)((plan.stretches - 1 + LM_EMBED_JOIN - 1) / LM_EMBED_JOIN),
+                (unsigned)((hidden + 255) / 256), 64 * LM_EMBED_JOIN_WAVES, 0, P, stream);
 }
 
 }  // extern "C"

@@ -344,12 +344,13 @@ __device__ __forceinline__ void rope_dw_sum(const lm_rope_params& P, float* red)
 //   sort   one workgroup per range of table rows.  Each scans all ids (they
 //          stay in L2): its 16 waves, each a stretch of the tokens in order,
 //          count their tokens per row in LDS; a scan over rows and waves
-//          gives every (row, wave) its place, and ids below the range the
-//          range's own; a second walk places the tokens.  Rows without tokens
-//          are zeroed here.
+//          gives every (row, wave) its place, and the ids below the range the
+//          range's own; a second walk places the tokens.  A wave requests
+//          1024 ids at a time, so up to 16384 tokens are one round trip.
 //   sum    one workgroup per stretch of `seg` sorted tokens and column slice:
 //          runs of one row are added in order and written; a run that crosses
-//          the stretch's ends is left as an fp32 partial row.
+//          the stretch's ends is left as an fp32 partial row.  Further
+//          workgroups zero the rows without tokens.
 //   join   the crossing runs' partial rows are added in order.
 
 template <typename T, int V>
@@ -373,8 +374,24 @@ __device__ __forceinline__ void embedding_fwd(const lm_embed_params& P) {
   }
 }
 
+// A wave's next 64 x LM_EMBED_BATCH tokens: each lane's rows within the range, -1 elsewhere.
+__device__ __forceinline__ void load_ids(const lm_embed_params& P, int64_t tb, int64_t t1, int lane, int64_t lo,
+                                         int64_t hi, int (&rel)[LM_EMBED_BATCH], int& below) {
+  int64_t id[LM_EMBED_BATCH];
+#pragma unroll
+  for (int i = 0; i < LM_EMBED_BATCH; ++i) {
+    const int64_t t = tb + i * 64 + lane;
+    id[i] = t < t1 ? index_at(P.ids, t, P.ids64) : -1;
+  }
+#pragma unroll
+  for (int i = 0; i < LM_EMBED_BATCH; ++i) {
+    const bool ok = id[i] >= 0 && id[i] != P.padding;
+    rel[i] = ok && id[i] >= lo && id[i] < hi ? (int)(id[i] - lo) : -1;
+    below += ok && id[i] < lo ? 1 : 0;
+  }
+}
+
 // cnt: LM_EMBED_WAVES x range counters; scan: one word per wave
-template <typename T, int V>
 __device__ __forceinline__ void embedding_sort(const lm_embed_params& P, int* cnt, int* scan) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int range = P.range;
@@ -386,12 +403,12 @@ __device__ __forceinline__ void embedding_sort(const lm_embed_params& P, int* cn
   const int64_t per = ((P.n + LM_EMBED_WAVES - 1) / LM_EMBED_WAVES + 63) / 64 * 64;
   const int64_t t0 = per * wave, t1 = t0 + per < P.n ? t0 + per : P.n;
   int below = 0;
-#pragma unroll 4
-  for (int64_t t = t0 + lane; t < t1; t += 64) {
-    const int64_t id = index_at(P.ids, t, P.ids64);
-    if (id == P.padding) continue;
-    if (id >= lo && id < hi) atomicAdd(&mine[id - lo], 1);
-    else if (id >= 0 && id < lo) ++below;
+  int rel[LM_EMBED_BATCH];
+  for (int64_t tb = t0; tb < t1; tb += 64 * LM_EMBED_BATCH) {
+    load_ids(P, tb, t1, lane, lo, hi, rel, below);
+#pragma unroll
+    for (int i = 0; i < LM_EMBED_BATCH; ++i)
+      if (rel[i] >= 0) atomicAdd(&mine[rel[i]], 1);
   }
   for (int m = 1; m < 64; m <<= 1) below += __shfl_xor(below, m);
   if (lane == 0) scan[wave] = below;
@@ -414,7 +431,10 @@ __device__ __forceinline__ void embedding_sort(const lm_embed_params& P, int* cn
   int at = base + incl - total;
   for (int i = 0; i < wave; ++i) at += scan[i];
   if (r < range) {
-    if (lo + r < P.rows) P.row_count[lo + r] = total;
+    if (lo + r < P.rows) {
+      P.row_count[lo + r] = total;
+      P.row_start[lo + r] = at;
+    }
     for (int i = 0; i < LM_EMBED_WAVES; ++i) {
       const int c = cnt[i * range + r];
       cnt[i * range + r] = at;
@@ -423,55 +443,72 @@ __device__ __forceinline__ void embedding_sort(const lm_embed_params& P, int* cn
   }
   if (blockIdx.x == gridDim.x - 1 && r == range - 1) P.counts[0] = at;  // tokens in all
   __syncthreads();
-  for (int64_t tb = t0; tb < t1; tb += 64) {
-    const int64_t t = tb + lane;
-    int64_t id = -1;
-    if (t < t1) id = index_at(P.ids, t, P.ids64);
-    const bool in = id >= lo && id < hi && id != P.padding;
-    const int row = (int)(id - lo);
-    uint64_t left = __ballot(in);
-    while (left != 0) {
-      const int lead = __builtin_ctzll(left);
-      const int rr = __builtin_amdgcn_readlane(row, lead);
-      const uint64_t same = __ballot(in && row == rr);
-      const int from = *(volatile int*)&mine[rr];
-      if (in && row == rr) {
-        const int p = from + __popcll(same & (((uint64_t)1 << lane) - 1));
-        P.sorted_token[p] = (int32_t)t;
-        P.sorted_row[p] = (int32_t)id;
+  // The walk that places: equal rows of a wave's 64 tokens take the next
+  // places in the order of the lanes.
+  for (int64_t tb = t0; tb < t1; tb += 64 * LM_EMBED_BATCH) {
+    if (per > 64 * LM_EMBED_BATCH) load_ids(P, tb, t1, lane, lo, hi, rel, below);
+#pragma unroll
+    for (int i = 0; i < LM_EMBED_BATCH; ++i) {
+      const int row = rel[i];
+      uint64_t left = __ballot(row >= 0);
+      while (left != 0) {
+        const int lead = __builtin_ctzll(left);
+        const int rr = __builtin_amdgcn_readlane(row, lead);
+        const uint64_t same = __ballot(row == rr);
+        const int from = *(volatile int*)&mine[rr];
+        if (row == rr) {
+          const int p = from + __popcll(same & (((uint64_t)1 << lane) - 1));
+          P.sorted_token[p] = (int32_t)(tb + i * 64 + lane);
+          P.sorted_row[p] = (int32_t)(lo + rr);
+        }
+        if (lane == lead) *(volatile int*)&mine[rr] = from + __popcll(same);
+        left &= ~same;
       }
-      if (lane == lead) *(volatile int*)&mine[rr] = from + __popcll(same);
-      left &= ~same;
     }
   }
 }
 
-// Rows without tokens get a zero gradient: a wave per row.
+// The rows without tokens among LM_EMBED_ZERO rows from row0, this slice's columns.
 template <typename T, int V>
-__device__ __forceinline__ void embedding_zero(const lm_embed_params& P) {
+__device__ __forceinline__ void embedding_zero(const lm_embed_params& P, int64_t row0) {
   const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6);
-  if (row >= P.rows || P.row_count[row] != 0) return;
+  const int64_t row = row0 + lane;
+  const bool none = lane < LM_EMBED_ZERO && row < P.rows && P.row_count[row < P.rows ? row : 0] == 0;
+  uint64_t left = __ballot(none);
+  const int c = blockIdx.y * blockDim.x + threadIdx.x;
+  if (c * V >= P.dim) return;
   float z[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) z[j] = 0.f;
-  for (int c = lane; c * V < P.dim; c += 64) store<T, V>(P.dw, row * P.dim + c * V, z);
+  while (left != 0) {
+    const int i = __builtin_ctzll(left);
+    store<T, V>(P.dw, (row0 + i) * P.dim + c * V, z);
+    left &= left - 1;
+  }
 }
 
 template <typename T, int V>
 __device__ __forceinline__ void embedding_sum(const lm_embed_params& P) {
   const int count = P.counts[0];
+  if ((int)blockIdx.x >= P.stretches) {
+    embedding_zero<T, V>(P, (int64_t)((int)blockIdx.x - P.stretches) * LM_EMBED_ZERO);
+    return;
+  }
   const int s0 = blockIdx.x * P.seg;
   if (s0 >= count) return;
   const int s1 = s0 + P.seg < count ? s0 + P.seg : count;
-  const int c = blockIdx.y * blockDim.x + threadIdx.x;
-  if (c * V >= P.dim) return;
+  // lane i: the stretch's i-th token and row (seg is at most 64)
+  const int lane = threadIdx.x & 63;
+  const int k = s0 + lane < s1 ? s0 + lane : s1 - 1;
+  const int toks = P.sorted_token[k], rows = P.sorted_row[k];
   const int before = s0 > 0 ? P.sorted_row[s0 - 1] : -1;
   const int after = s1 < count ? P.sorted_row[s1] : -1;
+  const int c = blockIdx.y * blockDim.x + threadIdx.x;
+  if (c * V >= P.dim) return;
   float acc[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) acc[j] = 0.f;
-  int row = P.sorted_row[s0];
+  int row = __builtin_amdgcn_readlane(rows, 0);
   auto flush = [&](bool end) {
     // crossing the start: partial 0; crossing the end only: partial 1
     const bool head = row == before, tail = end && row == after;
@@ -487,22 +524,20 @@ __device__ __forceinline__ void embedding_sum(const lm_embed_params& P) {
 #pragma unroll
     for (int j = 0; j < V; ++j) acc[j] = 0.f;
   };
-  constexpr int U = 4;
-  for (int i = s0; i < s1; i += U) {
+  constexpr int U = 8;
+  const int len = s1 - s0;
+  for (int i = 0; i < len; i += U) {
     float v[U][V];
-    int rows[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)  // lanes past the stretch repeat its last token
+      load<T, V>(P.g, (int64_t)__builtin_amdgcn_readlane(toks, i + u) * P.g_ld + c * V, v[u]);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int k = i + u < s1 ? i + u : s1 - 1;
-      rows[u] = P.sorted_row[k];
-      load<T, V>(P.g, (int64_t)P.sorted_token[k] * P.g_ld + c * V, v[u]);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (i + u < s1) {
-        if (rows[u] != row) {
+      if (i + u < len) {
+        const int r = __builtin_amdgcn_readlane(rows, i + u);
+        if (r != row) {
           flush(false);
-          row = rows[u];
+          row = r;
         }
 #pragma unroll
         for (int j = 0; j < V; ++j) acc[j] += v[u][j];
@@ -512,46 +547,81 @@ __device__ __forceinline__ void embedding_sum(const lm_embed_params& P) {
   flush(true);
 }
 
-// Workgroup (16 stretches, 64 columns): for each run that starts in one of the
-// stretches and leaves it, the 16 waves add every 16th partial row and then
-// each other's sums in order.
+// The partial rows first, first + step, ... of the run of stretches s .. e, 256
+// columns d of them, added in order.  Columns past the row's end repeat its
+// last: loads without a branch stay in flight together.
+__device__ __forceinline__ void add_partials(const lm_embed_params& P, int s, int first, int e, int step,
+                                             const int (&d)[4], float (&sum)[4]) {
+  constexpr int U = 8;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) sum[j] = 0.f;
+  for (int k = first; k <= e; k += U * step) {
+    float v[U][4];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int q = k + u * step <= e ? k + u * step : k;
+      const float* p = P.part + ((int64_t)q * 2 + (q == s ? 1 : 0)) * P.dim;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[u][j] = p[d[j]];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum[j] += k + u * step <= e ? v[u][j] : 0.f;
+  }
+}
+
+// Workgroup (LM_EMBED_JOIN stretches, 256 columns), for each run that starts in
+// one of them and leaves it.  A run of few partial rows is one wave's; the
+// partial rows of a longer one are dealt out to the waves, and their sums
+// added in order.  (One stretch per workgroup spent 27 us on dispatching 16368
+// workgroups that mostly found no run, at 16384 tokens x 4096.)
 template <typename T>
 __device__ __forceinline__ void embedding_join(const lm_embed_params& P, float* red) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int count = P.counts[0];
-  const int stretches = (count + P.seg - 1) / P.seg;
-  const int d = blockIdx.y * 64 + lane;
-  for (int i = 0; i < LM_EMBED_JOIN; ++i) {
+  const int total = P.counts[0];
+  const int mine = blockIdx.x * LM_EMBED_JOIN + (lane & (LM_EMBED_JOIN - 1));  // this lane's stretch
+  int row = -1, end = 0;
+  if (lane < LM_EMBED_JOIN && mine < P.stretches - 1 && (mine + 1) * P.seg < total) {
+    row = P.sorted_row[(mine + 1) * P.seg];
+    const int start = P.row_start[row];
+    if (start >= mine * P.seg && start < (mine + 1) * P.seg) end = (start + P.row_count[row] - 1) / P.seg;
+    else row = -1;  // the run at this end starts elsewhere, or at the next stretch
+  }
+  uint64_t left = __ballot(row >= 0);
+  const uint64_t lng = __ballot(row >= 0 && end - mine >= 2 * LM_EMBED_JOIN_WAVES);
+  int d[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    d[j] = blockIdx.y * 256 + 64 * j + lane;
+    d[j] = d[j] < P.dim ? d[j] : P.dim - 1;
+  }
+  float sum[4];
+  int turn = 0;
+  while (left != 0) {
+    const int i = __builtin_ctzll(left);
+    left &= left - 1;
     const int s = blockIdx.x * LM_EMBED_JOIN + i;
-    if (s + 1 >= stretches) return;
-    const int s0 = s * P.seg, s1 = s0 + P.seg;
-    const int row = P.sorted_row[s1];
-    if (P.sorted_row[s1 - 1] != row) continue;                                             // no run crosses this end
-    if (P.sorted_row[s0] == row && s0 > 0 && P.sorted_row[s0 - 1] == row) continue;      // it started earlier
-    // stretches s+1 .. e hold the rest of the run: the first whose first row is another ends it
-    int e = s + 1;
-    {
-      int lo = s + 1, hi = stretches - 1;  // the last stretch that begins with this row
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (P.sorted_row[mid * P.seg] == row) lo = mid;
-        else hi = mid - 1;
+    const int r = __builtin_amdgcn_readlane(row, i), e = __builtin_amdgcn_readlane(end, i);
+    if (((lng >> i) & 1) == 0) {
+      if ((turn++ & (LM_EMBED_JOIN_WAVES - 1)) != wave) continue;
+      add_partials(P, s, s, e, 1, d, sum);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float v = sum[j] * P.scale;
+        if ((int)(blockIdx.y * 256) + 64 * j + lane < P.dim) store<T, 1>(P.dw, (int64_t)r * P.dim + d[j], &v);
       }
-      e = lo;
+      continue;
     }
-    float sum = 0.f;
-    if (d < P.dim) {
-#pragma unroll 4
-      for (int k = s + wave; k <= e; k += LM_EMBED_WAVES)
-        sum += P.part[((int64_t)k * 2 + (k == s ? 1 : 0)) * P.dim + d];
-    }
-    red[wave * 64 + lane] = sum;
+    add_partials(P, s, s + wave, e, LM_EMBED_JOIN_WAVES, d, sum);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) red[wave * 256 + 64 * j + lane] = sum[j];
     __syncthreads();
-    if (wave == 0 && d < P.dim) {
-      float tot = 0.f;
-      for (int w = 0; w < LM_EMBED_WAVES; ++w) tot += red[w * 64 + lane];
-      tot *= P.scale;
-      store<T, 1>(P.dw, (int64_t)row * P.dim + d, &tot);
+    if (threadIdx.x < 256 && (int)(blockIdx.y * 256 + threadIdx.x) < P.dim) {
+      float v = 0.f;
+      for (int w = 0; w < LM_EMBED_JOIN_WAVES; ++w) v += red[w * 256 + threadIdx.x];
+      v *= P.scale;
+      store<T, 1>(P.dw, (int64_t)r * P.dim + blockIdx.y * 256 + threadIdx.x, &v);
     }
     __syncthreads();
   }
@@ -588,9 +658,6 @@ LM_ROPE_SUM(f32, F32)
   extern "C" __global__ void __launch_bounds__(256) attnres_embedding_fwd_##NAME(lm_embed_params P) {     \
     embedding_fwd<T, V>(P);                                                                               \
   }                                                                                                       \
-  extern "C" __global__ void __launch_bounds__(256) attnres_embedding_zero_##NAME(lm_embed_params P) {    \
-    embedding_zero<T, V>(P);                                                                              \
-  }                                                                                                       \
   extern "C" __global__ void __launch_bounds__(512) attnres_embedding_sum_##NAME(lm_embed_params P) {     \
     embedding_sum<T, V>(P);                                                                               \
   }
@@ -602,12 +669,13 @@ LM_EMBED(f32_v1, F32, 1)
 extern "C" __global__ void __launch_bounds__(64 * LM_EMBED_WAVES) attnres_embedding_sort(lm_embed_params P) {
   __shared__ int cnt[LM_EMBED_WAVES * LM_EMBED_MAX_RANGE];
   __shared__ int scan[LM_EMBED_WAVES];
-  embedding_sort<F32, 1>(P, cnt, scan);
+  embedding_sort(P, cnt, scan);
 }
-#define LM_EMBED_JOIN_K(NAME, T)                                                                                  \
-  extern "C" __global__ void __launch_bounds__(64 * LM_EMBED_WAVES) attnres_embedding_join_##NAME(lm_embed_params P) { \
-    __shared__ float red[64 * LM_EMBED_WAVES];                                                                    \
-    embedding_join<T>(P, red);                                                                                    \
+#define LM_EMBED_JOIN_K(NAME, T)                                                                       \
+  extern "C" __global__ void __launch_bounds__(64 * LM_EMBED_JOIN_WAVES)                              \
+      attnres_embedding_join_##NAME(lm_embed_params P) {                                              \
+    __shared__ float red[256 * LM_EMBED_JOIN_WAVES];                                                  \
+    embedding_join<T>(P, red);                                                                        \
   }
 LM_EMBED_JOIN_K(bf16, Bf16)
 LM_EMBED_JOIN_K(f32, F32)

@@ -97,9 +97,13 @@ typedef struct lm_rope_params {
 } lm_rope_params;
 
 /* Embedding lookup and its gradient. */
-#define LM_EMBED_WAVES 16       /* waves of the sort's and the join's workgroups */
+#define LM_EMBED_WAVES 16       /* waves of the sort's workgroups */
+#define LM_EMBED_BATCH 16       /* ids a lane requests at once there */
 #define LM_EMBED_MAX_RANGE 768  /* table rows per workgroup of the sort: 48 KiB of counters */
-#define LM_EMBED_JOIN 16        /* stretches per workgroup of the join */
+#define LM_EMBED_MAX_SEG 64     /* sorted tokens per stretch: one per lane */
+#define LM_EMBED_ZERO 32        /* table rows per zeroing workgroup */
+#define LM_EMBED_JOIN 32        /* stretches per workgroup of the join */
+#define LM_EMBED_JOIN_WAVES 8   /* waves of the join's workgroups */
 typedef struct lm_embed_params {
   const void* ids;       /* (n,) int32 or int64 */
   const void* w;         /* (rows, dim), rows w_ld apart */
@@ -108,6 +112,7 @@ typedef struct lm_embed_params {
   void* dw;              /* (rows, dim) */
   int32_t* counts;       /* [0]: tokens that count */
   int32_t* row_count;    /* (rows,) tokens of each row */
+  int32_t* row_start;    /* (rows,) and the place of its first among the sorted */
   int32_t* sorted_token; /* (n,) tokens by row, in order */
   int32_t* sorted_row;   /* (n,) their rows */
   float* part;           /* (stretches, 2, dim) */
@@ -120,6 +125,7 @@ typedef struct lm_embed_params {
   int32_t ids64;
   int32_t range;         /* table rows per workgroup of the sort */
   int32_t seg;           /* sorted tokens per stretch */
+  int32_t stretches;
   int32_t threads_per_row;
   float scale;
 } lm_embed_params;

@@ -31,6 +31,7 @@ import torch
 from torch import Tensor
 
 from . import _capi
+from ._native import native
 from .ops import _DeviceStream, _eager_direct, _require_device, dtype_code
 
 MAX_ATTENTION_DIM = 128
@@ -222,6 +223,10 @@ def qk_norm_rope(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, cos: 
     Returns tensors of q's and k's shapes over (B, T, H, D) memory.
     Differentiable in q, k and the weights; the tables have no gradient.
     """
+    if not torch.compiler.is_compiling():
+        res = native.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps)
+        if res is not None:
+            return res
     if torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad):
         raise NotImplementedError("qk_norm_rope: cos and sin have no gradient; detach them")
     if _eager_direct(q, k, q_weight, k_weight, cos, sin, positions):
@@ -382,6 +387,10 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, causal: bool = True, scale: Op
         value = int(q_start)
         if abs(value) > 1 << 40:
             raise ValueError(f"attention: q_start {value} is out of range")
+    if not torch.compiler.is_compiling():
+        res = native.attention(q, k, v, causal, scale, kv_lens, start, value, bool(want_lse))
+        if res is not None:
+            return res
     if _eager_direct(q, k, v, kv_lens, start):
         out, lse = _attention_impl(q, k, v, causal, scale, kv_lens, start, value, want_lse)
     else:
@@ -482,6 +491,10 @@ def embedding(ids: Tensor, weight: Tensor, scale: float = 1.0, padding_idx: Opti
         if not -rows <= pad < rows:
             raise ValueError(f"embedding: padding_idx {pad} is not a row of the table")
         pad %= rows
+    if not torch.compiler.is_compiling():
+        out = native.embedding(ids, weight, scale, pad)
+        if out is not None:
+            return out
     if _eager_direct(ids, weight):
         return _embedding_impl(ids, weight, scale, pad)
     _require_device(ids, weight)
