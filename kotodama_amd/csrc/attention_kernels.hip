@@ -19,6 +19,11 @@
 // ds_read_b64_tr_b16: four rows of one column per lane), so probabilities
 // never cross lanes or go through LDS.
 //
+// The rows of a key head's query group are taken together, query by query:
+// row r is head r % group of query r / group.  Consecutive rows then end at
+// (nearly) the same key, a workgroup reads a key tile once for the whole
+// group, and few queries still fill a tile.
+//
 // Tiles go from HBM to LDS directly (global_load_lds, 16 bytes per lane), the
 // next one requested before the current one is worked on.  A tile row is held
 // as 16-byte chunks, chunk c of row r at place c ^ g(r) with
@@ -137,69 +142,116 @@ template <typename T, int DP, int R>
 struct Tile {
   static constexpr int kRowBytes = DP * T::kBytes;
   static constexpr int kChunks = kRowBytes / 16;  // per row
+  static constexpr int kRows = R;
   static constexpr int kBytes = R * kRowBytes;
-  static constexpr int kLoads = kBytes / 1024;  // wave-wide 16-byte loads
 
   static __device__ __forceinline__ int place(int row) {
     if constexpr (kChunks >= 16) return ((row << 1) & 14) | ((row >> 3) & 1);
     return ((row & 6) | ((row >> 3) & 1));  // 8 chunks: row r and r + 1 share 256 bytes
   }
 
-  // Request rows row0 .. row0+R-1 of `src` (row stride `stride` bytes, `chunks`
-  // 16-byte chunks each) into `lds`; the wave `wave` of `waves` takes its part.
-  // Rows are clamped to first .. last, chunks to those that exist.
-  static __device__ __forceinline__ void request(char* lds, const char* src, int64_t stride, int row0, int first,
-                                                 int last, int chunks, int wave, int waves, int lane) {
+  // A workgroup's load i of kRound rows each is one wave-wide load per wave.
+  static constexpr int kRound = LM_ATTN_WAVES * 64 / kChunks;
+  static constexpr int kRounds = R / kRound;
+  static_assert(kRounds * kRound == R, "whole rounds");
+
+  // This lane's row within a round, and its chunk (even rounds; in odd ones
+  // ^ 1 where a round is 8 rows) among the `chunks` there are.
+  static __device__ __forceinline__ int round_row(int wave, int lane) { return (wave * 64 + lane) / kChunks; }
+  static __device__ __forceinline__ int round_chunk(int wave, int lane, int chunks, int odd) {
+    const int c = (lane % kChunks) ^ place(round_row(wave, lane)) ^ (kRound == 8 ? odd : 0);
+    return c < chunks ? c : chunks - 1;
+  }
+
+  // Offsets within a tile of this lane's part of its first two rounds, for rows `stride` bytes apart.
+  struct Lane {
+    uint32_t even, odd;
+  };
+  static __device__ __forceinline__ Lane lane_offsets(uint32_t stride, int chunks, int wave, int lane) {
+    const uint32_t row = (uint32_t)round_row(wave, lane) * stride;
+    return Lane{row + 16 * (uint32_t)round_chunk(wave, lane, chunks, 0),
+                row + 16 * (uint32_t)round_chunk(wave, lane, chunks, 1)};
+  }
+
+  // Request rows row0 .. row0+R-1 of `src` into `lds`.  Rows past `last` repeat
+  // it.  The base is uniform and the offset 32 bits wide, so a whole tile takes
+  // no address arithmetic in the vector unit.
+  static __device__ __forceinline__ void request(char* lds, const char* src, int64_t stride, int row0, int last,
+                                                 const Lane& at, int chunks, int wave, int lane) {
+    const char* base = src + (int64_t)row0 * stride;
+    if (row0 + R - 1 <= last) {
 #pragma unroll
-    for (int i = 0; i < (kLoads + LM_ATTN_WAVES - 1) / LM_ATTN_WAVES; ++i) {
-      const int ld = i * waves + wave;
-      const int p = ld * 64 + lane;  // place in the tile, in chunks
-      const int row = p / kChunks;
-      int c = (p % kChunks) ^ place(row);
-      c = c < chunks ? c : chunks - 1;
-      int r = row0 + row;
-      r = r < last ? r : last;
-      r = r > first ? r : first;
-      const char* g = src + (int64_t)r * stride + c * 16;
-      __builtin_amdgcn_global_load_lds((const LM_GLOBAL void*)g, (LM_LDS void*)(lds + ld * 1024), 16, 0, 0);
+      for (int i = 0; i < kRounds; ++i)
+        load_lds(lds + (i * LM_ATTN_WAVES + wave) * 1024, base + (int64_t)(i * kRound) * stride,
+                 (i & 1) ? at.odd : at.even);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kRounds; ++i) {
+        int row = i * kRound + round_row(wave, lane);
+        row = row < last - row0 ? row : last - row0;
+        load_lds(lds + (i * LM_ATTN_WAVES + wave) * 1024, base,
+                 (uint32_t)row * (uint32_t)stride + 16 * (uint32_t)round_chunk(wave, lane, chunks, i & 1));
+      }
+    }
+  }
+  static __device__ __forceinline__ void load_lds(char* lds, const char* base, uint32_t off) {
+    __builtin_amdgcn_global_load_lds((const LM_GLOBAL void*)(base + off), (LM_LDS void*)lds, 16, 0, 0);
+  }
+
+  // Lane offsets of the reads below.  A step's or a column block's place in the
+  // tile differs from the first's by an exclusive or, and rows 16 further down
+  // by a constant, so one offset serves a whole tile.
+  static __device__ __forceinline__ int row_at(int lane) {
+    const int row = lane & 31, h = lane >> 5;
+    return row * kRowBytes + (((T::kBytes == 2 ? h : 2 * h) ^ place(row)) << 4);
+  }
+  static __device__ __forceinline__ int col_at(int lane) {
+    const int h = lane >> 5;
+    if constexpr (T::kBytes == 2) {
+      const int s = lane & 15;
+      const int r = 4 * h + (s >> 2);
+      const int c = 2 * ((lane >> 4) & 1) + ((s & 3) >> 1);
+      return r * kRowBytes + ((c ^ place(r)) << 4) + ((s & 1) << 3);
+    } else {
+      const int d = lane & 31;
+      return 4 * h * kRowBytes + ((d >> 2) << 4) + ((d & 3) << 2);
     }
   }
 
-  // Row `row`'s elements 16 step + 8h .. + 7 (an A operand with rows along m).
-  static __device__ __forceinline__ typename T::Frag row_frag(const char* lds, int row, int step, int h) {
+  // Row row0 + lane % 32 (row0 a multiple of 32), elements 16 step + 8h .. + 7:
+  // an A operand with rows along m.  `at`: row_at(lane).
+  static __device__ __forceinline__ typename T::Frag row_frag(const char* lds, int row0, int step, int at) {
+    const char* p = lds + row0 * kRowBytes;
     typename T::Frag f;
     if constexpr (T::kBytes == 2) {
-      f.w = *reinterpret_cast<const u32x4*>(lds + row * kRowBytes + (((2 * step + h) ^ place(row)) << 4));
+      f.w = *reinterpret_cast<const u32x4*>(p + (at ^ (step << 5)));
     } else {
-      const int c = 4 * step + 2 * h;
-      f.lo = *reinterpret_cast<const f32x4*>(lds + row * kRowBytes + ((c ^ place(row)) << 4));
-      f.hi = *reinterpret_cast<const f32x4*>(lds + row * kRowBytes + (((c + 1) ^ place(row)) << 4));
+      f.lo = *reinterpret_cast<const f32x4*>(p + (at ^ (step << 6)));
+      f.hi = *reinterpret_cast<const f32x4*>(p + (at ^ (step << 6) ^ 16));
     }
     return f;
   }
 
   // Column 32 dt + lane % 32 over the rows row0 + 8 (j / 4) + 4h + j % 4, j = 0..7 (an A
   // operand with columns along m and a step's 16 rows along k); row0 a multiple of 16.
-  static __device__ __forceinline__ typename T::Frag col_frag(const char* lds, int row0, int dt, int lane) {
+  // `at`: col_at(lane).
+  static __device__ __forceinline__ typename T::Frag col_frag(const char* lds, int row0, int dt, int at, int lane) {
+    const char* p = lds + row0 * kRowBytes;
     typename T::Frag f;
-    const int h = lane >> 5;
     if constexpr (T::kBytes == 2) {
-      const int s = lane & 15;
-      const int r = row0 + 4 * h + (s >> 2);
-      const int c = 4 * dt + 2 * ((lane >> 4) & 1) + ((s & 3) >> 1);
-      const char* a = lds + r * kRowBytes + ((c ^ place(r)) << 4) + ((s & 1) << 3);
-      const char* b = lds + (r + 8) * kRowBytes + ((c ^ place(r + 8)) << 4) + ((s & 1) << 3);
-      const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LM_LDS i16x4*)a));
-      const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LM_LDS i16x4*)b));
+      // rows 8 further down: place() differs in its lowest bit
+      const int a = at ^ (dt << 6);
+      const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LM_LDS i16x4*)(p + a)));
+      const u32x2 hi = __builtin_bit_cast(
+          u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LM_LDS i16x4*)(p + 8 * kRowBytes + (a ^ 16))));
       f.w = u32x4{lo[0], lo[1], hi[0], hi[1]};
     } else {
-      const int d = 32 * dt + (lane & 31);
+      const int h4 = (lane >> 5) << 2;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int r = row0 + 4 * h + j;
-        f.lo[j] = *reinterpret_cast<const float*>(lds + r * kRowBytes + (((d >> 2) ^ place(r)) << 4) + ((d & 3) << 2));
-        f.hi[j] = *reinterpret_cast<const float*>(lds + (r + 8) * kRowBytes + (((d >> 2) ^ place(r + 8)) << 4) +
-                                                  ((d & 3) << 2));
+        const int a = at ^ (dt << 7);
+        f.lo[j] = *reinterpret_cast<const float*>(p + j * kRowBytes + (a ^ (place(h4 + j) << 4)));
+        f.hi[j] = *reinterpret_cast<const float*>(p + (j + 8) * kRowBytes + (a ^ (place(h4 + j + 8) << 4)));
       }
     }
     return f;
@@ -243,27 +295,66 @@ __device__ __forceinline__ void store_rows(char* row, const f32x16 (&acc)[DP / 3
   }
 }
 
+// ------------------------------------------------------------- schedules --
+
+// Orders the matrix instructions of the code before it (in its basic block): `ahead` LDS
+// reads, then N times one matrix instruction and the next reads, so that a
+// product waits for reads requested several products ago.  (Left to itself the
+// compiler reads one operand, waits, and multiplies.)  VALU: other vector
+// instructions placed behind each of the first VN products.
+template <int AHEAD, int N, int READS, int VN, int VALU>
+__device__ __forceinline__ void interleave() {
+  __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    if (AHEAD + (i + 1) * READS <= N * READS) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    if (i < VN) __builtin_amdgcn_sched_group_barrier(0x002, VALU, 0);
+  }
+}
+
 // ------------------------------------------------------------ work items --
 
-// Consecutive workgroups go to the eight XCDs in turn, each with an L2 of its
-// own; item w of XCD x is x * per + w, so a head's tiles stay on one XCD and
-// its keys and values in that L2.  -1: no work.
-__device__ __forceinline__ int work_item(int n) {
-  const int per = (n + 7) >> 3;
-  const int w = (int)(blockIdx.x >> 3);
-  const int item = (int)(blockIdx.x & 7) * per + w;
-  return w < per && item < n ? item : -1;
+// Workgroup -> (tile rank, sequence and key head).  Consecutive workgroups go
+// to the eight XCDs in turn, each with an L2 of its own: where the key heads
+// divide by eight, each XCD takes an eighth of them, so that a head's keys and
+// values stay in one L2.  Ranks are in order of falling work (causal), all
+// heads' first tiles before their second.  Where all of an XCD's workgroups
+// run at once, two on a CU, the second half is in rising order: a long one and
+// a short one meet on each CU.
+struct Item {
+  int rank, head;  // rank < 0: no work
+};
+__device__ __forceinline__ Item work_item(const lm_attn_params& P) {
+  const int heads = P.batch * P.kv_heads;
+  const int x = (int)(blockIdx.x & 7);
+  const int per = (int)(gridDim.x >> 3);
+  int w = (int)(blockIdx.x >> 3);
+  if (per <= 2 * P.cus_per_xcd && w >= P.cus_per_xcd) w = per - 1 - (w - P.cus_per_xcd);
+  Item it;
+  if ((heads & 7) == 0) {
+    const int hx = heads >> 3;
+    it.rank = w / hx;
+    it.head = x * hx + (w - it.rank * hx);
+  } else {
+    const int i = w * 8 + x;
+    it.rank = i / heads;
+    it.head = i - it.rank * heads;
+  }
+  if (it.rank >= P.n_tiles) it.rank = -1;
+  return it;
+}
+
+__device__ __forceinline__ int64_t index_at(const void* p, int i, int is64) {
+  return is64 ? ((const int64_t*)p)[i] : (int64_t)((const int32_t*)p)[i];
 }
 
 struct Seq {
   int kv_len;  // keys that exist
   int start;   // position of query 0
-  int lo, hi;  // queries lo .. hi-1 see keys (causal: those at positions 0 .. kv_len-1)
+  int lo, hi;  // rows lo .. hi-1 see keys (causal: those of queries at positions 0 .. kv_len-1)
 };
-__device__ __forceinline__ int64_t index_at(const void* p, int i, int is64) {
-  return is64 ? ((const int64_t*)p)[i] : (int64_t)((const int32_t*)p)[i];
-}
-__device__ __forceinline__ Seq sequence(const lm_attn_params& P, int b) {
+__device__ __forceinline__ Seq sequence(const lm_attn_params& P, int b, int group) {
   Seq s;
   int n = P.kv_len;
   if (P.kv_lens != nullptr) {
@@ -272,8 +363,9 @@ __device__ __forceinline__ Seq sequence(const lm_attn_params& P, int b) {
   }
   int64_t st = P.q_start_const;
   if (P.q_start != nullptr) st = index_at(P.q_start, b, P.start64);
-  st = st < -((int64_t)1 << 40) ? -((int64_t)1 << 40) : st > ((int64_t)1 << 40) ? (int64_t)1 << 40 : st;
   if (P.start_from_end) st = (int64_t)n - P.q_len;
+  // a start this far out leaves no query a key, and is held where 32 bits can count from it
+  st = st < -(1 << 30) ? -(1 << 30) : st > (1 << 30) ? (1 << 30) : st;
   int64_t lo = 0, hi = P.q_len;
   if (P.causal) {
     if (-st > lo) lo = -st;
@@ -284,326 +376,451 @@ __device__ __forceinline__ Seq sequence(const lm_attn_params& P, int b) {
   if (lo > P.q_len) lo = P.q_len;
   if (hi < lo) hi = lo;
   s.kv_len = n;
-  s.lo = (int)lo;
-  s.hi = (int)hi;
-  // out of range only where no query is live
-  s.start = (int)(st < -(1 << 30) ? -(1 << 30) : st > (1 << 30) ? (1 << 30) : st);
+  s.lo = (int)lo * group;
+  s.hi = (int)hi * group;
+  s.start = (int)st;
   return s;
+}
+
+// The keys that rows r0 .. r0+n-1 see: the most any sees, and what all see.
+struct Span {
+  int most, all;
+};
+__device__ __forceinline__ Span span(const lm_attn_params& P, const Seq& S, int group, int r0, int n) {
+  const int hi = r0 + n < S.hi ? r0 + n : S.hi, lo = r0 > S.lo ? r0 : S.lo;
+  Span k;
+  k.most = hi <= lo ? 0 : P.causal ? S.start + (hi - 1) / group + 1 : S.kv_len;
+  k.all = (r0 < S.lo || r0 + n > S.hi) ? 0 : P.causal ? S.start + r0 / group + 1 : S.kv_len;
+  return k;
+}
+
+// Where row `r` of a sequence's key head lies in a (batch, heads, tokens, dim) tensor.
+__device__ __forceinline__ int64_t row_offset(const lm_strides& s, int b, int head, int64_t i) {
+  return (int64_t)b * s.b + (int64_t)head * s.h + i * s.t;
+}
+
+// What a kernel whose waves own 32 rows each starts from.  KS waves share their
+// rows and split each key tile.
+template <int KS>
+struct Rows {
+  static constexpr int kPerGroup = 32 * LM_ATTN_WAVES / KS;  // rows of a workgroup
+  static constexpr int kKeys = KS == 4 ? 128 : 64;           // keys of a tile
+  static constexpr int kBlocks = kKeys / 32 / KS;            // 32-key blocks of a wave in a tile
+  int lane, wave, h, part;  // part: which of the KS
+  int b, kvh, head;         // this lane's row's query head
+  int row, query;           // this lane's row, and its query
+  bool exists, live;        // the row is there; it sees a key
+  int lim;                  // keys it sees
+  Span mine;                // the wave's rows'
+  int tiles;                // key tiles of the workgroup
+  Seq S;
+
+  __device__ __forceinline__ bool init(const lm_attn_params& P) {
+    const Item it = work_item(P);
+    if (it.rank < 0) return false;
+    lane = threadIdx.x & 63;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    h = lane >> 5;
+    part = wave % KS;
+    kvh = it.head % P.kv_heads;
+    b = it.head / P.kv_heads;
+    const int group = P.heads / P.kv_heads;
+    const int rows = P.q_len * group;
+    const int g0 = (P.n_tiles - 1 - it.rank) * kPerGroup;
+    const int r0 = g0 + wave / KS * 32;
+    S = sequence(P, b, group);
+    row = r0 + (lane & 31);
+    query = row / group;
+    head = kvh * group + (row - query * group);
+    exists = row < rows;
+    live = row >= S.lo && row < S.hi;
+    lim = live ? (P.causal ? S.start + query + 1 : S.kv_len) : 0;
+    mine = span(P, S, group, r0, 32);
+    tiles = (span(P, S, group, g0, kPerGroup).most + kKeys - 1) / kKeys;
+    return true;
+  }
+  __device__ __forceinline__ int64_t stat(const lm_attn_params& P) const {
+    return ((int64_t)b * P.heads + head) * P.q_len + query;
+  }
+};
+
+// Runs step(t, k, v) over the key tiles in LDS: with two buffers each, tile t+1
+// is requested before t is worked on; with one, the other workgroup of the CU
+// works meanwhile.
+template <typename KT, int NBUF, typename Step>
+__device__ __forceinline__ void over_keys(const char* kp, int64_t kst, const char* vp, int64_t vst, int tiles, int last,
+                                          int chunks, int wave, int lane, char* k0, char* k1, char* v0, char* v1,
+                                          Step&& step) {
+  const typename KT::Lane ka = KT::lane_offsets((uint32_t)kst, chunks, wave, lane);
+  const typename KT::Lane va = KT::lane_offsets((uint32_t)vst, chunks, wave, lane);
+  auto request = [&](int t, char* k, char* v) {
+    KT::request(k, kp, kst, t * KT::kRows, last, ka, chunks, wave, lane);
+    KT::request(v, vp, vst, t * KT::kRows, last, va, chunks, wave, lane);
+  };
+  auto arrived = [] {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  };
+  if constexpr (NBUF == 1) {
+    for (int t = 0; t < tiles; ++t) {
+      if (t > 0) __syncthreads();
+      request(t, k0, v0);
+      arrived();
+      step(t, k0, v0);
+    }
+  } else {
+    if (tiles > 0) request(0, k0, v0);
+    for (int t = 0; t < tiles; t += 2) {
+      arrived();
+      if (t + 1 < tiles) request(t + 1, k1, v1);
+      step(t, k0, v0);
+      if (t + 1 < tiles) {
+        arrived();
+        if (t + 2 < tiles) request(t + 2, k0, v0);
+        step(t + 1, k1, v1);
+      }
+    }
+  }
+}
+
+// The waves that share rows or keys add their results: part 0 receives.  `x`
+// holds 64 lanes x DP/2 floats per pair; every wave of the workgroup calls this.
+template <int DP>
+__device__ __forceinline__ void put(float* x, const f32x16 (&acc)[DP / 32], int lane) {
+#pragma unroll
+  for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[(dt * 16 + i) * 64 + lane] = acc[dt][i];
+}
+template <int DP>
+__device__ __forceinline__ void add(const float* x, f32x16 (&acc)[DP / 32], int lane, float mine, float theirs) {
+#pragma unroll
+  for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      acc[dt][i] = __builtin_fmaf(x[(dt * 16 + i) * 64 + lane], theirs, acc[dt][i] * mine);
 }
 
 // --------------------------------------------------------------- forward --
 
-template <typename T, int DP>
-__device__ __forceinline__ void attention_fwd(const lm_attn_params& P, char* k0, char* k1, char* v0, char* v1) {
-  using KT = Tile<T, DP, LM_ATTN_KEYS>;
-  const int item = work_item(P.n_items);
-  if (item < 0) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-  const int tile = P.n_tiles - 1 - item % P.n_tiles;  // the longest rows first
-  const int head = (item / P.n_tiles) % P.heads;
-  const int b = item / (P.n_tiles * P.heads);
-  const int kvh = head / (P.heads / P.kv_heads);
-  const Seq S = sequence(P, b);
-  const int row = tile * LM_ATTN_ROWS + wave * 32 + (lane & 31);
-  const bool live = row >= S.lo && row < S.hi;
-  const int lim = live ? (P.causal ? S.start + row + 1 : S.kv_len) : 0;  // keys the row sees
-  // over the wave's rows: the most any row sees, and what every row sees; over the workgroup's: tiles to read
-  const int r0 = tile * LM_ATTN_ROWS + wave * 32;
-  const int w_hi = r0 + 32 < S.hi ? r0 + 32 : S.hi, w_lo = r0 > S.lo ? r0 : S.lo;
-  const int w_max = w_hi <= w_lo ? 0 : P.causal ? S.start + w_hi : S.kv_len;
-  const int w_min = (r0 < S.lo || r0 + 32 > S.hi) ? 0 : P.causal ? S.start + r0 + 1 : S.kv_len;
-  const int g0 = tile * LM_ATTN_ROWS;
-  const int g_hi = g0 + LM_ATTN_ROWS < S.hi ? g0 + LM_ATTN_ROWS : S.hi, g_lo = g0 > S.lo ? g0 : S.lo;
-  const int g_max = g_hi <= g_lo ? 0 : P.causal ? S.start + g_hi : S.kv_len;
-  const int tiles = (g_max + LM_ATTN_KEYS - 1) / LM_ATTN_KEYS;
-
+template <typename T, int DP, int KS, int NBUF>
+__device__ __forceinline__ void attention_fwd(const lm_attn_params& P, char* k0, char* k1, char* v0, char* v1,
+                                              float* ml) {
+  using RW = Rows<KS>;
+  using KT = Tile<T, DP, RW::kKeys>;
+  RW R;
+  if (!R.init(P)) return;
+  const int lane = R.lane, h = R.h;
   const int chunks = P.dim * T::kBytes / 16;
-  const char* kp = (const char*)P.k + ((int64_t)b * P.sk.b + (int64_t)kvh * P.sk.h) * T::kBytes;
-  const char* vp = (const char*)P.v + ((int64_t)b * P.sv.b + (int64_t)kvh * P.sv.h) * T::kBytes;
-  const int64_t kst = P.sk.t * T::kBytes, vst = P.sv.t * T::kBytes;
-  const int last = S.kv_len - 1;
+  const char* kp = (const char*)P.k + ((int64_t)R.b * P.sk.b + (int64_t)R.kvh * P.sk.h) * T::kBytes;
+  const char* vp = (const char*)P.v + ((int64_t)R.b * P.sv.b + (int64_t)R.kvh * P.sv.h) * T::kBytes;
 
   typename T::Frag qf[DP / 16];
-  load_rows<T, DP>(qf, (const char*)P.q + ((int64_t)b * P.sq.b + (int64_t)head * P.sq.h + (int64_t)row * P.sq.t) * T::kBytes,
-                   P.dim, h, live);
+  load_rows<T, DP>(qf, (const char*)P.q + row_offset(P.sq, R.b, R.head, R.query) * T::kBytes, P.dim, h, R.live);
   f32x16 acc[DP / 32];
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i) acc[i] = zero16();
-  float m = kNegInf, l = 0.f;  // running maximum (of scores times log2 e) and this lane's part of the sum
+  float m = kNegInf, l = 0.f;  // reference maximum (of scores times log2 e) and this lane's part of the sum
+  const int row_at = KT::row_at(lane), col_at = KT::col_at(lane);
 
-  if (tiles > 0) {
-    KT::request(k0, kp, kst, 0, 0, last, chunks, wave, LM_ATTN_WAVES, lane);
-    KT::request(v0, vp, vst, 0, 0, last, chunks, wave, LM_ATTN_WAVES, lane);
-  }
-  auto step = [&](int t, const char* kc, const char* vc, char* kn, char* vn) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (t + 1 < tiles) {
-      KT::request(kn, kp, kst, (t + 1) * LM_ATTN_KEYS, 0, last, chunks, wave, LM_ATTN_WAVES, lane);
-      KT::request(vn, vp, vst, (t + 1) * LM_ATTN_KEYS, 0, last, chunks, wave, LM_ATTN_WAVES, lane);
-    }
-    const int key0 = t * LM_ATTN_KEYS;
-    if (key0 >= w_max) return;
-    f32x16 s[2];
+  over_keys<KT, NBUF>(
+      kp, P.sk.t * T::kBytes, vp, P.sv.t * T::kBytes, R.tiles, R.S.kv_len - 1, chunks, R.wave, lane, k0, k1, v0, v1,
+      [&](int t, const char* kc, const char* vc) {
+        constexpr int NB = RW::kBlocks;
+        const int first = KS == 1 ? 0 : 32 * NB * R.part;  // this wave's keys of the tile
+        const int key0 = t * RW::kKeys + first;
+        if (key0 >= R.mine.most) return;
+        f32x16 s[NB];
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      s[kb] = zero16();
+        for (int kb = 0; kb < NB; ++kb) {
+          s[kb] = zero16();
 #pragma unroll
-      for (int st = 0; st < DP / 16; ++st)
-        s[kb] = T::mma(KT::row_frag(kc, 32 * kb + (lane & 31), st, h), qf[st], s[kb]);
-    }
-    if (key0 + LM_ATTN_KEYS > w_min) {
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int key = key0 + 32 * kb + 8 * (i >> 2) + 4 * h + (i & 3);
-          s[kb][i] = key < lim ? s[kb][i] : kNegInf;
+          for (int st = 0; st < DP / 16; ++st)
+            s[kb] = T::mma(KT::row_frag(kc, first + 32 * kb, st, row_at), qf[st], s[kb]);
         }
-    }
-    float top = s[0][0];
+        if constexpr (T::kBytes == 2) interleave<4, NB * DP / 16, 1, 0, 0>();
+        if (key0 + 32 * NB > R.mine.all) {
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
+          for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kb][i]);
-    top = fmaxf(top, other_half(top)) * P.scale_log2;
-    const float mn = fmaxf(m, top);
-    const float ref = mn == kNegInf ? 0.f : mn;
-    const float fade = exp2_fast(m - ref);
-    m = mn;
-    float sum = 0.f;
+            for (int i = 0; i < 16; ++i) {
+              const int key = key0 + 32 * kb + 8 * (i >> 2) + 4 * h + (i & 3);
+              s[kb][i] = key < R.lim ? s[kb][i] : kNegInf;
+            }
+        }
+        float top = s[0][0];
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
+        for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[kb][i] = exp2_fast(__builtin_fmaf(s[kb][i], P.scale_log2, -ref));
-        sum += s[kb][i];
-      }
-    l = __builtin_fmaf(l, fade, sum);
+          for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kb][i]);
+        top = fmaxf(top, other_half(top)) * P.scale_log2;
+        // The reference only has to be near the maximum: probabilities up to
+        // 2^8 are as exact.  Most tiles after the first leave it, and so the
+        // accumulators, as they are.
+        if (__any(top > m + 8.f)) {
+          const float mn = fmaxf(m, top);
+          const float fade = mn == kNegInf ? 1.f : exp2_fast(m - mn);
+          m = mn;
+          l *= fade;
 #pragma unroll
-    for (int dt = 0; dt < DP / 32; ++dt)
+          for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) acc[dt][i] *= fade;
+            for (int i = 0; i < 16; ++i) acc[dt][i] *= fade;
+        }
+        const float ref = m == kNegInf ? 0.f : m;
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
+        for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        const typename T::Frag p = T::from_acc(s[kb], st);
+          for (int i = 0; i < 16; ++i) {
+            s[kb][i] = exp2_fast(__builtin_fmaf(s[kb][i], P.scale_log2, -ref));
+            l += s[kb][i];
+          }
 #pragma unroll
-        for (int dt = 0; dt < DP / 32; ++dt)
-          acc[dt] = T::mma(KT::col_frag(vc, 32 * kb + 16 * st, dt, lane), p, acc[dt]);
-      }
-  };
-  for (int t = 0; t < tiles; t += 2) {
-    step(t, k0, v0, k1, v1);
-    if (t + 1 < tiles) step(t + 1, k1, v1, k0, v0);
-  }
+        for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+          for (int st = 0; st < 2; ++st) {
+            const typename T::Frag p = T::from_acc(s[kb], st);
+#pragma unroll
+            for (int dt = 0; dt < DP / 32; ++dt)
+              acc[dt] = T::mma(KT::col_frag(vc, first + 32 * kb + 16 * st, dt, col_at, lane), p, acc[dt]);
+          }
+        if constexpr (T::kBytes == 2) interleave<8, NB * DP / 16, 2, (NB == 2 ? DP / 16 : 0), 7>();
+      });
 
   l += other_half(l);
-  if (row < P.q_len) {
+  if constexpr (KS > 1) {
+    // one part after another to part 0, which rescales both to their common maximum
+    float* x = reinterpret_cast<float*>((R.wave / KS) == 0 ? k0 : v0);
+    float* xm = ml + (R.wave / KS) * 128;
+#pragma unroll
+    for (int o = 1; o < KS; ++o) {
+      __syncthreads();
+      if (R.part == o) {
+        put<DP>(x, acc, lane);
+        xm[lane] = m;
+        xm[64 + lane] = l;
+      }
+      __syncthreads();
+      if (R.part == 0) {
+        const float om = xm[lane], ol = xm[64 + lane];
+        const float mn = fmaxf(m, om);
+        const float a = m == kNegInf ? 0.f : exp2_fast(m - mn), c = om == kNegInf ? 0.f : exp2_fast(om - mn);
+        add<DP>(x, acc, lane, a, c);
+        l = l * a + ol * c;
+        m = mn;
+      }
+    }
+    if (R.part != 0) return;
+  }
+  if (R.exists) {
     const float inv = l > 0.f ? 1.f / l : 0.f;
-    char* op = (char*)P.o + ((int64_t)b * P.so.b + (int64_t)head * P.so.h + (int64_t)row * P.so.t) * T::kBytes;
-    store_rows<T, DP>(op, acc, inv, P.dim, h);
-    if (P.lse != nullptr && h == 0)
-      P.lse[((int64_t)b * P.heads + head) * P.q_len + row] = l > 0.f ? (m + __builtin_amdgcn_logf(l)) * kLn2 : kNegInf;
+    store_rows<T, DP>((char*)P.o + row_offset(P.so, R.b, R.head, R.query) * T::kBytes, acc, inv, P.dim, h);
+    if (P.lse != nullptr && h == 0) P.lse[R.stat(P)] = l > 0.f ? (m + __builtin_amdgcn_logf(l)) * kLn2 : kNegInf;
   }
 }
 
 // -------------------------------------------------------- query gradients --
 
-template <typename T, int DP>
+template <typename T, int DP, int KS, int NBUF>
 __device__ __forceinline__ void attention_bwd_dq(const lm_attn_params& P, char* k0, char* k1, char* v0, char* v1) {
-  using KT = Tile<T, DP, LM_ATTN_KEYS>;
-  const int item = work_item(P.n_items);
-  if (item < 0) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-  const int tile = P.n_tiles - 1 - item % P.n_tiles;
-  const int head = (item / P.n_tiles) % P.heads;
-  const int b = item / (P.n_tiles * P.heads);
-  const int kvh = head / (P.heads / P.kv_heads);
-  const Seq S = sequence(P, b);
-  const int r0 = tile * LM_ATTN_ROWS + wave * 32;
-  const int row = r0 + (lane & 31);
-  const bool live = row >= S.lo && row < S.hi;
-  const int lim = live ? (P.causal ? S.start + row + 1 : S.kv_len) : 0;
-  const int w_hi = r0 + 32 < S.hi ? r0 + 32 : S.hi, w_lo = r0 > S.lo ? r0 : S.lo;
-  const int w_max = w_hi <= w_lo ? 0 : P.causal ? S.start + w_hi : S.kv_len;
-  const int w_min = (r0 < S.lo || r0 + 32 > S.hi) ? 0 : P.causal ? S.start + r0 + 1 : S.kv_len;
-  const int g0 = tile * LM_ATTN_ROWS;
-  const int g_hi = g0 + LM_ATTN_ROWS < S.hi ? g0 + LM_ATTN_ROWS : S.hi, g_lo = g0 > S.lo ? g0 : S.lo;
-  const int g_max = g_hi <= g_lo ? 0 : P.causal ? S.start + g_hi : S.kv_len;
-  const int tiles = (g_max + LM_ATTN_KEYS - 1) / LM_ATTN_KEYS;
-
+  using RW = Rows<KS>;
+  using KT = Tile<T, DP, RW::kKeys>;
+  RW R;
+  if (!R.init(P)) return;
+  const int lane = R.lane, h = R.h;
   const int chunks = P.dim * T::kBytes / 16;
-  const char* kp = (const char*)P.k + ((int64_t)b * P.sk.b + (int64_t)kvh * P.sk.h) * T::kBytes;
-  const char* vp = (const char*)P.v + ((int64_t)b * P.sv.b + (int64_t)kvh * P.sv.h) * T::kBytes;
-  const int64_t kst = P.sk.t * T::kBytes, vst = P.sv.t * T::kBytes;
-  const int last = S.kv_len - 1;
-  if (tiles > 0) {
-    KT::request(k0, kp, kst, 0, 0, last, chunks, wave, LM_ATTN_WAVES, lane);
-    KT::request(v0, vp, vst, 0, 0, last, chunks, wave, LM_ATTN_WAVES, lane);
-  }
+  const char* kp = (const char*)P.k + ((int64_t)R.b * P.sk.b + (int64_t)R.kvh * P.sk.h) * T::kBytes;
+  const char* vp = (const char*)P.v + ((int64_t)R.b * P.sv.b + (int64_t)R.kvh * P.sv.h) * T::kBytes;
 
   typename T::Frag qf[DP / 16], gf[DP / 16];
-  load_rows<T, DP>(qf, (const char*)P.q + ((int64_t)b * P.sq.b + (int64_t)head * P.sq.h + (int64_t)row * P.sq.t) * T::kBytes,
-                   P.dim, h, live);
-  load_rows<T, DP>(gf, (const char*)P.grad_out +
-                           ((int64_t)b * P.sdo.b + (int64_t)head * P.sdo.h + (int64_t)row * P.sdo.t) * T::kBytes,
-                   P.dim, h, live);
-  const int64_t stat = ((int64_t)b * P.heads + head) * P.q_len + row;
+  load_rows<T, DP>(qf, (const char*)P.q + row_offset(P.sq, R.b, R.head, R.query) * T::kBytes, P.dim, h, R.live);
+  load_rows<T, DP>(gf, (const char*)P.grad_out + row_offset(P.sdo, R.b, R.head, R.query) * T::kBytes, P.dim, h, R.live);
   float delta = 0.f, lse2 = 0.f;
   {
     typename T::Frag of[DP / 16];
-    load_rows<T, DP>(of, (const char*)P.out +
-                             ((int64_t)b * P.sout.b + (int64_t)head * P.sout.h + (int64_t)row * P.sout.t) * T::kBytes,
-                     P.dim, h, live);
+    load_rows<T, DP>(of, (const char*)P.out + row_offset(P.sout, R.b, R.head, R.query) * T::kBytes, P.dim, h, R.live);
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s)
 #pragma unroll
       for (int j = 0; j < 8; ++j) delta = __builtin_fmaf(T::get(gf[s], j), T::get(of[s], j), delta);
     delta += other_half(delta);
-    if (live) {
-      lse2 = P.lse[stat] * kLog2e;
-      if (P.grad_lse != nullptr) delta -= P.grad_lse[stat];
+    if (R.live) {
+      lse2 = P.lse[R.stat(P)] * kLog2e;
+      if (P.grad_lse != nullptr) delta -= P.grad_lse[R.stat(P)];
     }
-    if (row < P.q_len && h == 0) P.delta[stat] = delta;
+    if (R.exists && h == 0 && R.part == 0) P.delta[R.stat(P)] = delta;
   }
-
   f32x16 acc[DP / 32];
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i) acc[i] = zero16();
-  auto step = [&](int t, const char* kc, const char* vc, char* kn, char* vn) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (t + 1 < tiles) {
-      KT::request(kn, kp, kst, (t + 1) * LM_ATTN_KEYS, 0, last, chunks, wave, LM_ATTN_WAVES, lane);
-      KT::request(vn, vp, vst, (t + 1) * LM_ATTN_KEYS, 0, last, chunks, wave, LM_ATTN_WAVES, lane);
-    }
-    const int key0 = t * LM_ATTN_KEYS;
-    if (key0 >= w_max) return;
+  const int row_at = KT::row_at(lane), col_at = KT::col_at(lane);
+
+  over_keys<KT, NBUF>(
+      kp, P.sk.t * T::kBytes, vp, P.sv.t * T::kBytes, R.tiles, R.S.kv_len - 1, chunks, R.wave, lane, k0, k1, v0, v1,
+      [&](int t, const char* kc, const char* vc) {
+        constexpr int NB = RW::kBlocks;
+        const int first = KS == 1 ? 0 : 32 * NB * R.part;
+        const int key0 = t * RW::kKeys + first;
+        if (key0 >= R.mine.most) return;
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      f32x16 s = zero16(), dp = zero16();
+        for (int kb = 0; kb < NB; ++kb) {
+          f32x16 s = zero16(), dp = zero16();
 #pragma unroll
-      for (int st = 0; st < DP / 16; ++st) {
-        s = T::mma(KT::row_frag(kc, 32 * kb + (lane & 31), st, h), qf[st], s);
-        dp = T::mma(KT::row_frag(vc, 32 * kb + (lane & 31), st, h), gf[st], dp);
-      }
+          for (int st = 0; st < DP / 16; ++st) {
+            s = T::mma(KT::row_frag(kc, first + 32 * kb, st, row_at), qf[st], s);
+            dp = T::mma(KT::row_frag(vc, first + 32 * kb, st, row_at), gf[st], dp);
+          }
+          if constexpr (T::kBytes == 2) interleave<4, DP / 8, 1, 0, 0>();
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        s[i] = exp2_fast(__builtin_fmaf(s[i], P.scale_log2, -lse2)) * (dp[i] - delta);
-      if (key0 + LM_ATTN_KEYS > w_min) {
+          for (int i = 0; i < 16; ++i)
+            s[i] = exp2_fast(__builtin_fmaf(s[i], P.scale_log2, -lse2)) * (dp[i] - delta);
+          if (key0 + 32 * NB > R.mine.all) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int key = key0 + 32 * kb + 8 * (i >> 2) + 4 * h + (i & 3);
-          s[i] = key < lim ? s[i] : 0.f;
+            for (int i = 0; i < 16; ++i) {
+              const int key = key0 + 32 * kb + 8 * (i >> 2) + 4 * h + (i & 3);
+              s[i] = key < R.lim ? s[i] : 0.f;
+            }
+          }
+#pragma unroll
+          for (int st = 0; st < 2; ++st) {
+            const typename T::Frag ds = T::from_acc(s, st);
+#pragma unroll
+            for (int dt = 0; dt < DP / 32; ++dt)
+              acc[dt] = T::mma(KT::col_frag(kc, first + 32 * kb + 16 * st, dt, col_at, lane), ds, acc[dt]);
+          }
+          if constexpr (T::kBytes == 2) interleave<8, DP / 16, 2, 0, 0>();
         }
-      }
+      });
+
+  if constexpr (KS > 1) {
+    float* x = reinterpret_cast<float*>((R.wave / KS) == 0 ? k0 : v0);
 #pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        const typename T::Frag ds = T::from_acc(s, st);
-#pragma unroll
-        for (int dt = 0; dt < DP / 32; ++dt)
-          acc[dt] = T::mma(KT::col_frag(kc, 32 * kb + 16 * st, dt, lane), ds, acc[dt]);
-      }
+    for (int o = 1; o < KS; ++o) {
+      __syncthreads();
+      if (R.part == o) put<DP>(x, acc, lane);
+      __syncthreads();
+      if (R.part == 0) add<DP>(x, acc, lane, 1.f, 1.f);
     }
-  };
-  for (int t = 0; t < tiles; t += 2) {
-    step(t, k0, v0, k1, v1);
-    if (t + 1 < tiles) step(t + 1, k1, v1, k0, v0);
+    if (R.part != 0) return;
   }
-  if (row < P.q_len) {
-    char* op = (char*)P.dq + ((int64_t)b * P.sdq.b + (int64_t)head * P.sdq.h + (int64_t)row * P.sdq.t) * T::kBytes;
-    store_rows<T, DP>(op, acc, P.scale, P.dim, h);
-  }
+  if (R.exists)
+    store_rows<T, DP>((char*)P.dq + row_offset(P.sdq, R.b, R.head, R.query) * T::kBytes, acc, P.scale, P.dim, h);
 }
 
 // ------------------------------------------------ key and value gradients --
 
-template <typename T, int DP>
+// A wave owns 32 keys; KS waves share them and split each tile of 32 KS rows.
+template <typename T, int DP, int KS, int NBUF>
 __device__ __forceinline__ void attention_bwd_dkv(const lm_attn_params& P, char* q0, char* q1, char* g0, char* g1,
                                                   float* st0, float* st1) {
-  using QT = Tile<T, DP, LM_ATTN_BWD_ROWS>;
-  constexpr int R = LM_ATTN_BWD_ROWS;
-  const int item = work_item(P.n_items);
-  if (item < 0) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-  const int tile = item % P.n_tiles;  // causal: the first keys are seen by the most queries
-  const int kvh = (item / P.n_tiles) % P.kv_heads;
-  const int b = item / (P.n_tiles * P.kv_heads);
+  constexpr int R = 32 * KS;
+  using QT = Tile<T, DP, R>;
+  const Item it = work_item(P);
+  if (it.rank < 0) return;
+  const int lane = threadIdx.x & 63, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int part = wave % KS;
+  const int kvh = it.head % P.kv_heads, b = it.head / P.kv_heads;
   const int group = P.heads / P.kv_heads;
-  const Seq S = sequence(P, b);
-  const int w0 = tile * LM_ATTN_BWD_KEYS + wave * 32;
+  const Seq S = sequence(P, b, group);
+  const int wg0 = it.rank * (32 * LM_ATTN_WAVES / KS);  // causal: the first keys are seen by the most queries
+  const int w0 = wg0 + wave / KS * 32;
   const int key = w0 + (lane & 31);
   const bool live = key < S.kv_len;
 
   typename T::Frag kf[DP / 16], vf[DP / 16];
-  load_rows<T, DP>(kf, (const char*)P.k + ((int64_t)b * P.sk.b + (int64_t)kvh * P.sk.h + (int64_t)key * P.sk.t) * T::kBytes,
-                   P.dim, h, live);
-  load_rows<T, DP>(vf, (const char*)P.v + ((int64_t)b * P.sv.b + (int64_t)kvh * P.sv.h + (int64_t)key * P.sv.t) * T::kBytes,
-                   P.dim, h, live);
+  load_rows<T, DP>(kf, (const char*)P.k + row_offset(P.sk, b, kvh, key) * T::kBytes, P.dim, h, live);
+  load_rows<T, DP>(vf, (const char*)P.v + row_offset(P.sv, b, kvh, key) * T::kBytes, P.dim, h, live);
   f32x16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i) {
     dk[i] = zero16();
     dv[i] = zero16();
   }
-  // the first query that sees the workgroup's (the wave's) first key, rounded down to a tile; queries of a head
-  const int key_wg = tile * LM_ATTN_BWD_KEYS;
-  int first = S.lo, w_first = S.lo, w_full = S.lo;  // from w_full on a query sees all of the wave's keys
-  if (P.causal) {
-    if (key_wg - S.start > first) first = key_wg - S.start;
-    if (w0 - S.start > w_first) w_first = w0 - S.start;
-    if (w0 + 31 - S.start > w_full) w_full = w0 + 31 - S.start;
-  }
-  if (w0 + 32 > S.kv_len) w_full = S.hi;  // not every key exists
-  const int k_first = live ? (P.causal && key - S.start > S.lo ? key - S.start : S.lo) : S.hi;
+  // the first row that sees a key, of the workgroup's keys (rounded down to a
+  // tile), the wave's, and this lane's; from w_full on rows see all the wave's
+  auto first_row = [&](int k) {
+    const int64_t r = P.causal && k > S.start ? (int64_t)(k - S.start) * group : 0;
+    return (int)(r < S.lo ? S.lo : r > S.hi ? S.hi : r);
+  };
+  const int first = first_row(wg0);
   const int base = first / R * R;
-  const int per = key_wg < S.kv_len && first < S.hi ? (S.hi - base + R - 1) / R : 0;  // tiles of a head
-  const int tiles = per * group;
+  const int w_first = first_row(w0);
+  const int w_full = w0 + 32 > S.kv_len ? S.hi : first_row(w0 + 31);
+  const int k_first = live ? first_row(key) : S.hi;
+  const int tiles = wg0 < S.kv_len && first < S.hi ? (S.hi - base + R - 1) / R : 0;
 
   const int chunks = P.dim * T::kBytes / 16;
-  const int64_t qst = P.sq.t * T::kBytes, gst = P.sdo.t * T::kBytes;
+  const uint32_t qst = (uint32_t)(P.sq.t * T::kBytes), qsh = (uint32_t)(P.sq.h * T::kBytes);
+  const uint32_t gst = (uint32_t)(P.sdo.t * T::kBytes), gsh = (uint32_t)(P.sdo.h * T::kBytes);
+  const char* qp = (const char*)P.q + row_offset(P.sq, b, kvh * group, 0) * T::kBytes;
+  const char* gp = (const char*)P.grad_out + row_offset(P.sdo, b, kvh * group, 0) * T::kBytes;
+  const int64_t stat0 = ((int64_t)b * P.heads + kvh * group) * P.q_len;
   const int last = S.hi - 1;
-  auto request = [&](int t, char* qn, char* gn, float* sn) {
-    const int head = kvh * group + t / per;
-    const int row0 = base + (t % per) * R;
-    const char* qp = (const char*)P.q + ((int64_t)b * P.sq.b + (int64_t)head * P.sq.h) * T::kBytes;
-    const char* gp = (const char*)P.grad_out + ((int64_t)b * P.sdo.b + (int64_t)head * P.sdo.h) * T::kBytes;
-    QT::request(qn, qp, qst, row0, S.lo, last, chunks, wave, LM_ATTN_WAVES, lane);
-    QT::request(gn, gp, gst, row0, S.lo, last, chunks, wave, LM_ATTN_WAVES, lane);
-    if (wave == 0) {  // the rows' lse (lanes 0 .. 31) and delta
-      int r = row0 + (lane & (R - 1));
-      r = r < last ? r : last;
-      r = r > S.lo ? r : S.lo;
-      const float* src = (h ? P.delta : P.lse) + ((int64_t)b * P.heads + head) * P.q_len + r;
-      __builtin_amdgcn_global_load_lds((const LM_GLOBAL void*)src, (LM_LDS void*)sn, 4, 0, 0);
-    }
+  // tile t starts at row base + t R: query i0, head j0 of the group
+  int i0 = base / group, j0 = base - i0 * group, next = 0;
+  // row i0 * group + j0 + r as (query, head) after i0
+  auto split = [&](int r, int& i, int& j) {
+    const uint32_t n = (uint32_t)(j0 + r);
+    i = group == 1 ? (int)n : (int)__umulhi(n, P.group_magic);  // n / group: n is under group + 256
+    j = (int)n - i * group;
   };
-  if (tiles > 0) request(0, q0, g0, st0);
-  auto step = [&](int t, const char* qc, const char* gc, const float* sc, char* qn, char* gn, float* sn) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (t + 1 < tiles) request(t + 1, qn, gn, sn);
-    const int row0 = base + (t % per) * R;
-    if (row0 + R <= w_first || w0 >= S.kv_len) return;
+  auto request = [&](char* qn, char* gn, float* sn) {  // tile `next`
+    const int row0 = base + next * R;
+    const char* qb = qp + (int64_t)i0 * P.sq.t * T::kBytes;
+    const char* gb = gp + (int64_t)i0 * P.sdo.t * T::kBytes;
+    const int lo = S.lo - row0, hi = last - row0;  // rows that see keys, from the tile's first
+#pragma unroll
+    for (int n = 0; n < QT::kRounds; ++n) {
+      int r = n * QT::kRound + QT::round_row(wave, lane), i, j;
+      r = r < hi ? r : hi;
+      r = r > lo ? r : lo;
+      split(r, i, j);
+      const uint32_t c = 16 * (uint32_t)QT::round_chunk(wave, lane, chunks, n & 1);
+      QT::load_lds(qn + (n * LM_ATTN_WAVES + wave) * 1024, qb, (uint32_t)i * qst + (uint32_t)j * qsh + c);
+      QT::load_lds(gn + (n * LM_ATTN_WAVES + wave) * 1024, gb, (uint32_t)i * gst + (uint32_t)j * gsh + c);
+    }
+    if (wave < KS) {  // the rows' lse (lanes 0 .. 31) and delta, 32 rows a wave
+      int r = wave * 32 + (lane & 31), i, j;
+      r = r < hi ? r : hi;
+      r = r > lo ? r : lo;
+      split(r, i, j);
+      const float* src = (h ? P.delta : P.lse) + stat0 + (int64_t)j * P.q_len + (i0 + i);
+      __builtin_amdgcn_global_load_lds((const LM_GLOBAL void*)src, (LM_LDS void*)(sn + wave * 64), 4, 0, 0);
+    }
+    ++next;
+    int i, j;
+    split(R, i, j);
+    i0 += i;
+    j0 = j;
+  };
+  int row_at = QT::row_at(lane), col_at = QT::col_at(lane);
+  auto step = [&](int t, const char* qc, const char* gc, const float* sc) {
+    const int mine = KS == 1 ? 0 : 32 * part;  // this wave's rows of the tile
+    const int row0 = base + t * R + mine;
+    if (row0 + 32 <= w_first || row0 >= S.hi || w0 >= S.kv_len) return;
+    // opaque here, so that the offsets made from these are formed anew (one
+    // instruction each) instead of held in registers
+    asm volatile("" : "+v"(row_at), "+v"(col_at));
     f32x16 s = zero16(), dp = zero16();
 #pragma unroll
     for (int st = 0; st < DP / 16; ++st) {
-      s = T::mma(QT::row_frag(qc, lane & 31, st, h), kf[st], s);
-      dp = T::mma(QT::row_frag(gc, lane & 31, st, h), vf[st], dp);
+      s = T::mma(QT::row_frag(qc, mine, st, row_at), kf[st], s);
+      dp = T::mma(QT::row_frag(gc, mine, st, row_at), vf[st], dp);
     }
+    if constexpr (T::kBytes == 2) interleave<4, DP / 8, 1, 0, 0>();
+    const float* stats = sc + (KS == 1 ? 0 : 64 * part);
 #pragma unroll
     for (int a = 0; a < 4; ++a) {
-      const f32x4 lse = *reinterpret_cast<const f32x4*>(sc + 8 * a + 4 * h);
-      const f32x4 dl = *reinterpret_cast<const f32x4*>(sc + 32 + 8 * a + 4 * h);
+      const f32x4 lse = *reinterpret_cast<const f32x4*>(stats + 8 * a + 4 * h);
+      const f32x4 dl = *reinterpret_cast<const f32x4*>(stats + 32 + 8 * a + 4 * h);
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         s[4 * a + c] = exp2_fast(__builtin_fmaf(s[4 * a + c], P.scale_log2, -lse[c] * kLog2e));
         dp[4 * a + c] -= dl[c];
       }
     }
-    if (row0 < w_full || row0 + R > S.hi) {
+    if (row0 < w_full || row0 + 32 > S.hi) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int r = row0 + 8 * (i >> 2) + 4 * h + (i & 3);
@@ -619,68 +836,109 @@ __device__ __forceinline__ void attention_bwd_dkv(const lm_attn_params& P, char*
       const typename T::Frag p = T::from_acc(s, st), ds = T::from_acc(dp, st);
 #pragma unroll
       for (int dt = 0; dt < DP / 32; ++dt) {
-        dv[dt] = T::mma(QT::col_frag(gc, 16 * st, dt, lane), p, dv[dt]);
-        dk[dt] = T::mma(QT::col_frag(qc, 16 * st, dt, lane), ds, dk[dt]);
+        dv[dt] = T::mma(QT::col_frag(gc, mine + 16 * st, dt, col_at, lane), p, dv[dt]);
+        dk[dt] = T::mma(QT::col_frag(qc, mine + 16 * st, dt, col_at, lane), ds, dk[dt]);
       }
     }
+    if constexpr (T::kBytes == 2) interleave<4, DP / 8, 2, 0, 0>();
   };
-  for (int t = 0; t < tiles; t += 2) {
-    step(t, q0, g0, st0, q1, g1, st1);
-    if (t + 1 < tiles) step(t + 1, q1, g1, st1, q0, g0, st0);
+  auto arrived = [] {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  };
+  if constexpr (NBUF == 1) {
+    for (int t = 0; t < tiles; ++t) {
+      if (t > 0) __syncthreads();
+      request(q0, g0, st0);
+      arrived();
+      step(t, q0, g0, st0);
+    }
+  } else {
+    if (tiles > 0) request(q0, g0, st0);
+    for (int t = 0; t < tiles; t += 2) {
+      arrived();
+      if (t + 1 < tiles) request(q1, g1, st1);
+      step(t, q0, g0, st0);
+      if (t + 1 < tiles) {
+        arrived();
+        if (t + 2 < tiles) request(q0, g0, st0);
+        step(t + 1, q1, g1, st1);
+      }
+    }
+  }
+  if constexpr (KS > 1) {
+    float* xk = reinterpret_cast<float*>((wave / KS) == 0 ? q0 : q1);
+    float* xv = reinterpret_cast<float*>((wave / KS) == 0 ? g0 : g1);
+#pragma unroll
+    for (int o = 1; o < KS; ++o) {
+      __syncthreads();
+      if (part == o) {
+        put<DP>(xk, dk, lane);
+        put<DP>(xv, dv, lane);
+      }
+      __syncthreads();
+      if (part == 0) {
+        add<DP>(xk, dk, lane, 1.f, 1.f);
+        add<DP>(xv, dv, lane, 1.f, 1.f);
+      }
+    }
+    if (part != 0) return;
   }
   if (key < P.kv_len) {
-    char* kp = (char*)P.dk + ((int64_t)b * P.sdk.b + (int64_t)kvh * P.sdk.h + (int64_t)key * P.sdk.t) * T::kBytes;
-    char* vp = (char*)P.dv + ((int64_t)b * P.sdv.b + (int64_t)kvh * P.sdv.h + (int64_t)key * P.sdv.t) * T::kBytes;
-    store_rows<T, DP>(kp, dk, P.scale, P.dim, h);
-    store_rows<T, DP>(vp, dv, 1.f, P.dim, h);
+    store_rows<T, DP>((char*)P.dk + row_offset(P.sdk, b, kvh, key) * T::kBytes, dk, P.scale, P.dim, h);
+    store_rows<T, DP>((char*)P.dv + row_offset(P.sdv, b, kvh, key) * T::kBytes, dv, 1.f, P.dim, h);
   }
 }
 
 }  // namespace
 
-#define LM_ATTN_FWD(NAME, T, DP, WPE)                                                                   \
+// KS: waves that share rows (or keys); NBUF: LDS buffers of a tile; WPE: waves
+// per SIMD the registers are held to.
+#define LM_ATTN_KERNEL(KIND, NAME, WPE) \
   extern "C" __global__ void __launch_bounds__(64 * LM_ATTN_WAVES) __attribute__((amdgpu_waves_per_eu(WPE))) \
-      attnres_attention_fwd_##NAME(lm_attn_params P) {                                                  \
-    __shared__ __align__(16) char k0[Tile<T, DP, LM_ATTN_KEYS>::kBytes];                                \
-    __shared__ __align__(16) char k1[Tile<T, DP, LM_ATTN_KEYS>::kBytes];                                \
-    __shared__ __align__(16) char v0[Tile<T, DP, LM_ATTN_KEYS>::kBytes];                                \
-    __shared__ __align__(16) char v1[Tile<T, DP, LM_ATTN_KEYS>::kBytes];                                \
-    attention_fwd<T, DP>(P, k0, k1, v0, v1);                                                            \
-  }
-#define LM_ATTN_DQ(NAME, T, DP, WPE)                                                                    \
-  extern "C" __global__ void __launch_bounds__(64 * LM_ATTN_WAVES) __attribute__((amdgpu_waves_per_eu(WPE))) \
-      attnres_attention_dq_##NAME(lm_attn_params P) {                                                   \
-    __shared__ __align__(16) char k0[Tile<T, DP, LM_ATTN_KEYS>::kBytes];                                \
-    __shared__ __align__(16) char k1[Tile<T, DP, LM_ATTN_KEYS>::kBytes];                                \
-    __shared__ __align__(16) char v0[Tile<T, DP, LM_ATTN_KEYS>::kBytes];                                \
-    __shared__ __align__(16) char v1[Tile<T, DP, LM_ATTN_KEYS>::kBytes];                                \
-    attention_bwd_dq<T, DP>(P, k0, k1, v0, v1);                                                         \
-  }
-#define LM_ATTN_DKV(NAME, T, DP, WPE)                                                                   \
-  extern "C" __global__ void __launch_bounds__(64 * LM_ATTN_WAVES) __attribute__((amdgpu_waves_per_eu(WPE))) \
-      attnres_attention_dkv_##NAME(lm_attn_params P) {                                                  \
-    __shared__ __align__(16) char q0[Tile<T, DP, LM_ATTN_BWD_ROWS>::kBytes];                            \
-    __shared__ __align__(16) char q1[Tile<T, DP, LM_ATTN_BWD_ROWS>::kBytes];                            \
-    __shared__ __align__(16) char g0[Tile<T, DP, LM_ATTN_BWD_ROWS>::kBytes];                            \
-    __shared__ __align__(16) char g1[Tile<T, DP, LM_ATTN_BWD_ROWS>::kBytes];                            \
-    __shared__ __align__(16) float st0[64];                                                             \
-    __shared__ __align__(16) float st1[64];                                                             \
-    attention_bwd_dkv<T, DP>(P, q0, q1, g0, g1, st0, st1);                                              \
+      attnres_attention_##KIND##_##NAME(lm_attn_params P)
+#define LM_ATTN(NAME, T, DP, KS, NBUF, FWD_WPE, DQ_WPE, DKV_WPE)                                     \
+  LM_ATTN_KERNEL(fwd, NAME, FWD_WPE) {                                                               \
+    constexpr int kTile = Tile<T, DP, Rows<KS>::kKeys>::kBytes;                                      \
+    __shared__ __align__(16) char k0[kTile];                                                         \
+    __shared__ __align__(16) char v0[kTile];                                                         \
+    __shared__ __align__(16) char k1[NBUF == 2 ? kTile : 16];                                        \
+    __shared__ __align__(16) char v1[NBUF == 2 ? kTile : 16];                                        \
+    __shared__ float ml[KS > 1 ? LM_ATTN_WAVES / KS * 128 : 1];                                      \
+    attention_fwd<T, DP, KS, NBUF>(P, k0, k1, v0, v1, ml);                                           \
+  }                                                                                                  \
+  LM_ATTN_KERNEL(dq, NAME, DQ_WPE) {                                                                 \
+    constexpr int kTile = Tile<T, DP, Rows<KS>::kKeys>::kBytes;                                      \
+    __shared__ __align__(16) char k0[kTile];                                                         \
+    __shared__ __align__(16) char v0[kTile];                                                         \
+    __shared__ __align__(16) char k1[NBUF == 2 ? kTile : 16];                                        \
+    __shared__ __align__(16) char v1[NBUF == 2 ? kTile : 16];                                        \
+    attention_bwd_dq<T, DP, KS, NBUF>(P, k0, k1, v0, v1);                                            \
+  }                                                                                                  \
+  LM_ATTN_KERNEL(dkv, NAME, DKV_WPE) {                                                               \
+    constexpr int kTile = Tile<T, DP, 32 * KS>::kBytes;                                              \
+    __shared__ __align__(16) char q0[kTile];                                                         \
+    __shared__ __align__(16) char g0[kTile];                                                         \
+    __shared__ __align__(16) char q1[NBUF == 2 ? kTile : 16];                                        \
+    __shared__ __align__(16) char g1[NBUF == 2 ? kTile : 16];                                        \
+    __shared__ __align__(16) float st0[64 * KS];                                                     \
+    __shared__ __align__(16) float st1[NBUF == 2 ? 64 * KS : 4];                                     \
+    attention_bwd_dkv<T, DP, KS, NBUF>(P, q0, q1, g0, g1, st0, st1);                                 \
   }
 
 #if LM_PART == 13
-LM_ATTN_FWD(bf16_d64, Bf16, 64, 2)
-LM_ATTN_FWD(bf16_d128, Bf16, 128, 2)
-LM_ATTN_DQ(bf16_d64, Bf16, 64, 2)
-LM_ATTN_DQ(bf16_d128, Bf16, 128, 2)
-LM_ATTN_DKV(bf16_d64, Bf16, 64, 2)
-LM_ATTN_DKV(bf16_d128, Bf16, 128, 1)
+LM_ATTN(bf16_d64_s1, Bf16, 64, 1, 2, 2, 2, 2)
+LM_ATTN(bf16_d64_s2, Bf16, 64, 2, 2, 2, 2, 2)
+LM_ATTN(bf16_d64_s4, Bf16, 64, 4, 1, 2, 2, 2)
+LM_ATTN(bf16_d128_s1, Bf16, 128, 1, 2, 2, 2, 2)
+LM_ATTN(bf16_d128_s2, Bf16, 128, 2, 2, 2, 2, 2)
+LM_ATTN(bf16_d128_s4, Bf16, 128, 4, 1, 2, 2, 2)
 #endif
 #if LM_PART == 14
-LM_ATTN_FWD(f32_d64, F32, 64, 1)
-LM_ATTN_FWD(f32_d128, F32, 128, 1)
-LM_ATTN_DQ(f32_d64, F32, 64, 1)
-LM_ATTN_DQ(f32_d128, F32, 128, 1)
-LM_ATTN_DKV(f32_d64, F32, 64, 1)
-LM_ATTN_DKV(f32_d128, F32, 128, 1)
+LM_ATTN(f32_d64_s1, F32, 64, 1, 2, 1, 1, 1)
+LM_ATTN(f32_d64_s2, F32, 64, 2, 2, 1, 1, 1)
+LM_ATTN(f32_d64_s4, F32, 64, 4, 1, 1, 1, 1)
+LM_ATTN(f32_d128_s1, F32, 128, 1, 2, 1, 1, 1)
+LM_ATTN(f32_d128_s2, F32, 128, 2, 2, 1, 1, 1)
+LM_ATTN(f32_d128_s4, F32, 128, 4, 1, 1, 1, 1)
 #endif

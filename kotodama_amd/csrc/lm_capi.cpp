@@ -19,10 +19,10 @@ namespace {
 // Code-object parts and kernel slots.
 constexpr int kLmPart = 12, kAttnBf16Part = 13, kAttnF32Part = 14;
 enum Slot {
-  kAttnFwd = 0,                // + 2 * (fp32) + (head_dim > 64)
-  kAttnDq = kAttnFwd + 4,
-  kAttnDkv = kAttnDq + 4,
-  kRopeFwd = kAttnDkv + 4,     // + 4 * (fp32) + 2 * (scalar) + (4 heads per lane group)
+  kAttnFwd = 0,                // + 6 * (fp32) + 3 * (head_dim > 64) + log2 of the waves that share rows
+  kAttnDq = kAttnFwd + 12,
+  kAttnDkv = kAttnDq + 12,
+  kRopeFwd = kAttnDkv + 12,    // + 4 * (fp32) + 2 * (scalar) + (4 heads per lane group)
   kRopeBwd = kRopeFwd + 8,     // + 2 * (fp32) + (scalar)
   kRopeDw = kRopeBwd + 4,      // + (fp32)
   kEmbedFwd = kRopeDw + 2,     // + 2 * (fp32) + (scalar)
@@ -34,6 +34,7 @@ enum Slot {
 static_assert(kSlots <= ATTNRES_INTERNAL_SLOTS, "kernel slots");
 
 constexpr int64_t kMaxLen = (int64_t)1 << 30;  // tokens of one sequence
+constexpr int kMaxGroup = 4096;                // query heads per key head
 
 int fail(int code, const char* fmt, ...) {
   char buf[400];
@@ -88,8 +89,10 @@ int check_attention(int batch, int heads, int kv_heads, int64_t q_len, int64_t k
                 LM_ATTN_MAX_DIM);
   if (q_len > kMaxLen || kv_slots > kMaxLen)
     return fail(ATTNRES_ERR_UNSUPPORTED, "attention: sequences over 2^30 tokens");
-  const int64_t rows = (q_len + 31) / 32, keys = (kv_slots + 31) / 32;
-  if ((rows > keys ? rows : keys) * batch * heads > kMaxLen)
+  if (heads / kv_heads > kMaxGroup || q_len * (heads / kv_heads) > kMaxLen)
+    return fail(ATTNRES_ERR_UNSUPPORTED, "attention: over 4096 query heads per key head, or over 2^30 rows of them");
+  const int64_t rows = q_len * (heads / kv_heads), lines = rows > kv_slots ? rows : kv_slots;
+  if ((lines + 31) / 32 * batch * kv_heads > kMaxLen)
     return fail(ATTNRES_ERR_UNSUPPORTED, "attention: too many rows for one call");
   return ATTNRES_OK;
 }
@@ -120,19 +123,37 @@ int fill_attention(lm_attn_params* P, int batch, int heads, int kv_heads, int64_
   return ATTNRES_OK;
 }
 
-// One launch of the family at `base` over `tiles` x heads x batch workgroups.
-int launch_attention(int base, const char* kind, lm_attn_params& P, int dtype, int tiles, int heads, void* stream) {
-  const bool f32 = dtype == ATTNRES_DTYPE_F32, wide = P.dim > 64;
-  char name[64];
-  snprintf(name, sizeof(name), "attnres_attention_%s_%s_d%d", kind, f32 ? "f32" : "bf16", wide ? 128 : 64);
-  P.n_tiles = tiles;
-  P.n_items = tiles * heads * P.batch;
-  const unsigned grid = (unsigned)((P.n_items + 7) / 8 * 8);  // the XCDs' shares (work_item in the kernels)
-  return launch(base + (f32 ? 2 : 0) + (wide ? 1 : 0), f32 ? kAttnF32Part : kAttnBf16Part, name, grid, 1,
-                64 * LM_ATTN_WAVES, 0, P, stream);
+// Offsets within a tile (up to 128 rows, or their queries and heads) are 32 bits wide.
+int check_span(const char* what, const lm_strides& s, int64_t heads, int64_t tokens, int es) {
+  const int64_t t = s.t * es * (tokens < 130 ? tokens : 130), h = s.h * es * (heads - 1);
+  if (s.t < 0 || s.h < 0 || s.b < 0 || s.t > kMaxLen || s.h > ((int64_t)1 << 40) || t + h >= ((int64_t)1 << 32) - 4096)
+    return fail(ATTNRES_ERR_UNSUPPORTED, "%s: 130 tokens of a head group span over 4 GiB (or a stride is negative)",
+                what);
+  return ATTNRES_OK;
 }
 
-int tiles_of(int64_t n, int per) { return (int)((n + per - 1) / per); }
+// One launch of the family at `base`: `lines` rows (or keys) per key head, 32 a wave.
+int launch_attention(int base, const char* kind, lm_attn_params& P, int dtype, int64_t lines, void* stream) {
+  int cus = 0;
+  int rc = attnres_internal_num_cus(&cus);
+  if (rc != ATTNRES_OK) return rc;
+  const int64_t heads = (int64_t)P.batch * P.kv_heads;
+  // Waves share rows where there are fewer than two waves for every SIMD.
+  const int64_t waves = heads * ((lines + 31) / 32), full = (int64_t)cus * 8;
+  const int log = waves >= full ? 0 : waves * 2 >= full ? 1 : 2;
+  const int per = 32 * LM_ATTN_WAVES >> log;
+  P.n_tiles = (int32_t)((lines + per - 1) / per);
+  P.cus_per_xcd = cus / 8 > 0 ? cus / 8 : 1;
+  const int group = P.heads / P.kv_heads;
+  P.group_magic = (uint32_t)((((uint64_t)1 << 32) + group - 1) / group);
+  const int64_t items = P.n_tiles * heads;
+  if (items > INT32_MAX - 8) return fail(ATTNRES_ERR_UNSUPPORTED, "attention: too many rows for one call");
+  const bool f32 = dtype == ATTNRES_DTYPE_F32, wide = P.dim > 64;
+  char name[64];
+  snprintf(name, sizeof(name), "attnres_attention_%s_%s_d%d_s%d", kind, f32 ? "f32" : "bf16", wide ? 128 : 64, 1 << log);
+  return launch(base + (f32 ? 6 : 0) + (wide ? 3 : 0) + log, f32 ? kAttnF32Part : kAttnBf16Part, name,
+                (unsigned)((items + 7) / 8 * 8), 1, 64 * LM_ATTN_WAVES, 0, P, stream);
+}
 
 int64_t attention_workspace(int batch, int heads, int64_t q_len, int backward) {
   return backward ? (int64_t)batch * heads * q_len * 4 : 0;
@@ -314,6 +335,10 @@ int attnres_attention_fwd(const void* q, const int64_t* q_strides, const void* k
         (rc = take_strides("attention: v", v, v_strides, batch, kv_heads, kv_slots, es, 16, &P.sv)) != ATTNRES_OK)
       return rc;
   }
+  const int group = heads / kv_heads;
+  if ((rc = check_span("attention: k", P.sk, 1, kv_slots, es)) != ATTNRES_OK ||
+      (rc = check_span("attention: v", P.sv, 1, kv_slots, es)) != ATTNRES_OK)
+    return rc;
   const int64_t need = attention_workspace(batch, heads, q_len, 0);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return fail(ATTNRES_ERR_ARG, "attention: workspace of %lld bytes needed", (long long)need);
@@ -322,7 +347,7 @@ int attnres_attention_fwd(const void* q, const int64_t* q_strides, const void* k
   P.v = v;
   P.o = out;
   P.lse = lse;
-  return launch_attention(kAttnFwd, "fwd", P, dtype, tiles_of(q_len, LM_ATTN_ROWS), heads, stream);
+  return launch_attention(kAttnFwd, "fwd", P, dtype, q_len * group, stream);
 }
 
 int attnres_attention_bwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
@@ -366,6 +391,12 @@ int attnres_attention_bwd(const void* q, const int64_t* q_strides, const void* k
             ATTNRES_OK)
       return rc;
   }
+  const int group = heads / kv_heads;
+  if ((rc = check_span("attention: k", P.sk, 1, kv_slots, es)) != ATTNRES_OK ||
+      (rc = check_span("attention: v", P.sv, 1, kv_slots, es)) != ATTNRES_OK ||
+      (rc = check_span("attention: q", P.sq, group, q_len, es)) != ATTNRES_OK ||
+      (rc = check_span("attention: grad_out", P.sdo, group, q_len, es)) != ATTNRES_OK)
+    return rc;
   P.q = q;
   P.k = k;
   P.v = v;
@@ -378,11 +409,11 @@ int attnres_attention_bwd(const void* q, const int64_t* q_strides, const void* k
   P.dk = grad_k;
   P.dv = grad_v;
   if (q_len > 0) {
-    rc = launch_attention(kAttnDq, "dq", P, dtype, tiles_of(q_len, LM_ATTN_ROWS), heads, stream);
+    rc = launch_attention(kAttnDq, "dq", P, dtype, q_len * group, stream);
     if (rc != ATTNRES_OK) return rc;
   }
   if (kv_slots == 0) return ATTNRES_OK;
-  return launch_attention(kAttnDkv, "dkv", P, dtype, tiles_of(kv_slots, LM_ATTN_BWD_KEYS), kv_heads, stream);
+  return launch_attention(kAttnDkv, "dkv", P, dtype, kv_slots, stream);
 }
 
 int attnres_qk_norm_rope_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,

@@ -10,12 +10,7 @@
 
 #include <stdint.h>
 
-/* Attention: rows (queries) and keys of one workgroup's tile. */
-#define LM_ATTN_WAVES 4       /* waves per workgroup */
-#define LM_ATTN_ROWS 128      /* query rows per workgroup (forward, query gradient): 32 per wave */
-#define LM_ATTN_KEYS 64       /* keys per LDS tile of those kernels */
-#define LM_ATTN_BWD_KEYS 128  /* keys per workgroup of the key/value gradient: 32 per wave */
-#define LM_ATTN_BWD_ROWS 32   /* query rows per LDS tile there */
+#define LM_ATTN_WAVES 4 /* waves per workgroup of the attention kernels; a wave owns 32 rows or 32 keys */
 #define LM_ATTN_MAX_DIM 128
 
 /* Strides in elements; element (b, h, t, d) of X at X + b*sb + h*sh + t*st + d. */
@@ -59,8 +54,8 @@ typedef struct lm_attn_params {
   int32_t lens64;        /* kv_lens holds 64-bit numbers */
   int32_t start64;       /* q_start does */
   int32_t n_tiles;       /* tiles along the axis that the grid splits */
-  int32_t n_items;       /* workgroups with work: n_tiles * heads * batch (or kv_heads) */
-  int32_t splits;        /* parts of the key axis (few query rows) */
+  int32_t cus_per_xcd;
+  uint32_t group_magic;  /* ceil(2^32 / group): n / group = n * group_magic >> 32 for n under 2^32 / group */
   float scale;           /* of the scores */
   float scale_log2;      /* scale * log2(e) */
 } lm_attn_params;

@@ -91,6 +91,27 @@ def test_attention_masks(dtype, b, h, hk, tq, tk, d, causal, lens, start):
 
 
 @pytest.mark.parametrize("dtype", [BF, FP], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("b,h,hk,tq,tk,d,causal,lens,start", [
+    # enough rows that two waves share theirs, or none do
+    (4, 16, 16, 530, 530, 64, True, None, None),
+    (8, 16, 16, 530, 530, 64, True, None, None),
+    (4, 24, 8, 400, 300, 128, True, [300, 1, 0, 177], 0),
+    (8, 32, 16, 300, 500, 128, True, [500, 300, 200, 1, 0, 499, 64, 128], None),
+    (3, 21, 7, 700, 700, 72, False, [700, 64, 333], None),
+    (2, 40, 4, 515, 515, 128, True, None, 3),
+])
+def test_attention_of_many_rows(dtype, b, h, hk, tq, tk, d, causal, lens, start):
+    _attention_case(b, h, hk, tq, tk, d, dtype, seed=tq + b, causal=causal, lens=lens, start=start)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP], ids=["bf16", "fp32"])
+def test_attention_of_wide_groups(dtype):
+    _attention_case(1, 33, 1, 5, 70, 64, dtype, seed=5)
+    _attention_case(1, 200, 2, 3, 40, 128, dtype, seed=6, lens=[30])
+    _attention_case(2, 14, 2, 45, 45, 64, dtype, seed=7, lens=[45, 9], start=0)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP], ids=["bf16", "fp32"])
 def test_attention_gradient_through_lse(dtype):
     _attention_case(2, 4, 2, 90, 90, 64, dtype, seed=3, with_lse=True, scale=0.3)
     _attention_case(2, 2, 1, 50, 90, 128, dtype, seed=4, with_lse=True, lens=[90, 0], causal=False)
