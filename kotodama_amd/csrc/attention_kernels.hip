@@ -412,7 +412,8 @@ struct Rows {
   bool exists, live;        // the row is there; it sees a key
   int lim;                  // keys it sees
   Span mine;                // the wave's rows'
-  int tiles;                // key tiles of the workgroup
+  int split;                // which part of the key tiles this workgroup takes
+  int t0, t1;               // its key tiles
   Seq S;
 
   __device__ __forceinline__ bool init(const lm_attn_params& P) {
@@ -426,7 +427,13 @@ struct Rows {
     b = it.head / P.kv_heads;
     const int group = P.heads / P.kv_heads;
     const int rows = P.q_len * group;
-    const int g0 = (P.n_tiles - 1 - it.rank) * kPerGroup;
+    split = 0;
+    int rank = it.rank;
+    if (KS == 4 && P.splits > 1) {
+      rank = it.rank / P.splits;
+      split = it.rank - rank * P.splits;
+    }
+    const int g0 = (P.n_tiles / (KS == 4 ? P.splits : 1) - 1 - rank) * kPerGroup;
     const int r0 = g0 + wave / KS * 32;
     S = sequence(P, b, group);
     row = r0 + (lane & 31);
@@ -436,20 +443,30 @@ struct Rows {
     live = row >= S.lo && row < S.hi;
     lim = live ? (P.causal ? S.start + query + 1 : S.kv_len) : 0;
     mine = span(P, S, group, r0, 32);
-    tiles = (span(P, S, group, g0, kPerGroup).most + kKeys - 1) / kKeys;
+    t0 = 0;
+    t1 = (span(P, S, group, g0, kPerGroup).most + kKeys - 1) / kKeys;
+    if (KS == 4 && P.splits > 1) {
+      const int each = (t1 + P.splits - 1) / P.splits;
+      t0 = split * each < t1 ? split * each : t1;
+      t1 = t0 + each < t1 ? t0 + each : t1;
+    }
     return true;
+  }
+  // this row among all rows of the call
+  __device__ __forceinline__ int64_t index(const lm_attn_params& P) const {
+    return ((int64_t)b * P.kv_heads + kvh) * ((int64_t)P.q_len * (P.heads / P.kv_heads)) + row;
   }
   __device__ __forceinline__ int64_t stat(const lm_attn_params& P) const {
     return ((int64_t)b * P.heads + head) * P.q_len + query;
   }
 };
 
-// Runs step(t, k, v) over the key tiles in LDS: with two buffers each, tile t+1
+// Runs step(t, k, v) over the key tiles t0 .. t1-1 in LDS: with two buffers each, tile t+1
 // is requested before t is worked on; with one, the other workgroup of the CU
 // works meanwhile.
 template <typename KT, int NBUF, typename Step>
-__device__ __forceinline__ void over_keys(const char* kp, int64_t kst, const char* vp, int64_t vst, int tiles, int last,
-                                          int chunks, int wave, int lane, char* k0, char* k1, char* v0, char* v1,
+__device__ __forceinline__ void over_keys(const char* kp, int64_t kst, const char* vp, int64_t vst, int t0, int t1,
+                                          int last, int chunks, int wave, int lane, char* k0, char* k1, char* v0, char* v1,
                                           Step&& step) {
   const typename KT::Lane ka = KT::lane_offsets((uint32_t)kst, chunks, wave, lane);
   const typename KT::Lane va = KT::lane_offsets((uint32_t)vst, chunks, wave, lane);
@@ -462,21 +479,21 @@ __device__ __forceinline__ void over_keys(const char* kp, int64_t kst, const cha
     __syncthreads();
   };
   if constexpr (NBUF == 1) {
-    for (int t = 0; t < tiles; ++t) {
-      if (t > 0) __syncthreads();
+    for (int t = t0; t < t1; ++t) {
+      if (t > t0) __syncthreads();
       request(t, k0, v0);
       arrived();
       step(t, k0, v0);
     }
   } else {
-    if (tiles > 0) request(0, k0, v0);
-    for (int t = 0; t < tiles; t += 2) {
+    if (t0 < t1) request(t0, k0, v0);
+    for (int t = t0; t < t1; t += 2) {
       arrived();
-      if (t + 1 < tiles) request(t + 1, k1, v1);
+      if (t + 1 < t1) request(t + 1, k1, v1);
       step(t, k0, v0);
-      if (t + 1 < tiles) {
+      if (t + 1 < t1) {
         arrived();
-        if (t + 2 < tiles) request(t + 2, k0, v0);
+        if (t + 2 < t1) request(t + 2, k0, v0);
         step(t + 1, k1, v1);
       }
     }
@@ -524,13 +541,14 @@ __device__ __forceinline__ void attention_fwd(const lm_attn_params& P, char* k0,
   const int row_at = KT::row_at(lane), col_at = KT::col_at(lane);
 
   over_keys<KT, NBUF>(
-      kp, P.sk.t * T::kBytes, vp, P.sv.t * T::kBytes, R.tiles, R.S.kv_len - 1, chunks, R.wave, lane, k0, k1, v0, v1,
+      kp, P.sk.t * T::kBytes, vp, P.sv.t * T::kBytes, R.t0, R.t1, R.S.kv_len - 1, chunks, R.wave, lane, k0, k1, v0, v1,
       [&](int t, const char* kc, const char* vc) {
         constexpr int NB = RW::kBlocks;
         const int first = KS == 1 ? 0 : 32 * NB * R.part;  // this wave's keys of the tile
         const int key0 = t * RW::kKeys + first;
         if (key0 >= R.mine.most) return;
         f32x16 s[NB];
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int kb = 0; kb < NB; ++kb) {
           s[kb] = zero16();
@@ -539,6 +557,7 @@ __device__ __forceinline__ void attention_fwd(const lm_attn_params& P, char* k0,
             s[kb] = T::mma(KT::row_frag(kc, first + 32 * kb, st, row_at), qf[st], s[kb]);
         }
         if constexpr (T::kBytes == 2) interleave<4, NB * DP / 16, 1, 0, 0>();
+        __builtin_amdgcn_s_setprio(0);
         if (key0 + 32 * NB > R.mine.all) {
 #pragma unroll
           for (int kb = 0; kb < NB; ++kb)
@@ -612,10 +631,71 @@ __device__ __forceinline__ void attention_fwd(const lm_attn_params& P, char* k0,
     }
     if (R.part != 0) return;
   }
+  if constexpr (KS == 4) {
+    if (P.splits > 1) {  // this part's sums as they stand, for the join
+      if (!R.exists) return;
+      const int64_t at = R.index(P) * P.splits + R.split;
+      if (l > 0.f) store_rows<F32, DP>(reinterpret_cast<char*>(P.part + at * P.dim), acc, 1.f, P.dim, h);
+      if (h == 0) {
+        P.part_ml[at * 2] = m;
+        P.part_ml[at * 2 + 1] = l;
+      }
+      return;
+    }
+  }
   if (R.exists) {
     const float inv = l > 0.f ? 1.f / l : 0.f;
     store_rows<T, DP>((char*)P.o + row_offset(P.so, R.b, R.head, R.query) * T::kBytes, acc, inv, P.dim, h);
     if (P.lse != nullptr && h == 0) P.lse[R.stat(P)] = l > 0.f ? (m + __builtin_amdgcn_logf(l)) * kLn2 : kNegInf;
+  }
+}
+
+// Joins the parts of a row: a workgroup per row, 32 lanes over its columns (four
+// each), eight parts at a time.
+template <typename T>
+__device__ __forceinline__ void attention_join(const lm_attn_params& P, float* red) {
+  const int group = P.heads / P.kv_heads, rows = P.q_len * group;
+  const int64_t at = blockIdx.x;
+  const int row = (int)(at % rows), query = row / group;
+  const int kvh = (int)(at / rows % P.kv_heads), b = (int)(at / rows / P.kv_heads);
+  const int head = kvh * group + (row - query * group);
+  const int lane = threadIdx.x & 63;
+  const float* ml = P.part_ml + at * P.splits * 2;
+  // every wave: the common maximum and the sum
+  float m = kNegInf;
+  for (int s = lane; s < P.splits; s += 64) m = fmaxf(m, ml[2 * s]);
+  for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+  float l = 0.f;
+  for (int s = lane; s < P.splits; s += 64) l += ml[2 * s] == kNegInf ? 0.f : ml[2 * s + 1] * exp2_fast(ml[2 * s] - m);
+  for (int o = 1; o < 64; o <<= 1) l += __shfl_xor(l, o);
+  const int d = 4 * (threadIdx.x & 31), part = threadIdx.x >> 5;
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  if (d < P.dim) {
+#pragma unroll 4
+    for (int s = part; s < P.splits; s += 8) {
+      const float ms = ml[2 * s];
+      if (ms == kNegInf) continue;  // saw no key: nothing was written
+      const float w = exp2_fast(ms - m);
+      const f32x4 v = *reinterpret_cast<const f32x4*>(P.part + (at * P.splits + s) * P.dim + d);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum[j] = __builtin_fmaf(v[j], w, sum[j]);
+    }
+  }
+  *reinterpret_cast<f32x4*>(red + threadIdx.x * 4) = sum;
+  __syncthreads();
+  if (threadIdx.x < 32 && d < P.dim) {
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int p = 0; p < 8; ++p) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(red + (p * 32 + threadIdx.x) * 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] += v[j];
+    }
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    store4<T>((char*)P.o + (row_offset(P.so, b, head, query) + d) * T::kBytes, o[0] * inv, o[1] * inv, o[2] * inv,
+              o[3] * inv);
+    if (P.lse != nullptr && threadIdx.x == 0)
+      P.lse[((int64_t)b * P.heads + head) * P.q_len + query] =
+          l > 0.f ? (m + __builtin_amdgcn_logf(l)) * kLn2 : kNegInf;
   }
 }
 
@@ -656,7 +736,7 @@ __device__ __forceinline__ void attention_bwd_dq(const lm_attn_params& P, char* 
   const int row_at = KT::row_at(lane), col_at = KT::col_at(lane);
 
   over_keys<KT, NBUF>(
-      kp, P.sk.t * T::kBytes, vp, P.sv.t * T::kBytes, R.tiles, R.S.kv_len - 1, chunks, R.wave, lane, k0, k1, v0, v1,
+      kp, P.sk.t * T::kBytes, vp, P.sv.t * T::kBytes, R.t0, R.t1, R.S.kv_len - 1, chunks, R.wave, lane, k0, k1, v0, v1,
       [&](int t, const char* kc, const char* vc) {
         constexpr int NB = RW::kBlocks;
         const int first = KS == 1 ? 0 : 32 * NB * R.part;
@@ -665,12 +745,14 @@ __device__ __forceinline__ void attention_bwd_dq(const lm_attn_params& P, char* 
 #pragma unroll
         for (int kb = 0; kb < NB; ++kb) {
           f32x16 s = zero16(), dp = zero16();
+          __builtin_amdgcn_s_setprio(1);
 #pragma unroll
           for (int st = 0; st < DP / 16; ++st) {
             s = T::mma(KT::row_frag(kc, first + 32 * kb, st, row_at), qf[st], s);
             dp = T::mma(KT::row_frag(vc, first + 32 * kb, st, row_at), gf[st], dp);
           }
           if constexpr (T::kBytes == 2) interleave<4, DP / 8, 1, 0, 0>();
+          __builtin_amdgcn_s_setprio(0);
 #pragma unroll
           for (int i = 0; i < 16; ++i)
             s[i] = exp2_fast(__builtin_fmaf(s[i], P.scale_log2, -lse2)) * (dp[i] - delta);
@@ -803,12 +885,14 @@ __device__ __forceinline__ void attention_bwd_dkv(const lm_attn_params& P, char*
     // instruction each) instead of held in registers
     asm volatile("" : "+v"(row_at), "+v"(col_at));
     f32x16 s = zero16(), dp = zero16();
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int st = 0; st < DP / 16; ++st) {
       s = T::mma(QT::row_frag(qc, mine, st, row_at), kf[st], s);
       dp = T::mma(QT::row_frag(gc, mine, st, row_at), vf[st], dp);
     }
     if constexpr (T::kBytes == 2) interleave<4, DP / 8, 1, 0, 0>();
+    __builtin_amdgcn_s_setprio(0);
     const float* stats = sc + (KS == 1 ? 0 : 64 * part);
 #pragma unroll
     for (int a = 0; a < 4; ++a) {
@@ -926,7 +1010,14 @@ __device__ __forceinline__ void attention_bwd_dkv(const lm_attn_params& P, char*
     attention_bwd_dkv<T, DP, KS, NBUF>(P, q0, q1, g0, g1, st0, st1);                                 \
   }
 
+#define LM_ATTN_JOIN(NAME, T)                                                                       \
+  extern "C" __global__ void __launch_bounds__(256) attnres_attention_join_##NAME(lm_attn_params P) { \
+    __shared__ __align__(16) float red[1024];                                                       \
+    attention_join<T>(P, red);                                                                      \
+  }
+
 #if LM_PART == 13
+LM_ATTN_JOIN(bf16, Bf16)
 LM_ATTN(bf16_d64_s1, Bf16, 64, 1, 2, 2, 2, 2)
 LM_ATTN(bf16_d64_s2, Bf16, 64, 2, 2, 2, 2, 2)
 LM_ATTN(bf16_d64_s4, Bf16, 64, 4, 1, 2, 2, 2)
@@ -935,6 +1026,7 @@ LM_ATTN(bf16_d128_s2, Bf16, 128, 2, 2, 2, 2, 2)
 LM_ATTN(bf16_d128_s4, Bf16, 128, 4, 1, 2, 2, 2)
 #endif
 #if LM_PART == 14
+LM_ATTN_JOIN(f32, F32)
 LM_ATTN(f32_d64_s1, F32, 64, 1, 2, 1, 1, 1)
 LM_ATTN(f32_d64_s2, F32, 64, 2, 2, 1, 1, 1)
 LM_ATTN(f32_d64_s4, F32, 64, 4, 1, 1, 1, 1)

@@ -22,7 +22,8 @@ enum Slot {
   kAttnFwd = 0,                // + 6 * (fp32) + 3 * (head_dim > 64) + log2 of the waves that share rows
   kAttnDq = kAttnFwd + 12,
   kAttnDkv = kAttnDq + 12,
-  kRopeFwd = kAttnDkv + 12,    // + 4 * (fp32) + 2 * (scalar) + (4 heads per lane group)
+  kAttnJoin = kAttnDkv + 12,   // + (fp32)
+  kRopeFwd = kAttnJoin + 2,    // + 4 * (fp32) + 2 * (scalar) + (4 heads per lane group)
   kRopeBwd = kRopeFwd + 8,     // + 2 * (fp32) + (scalar)
   kRopeDw = kRopeBwd + 4,      // + (fp32)
   kEmbedFwd = kRopeDw + 2,     // + 2 * (fp32) + (scalar)
@@ -34,6 +35,7 @@ enum Slot {
 static_assert(kSlots <= ATTNRES_INTERNAL_SLOTS, "kernel slots");
 
 constexpr int64_t kMaxLen = (int64_t)1 << 30;  // tokens of one sequence
+constexpr int kSplitPerCu = 2;                 // workgroups per CU to split the key axis into
 constexpr int kMaxGroup = 4096;                // query heads per key head
 
 int fail(int code, const char* fmt, ...) {
@@ -132,17 +134,40 @@ int check_span(const char* what, const lm_strides& s, int64_t heads, int64_t tok
   return ATTNRES_OK;
 }
 
-// One launch of the family at `base`: `lines` rows (or keys) per key head, 32 a wave.
+// How the `lines` rows (or keys) of each key head are dealt out, 32 to a wave.
+struct AttnPlan {
+  int log = 0;     // 2^log waves share their rows
+  int splits = 1;  // parts of the key axis (forward)
+};
+
+// Waves share rows (and split the key tiles) where there are too few of them
+// for two or more on every SIMD: fwd and dq at the proxy training shape (1024
+// waves) take 38 + 46 us with two sharing against 54 + 65 us with none, at the
+// 8B one (8192) sharing costs 10-20%; dk and dv at the 8B shape (2048 waves)
+// 608 us with two sharing, 725 with none and 761 with four, as workgroups of
+// fewer keys balance the causal rows better.  Where even four sharing leave
+// CUs without work, the forward splits the key axis over workgroups too.
+AttnPlan attention_plan(int base, int64_t heads, int64_t lines, int64_t kv_slots, int cus) {
+  AttnPlan p;
+  const int64_t waves = heads * ((lines + 31) / 32), full = (int64_t)cus * (base == kAttnDkv ? 16 : 8);
+  p.log = waves >= full ? 0 : waves * 2 >= full ? 1 : 2;
+  if (base == kAttnFwd && p.log == 2) {
+    const int64_t most = (kv_slots + 127) / 128, want = (int64_t)cus * kSplitPerCu / (waves > 0 ? waves : 1);
+    const int64_t n = want < most ? want : most;
+    p.splits = n < 2 ? 1 : (int)n;
+  }
+  return p;
+}
+
 int launch_attention(int base, const char* kind, lm_attn_params& P, int dtype, int64_t lines, void* stream) {
   int cus = 0;
   int rc = attnres_internal_num_cus(&cus);
   if (rc != ATTNRES_OK) return rc;
   const int64_t heads = (int64_t)P.batch * P.kv_heads;
-  // Waves share rows where there are fewer than two waves for every SIMD.
-  const int64_t waves = heads * ((lines + 31) / 32), full = (int64_t)cus * 8;
-  const int log = waves >= full ? 0 : waves * 2 >= full ? 1 : 2;
-  const int per = 32 * LM_ATTN_WAVES >> log;
-  P.n_tiles = (int32_t)((lines + per - 1) / per);
+  const AttnPlan plan = attention_plan(base, heads, lines, P.kv_len, cus);
+  const int per = 32 * LM_ATTN_WAVES >> plan.log;
+  P.splits = plan.splits;
+  P.n_tiles = (int32_t)((lines + per - 1) / per * plan.splits);
   P.cus_per_xcd = cus / 8 > 0 ? cus / 8 : 1;
   const int group = P.heads / P.kv_heads;
   P.group_magic = (uint32_t)((((uint64_t)1 << 32) + group - 1) / group);
@@ -150,13 +175,24 @@ int launch_attention(int base, const char* kind, lm_attn_params& P, int dtype, i
   if (items > INT32_MAX - 8) return fail(ATTNRES_ERR_UNSUPPORTED, "attention: too many rows for one call");
   const bool f32 = dtype == ATTNRES_DTYPE_F32, wide = P.dim > 64;
   char name[64];
-  snprintf(name, sizeof(name), "attnres_attention_%s_%s_d%d_s%d", kind, f32 ? "f32" : "bf16", wide ? 128 : 64, 1 << log);
-  return launch(base + (f32 ? 6 : 0) + (wide ? 3 : 0) + log, f32 ? kAttnF32Part : kAttnBf16Part, name,
+  snprintf(name, sizeof(name), "attnres_attention_%s_%s_d%d_s%d", kind, f32 ? "f32" : "bf16", wide ? 128 : 64,
+           1 << plan.log);
+  return launch(base + (f32 ? 6 : 0) + (wide ? 3 : 0) + plan.log, f32 ? kAttnF32Part : kAttnBf16Part, name,
                 (unsigned)((items + 7) / 8 * 8), 1, 64 * LM_ATTN_WAVES, 0, P, stream);
 }
 
-int64_t attention_workspace(int batch, int heads, int64_t q_len, int backward) {
-  return backward ? (int64_t)batch * heads * q_len * 4 : 0;
+// Bytes of the forward's partial rows, and where their maxima and sums begin.
+int forward_workspace(int batch, int heads, int kv_heads, int64_t q_len, int64_t kv_slots, int head_dim, int64_t* ml,
+                      int64_t* bytes) {
+  int cus = 0;
+  int rc = attnres_internal_num_cus(&cus);
+  if (rc != ATTNRES_OK) return rc;
+  const int splits =
+      attention_plan(kAttnFwd, (int64_t)batch * kv_heads, q_len * (heads / kv_heads), kv_slots, cus).splits;
+  const int64_t parts = splits > 1 ? (int64_t)batch * heads * q_len * splits : 0;
+  *ml = parts * head_dim * 4;
+  *bytes = *ml + parts * 8;
+  return ATTNRES_OK;
 }
 
 // ------------------------------------------------------------------ rope --
@@ -308,8 +344,12 @@ int attnres_attention_workspace_size(int batch, int heads, int kv_heads, int64_t
   if (bytes == nullptr) return fail(ATTNRES_ERR_ARG, "attention: bytes is NULL");
   int rc = check_attention(batch, heads, kv_heads, q_len, kv_slots, head_dim, dtype);
   if (rc != ATTNRES_OK) return rc;
-  *bytes = attention_workspace(batch, heads, q_len, backward);
-  return ATTNRES_OK;
+  if (backward != 0) {
+    *bytes = (int64_t)batch * heads * q_len * 4;
+    return ATTNRES_OK;
+  }
+  int64_t ml = 0;
+  return forward_workspace(batch, heads, kv_heads, q_len, kv_slots, head_dim, &ml, bytes);
 }
 
 int attnres_attention_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
@@ -339,15 +379,25 @@ int attnres_attention_fwd(const void* q, const int64_t* q_strides, const void* k
   if ((rc = check_span("attention: k", P.sk, 1, kv_slots, es)) != ATTNRES_OK ||
       (rc = check_span("attention: v", P.sv, 1, kv_slots, es)) != ATTNRES_OK)
     return rc;
-  const int64_t need = attention_workspace(batch, heads, q_len, 0);
+  int64_t ml = 0, need = 0;
+  if ((rc = forward_workspace(batch, heads, kv_heads, q_len, kv_slots, head_dim, &ml, &need)) != ATTNRES_OK) return rc;
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return fail(ATTNRES_ERR_ARG, "attention: workspace of %lld bytes needed", (long long)need);
+  if (need > 0 && !aligned(workspace, 16))
+    return fail(ATTNRES_ERR_ALIGN, "attention: workspace must be 16-byte aligned");
+  P.part = static_cast<float*>(workspace);
+  P.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + ml);
   P.q = q;
   P.k = k;
   P.v = v;
   P.o = out;
   P.lse = lse;
-  return launch_attention(kAttnFwd, "fwd", P, dtype, q_len * group, stream);
+  rc = launch_attention(kAttnFwd, "fwd", P, dtype, q_len * group, stream);
+  if (rc != ATTNRES_OK || P.splits < 2) return rc;
+  const bool f32 = dtype == ATTNRES_DTYPE_F32;
+  return launch(kAttnJoin + (f32 ? 1 : 0), f32 ? kAttnF32Part : kAttnBf16Part,
+                f32 ? "attnres_attention_join_f32" : "attnres_attention_join_bf16", (unsigned)((int64_t)batch * heads * q_len),
+                1, 256, 0, P, stream);
 }
 
 int attnres_attention_bwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
@@ -376,7 +426,7 @@ int attnres_attention_bwd(const void* q, const int64_t* q_strides, const void* k
             ATTNRES_OK)
       return rc;
     if (lse == nullptr) return fail(ATTNRES_ERR_ARG, "attention: lse is NULL");
-    const int64_t need = attention_workspace(batch, heads, q_len, 1);
+    const int64_t need = (int64_t)batch * heads * q_len * 4;
     if (workspace == nullptr || workspace_bytes < need)
       return fail(ATTNRES_ERR_ARG, "attention: workspace of %lld bytes needed", (long long)need);
     if (!aligned(workspace, 16) || !aligned(lse, 4) || !aligned(grad_lse, 4))

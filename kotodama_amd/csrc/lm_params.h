@@ -38,7 +38,8 @@ typedef struct lm_attn_params {
   float* lse;            /* (batch, heads, q_len) natural log of the softmax sum; -inf for a row with no keys */
   float* delta;          /* (batch, heads, q_len): rowsum(grad_out * out) - grad_lse, written by the dq kernel */
   const float* grad_lse; /* (batch, heads, q_len) or NULL */
-  float* part;           /* split rows: partial outputs and their maxima and sums */
+  float* part;           /* (rows, splits, dim): sums of a part of the keys, where splits > 1 */
+  float* part_ml;        /* (rows, splits, 2): their maxima (times log2 e) and sums of weights */
   const void* kv_lens;   /* (batch,) int32 or int64, or NULL: kv_len */
   const void* q_start;   /* (batch,) int32 or int64, or NULL */
   lm_strides sq, sk, sv, so, sdo, sout, sdq, sdk, sdv;
@@ -54,6 +55,7 @@ typedef struct lm_attn_params {
   int32_t lens64;        /* kv_lens holds 64-bit numbers */
   int32_t start64;       /* q_start does */
   int32_t n_tiles;       /* tiles along the axis that the grid splits */
+  int32_t splits;        /* parts of the key axis, each a workgroup (forward, four waves a row) */
   int32_t cus_per_xcd;
   uint32_t group_magic;  /* ceil(2^32 / group): n / group = n * group_magic >> 32 for n under 2^32 / group */
   float scale;           /* of the scores */
