@@ -123,6 +123,9 @@ def parse_args():
     ap.add_argument("--residuals", default="standard,attnres,torch",
                     help="lmstep: comma-separated residual streams to time (standard, attnres, torch)")
     ap.add_argument("--eager-sublayers", action="store_true", help="lmstep: run the dense sublayers uncompiled")
+    ap.add_argument("--lm-kernels", action="store_true",
+                    help="lmstep: embedding, query and key norms with rotation, and attention on this package's "
+                         "kernels (kotodama_amd.lmops) in every residual stream")
     ap.add_argument("--graph", action="store_true",
                     help="cfg2train / cfg3train / cfg1btrain (list, eager): also time the step recorded in a HIP graph")
     ap.add_argument("--no-cpu-baseline", action="store_true", help="skip the CPU baseline leg")
@@ -982,14 +985,16 @@ def reference_routing_loop():
     return loop
 
 
-def bench_lmstep(steps: int, warmup: int, dev, lm: str, residuals, compiled: bool = True) -> dict:
+def bench_lmstep(steps: int, warmup: int, dev, lm: str, residuals, compiled: bool = True,
+                 kernels: bool = False) -> dict:
     """lmstep: one training step of the reference's Llama-family model
     (kotodama_amd.lmstep: forward, cross-entropy + z-loss, backward, AdamW step;
     train.py:610-640) with each residual stream in ``residuals``: "standard"
     (x + f(norm(x))), "attnres" (this package's routing kernels) and "torch"
     (the reference's routing ops compiled by inductor, :func:`reference_routing_loop`).
     The dense sublayers are the same torch functions in every variant, compiled
-    by inductor unless ``compiled`` is false.  HIP events split each step into
+    by inductor unless ``compiled`` is false; with ``kernels`` attention and
+    embedding run on this package's kernels instead.  HIP events split each step into
     forward (with the loss), backward and optimizer step."""
     import torch
 
@@ -998,11 +1003,13 @@ def bench_lmstep(steps: int, warmup: int, dev, lm: str, residuals, compiled: boo
     c = lmstep.PRESETS[lm]
     torch.backends.cuda.enable_math_sdp(False)  # SDPA runs a fused kernel or raises
     torch._dynamo.reset()
-    lmstep.compile_sublayers(compiled)
+    lmstep.compile_sublayers(compiled, kernels)
     ids, labels = lmstep.make_batch(c, dev)
     loops = {"standard": "standard", "attnres": "attnres", "torch": reference_routing_loop()}
     out = {"model": c.name, "hidden": c.hidden_size, "layers": c.num_layers, "batch": c.batch, "seq": c.seq,
            "vocab": c.vocab_size, "routing_points": 2 * c.num_layers + 1, "sublayers_compiled": compiled}
+    if kernels:
+        out["lm_kernels"] = True
     for name in residuals:
         residual = loops[name]
         model = lmstep.LanguageModel(c, dev, seed=3)  # every variant starts from the same weights
@@ -1204,7 +1211,8 @@ def main() -> int:
         }), flush=True)
         return 0
     if args.workload == "lmstep":
-        rec = bench_lmstep(args.steps, args.warmup, dev, args.lm, args.residuals.split(","), not args.eager_sublayers)
+        rec = bench_lmstep(args.steps, args.warmup, dev, args.lm, args.residuals.split(","), not args.eager_sublayers,
+                           args.lm_kernels)
         head = rec.get("attnres") or next(rec[k] for k in args.residuals.split(","))
         print(json.dumps({
             "metric": "whole training step tokens/s with AttnRes routing (and the standard residual stream beside it)",

@@ -28,7 +28,11 @@ The dense work (projections, attention, SwiGLU, norms, loss) is torch on ROCm
 (hipBLASLt GEMMs, SDPA's fused attention kernel).  :func:`compile_sublayers`
 compiles those functions with inductor once for every layer (the layers share
 shapes, so one graph serves them all); the routing loop around them stays
-eager, which is where this package's kernels run.
+eager, which is where this package's kernels run.  With its ``kernels`` the
+embedding, the norms and rotation of queries and keys and the attention run
+on this package's kernels too (:mod:`kotodama_amd.lmops`), compiled around or
+not.  :meth:`LanguageModel.logits` runs the model behind a KV cache (prefill
+and single tokens) through the engine's cached loop and those operators.
 """
 
 from __future__ import annotations
@@ -41,7 +45,7 @@ import torch
 import torch.nn.functional as F
 from torch import Tensor, nn
 
-from . import engine
+from . import engine, lmops
 
 
 @dataclass(frozen=True)
@@ -108,6 +112,40 @@ def _attention(x: Tensor, an: Tensor, wq: Tensor, wk: Tensor, wv: Tensor, wo: Te
     return F.linear(o.transpose(1, 2).reshape(b, t, heads * head_dim), wo)
 
 
+def _project(x: Tensor, an: Tensor, wq: Tensor, wk: Tensor, wv: Tensor, heads: int, kv_heads: int, head_dim: int,
+             eps: float) -> tuple:
+    b, t, _ = x.shape
+    x = _rms(x, an, eps)
+    return tuple(F.linear(x, w).view(b, t, n, head_dim).transpose(1, 2)
+                 for w, n in ((wq, heads), (wk, kv_heads), (wv, kv_heads)))
+
+
+def _attention_kernels(x: Tensor, an: Tensor, wq: Tensor, wk: Tensor, wv: Tensor, wo: Tensor, qn: Tensor, kn: Tensor,
+                       cos: Tensor, sin: Tensor, heads: int, kv_heads: int, head_dim: int, eps: float) -> Tensor:
+    """:func:`_attention` with its norms, rotation and attention on this package's kernels."""
+    b, t, _ = x.shape
+    q, k, v = _project(x, an, wq, wk, wv, heads, kv_heads, head_dim, eps)
+    q, k = lmops.qk_norm_rope(q, k, qn, kn, cos, sin, eps)
+    o = lmops.attention(q, k, v)
+    return F.linear(o.transpose(1, 2).reshape(b, t, heads * head_dim), wo)
+
+
+def _attention_cached(x: Tensor, an: Tensor, wq: Tensor, wk: Tensor, wv: Tensor, wo: Tensor, qn: Tensor, kn: Tensor,
+                      cos: Tensor, sin: Tensor, heads: int, kv_heads: int, head_dim: int, eps: float,
+                      past: Optional[tuple]) -> tuple:
+    """The same behind the keys and values of ``past`` (llama.py:384-401): (output, the grown (k, v))."""
+    b, t, _ = x.shape
+    q, k, v = _project(x, an, wq, wk, wv, heads, kv_heads, head_dim, eps)
+    n = 0 if past is None else past[0].shape[2]
+    if n + t > cos.shape[0]:
+        raise ValueError(f"{n + t} tokens, but the model's rope tables have {cos.shape[0]} rows")
+    q, k = lmops.qk_norm_rope(q, k, qn, kn, cos[n:n + t], sin[n:n + t], eps)
+    if past is not None:
+        k, v = torch.cat((past[0], k), 2), torch.cat((past[1], v), 2)
+    o = lmops.attention(q, k, v)
+    return F.linear(o.transpose(1, 2).reshape(b, t, heads * head_dim), wo), (k, v)
+
+
 def _swiglu(x: Tensor, fn: Tensor, wg: Tensor, wu: Tensor, wd: Tensor, eps: float) -> Tensor:
     x = _rms(x, fn, eps)
     return F.linear(F.silu(F.linear(x, wg)) * F.linear(x, wu), wd)
@@ -118,6 +156,21 @@ def _standard_layer(x: Tensor, an: Tensor, wq: Tensor, wk: Tensor, wv: Tensor, w
                     heads: int, kv_heads: int, head_dim: int, eps: float) -> Tensor:
     x = x + _attention(x, an, wq, wk, wv, wo, qn, kn, cos, sin, heads, kv_heads, head_dim, eps)
     return x + _swiglu(x, fn, wg, wu, wd, eps)
+
+
+def _standard_layer_kernels(x: Tensor, an: Tensor, wq: Tensor, wk: Tensor, wv: Tensor, wo: Tensor, qn: Tensor,
+                            kn: Tensor, fn: Tensor, wg: Tensor, wu: Tensor, wd: Tensor, cos: Tensor, sin: Tensor,
+                            heads: int, kv_heads: int, head_dim: int, eps: float) -> Tensor:
+    x = x + _attention_kernels(x, an, wq, wk, wv, wo, qn, kn, cos, sin, heads, kv_heads, head_dim, eps)
+    return x + _swiglu(x, fn, wg, wu, wd, eps)
+
+
+def _embedding(ids: Tensor, table: Tensor) -> Tensor:
+    return F.embedding(ids, table)
+
+
+def _embedding_kernels(ids: Tensor, table: Tensor) -> Tensor:
+    return lmops.embedding(ids, table)
 
 
 def _loss(x: Tensor, fw: Tensor, emb: Tensor, labels: Tensor, eps: float, z_weight: float) -> Tensor:
@@ -131,17 +184,22 @@ def _loss(x: Tensor, fw: Tensor, emb: Tensor, labels: Tensor, eps: float, z_weig
 
 
 _EAGER = {"rms": _rms, "attention": _attention, "swiglu": _swiglu, "standard_layer": _standard_layer,
-          "loss": _loss}
+          "loss": _loss, "embedding": _embedding}
+_KERNELS = {"attention": _attention_kernels, "standard_layer": _standard_layer_kernels,
+            "embedding": _embedding_kernels}
 _FN = dict(_EAGER)
 
 
-def compile_sublayers(enabled: bool = True) -> None:
-    """Run the dense functions compiled by inductor (``enabled``) or eagerly."""
+def compile_sublayers(enabled: bool = True, kernels: bool = False) -> None:
+    """Run the dense functions compiled by inductor (``enabled``) or eagerly, with ``kernels`` the
+    attention and the embedding on this package's kernels."""
+    fns = {**_EAGER, **_KERNELS} if kernels else dict(_EAGER)
     _FN.clear()
     if enabled:
-        _FN.update({k: torch.compile(f, dynamic=False) for k, f in _EAGER.items()})
+        # the embedding is one call outside the layers, as it was: nothing for inductor to fuse with
+        _FN.update({k: f if k == "embedding" else torch.compile(f, dynamic=False) for k, f in fns.items()})
     else:
-        _FN.update(_EAGER)
+        _FN.update(fns)
 
 
 # -------------------------------------------------------------------- modules --
@@ -184,13 +242,17 @@ class _Attention(nn.Module):
         self.q_norm = _Norm(c.head_dim, c.norm_eps, device, dtype)
         self.k_norm = _Norm(c.head_dim, c.norm_eps, device, dtype)
 
-    def forward(self, x: Tensor, rope_cos: Tensor, rope_sin: Tensor, mask: Optional[Tensor] = None) -> Tensor:
+    def forward(self, x: Tensor, rope_cos: Tensor, rope_sin: Tensor, mask: Optional[Tensor] = None,
+                layer_past: Optional[tuple] = None, use_cache: bool = False):
         if mask is not None:
             raise ValueError("the training step runs causal attention without a mask")
         c = self.c
-        return _FN["attention"](x, self.pre_norm.weight, self.wq, self.wk, self.wv, self.wo, self.q_norm.weight,
-                                self.k_norm.weight, rope_cos, rope_sin, c.num_attention_heads, c.num_kv_heads,
-                                c.head_dim, c.norm_eps)
+        args = (x, self.pre_norm.weight, self.wq, self.wk, self.wv, self.wo, self.q_norm.weight, self.k_norm.weight,
+                rope_cos, rope_sin, c.num_attention_heads, c.num_kv_heads, c.head_dim, c.norm_eps)
+        if use_cache or layer_past is not None:
+            out, kv = _attention_cached(*args, layer_past)
+            return (out, kv) if use_cache else out
+        return _FN["attention"](*args)
 
 
 class _SwiGLU(nn.Module):
@@ -278,7 +340,7 @@ class LanguageModel(nn.Module):
         """The last layer's output before the final norm.  ``residual`` is
         "standard", "attnres", or a caller loop ``fn(model, embed)`` in the
         form of llama.py:666-716."""
-        x = F.embedding(input_ids, self.embed)
+        x = _FN["embedding"](input_ids, self.embed)
         if residual == "standard":
             for layer in self.layers:
                 x = layer.standard(x, self.rope_cos, self.rope_sin)
@@ -293,6 +355,16 @@ class LanguageModel(nn.Module):
         x = self.hidden_states(input_ids, residual)
         c = self.config
         return _FN["loss"](x, self.norm.weight, self.embed, labels, c.norm_eps, c.z_loss_weight)
+
+
+    @torch.no_grad()
+    def logits(self, input_ids: Tensor, past_kv: Optional[list] = None) -> tuple[Tensor, list]:
+        """Logits of ``input_ids`` behind the cached keys and values of ``past_kv`` (None: a new
+        sequence), and the grown cache: the prefill and each decode step of llama.py:718-763 with
+        the AttnRes stream, on this package's kernels."""
+        x = lmops.embedding(input_ids, self.embed)
+        x, past_kv = engine.forward_attn_res_cached(self, x, None, past_kv)
+        return F.linear(_rms(x, self.norm.weight, self.config.norm_eps), self.embed), past_kv
 
 
 def make_batch(c: LMConfig, device, seed: int = 1) -> tuple[Tensor, Tensor]:
