@@ -199,7 +199,8 @@ int forward_workspace(int batch, int heads, int kv_heads, int64_t q_len, int64_t
 
 constexpr int kRopeMaxDim = 256;
 constexpr int kRopeThreads = 256;
-constexpr int kRopeBwdPerCu = 2;
+constexpr int kRopeBwdPerCu = 4;    // workgroups of the backward
+constexpr int kRopeMaxChunks = 64;  // head rows of its grid, for queries and for keys
 
 int rope_lanes(int half, int v) {
   int n = (half + v - 1) / v, g = 1;
@@ -216,8 +217,9 @@ int fill_rope(lm_rope_params* P, const void* q, const int64_t* q_strides, const 
   if (!valid_dtype(dtype)) return fail(ATTNRES_ERR_ARG, "qk_norm_rope: bad dtype %d", dtype);
   if (table_dtype != dtype && table_dtype != ATTNRES_DTYPE_F32)
     return fail(ATTNRES_ERR_ARG, "qk_norm_rope: the tables' dtype must be the rows' or fp32");
-  if (batch < 0 || q_heads < 0 || k_heads < 0 || tokens < 0 || tokens > kMaxLen)
-    return fail(ATTNRES_ERR_ARG, "qk_norm_rope: bad sizes");
+  if (batch < 0 || q_heads < 0 || k_heads < 0 || tokens < 0) return fail(ATTNRES_ERR_ARG, "qk_norm_rope: bad sizes");
+  if (tokens > kMaxLen || tokens * batch > kMaxLen || q_heads > (1 << 15) || k_heads > (1 << 15))
+    return fail(ATTNRES_ERR_UNSUPPORTED, "qk_norm_rope: over 2^30 tokens, or over 2^15 heads");
   if (head_dim < 2 || head_dim > kRopeMaxDim || head_dim % 2 != 0)
     return fail(ATTNRES_ERR_UNSUPPORTED, "qk_norm_rope: head_dim %d is not even and at most %d", head_dim, kRopeMaxDim);
   if (!std::isfinite(eps) || eps < 0) return fail(ATTNRES_ERR_ARG, "qk_norm_rope: bad eps");
@@ -493,15 +495,14 @@ int attnres_qk_norm_rope_fwd(const void* q, const int64_t* q_strides, const void
   // Four heads of a token per lane group share its table rows and keep more
   // reads in flight; with too few rows to fill the card that way, one.
   const int64_t n = (int64_t)batch * tokens;
-  const int64_t rows4 = n * ((q_heads + 3) / 4 + (k_heads + 3) / 4);
-  const bool h4 = rows4 * P.lanes >= (int64_t)cus * 1024;
-  const int64_t items = h4 ? rows4 : n * (q_heads + k_heads);
-  const int64_t grid = (items * P.lanes + kRopeThreads - 1) / kRopeThreads;
-  if (grid > INT32_MAX) return fail(ATTNRES_ERR_UNSUPPORTED, "qk_norm_rope: too many rows for one call");
+  const int rows4 = (q_heads + 3) / 4 + (k_heads + 3) / 4;
+  const bool h4 = n * rows4 * P.lanes >= (int64_t)cus * 256;
+  const int groups = kRopeThreads / P.lanes;
+  const int64_t grid = (n + groups - 1) / groups;
   char name[64];
   snprintf(name, sizeof(name), "attnres_qk_norm_rope_%s_h%d", rope_kind(f32, vec), h4 ? 4 : 1);
-  return launch(kRopeFwd + (f32 ? 4 : 0) + (vec ? 0 : 2) + (h4 ? 1 : 0), kLmPart, name, (unsigned)grid, 1,
-                kRopeThreads, 0, P, stream);
+  return launch(kRopeFwd + (f32 ? 4 : 0) + (vec ? 0 : 2) + (h4 ? 1 : 0), kLmPart, name, (unsigned)grid,
+                (unsigned)(h4 ? rows4 : q_heads + k_heads), kRopeThreads, 0, P, stream);
 }
 
 int attnres_qk_norm_rope_workspace_size(int head_dim, int64_t* bytes) {
@@ -510,7 +511,7 @@ int attnres_qk_norm_rope_workspace_size(int head_dim, int64_t* bytes) {
   int cus = 0;
   int rc = attnres_internal_num_cus(&cus);
   if (rc != ATTNRES_OK) return rc;
-  *bytes = (int64_t)2 * kRopeBwdPerCu * cus * head_dim * 4;
+  *bytes = ((int64_t)kRopeBwdPerCu * cus + 2 * kRopeMaxChunks) * head_dim * 4;
   return ATTNRES_OK;
 }
 
@@ -556,15 +557,20 @@ int attnres_qk_norm_rope_bwd(const void* q, const int64_t* q_strides, const void
     int cus = 0;
     if ((rc = attnres_internal_num_cus(&cus)) != ATTNRES_OK) return rc;
     const int groups = kRopeThreads / P.lanes;
-    const int heads = q_heads > k_heads ? q_heads : k_heads;
-    int64_t parts = ((int64_t)batch * tokens * ((heads + 1) / 2) + groups - 1) / groups;
-    if (parts > (int64_t)kRopeBwdPerCu * cus) parts = (int64_t)kRopeBwdPerCu * cus;
+    // rows of 4 heads (2 at a time), more where there would be too many rows
+    int chunk = 4;
+    while ((q_heads + chunk - 1) / chunk > kRopeMaxChunks || (k_heads + chunk - 1) / chunk > kRopeMaxChunks) chunk *= 2;
+    P.chunk = chunk;
+    P.q_chunks = (q_heads + chunk - 1) / chunk;
+    P.chunks = P.q_chunks + (k_heads + chunk - 1) / chunk;
+    int64_t parts = ((int64_t)batch * tokens + groups - 1) / groups, most = (int64_t)kRopeBwdPerCu * cus / P.chunks;
+    if (parts > most) parts = most > 0 ? most : 1;
     P.parts = (int)parts;
-    const int64_t need = 2 * parts * head_dim * 4;
+    const int64_t need = parts * P.chunks * head_dim * 4;
     if (workspace == nullptr || workspace_bytes < need)
       return fail(ATTNRES_ERR_ARG, "qk_norm_rope: workspace of %lld bytes needed", (long long)need);
     snprintf(name, sizeof(name), "attnres_qk_norm_rope_bwd_%s", rope_kind(f32, vec));
-    rc = launch(kRopeBwd + (f32 ? 2 : 0) + (vec ? 0 : 1), kLmPart, name, (unsigned)parts, 2, kRopeThreads,
+    rc = launch(kRopeBwd + (f32 ? 2 : 0) + (vec ? 0 : 1), kLmPart, name, (unsigned)parts, (unsigned)P.chunks, kRopeThreads,
                 (unsigned)(groups * head_dim * 4), P, stream);
     if (rc != ATTNRES_OK) return rc;
   }

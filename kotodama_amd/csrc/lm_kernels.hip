@@ -103,104 +103,120 @@ __device__ __forceinline__ float group_sum(float v, int g) {
 // each half, so the rotation needs nothing from other lanes and the mean is a
 // sum over the group.  Bound by memory: one read and one write of a row.
 
+// Lanes past the half (a group is a power of two) repeat its first elements,
+// so that no load has a branch, and count for nothing.
+template <typename T, int V, int C>
+struct Half {
+  int d[C];    // this lane's elements of each half
+  bool in[C];  // they exist
+  __device__ __forceinline__ Half(int half, int l, int g) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      d[c] = (c * g + l) * V;
+      in[c] = d[c] < half;
+      d[c] = in[c] ? d[c] : 0;
+    }
+  }
+  __device__ __forceinline__ void read(const void* base, int64_t at, int half, float (&lo)[C][V],
+                                       float (&hi)[C][V]) const {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      load<T, V>(base, at + d[c], lo[c]);
+      load<T, V>(base, at + half + d[c], hi[c]);
+    }
+  }
+  __device__ __forceinline__ void write(void* base, int64_t at, int half, int c, const float (&lo)[V],
+                                        const float (&hi)[V]) const {
+    if (!in[c]) return;
+    store<T, V>(base, at + d[c], lo);
+    store<T, V>(base, at + half + d[c], hi);
+  }
+};
+
+// cos and sin of a token: the tables' row, or NaN outside them.
 template <typename T, int V, int C>
 struct Rope {
   float clo[C][V], chi[C][V], slo[C][V], shi[C][V];
-};
-
-template <typename T, int V, int C>
-__device__ __forceinline__ void load_table(const lm_rope_params& P, int64_t pos, int l, int g, Rope<T, V, C>& R) {
-  const int half = P.dim >> 1;
-  const bool ok = pos >= 0 && pos < P.table_rows;
+  __device__ __forceinline__ void read(const lm_rope_params& P, int64_t pos, const Half<T, V, C>& H) {
+    const int half = P.dim >> 1;
+    if (pos < 0 || pos >= P.table_rows) {
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const int d = (c * g + l) * V;
-    const bool in = ok && d < half;
+      for (int c = 0; c < C; ++c)
 #pragma unroll
-    for (int j = 0; j < V; ++j) R.clo[c][j] = R.chi[c][j] = R.slo[c][j] = R.shi[c][j] = kNan;
-    if (in) {
-      const int64_t ac = pos * P.cos_ld + d, as = pos * P.sin_ld + d;
-      if (P.table_f32) {
+        for (int j = 0; j < V; ++j) clo[c][j] = chi[c][j] = slo[c][j] = shi[c][j] = kNan;
+      return;
+    }
+    const int64_t ac = pos * P.cos_ld, as = pos * P.sin_ld;
+    if (P.table_f32) {
+#pragma unroll
+      for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          R.clo[c][j] = ((const float*)P.cos)[ac + j];
-          R.chi[c][j] = ((const float*)P.cos)[ac + half + j];
-          R.slo[c][j] = ((const float*)P.sin)[as + j];
-          R.shi[c][j] = ((const float*)P.sin)[as + half + j];
+          clo[c][j] = ((const float*)P.cos)[ac + H.d[c] + j];
+          chi[c][j] = ((const float*)P.cos)[ac + half + H.d[c] + j];
+          slo[c][j] = ((const float*)P.sin)[as + H.d[c] + j];
+          shi[c][j] = ((const float*)P.sin)[as + half + H.d[c] + j];
         }
-      } else {
-        load<T, V>(P.cos, ac, R.clo[c]);
-        load<T, V>(P.cos, ac + half, R.chi[c]);
-        load<T, V>(P.sin, as, R.slo[c]);
-        load<T, V>(P.sin, as + half, R.shi[c]);
-      }
+    } else {
+      H.read(P.cos, ac, half, clo, chi);
+      H.read(P.sin, as, half, slo, shi);
     }
   }
-}
+};
 
-template <typename T, int V, int C>
-__device__ __forceinline__ void load_halves(const void* base, int64_t at, int half, int l, int g, bool live,
-                                            float (&lo)[C][V], float (&hi)[C][V]) {
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const int d = (c * g + l) * V;
-#pragma unroll
-    for (int j = 0; j < V; ++j) lo[c][j] = hi[c][j] = 0.f;
-    if (live && d < half) {
-      load<T, V>(base, at + d, lo[c]);
-      load<T, V>(base, at + half + d, hi[c]);
-    }
+// Token n of the call as (sequence, token of it), and the position it is rotated by.
+struct Token {
+  uint32_t b, t;
+  int64_t pos;
+  __device__ __forceinline__ Token(const lm_rope_params& P, uint32_t n) {
+    b = P.tokens == 1 ? n : n / (uint32_t)P.tokens;
+    t = n - b * (uint32_t)P.tokens;
+    pos = P.positions == nullptr ? (int64_t)t : index_at(P.positions, b * P.pos_b + t * P.pos_t, P.pos64);
   }
-}
+};
 
-__device__ __forceinline__ int64_t token_position(const lm_rope_params& P, int64_t b, int64_t t) {
-  return P.positions == nullptr ? t : index_at(P.positions, b * P.pos_b + t * P.pos_t, P.pos64);
-}
-
-// HPG heads of one token per lane group.
+// blockIdx.y: HPG heads of the queries, then of the keys; a lane group takes them for one token.
 template <typename T, int V, int C, int HPG>
 __device__ __forceinline__ void qk_norm_rope_fwd(const lm_rope_params& P) {
   const int g = P.lanes, l = threadIdx.x & (g - 1);
-  const int64_t item = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / g;
-  const int qc = (P.heads[0] + HPG - 1) / HPG, kc = (P.heads[1] + HPG - 1) / HPG;
-  if (item >= (int64_t)P.batch * P.tokens * (qc + kc)) return;
-  const int64_t n = item / (qc + kc);
-  const int part = (int)(item - n * (qc + kc));
-  const int x = part < qc ? 0 : 1;
-  const int h0 = (x ? part - qc : part) * HPG;
-  const int64_t b = n / P.tokens, t = n - b * P.tokens;
+  const uint32_t n = blockIdx.x * (blockDim.x / g) + threadIdx.x / g;
+  if (n >= (uint32_t)P.batch * (uint32_t)P.tokens) return;
+  const int qc = (P.heads[0] + HPG - 1) / HPG;
+  const int x = (int)blockIdx.y < qc ? 0 : 1;
+  const int h0 = ((int)blockIdx.y - (x ? qc : 0)) * HPG;
   const int half = P.dim >> 1;
-  const void* src = x ? P.x[1] : P.x[0];
-  void* dst = x ? P.y[1] : P.y[0];
-  const void* wp = x ? P.w[1] : P.w[0];
   const lm_strides sx = x ? P.sx[1] : P.sx[0], sy = x ? P.sy[1] : P.sy[0];
   const int heads = x ? P.heads[1] : P.heads[0];
+  const void* src = x ? P.x[1] : P.x[0];
+  void* dst = x ? P.y[1] : P.y[0];
+  const Token tok(P, n);
+  const Half<T, V, C> H(half, l, g);
+  const int64_t at = tok.b * sx.b + tok.t * sx.t, to = tok.b * sy.b + tok.t * sy.t;
 
-  float lo[HPG][C][V], hi[HPG][C][V];
+  float lo[HPG][C][V], hi[HPG][C][V], wlo[C][V], whi[C][V];
 #pragma unroll
-  for (int i = 0; i < HPG; ++i)
-    load_halves<T, V, C>(src, b * sx.b + (int64_t)(h0 + i) * sx.h + t * sx.t, half, l, g, h0 + i < heads, lo[i], hi[i]);
-  float wlo[C][V], whi[C][V];
-  load_halves<T, V, C>(wp, 0, half, l, g, true, wlo, whi);
+  for (int i = 0; i < HPG; ++i)  // heads past the last repeat it
+    H.read(src, at + (int64_t)(h0 + i < heads ? h0 + i : heads - 1) * sx.h, half, lo[i], hi[i]);
   Rope<T, V, C> R;
-  load_table<T, V, C>(P, token_position(P, b, t), l, g, R);
+  R.read(P, tok.pos, H);
+  H.read(x ? P.w[1] : P.w[0], 0, half, wlo, whi);
 #pragma unroll
   for (int i = 0; i < HPG; ++i) {
     float ss = 0.f;
 #pragma unroll
-    for (int c = 0; c < C; ++c)
+    for (int c = 0; c < C; ++c) {
+      float s = 0.f;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        ss = __builtin_fmaf(lo[i][c][j], lo[i][c][j], ss);
-        ss = __builtin_fmaf(hi[i][c][j], hi[i][c][j], ss);
+        s = __builtin_fmaf(lo[i][c][j], lo[i][c][j], s);
+        s = __builtin_fmaf(hi[i][c][j], hi[i][c][j], s);
       }
+      ss += H.in[c] ? s : 0.f;
+    }
     const float r = __builtin_amdgcn_rsqf(group_sum(ss, g) * P.inv_dim + P.eps);
-    if (h0 + i >= heads) continue;
-    const int64_t at = b * sy.b + (int64_t)(h0 + i) * sy.h + t * sy.t;
+    if (h0 + i >= heads) break;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const int d = (c * g + l) * V;
-      if (d >= half) continue;
       float ylo[V], yhi[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) {
@@ -208,100 +224,98 @@ __device__ __forceinline__ void qk_norm_rope_fwd(const lm_rope_params& P) {
         ylo[j] = a * R.clo[c][j] - e * R.slo[c][j];
         yhi[j] = e * R.chi[c][j] + a * R.shi[c][j];
       }
-      store<T, V>(dst, at + d, ylo);
-      store<T, V>(dst, at + half + d, yhi);
+      H.write(dst, to + (int64_t)(h0 + i) * sy.h, half, c, ylo, yhi);
     }
   }
 }
 
-// blockIdx.y: queries or keys.  The lane groups of the grid walk over (token,
-// HPG heads) items; each lane keeps its columns' weight gradient, the
+// blockIdx.y: P.chunk heads of the queries, then of the keys; the lane groups
+// walk over the tokens.  Each lane keeps its columns' weight gradient; the
 // workgroup adds its groups' in a fixed order and writes one row of partials.
 template <typename T, int V, int C, int HPG>
 __device__ __forceinline__ void qk_norm_rope_bwd(const lm_rope_params& P, float* red) {
   const int g = P.lanes, l = threadIdx.x & (g - 1);
-  const int x = blockIdx.y;
+  const int x = (int)blockIdx.y < P.q_chunks ? 0 : 1;
   const int half = P.dim >> 1;
+  const lm_strides sx = x ? P.sx[1] : P.sx[0], sy = x ? P.sy[1] : P.sy[0], sg = x ? P.sg[1] : P.sg[0];
   const void* src = x ? P.x[1] : P.x[0];
   const void* gsrc = x ? P.g[1] : P.g[0];
   void* dst = x ? P.y[1] : P.y[0];
-  const void* wp = x ? P.w[1] : P.w[0];
-  const lm_strides sx = x ? P.sx[1] : P.sx[0], sy = x ? P.sy[1] : P.sy[0], sg = x ? P.sg[1] : P.sg[0];
   const int heads = x ? P.heads[1] : P.heads[0];
-  const int hc = (heads + HPG - 1) / HPG;
-  const int64_t items = (int64_t)P.batch * P.tokens * hc;
+  const int first = ((int)blockIdx.y - (x ? P.q_chunks : 0)) * P.chunk;
+  const int end = first + P.chunk < heads ? first + P.chunk : heads;
   const int groups = blockDim.x / g, grp = threadIdx.x / g;
+  const uint32_t tokens = (uint32_t)P.batch * (uint32_t)P.tokens;
+  const Half<T, V, C> H(half, l, g);
   float wlo[C][V], whi[C][V], dwlo[C][V], dwhi[C][V];
-  load_halves<T, V, C>(wp, 0, half, l, g, true, wlo, whi);
+  H.read(x ? P.w[1] : P.w[0], 0, half, wlo, whi);
 #pragma unroll
   for (int c = 0; c < C; ++c)
 #pragma unroll
     for (int j = 0; j < V; ++j) dwlo[c][j] = dwhi[c][j] = 0.f;
-  for (int64_t item = (int64_t)blockIdx.x * groups + grp; item < items; item += (int64_t)gridDim.x * groups) {
-    const int64_t n = item / hc;
-    const int h0 = (int)(item - n * hc) * HPG;
-    const int64_t b = n / P.tokens, t = n - b * P.tokens;
-    float lo[HPG][C][V], hi[HPG][C][V], glo[HPG][C][V], ghi[HPG][C][V];
-#pragma unroll
-    for (int i = 0; i < HPG; ++i) {
-      const bool live = h0 + i < heads;
-      load_halves<T, V, C>(src, b * sx.b + (int64_t)(h0 + i) * sx.h + t * sx.t, half, l, g, live, lo[i], hi[i]);
-      load_halves<T, V, C>(gsrc, b * sg.b + (int64_t)(h0 + i) * sg.h + t * sg.t, half, l, g, live, glo[i], ghi[i]);
-    }
+  for (uint32_t n = blockIdx.x * groups + grp; n < tokens; n += gridDim.x * groups) {
+    const Token tok(P, n);
+    const int64_t ax = tok.b * sx.b + tok.t * sx.t, ag = tok.b * sg.b + tok.t * sg.t, ay = tok.b * sy.b + tok.t * sy.t;
     Rope<T, V, C> R;
-    load_table<T, V, C>(P, token_position(P, b, t), l, g, R);
+    for (int h0 = first; h0 < end; h0 += HPG) {
+      float lo[HPG][C][V], hi[HPG][C][V], glo[HPG][C][V], ghi[HPG][C][V];
 #pragma unroll
-    for (int i = 0; i < HPG; ++i) {
-      float ss = 0.f, mx = 0.f;
-#pragma unroll
-      for (int c = 0; c < C; ++c) {
-        const bool in = (c * g + l) * V < half;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float a = lo[i][c][j], e = hi[i][c][j];
-          ss = __builtin_fmaf(a, a, ss);
-          ss = __builtin_fmaf(e, e, ss);
-          const float da = in ? glo[i][c][j] * R.clo[c][j] + ghi[i][c][j] * R.shi[c][j] : 0.f;
-          const float de = in ? ghi[i][c][j] * R.chi[c][j] - glo[i][c][j] * R.slo[c][j] : 0.f;
-          glo[i][c][j] = da;
-          ghi[i][c][j] = de;
-          mx = __builtin_fmaf(da * wlo[c][j], a, mx);
-          mx = __builtin_fmaf(de * whi[c][j], e, mx);
-        }
+      for (int i = 0; i < HPG; ++i) {
+        const int64_t h = h0 + i < end ? h0 + i : end - 1;
+        H.read(src, ax + h * sx.h, half, lo[i], hi[i]);
+        H.read(gsrc, ag + h * sg.h, half, glo[i], ghi[i]);
       }
-      ss = group_sum(ss, g);
-      mx = group_sum(mx, g);
-      const float r = __builtin_amdgcn_rsqf(ss * P.inv_dim + P.eps);
-      const float k = r * r * mx * P.inv_dim;
-      if (h0 + i >= heads) continue;
-      const int64_t at = b * sy.b + (int64_t)(h0 + i) * sy.h + t * sy.t;
+      if (h0 == first) R.read(P, tok.pos, H);
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        const int d = (c * g + l) * V;
-        if (d >= half) continue;
-        float olo[V], ohi[V];
+      for (int i = 0; i < HPG; ++i) {
+        float ss = 0.f, mx = 0.f;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float a = lo[i][c][j], e = hi[i][c][j], da = glo[i][c][j], de = ghi[i][c][j];
-          olo[j] = r * (wlo[c][j] * da - a * k);
-          ohi[j] = r * (whi[c][j] * de - e * k);
-          dwlo[c][j] = __builtin_fmaf(da * a, r, dwlo[c][j]);
-          dwhi[c][j] = __builtin_fmaf(de * e, r, dwhi[c][j]);
+        for (int c = 0; c < C; ++c) {
+          float s = 0.f, m = 0.f;
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const float a = lo[i][c][j], e = hi[i][c][j];
+            s = __builtin_fmaf(a, a, s);
+            s = __builtin_fmaf(e, e, s);
+            const float da = glo[i][c][j] * R.clo[c][j] + ghi[i][c][j] * R.shi[c][j];
+            const float de = ghi[i][c][j] * R.chi[c][j] - glo[i][c][j] * R.slo[c][j];
+            glo[i][c][j] = da;
+            ghi[i][c][j] = de;
+            m = __builtin_fmaf(da * wlo[c][j], a, m);
+            m = __builtin_fmaf(de * whi[c][j], e, m);
+          }
+          ss += H.in[c] ? s : 0.f;
+          mx += H.in[c] ? m : 0.f;
         }
-        store<T, V>(dst, at + d, olo);
-        store<T, V>(dst, at + half + d, ohi);
+        ss = group_sum(ss, g);
+        mx = group_sum(mx, g);
+        const float r = __builtin_amdgcn_rsqf(ss * P.inv_dim + P.eps);
+        const float k = r * r * mx * P.inv_dim;
+        if (h0 + i >= end) break;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          float olo[V], ohi[V];
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const float a = lo[i][c][j], e = hi[i][c][j], da = glo[i][c][j], de = ghi[i][c][j];
+            olo[j] = r * (wlo[c][j] * da - a * k);
+            ohi[j] = r * (whi[c][j] * de - e * k);
+            dwlo[c][j] = __builtin_fmaf(da * a, r, dwlo[c][j]);
+            dwhi[c][j] = __builtin_fmaf(de * e, r, dwhi[c][j]);
+          }
+          H.write(dst, ay + (int64_t)(h0 + i) * sy.h, half, c, olo, ohi);
+        }
       }
     }
   }
-  // the workgroup's weight gradient, one column after another, groups in order
+  // the workgroup's weight gradient: groups in order
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    const int d = (c * g + l) * V;
-    if (d < half) {
+    if (H.in[c]) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        red[grp * P.dim + d + j] = dwlo[c][j];
-        red[grp * P.dim + half + d + j] = dwhi[c][j];
+        red[grp * P.dim + H.d[c] + j] = dwlo[c][j];
+        red[grp * P.dim + half + H.d[c] + j] = dwhi[c][j];
       }
     }
   }
@@ -309,21 +323,21 @@ __device__ __forceinline__ void qk_norm_rope_bwd(const lm_rope_params& P, float*
   for (int d = threadIdx.x; d < P.dim; d += blockDim.x) {
     float s = 0.f;
     for (int i = 0; i < groups; ++i) s += red[i * P.dim + d];
-    P.dw_part[((int64_t)x * gridDim.x + blockIdx.x) * P.dim + d] = s;
+    P.dw_part[((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * P.dim + d] = s;
   }
 }
 
-// Sums the partial rows: workgroup (column block, queries or keys) of 32
-// columns x 8 row strides, added in a fixed order.
+// Sums the partial rows: workgroup (32 columns, queries or keys), 32 row
+// strides, added in a fixed order.
 template <typename T>
 __device__ __forceinline__ void rope_dw_sum(const lm_rope_params& P, float* red) {
   const int x = blockIdx.y, col = threadIdx.x & 31, str = threadIdx.x >> 5;
   const int d = blockIdx.x * 32 + col;
+  const int first = x ? P.parts * P.q_chunks : 0, end = P.parts * (x ? P.chunks : P.q_chunks);
   float s = 0.f;
   if (d < P.dim) {
-    const float* p = P.dw_part + (int64_t)x * P.parts * P.dim + d;
-#pragma unroll 4
-    for (int i = str; i < P.parts; i += 32) s += p[(int64_t)i * P.dim];
+#pragma unroll 8
+    for (int i = first + str; i < end; i += 32) s += P.dw_part[(int64_t)i * P.dim + d];
   }
   red[str * 33 + col] = s;
   __syncthreads();

@@ -73,7 +73,7 @@ typedef struct lm_rope_params {
   void* y[2];        /* outputs; backward: dL/dx */
   const void* w[2];
   void* dw[2];       /* weight gradients */
-  float* dw_part;    /* (2, parts, dim) */
+  float* dw_part;    /* (chunks, parts, dim) */
   const void* cos;   /* (table_rows, dim), rows cos_ld apart, x's type or (table_f32) fp32 */
   const void* sin;
   const void* positions;
@@ -86,7 +86,10 @@ typedef struct lm_rope_params {
   int32_t heads[2];
   int32_t dim;
   int32_t lanes;     /* lanes per head row (a power of two) */
-  int32_t parts;
+  int32_t chunk;     /* backward: heads per workgroup row, */
+  int32_t q_chunks;  /* rows of the queries, */
+  int32_t chunks;    /* rows in all, */
+  int32_t parts;     /* workgroups per row */
   int32_t table_f32;
   int32_t pos64;
   float eps;
