@@ -55,6 +55,7 @@ namespace {
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kNegInf = -__builtin_inff();
+constexpr int kExactKeys = 256;  // rows of up to so many keys: delta from the probabilities (attention_bwd_dq)
 
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   bf16x2 r = {(__bf16)lo, (__bf16)hi};
@@ -260,10 +261,10 @@ struct Tile {
 
 // A global row as B operands: elements 16 step + 8h .. + 7; zero past `dim` or
 // where the row does not exist.
-template <typename T, int DP>
-__device__ __forceinline__ void load_rows(typename T::Frag (&f)[DP / 16], const char* row, int dim, int h, bool live) {
+template <typename T, int DC>
+__device__ __forceinline__ void load_rows(typename T::Frag (&f)[DC / 16], const char* row, int dim, int h, bool live) {
 #pragma unroll
-  for (int s = 0; s < DP / 16; ++s) {
+  for (int s = 0; s < DC / 16; ++s) {
     const int d = 16 * s + 8 * h;
     f[s] = (live && d < dim) ? T::load(row + d * T::kBytes) : T::zero();
   }
@@ -279,12 +280,12 @@ __device__ __forceinline__ void store4(char* p, float a, float b, float c, float
   }
 }
 
-// A wave's 32 rows x DP result held as its transpose (lane: row lane % 32,
+// A wave's 32 rows x DC result held as its transpose (lane: row lane % 32,
 // registers: columns), scaled and stored; only columns under dim.
-template <typename T, int DP>
-__device__ __forceinline__ void store_rows(char* row, const f32x16 (&acc)[DP / 32], float scale, int dim, int h) {
+template <typename T, int DC>
+__device__ __forceinline__ void store_rows(char* row, const f32x16 (&acc)[DC / 32], float scale, int dim, int h) {
 #pragma unroll
-  for (int dt = 0; dt < DP / 32; ++dt) {
+  for (int dt = 0; dt < DC / 32; ++dt) {
 #pragma unroll
     for (int a = 0; a < 4; ++a) {
       const int d = 32 * dt + 8 * a + 4 * h;
@@ -501,18 +502,18 @@ __device__ __forceinline__ void over_keys(const char* kp, int64_t kst, const cha
 }
 
 // The waves that share rows or keys add their results: part 0 receives.  `x`
-// holds 64 lanes x DP/2 floats per pair; every wave of the workgroup calls this.
-template <int DP>
-__device__ __forceinline__ void put(float* x, const f32x16 (&acc)[DP / 32], int lane) {
+// holds 64 lanes x DC/2 floats per pair; every wave of the workgroup calls this.
+template <int DC>
+__device__ __forceinline__ void put(float* x, const f32x16 (&acc)[DC / 32], int lane) {
 #pragma unroll
-  for (int dt = 0; dt < DP / 32; ++dt)
+  for (int dt = 0; dt < DC / 32; ++dt)
 #pragma unroll
     for (int i = 0; i < 16; ++i) x[(dt * 16 + i) * 64 + lane] = acc[dt][i];
 }
-template <int DP>
-__device__ __forceinline__ void add(const float* x, f32x16 (&acc)[DP / 32], int lane, float mine, float theirs) {
+template <int DC>
+__device__ __forceinline__ void add(const float* x, f32x16 (&acc)[DC / 32], int lane, float mine, float theirs) {
 #pragma unroll
-  for (int dt = 0; dt < DP / 32; ++dt)
+  for (int dt = 0; dt < DC / 32; ++dt)
 #pragma unroll
     for (int i = 0; i < 16; ++i)
       acc[dt][i] = __builtin_fmaf(x[(dt * 16 + i) * 64 + lane], theirs, acc[dt][i] * mine);
@@ -520,7 +521,7 @@ __device__ __forceinline__ void add(const float* x, f32x16 (&acc)[DP / 32], int 
 
 // --------------------------------------------------------------- forward --
 
-template <typename T, int DP, int KS, int NBUF>
+template <typename T, int DP, int DC, int KS, int NBUF>
 __device__ __forceinline__ void attention_fwd(const lm_attn_params& P, char* k0, char* k1, char* v0, char* v1,
                                               float* ml) {
   using RW = Rows<KS>;
@@ -532,11 +533,11 @@ __device__ __forceinline__ void attention_fwd(const lm_attn_params& P, char* k0,
   const char* kp = (const char*)P.k + ((int64_t)R.b * P.sk.b + (int64_t)R.kvh * P.sk.h) * T::kBytes;
   const char* vp = (const char*)P.v + ((int64_t)R.b * P.sv.b + (int64_t)R.kvh * P.sv.h) * T::kBytes;
 
-  typename T::Frag qf[DP / 16];
-  load_rows<T, DP>(qf, (const char*)P.q + row_offset(P.sq, R.b, R.head, R.query) * T::kBytes, P.dim, h, R.live);
-  f32x16 acc[DP / 32];
+  typename T::Frag qf[DC / 16];
+  load_rows<T, DC>(qf, (const char*)P.q + row_offset(P.sq, R.b, R.head, R.query) * T::kBytes, P.dim, h, R.live);
+  f32x16 acc[DC / 32];
 #pragma unroll
-  for (int i = 0; i < DP / 32; ++i) acc[i] = zero16();
+  for (int i = 0; i < DC / 32; ++i) acc[i] = zero16();
   float m = kNegInf, l = 0.f;  // reference maximum (of scores times log2 e) and this lane's part of the sum
   const int row_at = KT::row_at(lane), col_at = KT::col_at(lane);
 
@@ -553,10 +554,10 @@ __device__ __forceinline__ void attention_fwd(const lm_attn_params& P, char* k0,
         for (int kb = 0; kb < NB; ++kb) {
           s[kb] = zero16();
 #pragma unroll
-          for (int st = 0; st < DP / 16; ++st)
+          for (int st = 0; st < DC / 16; ++st)
             s[kb] = T::mma(KT::row_frag(kc, first + 32 * kb, st, row_at), qf[st], s[kb]);
         }
-        if constexpr (T::kBytes == 2) interleave<4, NB * DP / 16, 1, 0, 0>();
+        if constexpr (T::kBytes == 2) interleave<4, NB * DC / 16, 1, 0, 0>();
         __builtin_amdgcn_s_setprio(0);
         if (key0 + 32 * NB > R.mine.all) {
 #pragma unroll
@@ -582,7 +583,7 @@ __device__ __forceinline__ void attention_fwd(const lm_attn_params& P, char* k0,
           m = mn;
           l *= fade;
 #pragma unroll
-          for (int dt = 0; dt < DP / 32; ++dt)
+          for (int dt = 0; dt < DC / 32; ++dt)
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[dt][i] *= fade;
         }
@@ -600,10 +601,10 @@ __device__ __forceinline__ void attention_fwd(const lm_attn_params& P, char* k0,
           for (int st = 0; st < 2; ++st) {
             const typename T::Frag p = T::from_acc(s[kb], st);
 #pragma unroll
-            for (int dt = 0; dt < DP / 32; ++dt)
+            for (int dt = 0; dt < DC / 32; ++dt)
               acc[dt] = T::mma(KT::col_frag(vc, first + 32 * kb + 16 * st, dt, col_at, lane), p, acc[dt]);
           }
-        if constexpr (T::kBytes == 2) interleave<8, NB * DP / 16, 2, (NB == 2 ? DP / 16 : 0), 7>();
+        if constexpr (T::kBytes == 2) interleave<8, NB * DC / 16, 2, (NB == 2 ? DC / 16 : 0), 7>();
       });
 
   l += other_half(l);
@@ -615,7 +616,7 @@ __device__ __forceinline__ void attention_fwd(const lm_attn_params& P, char* k0,
     for (int o = 1; o < KS; ++o) {
       __syncthreads();
       if (R.part == o) {
-        put<DP>(x, acc, lane);
+        put<DC>(x, acc, lane);
         xm[lane] = m;
         xm[64 + lane] = l;
       }
@@ -624,7 +625,7 @@ __device__ __forceinline__ void attention_fwd(const lm_attn_params& P, char* k0,
         const float om = xm[lane], ol = xm[64 + lane];
         const float mn = fmaxf(m, om);
         const float a = m == kNegInf ? 0.f : exp2_fast(m - mn), c = om == kNegInf ? 0.f : exp2_fast(om - mn);
-        add<DP>(x, acc, lane, a, c);
+        add<DC>(x, acc, lane, a, c);
         l = l * a + ol * c;
         m = mn;
       }
@@ -635,7 +636,7 @@ __device__ __forceinline__ void attention_fwd(const lm_attn_params& P, char* k0,
     if (P.splits > 1) {  // this part's sums as they stand, for the join
       if (!R.exists) return;
       const int64_t at = R.index(P) * P.splits + R.split;
-      if (l > 0.f) store_rows<F32, DP>(reinterpret_cast<char*>(P.part + at * P.dim), acc, 1.f, P.dim, h);
+      if (l > 0.f) store_rows<F32, DC>(reinterpret_cast<char*>(P.part + at * P.dim), acc, 1.f, P.dim, h);
       if (h == 0) {
         P.part_ml[at * 2] = m;
         P.part_ml[at * 2 + 1] = l;
@@ -645,7 +646,7 @@ __device__ __forceinline__ void attention_fwd(const lm_attn_params& P, char* k0,
   }
   if (R.exists) {
     const float inv = l > 0.f ? 1.f / l : 0.f;
-    store_rows<T, DP>((char*)P.o + row_offset(P.so, R.b, R.head, R.query) * T::kBytes, acc, inv, P.dim, h);
+    store_rows<T, DC>((char*)P.o + row_offset(P.so, R.b, R.head, R.query) * T::kBytes, acc, inv, P.dim, h);
     if (P.lse != nullptr && h == 0) P.lse[R.stat(P)] = l > 0.f ? (m + __builtin_amdgcn_logf(l)) * kLn2 : kNegInf;
   }
 }
@@ -701,7 +702,7 @@ __device__ __forceinline__ void attention_join(const lm_attn_params& P, float* r
 
 // -------------------------------------------------------- query gradients --
 
-template <typename T, int DP, int KS, int NBUF>
+template <typename T, int DP, int DC, int KS, int NBUF>
 __device__ __forceinline__ void attention_bwd_dq(const lm_attn_params& P, char* k0, char* k1, char* v0, char* v1) {
   using RW = Rows<KS>;
   using KT = Tile<T, DP, RW::kKeys>;
@@ -712,87 +713,125 @@ __device__ __forceinline__ void attention_bwd_dq(const lm_attn_params& P, char* 
   const char* kp = (const char*)P.k + ((int64_t)R.b * P.sk.b + (int64_t)R.kvh * P.sk.h) * T::kBytes;
   const char* vp = (const char*)P.v + ((int64_t)R.b * P.sv.b + (int64_t)R.kvh * P.sv.h) * T::kBytes;
 
-  typename T::Frag qf[DP / 16], gf[DP / 16];
-  load_rows<T, DP>(qf, (const char*)P.q + row_offset(P.sq, R.b, R.head, R.query) * T::kBytes, P.dim, h, R.live);
-  load_rows<T, DP>(gf, (const char*)P.grad_out + row_offset(P.sdo, R.b, R.head, R.query) * T::kBytes, P.dim, h, R.live);
+  typename T::Frag qf[DC / 16], gf[DC / 16];
+  load_rows<T, DC>(qf, (const char*)P.q + row_offset(P.sq, R.b, R.head, R.query) * T::kBytes, P.dim, h, R.live);
+  load_rows<T, DC>(gf, (const char*)P.grad_out + row_offset(P.sdo, R.b, R.head, R.query) * T::kBytes, P.dim, h, R.live);
   float delta = 0.f, lse2 = 0.f;
   {
-    typename T::Frag of[DP / 16];
-    load_rows<T, DP>(of, (const char*)P.out + row_offset(P.sout, R.b, R.head, R.query) * T::kBytes, P.dim, h, R.live);
+    typename T::Frag of[DC / 16];
+    load_rows<T, DC>(of, (const char*)P.out + row_offset(P.sout, R.b, R.head, R.query) * T::kBytes, P.dim, h, R.live);
 #pragma unroll
-    for (int s = 0; s < DP / 16; ++s)
+    for (int s = 0; s < DC / 16; ++s)
 #pragma unroll
       for (int j = 0; j < 8; ++j) delta = __builtin_fmaf(T::get(gf[s], j), T::get(of[s], j), delta);
     delta += other_half(delta);
-    if (R.live) {
-      lse2 = P.lse[R.stat(P)] * kLog2e;
-      if (P.grad_lse != nullptr) delta -= P.grad_lse[R.stat(P)];
-    }
-    if (R.exists && h == 0 && R.part == 0) P.delta[R.stat(P)] = delta;
+    if (R.live) lse2 = P.lse[R.stat(P)] * kLog2e;
   }
-  f32x16 acc[DP / 32];
-#pragma unroll
-  for (int i = 0; i < DP / 32; ++i) acc[i] = zero16();
   const int row_at = KT::row_at(lane), col_at = KT::col_at(lane);
-
-  over_keys<KT, NBUF>(
-      kp, P.sk.t * T::kBytes, vp, P.sv.t * T::kBytes, R.t0, R.t1, R.S.kv_len - 1, chunks, R.wave, lane, k0, k1, v0, v1,
-      [&](int t, const char* kc, const char* vc) {
-        constexpr int NB = RW::kBlocks;
-        const int first = KS == 1 ? 0 : 32 * NB * R.part;
-        const int key0 = t * RW::kKeys + first;
-        if (key0 >= R.mine.most) return;
+  // One 32-key block of a tile: the probabilities in s, do v^T in dp, for the keys from `first` of the tile.
+  auto recompute = [&](const char* kc, const char* vc, int first, int key0, f32x16& s, f32x16& dp) {
+    s = zero16();
+    dp = zero16();
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-        for (int kb = 0; kb < NB; ++kb) {
-          f32x16 s = zero16(), dp = zero16();
-          __builtin_amdgcn_s_setprio(1);
+    for (int st = 0; st < DC / 16; ++st) {
+      s = T::mma(KT::row_frag(kc, first, st, row_at), qf[st], s);
+      dp = T::mma(KT::row_frag(vc, first, st, row_at), gf[st], dp);
+    }
+    if constexpr (T::kBytes == 2) interleave<4, DC / 8, 1, 0, 0>();
+    __builtin_amdgcn_s_setprio(0);
 #pragma unroll
-          for (int st = 0; st < DP / 16; ++st) {
-            s = T::mma(KT::row_frag(kc, first + 32 * kb, st, row_at), qf[st], s);
-            dp = T::mma(KT::row_frag(vc, first + 32 * kb, st, row_at), gf[st], dp);
-          }
-          if constexpr (T::kBytes == 2) interleave<4, DP / 8, 1, 0, 0>();
-          __builtin_amdgcn_s_setprio(0);
+    for (int i = 0; i < 16; ++i) s[i] = exp2_fast(__builtin_fmaf(s[i], P.scale_log2, -lse2));
+    if (key0 + 32 > R.mine.all) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            s[i] = exp2_fast(__builtin_fmaf(s[i], P.scale_log2, -lse2)) * (dp[i] - delta);
-          if (key0 + 32 * NB > R.mine.all) {
+      for (int i = 0; i < 16; ++i) {
+        const bool seen = key0 + 8 * (i >> 2) + 4 * h + (i & 3) < R.lim;
+        s[i] = seen ? s[i] : 0.f;
+        dp[i] = seen ? dp[i] : 0.f;
+      }
+    }
+  };
+  constexpr int NB = RW::kBlocks;
+  const int mine = KS == 1 ? 0 : 32 * NB * R.part;  // this wave's keys of a tile
+  // sum_d do o = sum_j p dp.  The first is one product a row, but the output it
+  // reads was rounded to bf16; where a row sees few keys that rounding is as
+  // large as any other in dq (an output of few values is as large as they
+  // are).  Tiles of such rows are walked once more for the second: 1% of the
+  // pairs of a sequence of 4096, and dq and dk keep the error of their own
+  // roundings (2.4e-3 against 2.6e-3 of the norm at 777 tokens).
+  if constexpr (T::kBytes == 2) {
+    if (R.t1 * RW::kKeys <= kExactKeys && R.t1 > 0) {
+      float d = 0.f;
+      over_keys<KT, NBUF>(kp, P.sk.t * T::kBytes, vp, P.sv.t * T::kBytes, 0, R.t1, R.S.kv_len - 1, chunks, R.wave, lane,
+                          k0, k1, v0, v1, [&](int t, const char* kc, const char* vc) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int key = key0 + 32 * kb + 8 * (i >> 2) + 4 * h + (i & 3);
-              s[i] = key < R.lim ? s[i] : 0.f;
-            }
-          }
+                            for (int kb = 0; kb < NB; ++kb) {
+                              const int key0 = t * RW::kKeys + mine + 32 * kb;
+                              if (key0 >= R.mine.most) continue;
+                              f32x16 s, dp;
+                              recompute(kc, vc, mine + 32 * kb, key0, s, dp);
 #pragma unroll
-          for (int st = 0; st < 2; ++st) {
-            const typename T::Frag ds = T::from_acc(s, st);
+                              for (int i = 0; i < 16; ++i) d = __builtin_fmaf(s[i], dp[i], d);
+                            }
+                          });
+      delta = d + other_half(d);
+      __syncthreads();  // the tiles' last readers are done
+      if constexpr (KS > 1) {
+        float* x = reinterpret_cast<float*>(k0);
+        x[R.wave * 64 + lane] = delta;
+        __syncthreads();
+        delta = 0.f;
 #pragma unroll
-            for (int dt = 0; dt < DP / 32; ++dt)
-              acc[dt] = T::mma(KT::col_frag(kc, first + 32 * kb + 16 * st, dt, col_at, lane), ds, acc[dt]);
-          }
-          if constexpr (T::kBytes == 2) interleave<8, DP / 16, 2, 0, 0>();
-        }
-      });
+        for (int o = 0; o < KS; ++o) delta += x[(R.wave - R.part + o) * 64 + lane];
+        __syncthreads();
+      }
+    }
+  }
+  if (R.live && P.grad_lse != nullptr) delta -= P.grad_lse[R.stat(P)];
+  if (R.exists && h == 0 && R.part == 0) P.delta[R.stat(P)] = delta;
+  f32x16 acc[DC / 32];
+#pragma unroll
+  for (int i = 0; i < DC / 32; ++i) acc[i] = zero16();
+  over_keys<KT, NBUF>(kp, P.sk.t * T::kBytes, vp, P.sv.t * T::kBytes, 0, R.t1, R.S.kv_len - 1, chunks, R.wave, lane, k0,
+                      k1, v0, v1, [&](int t, const char* kc, const char* vc) {
+#pragma unroll
+                        for (int kb = 0; kb < NB; ++kb) {
+                          const int key0 = t * RW::kKeys + mine + 32 * kb;
+                          if (key0 >= R.mine.most) continue;
+                          f32x16 s, dp;
+                          recompute(kc, vc, mine + 32 * kb, key0, s, dp);
+#pragma unroll
+                          for (int i = 0; i < 16; ++i) s[i] *= dp[i] - delta;
+#pragma unroll
+                          for (int st = 0; st < 2; ++st) {
+                            const typename T::Frag ds = T::from_acc(s, st);
+#pragma unroll
+                            for (int dt = 0; dt < DC / 32; ++dt)
+                              acc[dt] = T::mma(KT::col_frag(kc, mine + 32 * kb + 16 * st, dt, col_at, lane), ds, acc[dt]);
+                          }
+                          if constexpr (T::kBytes == 2) interleave<8, DC / 16, 2, 0, 0>();
+                        }
+                      });
 
   if constexpr (KS > 1) {
     float* x = reinterpret_cast<float*>((R.wave / KS) == 0 ? k0 : v0);
 #pragma unroll
     for (int o = 1; o < KS; ++o) {
       __syncthreads();
-      if (R.part == o) put<DP>(x, acc, lane);
+      if (R.part == o) put<DC>(x, acc, lane);
       __syncthreads();
-      if (R.part == 0) add<DP>(x, acc, lane, 1.f, 1.f);
+      if (R.part == 0) add<DC>(x, acc, lane, 1.f, 1.f);
     }
     if (R.part != 0) return;
   }
   if (R.exists)
-    store_rows<T, DP>((char*)P.dq + row_offset(P.sdq, R.b, R.head, R.query) * T::kBytes, acc, P.scale, P.dim, h);
+    store_rows<T, DC>((char*)P.dq + row_offset(P.sdq, R.b, R.head, R.query) * T::kBytes, acc, P.scale, P.dim, h);
 }
 
 // ------------------------------------------------ key and value gradients --
 
 // A wave owns 32 keys; KS waves share them and split each tile of 32 KS rows.
-template <typename T, int DP, int KS, int NBUF>
+template <typename T, int DP, int DC, int KS, int NBUF>
 __device__ __forceinline__ void attention_bwd_dkv(const lm_attn_params& P, char* q0, char* q1, char* g0, char* g1,
                                                   float* st0, float* st1) {
   constexpr int R = 32 * KS;
@@ -810,12 +849,12 @@ __device__ __forceinline__ void attention_bwd_dkv(const lm_attn_params& P, char*
   const int key = w0 + (lane & 31);
   const bool live = key < S.kv_len;
 
-  typename T::Frag kf[DP / 16], vf[DP / 16];
-  load_rows<T, DP>(kf, (const char*)P.k + row_offset(P.sk, b, kvh, key) * T::kBytes, P.dim, h, live);
-  load_rows<T, DP>(vf, (const char*)P.v + row_offset(P.sv, b, kvh, key) * T::kBytes, P.dim, h, live);
-  f32x16 dk[DP / 32], dv[DP / 32];
+  typename T::Frag kf[DC / 16], vf[DC / 16];
+  load_rows<T, DC>(kf, (const char*)P.k + row_offset(P.sk, b, kvh, key) * T::kBytes, P.dim, h, live);
+  load_rows<T, DC>(vf, (const char*)P.v + row_offset(P.sv, b, kvh, key) * T::kBytes, P.dim, h, live);
+  f32x16 dk[DC / 32], dv[DC / 32];
 #pragma unroll
-  for (int i = 0; i < DP / 32; ++i) {
+  for (int i = 0; i < DC / 32; ++i) {
     dk[i] = zero16();
     dv[i] = zero16();
   }
@@ -887,11 +926,11 @@ __device__ __forceinline__ void attention_bwd_dkv(const lm_attn_params& P, char*
     f32x16 s = zero16(), dp = zero16();
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-    for (int st = 0; st < DP / 16; ++st) {
+    for (int st = 0; st < DC / 16; ++st) {
       s = T::mma(QT::row_frag(qc, mine, st, row_at), kf[st], s);
       dp = T::mma(QT::row_frag(gc, mine, st, row_at), vf[st], dp);
     }
-    if constexpr (T::kBytes == 2) interleave<4, DP / 8, 1, 0, 0>();
+    if constexpr (T::kBytes == 2) interleave<4, DC / 8, 1, 0, 0>();
     __builtin_amdgcn_s_setprio(0);
     const float* stats = sc + (KS == 1 ? 0 : 64 * part);
 #pragma unroll
@@ -919,12 +958,12 @@ __device__ __forceinline__ void attention_bwd_dkv(const lm_attn_params& P, char*
     for (int st = 0; st < 2; ++st) {
       const typename T::Frag p = T::from_acc(s, st), ds = T::from_acc(dp, st);
 #pragma unroll
-      for (int dt = 0; dt < DP / 32; ++dt) {
+      for (int dt = 0; dt < DC / 32; ++dt) {
         dv[dt] = T::mma(QT::col_frag(gc, mine + 16 * st, dt, col_at, lane), p, dv[dt]);
         dk[dt] = T::mma(QT::col_frag(qc, mine + 16 * st, dt, col_at, lane), ds, dk[dt]);
       }
     }
-    if constexpr (T::kBytes == 2) interleave<4, DP / 8, 2, 0, 0>();
+    if constexpr (T::kBytes == 2) interleave<4, DC / 8, 2, 0, 0>();
   };
   auto arrived = [] {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -957,31 +996,32 @@ __device__ __forceinline__ void attention_bwd_dkv(const lm_attn_params& P, char*
     for (int o = 1; o < KS; ++o) {
       __syncthreads();
       if (part == o) {
-        put<DP>(xk, dk, lane);
-        put<DP>(xv, dv, lane);
+        put<DC>(xk, dk, lane);
+        put<DC>(xv, dv, lane);
       }
       __syncthreads();
       if (part == 0) {
-        add<DP>(xk, dk, lane, 1.f, 1.f);
-        add<DP>(xv, dv, lane, 1.f, 1.f);
+        add<DC>(xk, dk, lane, 1.f, 1.f);
+        add<DC>(xv, dv, lane, 1.f, 1.f);
       }
     }
     if (part != 0) return;
   }
   if (key < P.kv_len) {
-    store_rows<T, DP>((char*)P.dk + row_offset(P.sdk, b, kvh, key) * T::kBytes, dk, P.scale, P.dim, h);
-    store_rows<T, DP>((char*)P.dv + row_offset(P.sdv, b, kvh, key) * T::kBytes, dv, 1.f, P.dim, h);
+    store_rows<T, DC>((char*)P.dk + row_offset(P.sdk, b, kvh, key) * T::kBytes, dk, P.scale, P.dim, h);
+    store_rows<T, DC>((char*)P.dv + row_offset(P.sdv, b, kvh, key) * T::kBytes, dv, 1.f, P.dim, h);
   }
 }
 
 }  // namespace
 
-// KS: waves that share rows (or keys); NBUF: LDS buffers of a tile; WPE: waves
+// DP: elements of a tile's row in LDS; DC: columns worked on, the head size
+// rounded up to 32; KS: waves that share rows (or keys); NBUF: LDS buffers of a tile; WPE: waves
 // per SIMD the registers are held to.
 #define LM_ATTN_KERNEL(KIND, NAME, WPE) \
   extern "C" __global__ void __launch_bounds__(64 * LM_ATTN_WAVES) __attribute__((amdgpu_waves_per_eu(WPE))) \
       attnres_attention_##KIND##_##NAME(lm_attn_params P)
-#define LM_ATTN(NAME, T, DP, KS, NBUF, FWD_WPE, DQ_WPE, DKV_WPE)                                     \
+#define LM_ATTN(NAME, T, DP, DC, KS, NBUF, FWD_WPE, DQ_WPE, DKV_WPE)                                     \
   LM_ATTN_KERNEL(fwd, NAME, FWD_WPE) {                                                               \
     constexpr int kTile = Tile<T, DP, Rows<KS>::kKeys>::kBytes;                                      \
     __shared__ __align__(16) char k0[kTile];                                                         \
@@ -989,7 +1029,7 @@ __device__ __forceinline__ void attention_bwd_dkv(const lm_attn_params& P, char*
     __shared__ __align__(16) char k1[NBUF == 2 ? kTile : 16];                                        \
     __shared__ __align__(16) char v1[NBUF == 2 ? kTile : 16];                                        \
     __shared__ float ml[KS > 1 ? LM_ATTN_WAVES / KS * 128 : 1];                                      \
-    attention_fwd<T, DP, KS, NBUF>(P, k0, k1, v0, v1, ml);                                           \
+    attention_fwd<T, DP, DC, KS, NBUF>(P, k0, k1, v0, v1, ml);                                           \
   }                                                                                                  \
   LM_ATTN_KERNEL(dq, NAME, DQ_WPE) {                                                                 \
     constexpr int kTile = Tile<T, DP, Rows<KS>::kKeys>::kBytes;                                      \
@@ -997,7 +1037,7 @@ __device__ __forceinline__ void attention_bwd_dkv(const lm_attn_params& P, char*
     __shared__ __align__(16) char v0[kTile];                                                         \
     __shared__ __align__(16) char k1[NBUF == 2 ? kTile : 16];                                        \
     __shared__ __align__(16) char v1[NBUF == 2 ? kTile : 16];                                        \
-    attention_bwd_dq<T, DP, KS, NBUF>(P, k0, k1, v0, v1);                                            \
+    attention_bwd_dq<T, DP, DC, KS, NBUF>(P, k0, k1, v0, v1);                                            \
   }                                                                                                  \
   LM_ATTN_KERNEL(dkv, NAME, DKV_WPE) {                                                               \
     constexpr int kTile = Tile<T, DP, 32 * KS>::kBytes;                                              \
@@ -1007,7 +1047,7 @@ __device__ __forceinline__ void attention_bwd_dkv(const lm_attn_params& P, char*
     __shared__ __align__(16) char g1[NBUF == 2 ? kTile : 16];                                        \
     __shared__ __align__(16) float st0[64 * KS];                                                     \
     __shared__ __align__(16) float st1[NBUF == 2 ? 64 * KS : 4];                                     \
-    attention_bwd_dkv<T, DP, KS, NBUF>(P, q0, q1, g0, g1, st0, st1);                                 \
+    attention_bwd_dkv<T, DP, DC, KS, NBUF>(P, q0, q1, g0, g1, st0, st1);                                 \
   }
 
 #define LM_ATTN_JOIN(NAME, T)                                                                       \
@@ -1018,19 +1058,23 @@ __device__ __forceinline__ void attention_bwd_dkv(const lm_attn_params& P, char*
 
 #if LM_PART == 13
 LM_ATTN_JOIN(bf16, Bf16)
-LM_ATTN(bf16_d64_s1, Bf16, 64, 1, 2, 2, 2, 2)
-LM_ATTN(bf16_d64_s2, Bf16, 64, 2, 2, 2, 2, 2)
-LM_ATTN(bf16_d64_s4, Bf16, 64, 4, 1, 2, 2, 2)
-LM_ATTN(bf16_d128_s1, Bf16, 128, 1, 2, 2, 2, 2)
-LM_ATTN(bf16_d128_s2, Bf16, 128, 2, 2, 2, 2, 2)
-LM_ATTN(bf16_d128_s4, Bf16, 128, 4, 1, 2, 2, 2)
+#define LM_ATTN_BF16(DP, DC)                              \
+  LM_ATTN(bf16_d##DC##_s1, Bf16, DP, DC, 1, 2, 2, 2, 2)   \
+  LM_ATTN(bf16_d##DC##_s2, Bf16, DP, DC, 2, 2, 2, 2, 2)   \
+  LM_ATTN(bf16_d##DC##_s4, Bf16, DP, DC, 4, 1, 2, 2, 2)
+LM_ATTN_BF16(64, 32)
+LM_ATTN_BF16(64, 64)
+LM_ATTN_BF16(128, 96)
+LM_ATTN_BF16(128, 128)
 #endif
 #if LM_PART == 14
 LM_ATTN_JOIN(f32, F32)
-LM_ATTN(f32_d64_s1, F32, 64, 1, 2, 1, 1, 1)
-LM_ATTN(f32_d64_s2, F32, 64, 2, 2, 1, 1, 1)
-LM_ATTN(f32_d64_s4, F32, 64, 4, 1, 1, 1, 1)
-LM_ATTN(f32_d128_s1, F32, 128, 1, 2, 1, 1, 1)
-LM_ATTN(f32_d128_s2, F32, 128, 2, 2, 1, 1, 1)
-LM_ATTN(f32_d128_s4, F32, 128, 4, 1, 1, 1, 1)
+#define LM_ATTN_F32(DP, DC)                              \
+  LM_ATTN(f32_d##DC##_s1, F32, DP, DC, 1, 2, 1, 1, 1)    \
+  LM_ATTN(f32_d##DC##_s2, F32, DP, DC, 2, 2, 1, 1, 1)    \
+  LM_ATTN(f32_d##DC##_s4, F32, DP, DC, 4, 1, 1, 1, 1)
+LM_ATTN_F32(64, 32)
+LM_ATTN_F32(64, 64)
+LM_ATTN_F32(128, 96)
+LM_ATTN_F32(128, 128)
 #endif

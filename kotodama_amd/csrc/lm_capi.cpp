@@ -19,10 +19,10 @@ namespace {
 // Code-object parts and kernel slots.
 constexpr int kLmPart = 12, kAttnBf16Part = 13, kAttnF32Part = 14;
 enum Slot {
-  kAttnFwd = 0,                // + 6 * (fp32) + 3 * (head_dim > 64) + log2 of the waves that share rows
-  kAttnDq = kAttnFwd + 12,
-  kAttnDkv = kAttnDq + 12,
-  kAttnJoin = kAttnDkv + 12,   // + (fp32)
+  kAttnFwd = 0,                // + 12 * (fp32) + 3 * ((head_dim - 1) / 32) + log2 of the waves that share rows
+  kAttnDq = kAttnFwd + 24,
+  kAttnDkv = kAttnDq + 24,
+  kAttnJoin = kAttnDkv + 24,   // + (fp32)
   kRopeFwd = kAttnJoin + 2,    // + 4 * (fp32) + 2 * (scalar) + (4 heads per lane group)
   kRopeBwd = kRopeFwd + 8,     // + 2 * (fp32) + (scalar)
   kRopeDw = kRopeBwd + 4,      // + (fp32)
@@ -152,7 +152,9 @@ AttnPlan attention_plan(int base, int64_t heads, int64_t lines, int64_t kv_slots
   const int64_t waves = heads * ((lines + 31) / 32), full = (int64_t)cus * (base == kAttnDkv ? 16 : 8);
   p.log = waves >= full ? 0 : waves * 2 >= full ? 1 : 2;
   if (base == kAttnFwd && p.log == 2) {
-    const int64_t most = (kv_slots + 127) / 128, want = (int64_t)cus * kSplitPerCu / (waves > 0 ? waves : 1);
+    // tiles of 128 keys; four at least a part where there are many rows to join
+    const int64_t least = heads * lines <= (int64_t)cus * 4 ? 1 : 4;
+    const int64_t most = (kv_slots + 127) / 128 / least, want = (int64_t)cus * kSplitPerCu / (waves > 0 ? waves : 1);
     const int64_t n = want < most ? want : most;
     p.splits = n < 2 ? 1 : (int)n;
   }
@@ -173,11 +175,12 @@ int launch_attention(int base, const char* kind, lm_attn_params& P, int dtype, i
   P.group_magic = (uint32_t)((((uint64_t)1 << 32) + group - 1) / group);
   const int64_t items = P.n_tiles * heads;
   if (items > INT32_MAX - 8) return fail(ATTNRES_ERR_UNSUPPORTED, "attention: too many rows for one call");
-  const bool f32 = dtype == ATTNRES_DTYPE_F32, wide = P.dim > 64;
+  const bool f32 = dtype == ATTNRES_DTYPE_F32;
+  const int blocks = (P.dim - 1) / 32;
   char name[64];
-  snprintf(name, sizeof(name), "attnres_attention_%s_%s_d%d_s%d", kind, f32 ? "f32" : "bf16", wide ? 128 : 64,
+  snprintf(name, sizeof(name), "attnres_attention_%s_%s_d%d_s%d", kind, f32 ? "f32" : "bf16", 32 * (blocks + 1),
            1 << plan.log);
-  return launch(base + (f32 ? 6 : 0) + (wide ? 3 : 0) + plan.log, f32 ? kAttnF32Part : kAttnBf16Part, name,
+  return launch(base + (f32 ? 12 : 0) + 3 * blocks + plan.log, f32 ? kAttnF32Part : kAttnBf16Part, name,
                 (unsigned)((items + 7) / 8 * 8), 1, 64 * LM_ATTN_WAVES, 0, P, stream);
 }
 
