@@ -830,7 +830,8 @@ __device__ __forceinline__ void attention_bwd_dq(const lm_attn_params& P, char* 
 
 // ------------------------------------------------ key and value gradients --
 
-// A wave owns 32 keys; KS waves share them and split each tile of 32 KS rows.
+// A wave owns 32 keys; KS waves share them and split each tile of 32 KS rows:
+// queries of one head, the heads of the group one after another.
 template <typename T, int DP, int DC, int KS, int NBUF>
 __device__ __forceinline__ void attention_bwd_dkv(const lm_attn_params& P, char* q0, char* q1, char* g0, char* g1,
                                                   float* st0, float* st1) {
@@ -843,7 +844,7 @@ __device__ __forceinline__ void attention_bwd_dkv(const lm_attn_params& P, char*
   const int part = wave % KS;
   const int kvh = it.head % P.kv_heads, b = it.head / P.kv_heads;
   const int group = P.heads / P.kv_heads;
-  const Seq S = sequence(P, b, group);
+  const Seq S = sequence(P, b, 1);
   const int wg0 = it.rank * (32 * LM_ATTN_WAVES / KS);  // causal: the first keys are seen by the most queries
   const int w0 = wg0 + wave / KS * 32;
   const int key = w0 + (lane & 31);
@@ -858,67 +859,50 @@ __device__ __forceinline__ void attention_bwd_dkv(const lm_attn_params& P, char*
     dk[i] = zero16();
     dv[i] = zero16();
   }
-  // the first row that sees a key, of the workgroup's keys (rounded down to a
-  // tile), the wave's, and this lane's; from w_full on rows see all the wave's
-  auto first_row = [&](int k) {
-    const int64_t r = P.causal && k > S.start ? (int64_t)(k - S.start) * group : 0;
+  // the first query that sees a key, of the workgroup's keys, the wave's, and
+  // this lane's; from w_full on queries see all the wave's
+  auto first_query = [&](int k) {
+    const int64_t r = P.causal ? (int64_t)k - S.start : 0;
     return (int)(r < S.lo ? S.lo : r > S.hi ? S.hi : r);
   };
-  const int first = first_row(wg0);
-  const int base = first / R * R;
-  const int w_first = first_row(w0);
-  const int w_full = w0 + 32 > S.kv_len ? S.hi : first_row(w0 + 31);
-  const int k_first = live ? first_row(key) : S.hi;
-  const int tiles = wg0 < S.kv_len && first < S.hi ? (S.hi - base + R - 1) / R : 0;
+  const int base = first_query(wg0);
+  const int w_first = first_query(w0);
+  const int w_full = w0 + 32 > S.kv_len ? S.hi : first_query(w0 + 31);
+  const int k_first = live ? first_query(key) : S.hi;
+  const int per = wg0 < S.kv_len ? (S.hi - base + R - 1) / R : 0;  // tiles of a head
+  const int tiles = per * group;
 
   const int chunks = P.dim * T::kBytes / 16;
-  const uint32_t qst = (uint32_t)(P.sq.t * T::kBytes), qsh = (uint32_t)(P.sq.h * T::kBytes);
-  const uint32_t gst = (uint32_t)(P.sdo.t * T::kBytes), gsh = (uint32_t)(P.sdo.h * T::kBytes);
+  const int64_t qst = P.sq.t * T::kBytes, qsh = P.sq.h * T::kBytes, gst = P.sdo.t * T::kBytes, gsh = P.sdo.h * T::kBytes;
   const char* qp = (const char*)P.q + row_offset(P.sq, b, kvh * group, 0) * T::kBytes;
   const char* gp = (const char*)P.grad_out + row_offset(P.sdo, b, kvh * group, 0) * T::kBytes;
-  const int64_t stat0 = ((int64_t)b * P.heads + kvh * group) * P.q_len;
-  const int last = S.hi - 1;
-  // tile t starts at row base + t R: query i0, head j0 of the group
-  int i0 = base / group, j0 = base - i0 * group, next = 0;
-  // row i0 * group + j0 + r as (query, head) after i0
-  auto split = [&](int r, int& i, int& j) {
-    const uint32_t n = (uint32_t)(j0 + r);
-    i = group == 1 ? (int)n : (int)__umulhi(n, P.group_magic);  // n / group: n is under group + 256
-    j = (int)n - i * group;
-  };
-  auto request = [&](char* qn, char* gn, float* sn) {  // tile `next`
+  int64_t stat = ((int64_t)b * P.heads + kvh * group) * P.q_len;
+  int next = 0;  // the tile of its head to request
+  auto request = [&](char* qn, char* gn, float* sn) {
     const int row0 = base + next * R;
-    const char* qb = qp + (int64_t)i0 * P.sq.t * T::kBytes;
-    const char* gb = gp + (int64_t)i0 * P.sdo.t * T::kBytes;
-    const int lo = S.lo - row0, hi = last - row0;  // rows that see keys, from the tile's first
-#pragma unroll
-    for (int n = 0; n < QT::kRounds; ++n) {
-      int r = n * QT::kRound + QT::round_row(wave, lane), i, j;
-      r = r < hi ? r : hi;
-      r = r > lo ? r : lo;
-      split(r, i, j);
-      const uint32_t c = 16 * (uint32_t)QT::round_chunk(wave, lane, chunks, n & 1);
-      QT::load_lds(qn + (n * LM_ATTN_WAVES + wave) * 1024, qb, (uint32_t)i * qst + (uint32_t)j * qsh + c);
-      QT::load_lds(gn + (n * LM_ATTN_WAVES + wave) * 1024, gb, (uint32_t)i * gst + (uint32_t)j * gsh + c);
-    }
-    if (wave < KS) {  // the rows' lse (lanes 0 .. 31) and delta, 32 rows a wave
-      int r = wave * 32 + (lane & 31), i, j;
-      r = r < hi ? r : hi;
-      r = r > lo ? r : lo;
-      split(r, i, j);
-      const float* src = (h ? P.delta : P.lse) + stat0 + (int64_t)j * P.q_len + (i0 + i);
+    int ln = lane;  // opaque: the lane's offsets are formed anew for each tile, registers being short
+    asm volatile("" : "+v"(ln));
+    QT::request(qn, qp, qst, row0, S.hi - 1, QT::lane_offsets((uint32_t)qst, chunks, wave, ln), chunks, wave, ln);
+    QT::request(gn, gp, gst, row0, S.hi - 1, QT::lane_offsets((uint32_t)gst, chunks, wave, ln), chunks, wave, ln);
+    if (wave < KS) {  // the queries' lse (lanes 0 .. 31) and delta, 32 a wave
+      int r = row0 + wave * 32 + (ln & 31);
+      r = r < S.hi ? r : S.hi - 1;
+      const float* src = ((ln >> 5) ? P.delta : P.lse) + stat + r;
       __builtin_amdgcn_global_load_lds((const LM_GLOBAL void*)src, (LM_LDS void*)(sn + wave * 64), 4, 0, 0);
     }
-    ++next;
-    int i, j;
-    split(R, i, j);
-    i0 += i;
-    j0 = j;
+    if (++next == per) {
+      next = 0;
+      qp += qsh;
+      gp += gsh;
+      stat += P.q_len;
+    }
   };
+  int now = 0;  // the tile of its head to work on
   int row_at = QT::row_at(lane), col_at = QT::col_at(lane);
-  auto step = [&](int t, const char* qc, const char* gc, const float* sc) {
+  auto step = [&](const char* qc, const char* gc, const float* sc) {
     const int mine = KS == 1 ? 0 : 32 * part;  // this wave's rows of the tile
-    const int row0 = base + t * R + mine;
+    const int row0 = base + now * R + mine;
+    now = now + 1 == per ? 0 : now + 1;
     if (row0 + 32 <= w_first || row0 >= S.hi || w0 >= S.kv_len) return;
     // opaque here, so that the offsets made from these are formed anew (one
     // instruction each) instead of held in registers
@@ -974,18 +958,18 @@ __device__ __forceinline__ void attention_bwd_dkv(const lm_attn_params& P, char*
       if (t > 0) __syncthreads();
       request(q0, g0, st0);
       arrived();
-      step(t, q0, g0, st0);
+      step(q0, g0, st0);
     }
   } else {
     if (tiles > 0) request(q0, g0, st0);
     for (int t = 0; t < tiles; t += 2) {
       arrived();
       if (t + 1 < tiles) request(q1, g1, st1);
-      step(t, q0, g0, st0);
+      step(q0, g0, st0);
       if (t + 1 < tiles) {
         arrived();
         if (t + 2 < tiles) request(q0, g0, st0);
-        step(t + 1, q1, g1, st1);
+        step(q1, g1, st1);
       }
     }
   }

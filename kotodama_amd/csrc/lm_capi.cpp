@@ -171,8 +171,6 @@ int launch_attention(int base, const char* kind, lm_attn_params& P, int dtype, i
   P.splits = plan.splits;
   P.n_tiles = (int32_t)((lines + per - 1) / per * plan.splits);
   P.cus_per_xcd = cus / 8 > 0 ? cus / 8 : 1;
-  const int group = P.heads / P.kv_heads;
-  P.group_magic = (uint32_t)((((uint64_t)1 << 32) + group - 1) / group);
   const int64_t items = P.n_tiles * heads;
   if (items > INT32_MAX - 8) return fail(ATTNRES_ERR_UNSUPPORTED, "attention: too many rows for one call");
   const bool f32 = dtype == ATTNRES_DTYPE_F32;

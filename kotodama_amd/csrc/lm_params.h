@@ -57,7 +57,6 @@ typedef struct lm_attn_params {
   int32_t n_tiles;       /* tiles along the axis that the grid splits */
   int32_t splits;        /* parts of the key axis, each a workgroup (forward, four waves a row) */
   int32_t cus_per_xcd;
-  uint32_t group_magic;  /* ceil(2^32 / group): n / group = n * group_magic >> 32 for n under 2^32 / group */
   float scale;           /* of the scores */
   float scale_log2;      /* scale * log2(e) */
 } lm_attn_params;
