@@ -478,7 +478,8 @@ int attnres_merge_bwd(const void* partial, int64_t num_tokens, int hidden, int p
  * every query of its sequence.
  *
  * dtype: bf16 or fp32 (all of q, k, v, out); head_dim a multiple of 8 up to
- * 128; 16-byte aligned pointers and strides.  lse ((batch, heads, q_len) fp32)
+ * 128; scale positive; 16-byte aligned pointers and strides, tokens less than
+ * 32 MiB apart; at most 4096 query heads per key head.  lse ((batch, heads, q_len) fp32)
  * may be NULL.  Scores and sums are fp32; the probabilities are rounded to the
  * dtype for the product with v, the result once.  workspace: device memory of
  * attnres_attention_workspace_size bytes (backward 0 or 1).

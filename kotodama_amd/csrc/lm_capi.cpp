@@ -36,6 +36,7 @@ static_assert(kSlots <= ATTNRES_INTERNAL_SLOTS, "kernel slots");
 
 constexpr int64_t kMaxLen = (int64_t)1 << 30;  // tokens of one sequence
 constexpr int kSplitPerCu = 2;                 // workgroups per CU to split the key axis into
+constexpr int64_t kMaxTokenStride = (int64_t)32 << 20;  // bytes
 constexpr int kMaxGroup = 4096;                // query heads per key head
 
 int fail(int code, const char* fmt, ...) {
@@ -103,7 +104,9 @@ int fill_attention(lm_attn_params* P, int batch, int heads, int kv_heads, int64_
                    int head_dim, int causal, float scale, const void* kv_lens, const void* q_start, int index_dtype,
                    int64_t q_start_value) {
   if (causal != 0 && causal != 1) return fail(ATTNRES_ERR_ARG, "attention: causal is 0 or 1");
-  if (!std::isfinite(scale)) return fail(ATTNRES_ERR_ARG, "attention: scale is not finite");
+  // masked scores are -inf before they are scaled, and the largest score has to be the largest scaled one
+  if (!(scale > 0.f) || !std::isfinite(scale * 1.44269504088896340736f))
+    return fail(ATTNRES_ERR_ARG, "attention: scale is not positive and finite");
   if (!valid_index(index_dtype)) return fail(ATTNRES_ERR_ARG, "attention: bad index_dtype %d", index_dtype);
   const int is = index_dtype == ATTNRES_INDEX_I64 ? 8 : 4;
   if (!aligned(kv_lens, is) || !aligned(q_start, is))
@@ -125,12 +128,11 @@ int fill_attention(lm_attn_params* P, int batch, int heads, int kv_heads, int64_
   return ATTNRES_OK;
 }
 
-// Offsets within a tile (up to 128 rows, or their queries and heads) are 32 bits wide.
-int check_span(const char* what, const lm_strides& s, int64_t heads, int64_t tokens, int es) {
-  const int64_t t = s.t * es * (tokens < 130 ? tokens : 130), h = s.h * es * (heads - 1);
-  if (s.t < 0 || s.h < 0 || s.b < 0 || s.t > kMaxLen || s.h > ((int64_t)1 << 40) || t + h >= ((int64_t)1 << 32) - 4096)
-    return fail(ATTNRES_ERR_UNSUPPORTED, "%s: 130 tokens of a head group span over 4 GiB (or a stride is negative)",
-                what);
+// Offsets within a tile (up to 128 rows) are 32 bits wide.
+int check_span(const char* what, const lm_strides& s, int es) {
+  if (s.b < 0 || s.h < 0 || s.t < 0) return fail(ATTNRES_ERR_ARG, "%s: a stride is negative", what);
+  if (s.t * es >= kMaxTokenStride)
+    return fail(ATTNRES_ERR_UNSUPPORTED, "%s: tokens are 32 MiB apart or more", what);
   return ATTNRES_OK;
 }
 
@@ -219,8 +221,8 @@ int fill_rope(lm_rope_params* P, const void* q, const int64_t* q_strides, const 
   if (table_dtype != dtype && table_dtype != ATTNRES_DTYPE_F32)
     return fail(ATTNRES_ERR_ARG, "qk_norm_rope: the tables' dtype must be the rows' or fp32");
   if (batch < 0 || q_heads < 0 || k_heads < 0 || tokens < 0) return fail(ATTNRES_ERR_ARG, "qk_norm_rope: bad sizes");
-  if (tokens > kMaxLen || tokens * batch > kMaxLen || q_heads > (1 << 15) || k_heads > (1 << 15))
-    return fail(ATTNRES_ERR_UNSUPPORTED, "qk_norm_rope: over 2^30 tokens, or over 2^15 heads");
+  if (tokens > kMaxLen || tokens * batch > kMaxLen || q_heads > (1 << 14) || k_heads > (1 << 14))
+    return fail(ATTNRES_ERR_UNSUPPORTED, "qk_norm_rope: over 2^30 tokens, or over 2^14 heads");
   if (head_dim < 2 || head_dim > kRopeMaxDim || head_dim % 2 != 0)
     return fail(ATTNRES_ERR_UNSUPPORTED, "qk_norm_rope: head_dim %d is not even and at most %d", head_dim, kRopeMaxDim);
   if (!std::isfinite(eps) || eps < 0) return fail(ATTNRES_ERR_ARG, "qk_norm_rope: bad eps");
@@ -318,8 +320,8 @@ EmbedPlan embed_plan(int64_t n, int64_t rows, int hidden) {
 
 int check_embedding_sizes(int64_t num_ids, int64_t rows, int hidden) {
   if (num_ids < 0 || rows < 0 || hidden < 1) return fail(ATTNRES_ERR_ARG, "embedding: bad sizes");
-  if (num_ids > INT32_MAX - 64 || rows > INT32_MAX - LM_EMBED_MAX_RANGE || hidden > (1 << 24))
-    return fail(ATTNRES_ERR_UNSUPPORTED, "embedding: more than 2^31 ids or rows, or a row over 2^24");
+  if (num_ids > INT32_MAX - 64 || rows > INT32_MAX - LM_EMBED_MAX_RANGE || hidden > (1 << 23))
+    return fail(ATTNRES_ERR_UNSUPPORTED, "embedding: more than 2^31 ids or rows, or a row over 2^23");
   return ATTNRES_OK;
 }
 
@@ -379,8 +381,8 @@ int attnres_attention_fwd(const void* q, const int64_t* q_strides, const void* k
       return rc;
   }
   const int group = heads / kv_heads;
-  if ((rc = check_span("attention: k", P.sk, 1, kv_slots, es)) != ATTNRES_OK ||
-      (rc = check_span("attention: v", P.sv, 1, kv_slots, es)) != ATTNRES_OK)
+  if ((rc = check_span("attention: k", P.sk, es)) != ATTNRES_OK ||
+      (rc = check_span("attention: v", P.sv, es)) != ATTNRES_OK)
     return rc;
   int64_t ml = 0, need = 0;
   if ((rc = forward_workspace(batch, heads, kv_heads, q_len, kv_slots, head_dim, &ml, &need)) != ATTNRES_OK) return rc;
@@ -445,10 +447,10 @@ int attnres_attention_bwd(const void* q, const int64_t* q_strides, const void* k
       return rc;
   }
   const int group = heads / kv_heads;
-  if ((rc = check_span("attention: k", P.sk, 1, kv_slots, es)) != ATTNRES_OK ||
-      (rc = check_span("attention: v", P.sv, 1, kv_slots, es)) != ATTNRES_OK ||
-      (rc = check_span("attention: q", P.sq, group, q_len, es)) != ATTNRES_OK ||
-      (rc = check_span("attention: grad_out", P.sdo, group, q_len, es)) != ATTNRES_OK)
+  if ((rc = check_span("attention: k", P.sk, es)) != ATTNRES_OK ||
+      (rc = check_span("attention: v", P.sv, es)) != ATTNRES_OK ||
+      (rc = check_span("attention: q", P.sq, es)) != ATTNRES_OK ||
+      (rc = check_span("attention: grad_out", P.sdo, es)) != ATTNRES_OK)
     return rc;
   P.q = q;
   P.k = k;

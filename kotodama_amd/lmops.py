@@ -36,6 +36,7 @@ from .ops import _DeviceStream, _eager_direct, _require_device, dtype_code
 
 MAX_ATTENTION_DIM = 128
 MAX_ROPE_DIM = 256
+MAX_TOKEN_STRIDE = 32 << 20  # bytes from a token's row to the next that the attention kernels address
 
 
 def _index_code(name: str, t: Tensor) -> int:
@@ -76,7 +77,8 @@ def _chunked(t: Tensor) -> Tensor:
     """``t`` with rows that load in 16-byte pieces."""
     m = 16 // t.element_size()
     if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(
-            t.stride(i) % m == 0 for i in range(t.dim() - 1) if t.shape[i] > 1):
+            t.stride(i) % m == 0 for i in range(t.dim() - 1) if t.shape[i] > 1) and (
+            t.shape[2] <= 1 or t.stride(2) * t.element_size() < MAX_TOKEN_STRIDE):
         return t
     # contiguous() leaves a contiguous tensor at its (unaligned) place
     return t.clone(memory_format=torch.contiguous_format)
@@ -359,8 +361,8 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, causal: bool = True, scale: Op
               kv_lens: Optional[Tensor] = None, q_start: Union[None, int, Tensor] = None, want_lse: bool = False):
     """softmax(scale q k^T) v for ``q`` (B, H, Tq, D) over ``k`` and ``v`` (B, Hk, Tk, D), H a multiple of Hk.
 
-    Query head h reads key head ``h // (H // Hk)``.  ``scale`` is 1/sqrt(D)
-    unless given.  ``kv_lens`` ((B,) whole numbers on the device) is how many
+    Query head h reads key head ``h // (H // Hk)``.  ``scale`` (positive) is
+    1/sqrt(D) unless given.  ``kv_lens`` ((B,) whole numbers on the device) is how many
     keys of each sequence exist, Tk unless given: a cache's fill, a padded
     batch's lengths.  What the other slots hold, NaN included, is not used.
     Query i is at position ``q_start + i`` of its sequence, ``q_start`` a
@@ -380,6 +382,10 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, causal: bool = True, scale: Op
     """
     causal = bool(causal)
     scale = 1.0 / math.sqrt(max(1, q.shape[-1])) if scale is None else float(scale)
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"attention: scale must be positive and finite, got {scale}")
+    if kv_lens is not None and not isinstance(kv_lens, Tensor):
+        raise TypeError(f"attention: kv_lens must be a tensor, got {type(kv_lens).__name__}")
     start, value = None, _capi.START_FROM_END
     if isinstance(q_start, Tensor):
         start = q_start

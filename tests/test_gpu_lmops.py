@@ -191,6 +191,43 @@ def test_attention_peaked_and_equal_scores():
         _within("out", kotodama_amd.attention(zero, k, v), LO.attention(zero, k, v)["out"])
 
 
+def test_attention_tokens_far_apart():
+    # rows 40 MiB apart (a view of every 20th million elements) are copied; 20 MiB apart they are read in place
+    g = _gen(13)
+    for step in (20 << 20, 10 << 20):
+        store = torch.zeros(5 * step + 64, device=DEV, dtype=BF)
+        k = store[:5 * step].view(5, step)[:, :64].view(1, 1, 5, 64)
+        k.copy_(_randn(g, 1, 1, 5, 64))
+        q = _heads(g, 1, 2, 5, 64, BF)
+        assert torch.equal(kotodama_amd.attention(q, k, k), kotodama_amd.attention(q, k.contiguous(), k.contiguous()))
+
+
+def test_no_gradients_of_gradients():
+    g = _gen(14)
+    q = _heads(g, 1, 2, 9, 64, FP).requires_grad_(True)
+    out = kotodama_amd.attention(q, q, q)
+    (d,) = torch.autograd.grad(out.sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(d.sum(), q)
+
+
+def test_attention_index_forms():
+    # starts and lengths of any whole-number type and stride, together and apart, give the same rows
+    g = _gen(15)
+    q, k, v = _heads(g, 3, 4, 6, 64, BF), _heads(g, 3, 2, 90, 64, BF), _heads(g, 3, 2, 90, 64, BF)
+    lens, start = torch.tensor([90, 40, 7], device=DEV), torch.tensor([80, 34, 1], device=DEV)
+    want = kotodama_amd.attention(q, k, v, kv_lens=lens, q_start=start)
+    for a in (lens, lens.int(), lens.repeat_interleave(2)[::2]):
+        for b in (start, start.int(), start.repeat_interleave(3)[::3]):
+            assert torch.equal(kotodama_amd.attention(q, k, v, kv_lens=a, q_start=b), want)
+    far = torch.tensor([1 << 45, -(1 << 45), 1 << 62], device=DEV)
+    assert not kotodama_amd.attention(q, k, v, q_start=far).any()
+    assert torch.equal(kotodama_amd.attention(q, k, v, kv_lens=far),
+                       kotodama_amd.attention(q, k, v, kv_lens=torch.tensor([90, 0, 90], device=DEV)))
+    one = lens[:1].expand(3)
+    assert torch.equal(kotodama_amd.attention(q, k, v, kv_lens=one), kotodama_amd.attention(q, k, v))
+
+
 @pytest.mark.parametrize("b,h,hk,tq,tk,d", [(0, 2, 1, 4, 4, 64), (2, 2, 1, 0, 4, 64), (2, 2, 1, 4, 0, 64)])
 def test_attention_of_nothing(b, h, hk, tq, tk, d):
     q, k, v = (torch.ones((b, n, t, d), device=DEV, dtype=BF, requires_grad=True)
@@ -298,6 +335,24 @@ def test_qk_norm_rope_one_result_used():
     _within("dw", dwk, res["dw"])
 
 
+def test_qk_norm_rope_without_keys():
+    g = _gen(23)
+    cos, sin = _tables(9, 64, BF)
+    q = _heads(g, 2, 4, 9, 64, BF).requires_grad_(True)
+    none = torch.empty((2, 0, 9, 64), device=DEV, dtype=BF, requires_grad=True)
+    w = [_randn(g, 64).requires_grad_(True) for _ in range(2)]
+    yq, yk = kotodama_amd.qk_norm_rope(q, none, *w, cos, sin, 1e-5)
+    want, _ = kotodama_amd.qk_norm_rope(q, q[:, :2], *w, cos, sin, 1e-5)
+    assert torch.equal(yq, want) and yk.shape == none.shape
+    dq, dk, dwq, dwk = torch.autograd.grad((yq, yk), (q, none, *w), (torch.ones_like(yq), torch.ones_like(yk)))
+    assert dk.shape == none.shape and not dwk.any() and dq.any() and dwq.any()
+
+
+def test_qk_norm_rope_of_many_heads():
+    _qk_case(1, 300, 130, 3, 64, BF, seed=9)  # more head rows than the backward's grid has
+    _qk_case(40, 6, 2, 1, 128, BF, seed=10)
+
+
 @pytest.mark.parametrize("b,t", [(0, 4), (2, 0)])
 def test_qk_norm_rope_of_nothing(b, t):
     leaves = [torch.ones(s, device=DEV, dtype=BF, requires_grad=True) for s in ((b, 2, t, 64), (b, 1, t, 64), (64,), (64,))]
@@ -366,6 +421,18 @@ def test_embedding_strides():
     (one,) = torch.autograd.grad(out.sum(), w)  # a broadcast gradient
     (two,) = torch.autograd.grad(kotodama_amd.embedding(ids, w), w, torch.ones_like(out))
     assert torch.equal(one, two)
+
+
+def test_embedding_of_one_id_without_dimensions():
+    _embed_case(torch.tensor(3, device=DEV), 7, 64, BF, scale=2.0)
+
+
+def test_embedding_in_an_empty_table():
+    w = torch.empty((0, 8), device=DEV, requires_grad=True)
+    out = kotodama_amd.embedding(torch.tensor([0, 1], device=DEV), w)
+    assert out.isnan().all() and out.shape == (2, 8)
+    (dw,) = torch.autograd.grad(out, w, torch.ones_like(out))
+    assert dw.shape == (0, 8)
 
 
 def test_embedding_of_nothing():
@@ -446,6 +513,38 @@ def test_another_stream():
         got = [out.detach(), *torch.autograd.grad(out, leaves, go)]
     torch.cuda.current_stream().wait_stream(side)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_two_threads_at_once():
+    import threading
+
+    cases = [_layer_inputs(50 + i) for i in range(2)]
+    want = []
+    for args, leaves, go in cases:
+        out = _layer(*args)
+        want.append([out.detach(), *torch.autograd.grad(out, leaves, go)])
+    torch.cuda.synchronize()
+    got, errors = [[], []], []
+
+    def work(i):
+        try:
+            args, leaves, go = cases[i]
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(10):
+                    out = _layer(*args)
+                    got[i] = [out.detach(), *torch.autograd.grad(out, leaves, go)]
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001 - reported below
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for a, b in zip(got, want):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
 def test_graphs_that_replay_in_turn():

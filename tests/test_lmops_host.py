@@ -46,9 +46,14 @@ def test_attention_refusals():
                dict(start=torch.zeros(2, dtype=torch.int16))):
         with pytest.raises(TypeError):
             _attn(**kw)
+    t = torch.empty(1, 1, 1, 64)
     with pytest.raises(ValueError, match="q_start"):
-        t = torch.empty(1, 1, 1, 64)
         kotodama_amd.attention(t, t, t, q_start=1 << 41)
+    for scale in (0.0, -0.5, float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="scale"):
+            kotodama_amd.attention(t, t, t, scale=scale)
+    with pytest.raises(TypeError, match="kv_lens"):
+        kotodama_amd.attention(t, t, t, kv_lens=[1])
 
 
 def test_qk_norm_rope_refusals():
@@ -101,10 +106,11 @@ def attention_fwd(b=2, h=4, hk=2, tq=5, tk=7, d=64, dt=BF, causal=1, scale=0.1, 
 def test_attention_abi_refusals():
     assert attention_fwd(b=0) == _capi.OK  # nothing to do: returns before any HIP call
     assert attention_fwd(tq=0) == _capi.OK
-    for kw in (dict(b=-1), dict(h=3), dict(hk=0), dict(tq=-1), dict(dt=5), dict(causal=2), dict(scale=float("nan")),
-               dict(q=None), dict(out=None), dict(index=7)):
+    for kw in (dict(b=-1), dict(h=3), dict(hk=0), dict(tq=-1), dict(dt=5), dict(causal=2), dict(scale=float("nan")), dict(scale=0.0),
+               dict(scale=-1.0), dict(scale=3e38), dict(q=None), dict(out=None), dict(index=7)):
         assert attention_fwd(**kw) == _capi.ERR_ARG, kw
-    for kw in (dict(d=4), dict(d=68), dict(d=136), dict(tk=1 << 31), dict(b=1 << 20, tq=1 << 20)):
+    for kw in (dict(d=4), dict(d=68), dict(d=136), dict(tk=1 << 31), dict(b=1 << 20, tq=1 << 20),
+               dict(h=8194, hk=2), dict(st=(4096, 64, 1 << 24))):
         assert attention_fwd(**kw) == _capi.ERR_UNSUPPORTED, kw
     for kw in (dict(q=FAKE + 8), dict(st=(4096, 64, 257)), dict(lens=FAKE + 2), dict(lens=FAKE + 4, index=1)):
         assert attention_fwd(**kw) == _capi.ERR_ALIGN, kw
@@ -138,7 +144,7 @@ def test_qk_norm_rope_abi_refusals():
     for kw in (dict(b=-1), dict(dt=9), dict(tdt=9), dict(dt=F32, tdt=BF), dict(q=None), dict(w=None), dict(cos=None),
                dict(ld=63), dict(eps=-1.0), dict(eps=float("nan")), dict(index=3), dict()):  # k_out is NULL in all
         assert fwd(**kw) == _capi.ERR_ARG, kw
-    for kw in (dict(d=3), dict(d=258)):
+    for kw in (dict(d=3), dict(d=258), dict(b=1 << 20, t=1 << 20)):
         assert fwd(**kw) == _capi.ERR_UNSUPPORTED, kw
     for kw in (dict(q=FAKE + 1), dict(cos=FAKE + 1), dict(pos=FAKE + 2)):
         assert fwd(**kw) == _capi.ERR_ALIGN, kw
@@ -156,6 +162,7 @@ def test_embedding_abi_refusals():
                dict(out=None), dict(index=2)):
         assert fwd(**kw) == _capi.ERR_ARG, kw
     assert fwd(n=1 << 31) == _capi.ERR_UNSUPPORTED
+    assert fwd(hidden=1 << 24, ld=1 << 24) == _capi.ERR_UNSUPPORTED
     assert fwd(ids=FAKE + 4) == _capi.ERR_ALIGN
     assert fwd(out=FAKE + 1) == _capi.ERR_ALIGN
     assert bwd(rows=0) == _capi.OK
