@@ -306,7 +306,7 @@ EmbedPlan embed_plan(int64_t n, int64_t rows, int hidden) {
   p.range = (int)range;
   p.ranges = (int)((rows + range - 1) / range);
   int64_t seg = 8;
-  while (seg < LM_EMBED_MAX_SEG && seg * 1024 < n) seg <<= 1;
+  while (seg < LM_EMBED_MAX_SEG && seg * 256 < n) seg <<= 1;
   p.seg = (int)seg;
   p.stretches = (n + seg - 1) / seg;
   p.at_rows = 256;
