@@ -101,7 +101,10 @@ __device__ __forceinline__ float group_sum(float v, int g) {
 //
 // A group of G lanes holds one head row, a lane the V elements from V l of
 // each half, so the rotation needs nothing from other lanes and the mean is a
-// sum over the group.  Bound by memory: one read and one write of a row.
+// sum over the group.  Bound by memory: one read and one write of a row.  8192
+// tokens x 12 heads x 128 in bf16: 10.8 us (50 MB at 4.6 TB/s), backward 18.7
+// (75 MB at 4.0) and 3.1 for the weights' partial rows; a copy runs at 5.0.
+// Four heads of a token per lane group share its table row (one: 11.8 us).
 
 // Lanes past the half (a group is a power of two) repeat its first elements,
 // so that no load has a branch, and count for nothing.
@@ -366,6 +369,8 @@ __device__ __forceinline__ void rope_dw_sum(const lm_rope_params& P, float* red)
 //          the stretch's ends is left as an fp32 partial row.  Further
 //          workgroups zero the rows without tokens.
 //   join   the crossing runs' partial rows are added in order.
+// 16384 tokens of a text's frequencies, 49152 x 4096 in bf16: 13 + 89 (530 MB
+// at 5.9 TB/s) + 9 us, the lookup 40 (190 MB or more at 4.7).
 
 template <typename T, int V>
 __device__ __forceinline__ void embedding_fwd(const lm_embed_params& P) {
@@ -589,7 +594,7 @@ __device__ __forceinline__ void add_partials(const lm_embed_params& P, int s, in
 // one of them and leaves it.  A run of few partial rows is one wave's; the
 // partial rows of a longer one are dealt out to the waves, and their sums
 // added in order.  (One stretch per workgroup spent 27 us on dispatching 16368
-// workgroups that mostly found no run, at 16384 tokens x 4096.)
+// workgroups that mostly found no run, at 16384 tokens x 4096 in stretches of 16.)
 template <typename T>
 __device__ __forceinline__ void embedding_join(const lm_embed_params& P, float* red) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
