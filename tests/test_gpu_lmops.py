@@ -588,6 +588,97 @@ def test_compiled_whole():
         assert (a.float() - b.float()).abs().max() <= 2.0**-5 * b.float().abs().max()
 
 
+class _Native:
+    """The native functions: ``taken`` counts the calls they took; with ``off`` they take none."""
+
+    def __init__(self, off):
+        self.off, self.taken = off, []
+
+    def __getattr__(self, name):
+        from kotodama_amd._native import native
+
+        def call(*args):
+            res = None if self.off else getattr(native, name)(*args)
+            if res is not None:
+                self.taken.append(name)
+            return res
+
+        return call
+
+
+@pytest.mark.parametrize("dtype", [BF, FP], ids=["bf16", "fp32"])
+def test_native_calls_equal_the_ops(monkeypatch, dtype):
+    # bit for bit, recorded and not, and the native path is the one that plain calls take
+    results = {}
+    for off in (False, True):
+        stub = _Native(off)
+        monkeypatch.setattr(lmops, "native", stub)
+        args, leaves, go = _layer_inputs(46, dtype)
+        out = _layer(*args)
+        res = [out.detach(), *torch.autograd.grad(out, leaves, go)]
+        q = _heads(_gen(47), 2, 4, 30, 64, dtype)
+        o, lse = kotodama_amd.attention(q, q[:, :2], q[:, 2:], want_lse=True, scale=0.2, q_start=-3)
+        results[off] = [*res, o, lse]
+        assert stub.taken == ([] if off else ["embedding", "qk_norm_rope", "attention", "attention"])
+    assert all(torch.equal(a, b) for a, b in zip(results[False], results[True]))
+
+
+def test_calls_left_to_the_ops(monkeypatch):
+    stub = _Native(False)
+    monkeypatch.setattr(lmops, "native", stub)
+    g = _gen(48)
+    q = _heads(g, 1, 2, 9, 64, BF)
+    odd = _randn(g, 1, 2, 9, 65)[..., 1:]
+    kotodama_amd.attention(odd, q, q)  # unaligned rows
+    kotodama_amd.embedding(torch.zeros((4, 4), device=DEV, dtype=torch.int64).t()[::2], _randn(g, 5, 8))
+    w = _randn(g, 64)
+    cos, sin = _tables(9, 64, BF)
+    kotodama_amd.qk_norm_rope(q.transpose(-1, -2).contiguous().transpose(-1, -2), q, w, w, cos, sin, 1e-5)
+    with torch.overrides.BaseTorchFunctionMode():
+        kotodama_amd.attention(q, q, q)
+    assert stub.taken == []
+
+
+@pytest.mark.parametrize("op", ["attention", "qk_norm_rope", "embedding"])
+def test_backward_under_compiled_autograd(op):
+    # the whole backward of a recorded native call is traced, without a graph break
+    def compiler(graph):
+        return torch.compile(graph, backend="aot_eager", fullgraph=True)
+
+    g = _gen(49)
+    q, k = _heads(g, 2, 4, 9, 64, FP).requires_grad_(True), _heads(g, 2, 2, 9, 64, FP).requires_grad_(True)
+    w = [_randn(g, 64, dtype=FP).requires_grad_(True) for _ in range(2)]
+    cos, sin = _tables(9, 64, FP)
+    ids = torch.randint(0, 64, (5, 7), generator=g, device=DEV)
+    lens = torch.tensor([9, 4], device=DEV)
+    calls = {
+        "attention": ((q, k), lambda: kotodama_amd.attention(q, k, k, kv_lens=lens, q_start=0)),
+        "qk_norm_rope": ((q, k, *w), lambda: sum(y.sum(1) for y in kotodama_amd.qk_norm_rope(q, k, *w, cos, sin, 1e-5))),
+        "embedding": ((q,), lambda: kotodama_amd.embedding(ids, q[0, 0].reshape(9, 64), scale=0.5)),
+    }
+    leaves, call = calls[op]
+    if op == "embedding":
+        ids.remainder_(9)
+    torch._dynamo.reset()
+    want = torch.autograd.grad(call().square().sum(), leaves)
+    for _ in range(2):
+        for t in leaves:
+            t.grad = None
+        loss = call().square().sum()
+        with torch._dynamo.compiled_autograd._enable(compiler):
+            loss.backward()
+        for t, x in zip(leaves, want):
+            torch.testing.assert_close(t.grad, x, rtol=1e-6, atol=1e-6)
+
+
+def test_recorded_calls_appear_in_a_profile():
+    args, leaves, go = _layer_inputs(51)
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU]) as prof:
+        torch.autograd.grad(_layer(*args), leaves, go)
+    seen = {e.key for e in prof.key_averages() if e.key.startswith("attnres_hip::")}
+    assert seen == {f"attnres_hip::{n}{d}" for n in ("attention", "qk_norm_rope", "embedding") for d in ("", "_bwd")}
+
+
 def test_op_registrations():
     args, _, _ = _layer_inputs(45)
     x, ids, table, w, norm, cos, sin, lens = args
