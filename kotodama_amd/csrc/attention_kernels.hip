@@ -138,8 +138,9 @@ struct F32 {
 
 // ------------------------------------------------------------- LDS tiles --
 
-// A tile of R rows of DP elements in LDS (layout in the head comment).
-template <typename T, int DP, int R>
+// A tile of R rows of DP elements in LDS (layout in the head comment), loaded
+// by WAVES waves.
+template <typename T, int DP, int R, int WAVES = LM_ATTN_WAVES>
 struct Tile {
   static constexpr int kRowBytes = DP * T::kBytes;
   static constexpr int kChunks = kRowBytes / 16;  // per row
@@ -151,47 +152,39 @@ struct Tile {
     return ((row & 6) | ((row >> 3) & 1));  // 8 chunks: row r and r + 1 share 256 bytes
   }
 
-  // A workgroup's load i of kRound rows each is one wave-wide load per wave.
-  static constexpr int kRound = LM_ATTN_WAVES * 64 / kChunks;
+  using Mine = Tile<T, DP, 32, 1>;  // 32 of its rows, loaded by the wave that reads them
+  // Round i, of kRound rows, is one wave-wide load per wave.
+  static constexpr int kRound = WAVES * 64 / kChunks;
   static constexpr int kRounds = R / kRound;
   static_assert(kRounds * kRound == R, "whole rounds");
 
-  // This lane's row within a round, and its chunk (even rounds; in odd ones
-  // ^ 1 where a round is 8 rows) among the `chunks` there are.
+  // This lane's row within a round, and the offset within the round of its part.
   static __device__ __forceinline__ int round_row(int wave, int lane) { return (wave * 64 + lane) / kChunks; }
-  static __device__ __forceinline__ int round_chunk(int wave, int lane, int chunks, int odd) {
-    const int c = (lane % kChunks) ^ place(round_row(wave, lane)) ^ (kRound == 8 ? odd : 0);
-    return c < chunks ? c : chunks - 1;
+  static __device__ __forceinline__ uint32_t chunk_offset(int round, int wave, int lane, int chunks) {
+    const int c = (lane % kChunks) ^ place(round * kRound + round_row(wave, lane));
+    return 16 * (uint32_t)(c < chunks ? c : chunks - 1);  // chunks past the row's end repeat its last
   }
 
-  // Offsets within a tile of this lane's part of its first two rounds, for rows `stride` bytes apart.
-  struct Lane {
-    uint32_t even, odd;
-  };
-  static __device__ __forceinline__ Lane lane_offsets(uint32_t stride, int chunks, int wave, int lane) {
-    const uint32_t row = (uint32_t)round_row(wave, lane) * stride;
-    return Lane{row + 16 * (uint32_t)round_chunk(wave, lane, chunks, 0),
-                row + 16 * (uint32_t)round_chunk(wave, lane, chunks, 1)};
-  }
-
-  // Request rows row0 .. row0+R-1 of `src` into `lds`.  Rows past `last` repeat
-  // it.  The base is uniform and the offset 32 bits wide, so a whole tile takes
-  // no address arithmetic in the vector unit.
+  // Request rows row0 .. row0+R-1 of `src` into `lds`.  Rows past `last` (at
+  // least row0) repeat it.  The base is uniform and the offset 32 bits wide; the
+  // places of rows 16 apart are the same, so that rounds of 16 rows or more
+  // share one offset.
   static __device__ __forceinline__ void request(char* lds, const char* src, int64_t stride, int row0, int last,
-                                                 const Lane& at, int chunks, int wave, int lane) {
+                                                 int chunks, int wave, int lane) {
     const char* base = src + (int64_t)row0 * stride;
     if (row0 + R - 1 <= last) {
+      const uint32_t row = (uint32_t)round_row(wave, lane) * (uint32_t)stride;
 #pragma unroll
       for (int i = 0; i < kRounds; ++i)
-        load_lds(lds + (i * LM_ATTN_WAVES + wave) * 1024, base + (int64_t)(i * kRound) * stride,
-                 (i & 1) ? at.odd : at.even);
+        load_lds(lds + (i * WAVES + wave) * 1024, base + (int64_t)(i * kRound) * stride,
+                 row + chunk_offset(i, wave, lane, chunks));
     } else {
 #pragma unroll
       for (int i = 0; i < kRounds; ++i) {
         int row = i * kRound + round_row(wave, lane);
         row = row < last - row0 ? row : last - row0;
-        load_lds(lds + (i * LM_ATTN_WAVES + wave) * 1024, base,
-                 (uint32_t)row * (uint32_t)stride + 16 * (uint32_t)round_chunk(wave, lane, chunks, i & 1));
+        load_lds(lds + (i * WAVES + wave) * 1024, base,
+                 (uint32_t)row * (uint32_t)stride + chunk_offset(i, wave, lane, chunks));
       }
     }
   }
@@ -462,31 +455,35 @@ struct Rows {
   }
 };
 
-// Runs step(t, k, v) over the key tiles t0 .. t1-1 in LDS: with two buffers each, tile t+1
-// is requested before t is worked on; with one, the other workgroup of the CU
-// works meanwhile.
+// Runs step(t, k, v) over the key tiles t0 .. t1-1 in LDS.  NBUF 2: the waves
+// share the tiles; tile t+1 is requested before t is worked on.  NBUF 1 (four
+// waves share their rows): each reads only its own 32 keys of a tile, so it
+// loads them itself, up to `most` keys, and no wave waits for another.
 template <typename KT, int NBUF, typename Step>
 __device__ __forceinline__ void over_keys(const char* kp, int64_t kst, const char* vp, int64_t vst, int t0, int t1,
-                                          int last, int chunks, int wave, int lane, char* k0, char* k1, char* v0, char* v1,
-                                          Step&& step) {
-  const typename KT::Lane ka = KT::lane_offsets((uint32_t)kst, chunks, wave, lane);
-  const typename KT::Lane va = KT::lane_offsets((uint32_t)vst, chunks, wave, lane);
-  auto request = [&](int t, char* k, char* v) {
-    KT::request(k, kp, kst, t * KT::kRows, last, ka, chunks, wave, lane);
-    KT::request(v, vp, vst, t * KT::kRows, last, va, chunks, wave, lane);
-  };
-  auto arrived = [] {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-  };
+                                          int last, int chunks, int wave, int lane, int most, char* k0, char* k1,
+                                          char* v0, char* v1, Step&& step) {
   if constexpr (NBUF == 1) {
-    for (int t = t0; t < t1; ++t) {
-      if (t > t0) __syncthreads();
-      request(t, k0, v0);
-      arrived();
+    using MT = typename KT::Mine;
+    static_assert(KT::kRows == 32 * LM_ATTN_WAVES, "a tile has 32 keys for each wave");
+    const int own = 32 * wave;
+    for (int t = t0; t < t1 && t * KT::kRows + own < most; ++t) {
+      int ln = lane;  // opaque: offsets formed anew for each tile instead of held in registers
+      asm volatile("" : "+v"(ln));
+      MT::request(k0 + own * KT::kRowBytes, kp, kst, t * KT::kRows + own, last, chunks, 0, ln);
+      MT::request(v0 + own * KT::kRowBytes, vp, vst, t * KT::kRows + own, last, chunks, 0, ln);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       step(t, k0, v0);
     }
   } else {
+    auto request = [&](int t, char* k, char* v) {
+      KT::request(k, kp, kst, t * KT::kRows, last, chunks, wave, lane);
+      KT::request(v, vp, vst, t * KT::kRows, last, chunks, wave, lane);
+    };
+    auto arrived = [] {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+    };
     if (t0 < t1) request(t0, k0, v0);
     for (int t = t0; t < t1; t += 2) {
       arrived();
@@ -550,7 +547,8 @@ __device__ __forceinline__ void attention_fwd(const lm_attn_params& P, char* k0,
   const int row_at = KT::row_at(lane), col_at = KT::col_at(lane);
 
   over_keys<KT, NBUF>(
-      kp, P.sk.t * T::kBytes, vp, P.sv.t * T::kBytes, R.t0, R.t1, R.S.kv_len - 1, chunks, R.wave, lane, k0, k1, v0, v1,
+      kp, P.sk.t * T::kBytes, vp, P.sv.t * T::kBytes, R.t0, R.t1, R.S.kv_len - 1, chunks, R.wave, lane, R.mine.most, k0,
+      k1, v0, v1,
       [&](int t, const char* kc, const char* vc) {
         constexpr int NB = RW::kBlocks;
         const int first = KS == 1 ? 0 : 32 * NB * R.part;  // this wave's keys of the tile
@@ -773,7 +771,7 @@ __device__ __forceinline__ void attention_bwd_dq(const lm_attn_params& P, char* 
     if (R.t1 * RW::kKeys <= kExactKeys && R.t1 > 0) {
       float d = 0.f;
       over_keys<KT, NBUF>(kp, P.sk.t * T::kBytes, vp, P.sv.t * T::kBytes, 0, R.t1, R.S.kv_len - 1, chunks, R.wave, lane,
-                          k0, k1, v0, v1, [&](int t, const char* kc, const char* vc) {
+                          R.mine.most, k0, k1, v0, v1, [&](int t, const char* kc, const char* vc) {
 #pragma unroll
                             for (int kb = 0; kb < NB; ++kb) {
                               const int key0 = t * RW::kKeys + mine + 32 * kb;
@@ -802,8 +800,8 @@ __device__ __forceinline__ void attention_bwd_dq(const lm_attn_params& P, char* 
   f32x16 acc[DC / 32];
 #pragma unroll
   for (int i = 0; i < DC / 32; ++i) acc[i] = zero16();
-  over_keys<KT, NBUF>(kp, P.sk.t * T::kBytes, vp, P.sv.t * T::kBytes, 0, R.t1, R.S.kv_len - 1, chunks, R.wave, lane, k0,
-                      k1, v0, v1, [&](int t, const char* kc, const char* vc) {
+  over_keys<KT, NBUF>(kp, P.sk.t * T::kBytes, vp, P.sv.t * T::kBytes, 0, R.t1, R.S.kv_len - 1, chunks, R.wave, lane,
+                      R.mine.most, k0, k1, v0, v1, [&](int t, const char* kc, const char* vc) {
 #pragma unroll
                         for (int kb = 0; kb < NB; ++kb) {
                           const int key0 = t * RW::kKeys + mine + 32 * kb;
@@ -893,13 +891,21 @@ __device__ __forceinline__ void attention_bwd_dkv(const lm_attn_params& P, char*
   int64_t stat = ((int64_t)b * P.heads + kvh * group) * P.q_len;
   int next = 0;  // the tile of its head to request
   auto request = [&](char* qn, char* gn, float* sn) {
-    const int row0 = base + next * R;
     int ln = lane;  // opaque: the lane's offsets are formed anew for each tile, registers being short
     asm volatile("" : "+v"(ln));
-    QT::request(qn, qp, qst, row0, S.hi - 1, QT::lane_offsets((uint32_t)qst, chunks, wave, ln), chunks, wave, ln);
-    QT::request(gn, gp, gst, row0, S.hi - 1, QT::lane_offsets((uint32_t)gst, chunks, wave, ln), chunks, wave, ln);
+    if constexpr (NBUF == 1) {  // this wave's own 32 rows, where there are any
+      using MT = typename QT::Mine;
+      const int row0 = base + next * R + 32 * wave;
+      if (row0 < S.hi) {
+        MT::request(qn + 32 * wave * QT::kRowBytes, qp, qst, row0, S.hi - 1, chunks, 0, ln);
+        MT::request(gn + 32 * wave * QT::kRowBytes, gp, gst, row0, S.hi - 1, chunks, 0, ln);
+      }
+    } else {
+      QT::request(qn, qp, qst, base + next * R, S.hi - 1, chunks, wave, ln);
+      QT::request(gn, gp, gst, base + next * R, S.hi - 1, chunks, wave, ln);
+    }
     if (wave < KS) {  // the queries' lse (lanes 0 .. 31) and delta, 32 a wave
-      int r = row0 + wave * 32 + (ln & 31);
+      int r = base + next * R + wave * 32 + (ln & 31);
       r = r < S.hi ? r : S.hi - 1;
       const float* src = ((ln >> 5) ? P.delta : P.lse) + stat + r;
       __builtin_amdgcn_global_load_lds((const LM_GLOBAL void*)src, (LM_LDS void*)(sn + wave * 64), 4, 0, 0);
@@ -967,11 +973,11 @@ __device__ __forceinline__ void attention_bwd_dkv(const lm_attn_params& P, char*
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
   };
-  if constexpr (NBUF == 1) {
+  if constexpr (NBUF == 1) {  // four waves share their keys: each loads the rows it reads itself
+    static_assert(KS == LM_ATTN_WAVES, "a tile has 32 rows for each wave");
     for (int t = 0; t < tiles; ++t) {
-      if (t > 0) __syncthreads();
       request(q0, g0, st0);
-      arrived();
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       step(q0, g0, st0);
     }
   } else {
