@@ -525,7 +525,7 @@ __device__ __forceinline__ void add(const float* x, f32x16 (&acc)[DC / 32], int 
 // reaches 1.17).  There matrix, vector and LDS units are busy 48, 44 and 37% of
 // the cycles, at a clock that the load holds to 1.8 GHz: two waves a SIMD
 // overlap them in part.  One token over 32768 keys (8 key heads): 27 us, its
-// 134 MB at 5.0 TB/s, and 6 us for the join.
+// 134 MB at 5.0 TB/s, and 4 us for the join of 64 parts.
 template <typename T, int DP, int DC, int KS, int NBUF>
 __device__ __forceinline__ void attention_fwd(const lm_attn_params& P, char* k0, char* k1, char* v0, char* v1,
                                               float* ml) {
@@ -642,7 +642,7 @@ __device__ __forceinline__ void attention_fwd(const lm_attn_params& P, char* k0,
     if (P.splits > 1) {  // this part's sums as they stand, for the join
       if (!R.exists) return;
       const int64_t at = R.index(P) * P.splits + R.split;
-      if (l > 0.f) store_rows<F32, DC>(reinterpret_cast<char*>(P.part + at * P.dim), acc, 1.f, P.dim, h);
+      if (l != 0.f) store_rows<F32, DC>(reinterpret_cast<char*>(P.part + at * P.dim), acc, 1.f, P.dim, h);
       if (h == 0) {
         P.part_ml[at * 2] = m;
         P.part_ml[at * 2 + 1] = l;
@@ -651,16 +651,19 @@ __device__ __forceinline__ void attention_fwd(const lm_attn_params& P, char* k0,
     }
   }
   if (R.exists) {
-    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const float inv = l == 0.f ? 0.f : 1.f / l;  // a NaN stays one
     store_rows<T, DC>((char*)P.o + row_offset(P.so, R.b, R.head, R.query) * T::kBytes, acc, inv, P.dim, h);
-    if (P.lse != nullptr && h == 0) P.lse[R.stat(P)] = l > 0.f ? (m + __builtin_amdgcn_logf(l)) * kLn2 : kNegInf;
+    if (P.lse != nullptr && h == 0) P.lse[R.stat(P)] = l == 0.f ? kNegInf : (m + __builtin_amdgcn_logf(l)) * kLn2;
   }
 }
 
-// Joins the parts of a row: a workgroup per row, 32 lanes over its columns (four
-// each), eight parts at a time.
+// Joins the parts of a row (64 parts of 32 rows: 4.0 us, 6.3 with the parts'
+// weights found on the way): a workgroup per row, 32 lanes over its columns (four
+// each), eight parts at a time.  All of a row's maxima and sums are requested
+// together with the first parts, so that the join is one round trip to memory
+// for up to 64 parts.  weights: one float per part.
 template <typename T>
-__device__ __forceinline__ void attention_join(const lm_attn_params& P, float* red) {
+__device__ __forceinline__ void attention_join(const lm_attn_params& P, float* red, float* weights) {
   const int group = P.heads / P.kv_heads, rows = P.q_len * group;
   const int64_t at = blockIdx.x;
   const int row = (int)(at % rows), query = row / group;
@@ -668,24 +671,47 @@ __device__ __forceinline__ void attention_join(const lm_attn_params& P, float* r
   const int head = kvh * group + (row - query * group);
   const int lane = threadIdx.x & 63;
   const float* ml = P.part_ml + at * P.splits * 2;
-  // every wave: the common maximum and the sum
-  float m = kNegInf;
-  for (int s = lane; s < P.splits; s += 64) m = fmaxf(m, ml[2 * s]);
-  for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
-  float l = 0.f;
-  for (int s = lane; s < P.splits; s += 64) l += ml[2 * s] == kNegInf ? 0.f : ml[2 * s + 1] * exp2_fast(ml[2 * s] - m);
-  for (int o = 1; o < 64; o <<= 1) l += __shfl_xor(l, o);
   const int d = 4 * (threadIdx.x & 31), part = threadIdx.x >> 5;
-  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-  if (d < P.dim) {
-#pragma unroll 4
-    for (int s = part; s < P.splits; s += 8) {
-      const float ms = ml[2 * s];
-      if (ms == kNegInf) continue;  // saw no key: nothing was written
-      const float w = exp2_fast(ms - m);
-      const f32x4 v = *reinterpret_cast<const f32x4*>(P.part + (at * P.splits + s) * P.dim + d);
+  const float* rowp = P.part + at * P.splits * P.dim + (d < P.dim ? d : 0);
+  constexpr int U = 8;
+  f32x4 v[U];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sum[j] = __builtin_fmaf(v[j], w, sum[j]);
+  for (int u = 0; u < U; ++u) {
+    const int s = part + 8 * u < P.splits ? part + 8 * u : 0;
+    v[u] = *reinterpret_cast<const f32x4*>(rowp + (int64_t)s * P.dim);
+  }
+  // every wave: the common maximum and the sum; wave 0: the parts' weights
+  float ms[LM_ATTN_MAX_SPLITS / 64], ls[LM_ATTN_MAX_SPLITS / 64], m = kNegInf, l = 0.f;
+#pragma unroll
+  for (int i = 0; i < LM_ATTN_MAX_SPLITS / 64; ++i) {
+    const int s = i * 64 + lane;
+    ms[i] = s < P.splits ? ml[2 * s] : kNegInf;
+    ls[i] = s < P.splits ? ml[2 * s + 1] : 0.f;
+    m = fmaxf(m, ms[i]);
+  }
+  for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+#pragma unroll
+  for (int i = 0; i < LM_ATTN_MAX_SPLITS / 64; ++i) {
+    const float w = ls[i] == 0.f ? 0.f : exp2_fast(ms[i] - m);  // 0: saw no key, nothing was written
+    l = __builtin_fmaf(w, ls[i], l);
+    if (threadIdx.x < 64 && i * 64 + lane < P.splits) weights[i * 64 + lane] = w;
+  }
+  for (int o = 1; o < 64; o <<= 1) l += __shfl_xor(l, o);
+  __syncthreads();
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = part; s0 < P.splits; s0 += 8 * U) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float w = s0 + 8 * u < P.splits ? weights[s0 + 8 * u] : 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum[j] = w != 0.f ? __builtin_fmaf(v[u][j], w, sum[j]) : sum[j];
+    }
+    if (s0 + 8 * U < P.splits) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int s = s0 + 8 * (U + u) < P.splits ? s0 + 8 * (U + u) : 0;
+        v[u] = *reinterpret_cast<const f32x4*>(rowp + (int64_t)s * P.dim);
+      }
     }
   }
   *reinterpret_cast<f32x4*>(red + threadIdx.x * 4) = sum;
@@ -693,16 +719,16 @@ __device__ __forceinline__ void attention_join(const lm_attn_params& P, float* r
   if (threadIdx.x < 32 && d < P.dim) {
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     for (int p = 0; p < 8; ++p) {
-      const f32x4 v = *reinterpret_cast<const f32x4*>(red + (p * 32 + threadIdx.x) * 4);
+      const f32x4 x = *reinterpret_cast<const f32x4*>(red + (p * 32 + threadIdx.x) * 4);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] += v[j];
+      for (int j = 0; j < 4; ++j) o[j] += x[j];
     }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const float inv = l == 0.f ? 0.f : 1.f / l;  // a NaN stays one
     store4<T>((char*)P.o + (row_offset(P.so, b, head, query) + d) * T::kBytes, o[0] * inv, o[1] * inv, o[2] * inv,
               o[3] * inv);
     if (P.lse != nullptr && threadIdx.x == 0)
       P.lse[((int64_t)b * P.heads + head) * P.q_len + query] =
-          l > 0.f ? (m + __builtin_amdgcn_logf(l)) * kLn2 : kNegInf;
+          l == 0.f ? kNegInf : (m + __builtin_amdgcn_logf(l)) * kLn2;
   }
 }
 
@@ -1057,7 +1083,8 @@ __device__ __forceinline__ void attention_bwd_dkv(const lm_attn_params& P, char*
 #define LM_ATTN_JOIN(NAME, T)                                                                       \
   extern "C" __global__ void __launch_bounds__(256) attnres_attention_join_##NAME(lm_attn_params P) { \
     __shared__ __align__(16) float red[1024];                                                       \
-    attention_join<T>(P, red);                                                                      \
+    __shared__ float weights[LM_ATTN_MAX_SPLITS];                                                   \
+    attention_join<T>(P, red, weights);                                                             \
   }
 
 #if LM_PART == 13

@@ -158,7 +158,7 @@ AttnPlan attention_plan(int base, int64_t heads, int64_t lines, int64_t kv_slots
     const int64_t least = heads * lines <= (int64_t)cus * 4 ? 1 : 4;
     const int64_t most = (kv_slots + 127) / 128 / least, want = (int64_t)cus * kSplitPerCu / (waves > 0 ? waves : 1);
     const int64_t n = want < most ? want : most;
-    p.splits = n < 2 ? 1 : (int)n;
+    p.splits = n < 2 ? 1 : n < LM_ATTN_MAX_SPLITS ? (int)n : LM_ATTN_MAX_SPLITS;
   }
   return p;
 }

@@ -12,6 +12,7 @@
 
 #define LM_ATTN_WAVES 4 /* waves per workgroup of the attention kernels; a wave owns 32 rows or 32 keys */
 #define LM_ATTN_MAX_DIM 128
+#define LM_ATTN_MAX_SPLITS 512 /* parts of the key axis */
 
 /* Strides in elements; element (b, h, t, d) of X at X + b*sb + h*sh + t*st + d. */
 typedef struct lm_strides {

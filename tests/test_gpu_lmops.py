@@ -105,6 +105,66 @@ def test_attention_of_many_rows(dtype, b, h, hk, tq, tk, d, causal, lens, start)
 
 
 @pytest.mark.parametrize("dtype", [BF, FP], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("b,h,hk,tq,tk,d,lens", [
+    (1, 1, 1, 1, 70000, 64, None),      # more parts than a workgroup's waves hold at once
+    (1, 3, 1, 2, 9000, 128, None),
+    (5, 4, 2, 1, 3000, 80, [3000, 1, 0, 129, 2500]),  # parts without keys
+    (2, 2, 2, 40, 5000, 128, [5000, 41]),
+])
+def test_attention_over_a_split_cache(dtype, b, h, hk, tq, tk, d, lens):
+    g = _gen(tk)
+    print(f"attention over a cache b={b} h={h}/{hk} q={tq} k={tk} d={d} {dtype} lens={lens}", flush=True)
+    q, k, v = _heads(g, b, h, tq, d, dtype, 1.5), _heads(g, b, hk, tk, d, dtype), _heads(g, b, hk, tk, d, dtype)
+    kv_lens = None if lens is None else torch.tensor(lens, device=DEV)
+    if lens is not None:  # what is not written yet
+        gone = torch.arange(tk, device=DEV)[None, None, :, None] >= kv_lens[:, None, None, None]
+        k, v = k.masked_fill(gone, math.nan), v.masked_fill(gone, math.inf)
+    out, lse = kotodama_amd.attention(q, k, v, kv_lens=kv_lens, want_lse=True)
+    res = LO.attention(q, k, v, kv_lens=lens)
+    _within("out", out, res["out"])
+    _within("lse", lse, res["lse"])
+
+
+@pytest.mark.parametrize("dtype", [BF, FP], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("tq,tk", [(1, 9000), (1, 100), (70, 70), (300, 5000)])
+def test_attention_shows_a_nan(dtype, tq, tk):
+    # a row that sees a NaN is one, whether its keys are split over workgroups or not
+    g = _gen(tk + 1)
+    b, h, hk, d = 2, 4, 2, 64
+    q, k, v = _heads(g, b, h, tq, d, dtype), _heads(g, b, hk, tk, d, dtype), _heads(g, b, hk, tk, d, dtype)
+    print(f"attention of a NaN q={tq} k={tk} {dtype}", flush=True)
+    out, lse = kotodama_amd.attention(q, k, v, causal=False, want_lse=True)
+    for which in range(3):
+        bad = [q.clone(), k.clone(), v.clone()]
+        at = (1, 2, tq - 1) if which == 0 else (1, 1, tk // 2)
+        bad[which][at][3] = math.nan
+        got, got_lse = kotodama_amd.attention(*bad, causal=False, want_lse=True)
+        hit = torch.zeros((b, h, tq), dtype=torch.bool, device=DEV)
+        if which == 0:
+            hit[at] = True
+        else:
+            hit[1, 2:] = True  # both query heads of the key head
+        if which == 2:
+            assert got[..., 3][hit].isnan().all() and torch.equal(got_lse, lse)
+        else:
+            assert got[hit].isnan().all() and got_lse[hit].isnan().all()
+            assert torch.equal(got_lse[~hit], lse[~hit])
+        assert torch.equal(got[~hit], out[~hit])
+
+
+def test_attention_gradient_shows_a_nan():
+    g = _gen(2)
+    q, k, v, go = (_heads(g, 1, 2, 40, 64, BF) for _ in range(4))
+    q[0, 1, 7, 0] = math.nan
+    leaves = [x.requires_grad_(True) for x in (q, k, v)]
+    dq, dk, dv = torch.autograd.grad(kotodama_amd.attention(*leaves), leaves, go)
+    seen = torch.arange(40, device=DEV) <= 7
+    assert dq[0, 1, 7].isnan().all() and not dq[0, 1, 8:].isnan().any() and not dq[0, 0].isnan().any()
+    assert dk[0, 1, seen].isnan().all() and dv[0, 1, seen].isnan().all()
+    assert not dk[0, 0].isnan().any() and not dv[0, 0].isnan().any()
+
+
+@pytest.mark.parametrize("dtype", [BF, FP], ids=["bf16", "fp32"])
 def test_attention_of_wide_groups(dtype):
     _attention_case(1, 33, 1, 5, 70, 64, dtype, seed=5)
     _attention_case(1, 200, 2, 3, 40, 128, dtype, seed=6, lens=[30])
