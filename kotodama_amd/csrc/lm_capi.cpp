@@ -56,6 +56,8 @@ bool aligned(const void* p, int n) { return ((uintptr_t)p & (uintptr_t)(n - 1)) 
 template <typename Params>
 int launch(int slot, int part, const char* name, unsigned gx, unsigned gy, unsigned block, unsigned lds, Params& P,
            void* stream) {
+  if ((uint64_t)gx * block > UINT32_MAX)  // a launch's threads along one axis
+    return fail(ATTNRES_ERR_UNSUPPORTED, "%s: too many rows for one call", name);
   hipFunction_t f = nullptr;
   int cus = 0;
   int rc = attnres_internal_kernel(slot, part, name, &f, &cus);

@@ -522,8 +522,12 @@ __device__ __forceinline__ void embedding_sum(const lm_embed_params& P) {
   const int toks = P.sorted_token[k], rows = P.sorted_row[k];
   const int before = s0 > 0 ? P.sorted_row[s0 - 1] : -1;
   const int after = s1 < count ? P.sorted_row[s1] : -1;
-  const int c = blockIdx.y * blockDim.x + threadIdx.x;
-  if (c * V >= P.dim) return;
+  // Lanes past the row's end stay on, as they hold tokens and rows that the
+  // others read: they sum its first columns and write nothing.
+  const int at = blockIdx.y * blockDim.x + threadIdx.x;
+  if ((at - lane) * V >= P.dim) return;
+  const bool writes = at * V < P.dim;
+  const int c = writes ? at : 0;
   float acc[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) acc[j] = 0.f;
@@ -531,7 +535,8 @@ __device__ __forceinline__ void embedding_sum(const lm_embed_params& P) {
   auto flush = [&](bool end) {
     // crossing the start: partial 0; crossing the end only: partial 1
     const bool head = row == before, tail = end && row == after;
-    if (head || tail) {
+    if (!writes) {
+    } else if (head || tail) {
       float* p = P.part + ((int64_t)blockIdx.x * 2 + (head ? 0 : 1)) * P.dim + c * V;
 #pragma unroll
       for (int j = 0; j < V; ++j) p[j] = acc[j];

@@ -19,6 +19,8 @@ struct Strides {
   Strides(const Tensor& t, bool align) {
     if (!t.defined() || !dense(t) || !dtype_ok(t.scalar_type()) || t.dim() != 4) return;
     if (t.size(3) > 1 && t.stride(3) != 1) return;
+    for (const int64_t n : t.sizes())
+      if (n > INT32_MAX) return;
     const int64_t m = 16 / (int64_t)t.element_size();
     if (align && (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15) != 0) return;
     for (int i = 0; i < 3; ++i) {
@@ -267,7 +269,7 @@ struct NormRope : public torch::autograd::Function<NormRope> {
 // -------------------------------------------------------------- embedding --
 
 bool table(const Tensor& t) {
-  return dense(t) && dtype_ok(t.scalar_type()) && t.dim() == 2 && t.size(1) > 0 &&
+  return dense(t) && dtype_ok(t.scalar_type()) && t.dim() == 2 && t.size(1) > 0 && t.size(1) <= INT32_MAX &&
          (t.stride(1) == 1 || t.size(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1));
 }
 
@@ -285,8 +287,8 @@ bool embedding_rows(const Tensor& ids, const Tensor& w, double scale, Tensor* ou
 
 bool embedding_rows_bwd(const Tensor& ids, const Tensor& go, at::ScalarType dtype, int64_t rows, double scale,
                         int64_t padding, Tensor* dw) {
-  if (!plain(go) || go.scalar_type() != dtype || go.dim() < 1 || go.size(-1) < 1 || !index_tensor(ids, go) ||
-      !ids.is_contiguous())
+  if (!plain(go) || go.scalar_type() != dtype || go.dim() < 1 || go.size(-1) < 1 || go.size(-1) > INT32_MAX ||
+      !index_tensor(ids, go) || !ids.is_contiguous())
     return false;
   ATTNRES_RECORD("attnres_hip::embedding_bwd");
   const int64_t hidden = go.size(-1);

@@ -55,6 +55,13 @@ def _same_dtype(op: str, **tensors: Tensor) -> None:
             raise TypeError(f"{op}: {n} is {t.dtype}, {next(iter(tensors))} is {first}")
 
 
+def _check_sizes(op: str, *tensors: Tensor) -> None:
+    """The C calls take most sizes as 32-bit numbers."""
+    for t in tensors:
+        if max(t.shape, default=0) >= 1 << 31:
+            raise ValueError(f"{op}: a size of {max(t.shape)} is over 2^31")
+
+
 _i64x3 = ctypes.c_int64 * 3
 
 
@@ -141,6 +148,7 @@ def _qk_args(q, k, q_weight, k_weight, cos, sin, positions, eps) -> tuple:
 def _qk_norm_rope_impl(q, k, q_weight, k_weight, cos, sin, positions, eps) -> tuple[Tensor, Tensor]:
     device = _require_device(q, k, q_weight, k_weight, cos, sin, positions)
     _check_qk(q, k, q_weight, k_weight, cos, sin, positions)
+    _check_sizes("qk_norm_rope", q, k)
     q, k, cos, sin = _rows(q), _rows(k), _table(cos), _table(sin)
     q_weight, k_weight = q_weight.contiguous(), k_weight.contiguous()
     b, h, t, d = q.shape
@@ -166,6 +174,7 @@ def _qk_norm_rope_fake(q, k, q_weight, k_weight, cos, sin, positions, eps):
 def _qk_norm_rope_bwd_impl(q, k, q_weight, k_weight, cos, sin, positions, eps, grad_q, grad_k):
     device = _require_device(q, k, q_weight, k_weight, cos, sin, positions, grad_q, grad_k)
     _check_qk(q, k, q_weight, k_weight, cos, sin, positions)
+    _check_sizes("qk_norm_rope", q, k)
     q, k, cos, sin = _rows(q), _rows(k), _table(cos), _table(sin)
     q_weight, k_weight = q_weight.contiguous(), k_weight.contiguous()
     grad_q, grad_k = _rows(grad_q.to(q.dtype)), _rows(grad_k.to(k.dtype))
@@ -271,6 +280,7 @@ def _attn_index(kv_lens: Optional[Tensor], q_start: Optional[Tensor]) -> tuple:
 def _attention_impl(q, k, v, causal, scale, kv_lens, q_start, q_start_value, want_lse=True):
     device = _require_device(q, k, v, kv_lens, q_start)
     _check_attention(q, k, v, kv_lens, q_start)
+    _check_sizes("attention", q, k)
     q, k, v = _chunked(q), _chunked(k), _chunked(v)
     kv_lens, q_start, index = _attn_index(kv_lens, q_start)
     b, h, tq, d = q.shape
@@ -302,6 +312,7 @@ def _attention_fake(q, k, v, causal, scale, kv_lens, q_start, q_start_value):
 def _attention_bwd_impl(q, k, v, out, lse, grad_out, grad_lse, causal, scale, kv_lens, q_start, q_start_value):
     device = _require_device(q, k, v, out, lse, grad_out, grad_lse, kv_lens, q_start)
     _check_attention(q, k, v, kv_lens, q_start)
+    _check_sizes("attention", q, k)
     q, k, v, out, grad_out = _chunked(q), _chunked(k), _chunked(v), _chunked(out), _chunked(grad_out.to(q.dtype))
     lse = lse.contiguous()
     grad_lse = None if grad_lse is None else grad_lse.to(torch.float32).contiguous()
@@ -421,6 +432,7 @@ def _check_embedding(ids: Tensor, weight: Tensor, padding_idx: int) -> None:
 def _embedding_impl(ids, weight, scale, padding_idx) -> Tensor:
     device = _require_device(ids, weight)
     _check_embedding(ids, weight, padding_idx)
+    _check_sizes("embedding", weight)
     weight, flat = _table(weight), ids.contiguous()
     out = torch.empty((*ids.shape, weight.shape[1]), device=device, dtype=weight.dtype)
     with _DeviceStream(device) as stream:

@@ -449,6 +449,14 @@ def test_embedding(dtype, n, rows, hidden):
     _embed_case(ids, rows, hidden, dtype, scale=1.5)
 
 
+@pytest.mark.parametrize("dtype", [BF, FP], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("hidden", [257, 260, 520, 1031])
+def test_embedding_of_long_stretches_by_few_lanes(dtype, hidden):
+    # stretches of 64 tokens, rows whose last columns a few lanes of a wave hold
+    ids = torch.randint(0, 700, (20000,), generator=_gen(hidden), device=DEV)
+    _embed_case(ids, 700, hidden, dtype, scale=0.5, padding_idx=3)
+
+
 @pytest.mark.parametrize("index", [torch.int32, torch.int64])
 def test_embedding_skewed_and_padded(index):
     g = _gen(30)

@@ -56,6 +56,12 @@ def test_attention_refusals():
         kotodama_amd.attention(t, t, t, kv_lens=[1])
 
 
+def test_sizes_over_32_bits_are_refused():
+    lmops._check_sizes("x", torch.empty((2**31 - 1, 2), device="meta"), torch.empty((), device="meta"))
+    with pytest.raises(ValueError, match="2\\^31"):
+        lmops._check_sizes("x", torch.empty((1, 2**31), device="meta"))
+
+
 def test_qk_norm_rope_refusals():
     def check(q=(2, 4, 5, 64), k=(2, 2, 5, 64), w=(64,), cos=(9, 64), sin=None, dt=torch.bfloat16, tdt=None, pos=None,
               wdt=None):
