@@ -93,9 +93,12 @@ bool attention_rows(const AttnCall& c, bool want_lse, Tensor* out, Tensor* lse) 
 
 bool attention_rows_bwd(const AttnCall& c, const Tensor& out, const Tensor& lse, Tensor go, const Tensor& gl,
                         Tensor* dq, Tensor* dk, Tensor* dv) {
-  if (!c.fits() || !go.is_cuda() || go.scalar_type() != c.q.scalar_type() || go.sizes() != c.q.sizes() ||
-      go.get_device() != c.q.get_device())
-    return false;
+  if (!c.fits()) return false;
+  // what was saved passes through the caller's saved-tensor hooks
+  for (const Tensor* t : {static_cast<const Tensor*>(&go), &out})
+    if (!t->is_cuda() || t->scalar_type() != c.q.scalar_type() || t->sizes() != c.q.sizes() ||
+        t->get_device() != c.q.get_device())
+      return false;
   Strides sgo(go, true);
   if (!sgo.ok) {
     if (!dense(go)) return false;
@@ -103,7 +106,9 @@ bool attention_rows_bwd(const AttnCall& c, const Tensor& out, const Tensor& lse,
     sgo = Strides(go, true);
   }
   const Strides sq(c.q, true), sk(c.k, true), sv(c.v, true), so(out, true);
-  if (!sq.ok || !sk.ok || !sv.ok || !so.ok || !sgo.ok || !plain(lse)) return false;
+  if (!sq.ok || !sk.ok || !sv.ok || !so.ok || !sgo.ok || !plain(lse) || lse.scalar_type() != at::kFloat ||
+      lse.sizes() != c.q.sizes().slice(0, 3) || lse.get_device() != c.q.get_device())
+    return false;
   if (gl.defined() && (!plain(gl) || gl.scalar_type() != at::kFloat || gl.sizes() != lse.sizes() ||
                        gl.get_device() != c.q.get_device()))
     return false;
@@ -288,7 +293,7 @@ bool embedding_rows(const Tensor& ids, const Tensor& w, double scale, Tensor* ou
 bool embedding_rows_bwd(const Tensor& ids, const Tensor& go, at::ScalarType dtype, int64_t rows, double scale,
                         int64_t padding, Tensor* dw) {
   if (!plain(go) || go.scalar_type() != dtype || go.dim() < 1 || go.size(-1) < 1 || go.size(-1) > INT32_MAX ||
-      !index_tensor(ids, go) || !ids.is_contiguous())
+      !index_tensor(ids, go) || !ids.is_contiguous() || ids.sizes() != go.sizes().slice(0, go.dim() - 1))
     return false;
   ATTNRES_RECORD("attnres_hip::embedding_bwd");
   const int64_t hidden = go.size(-1);

@@ -55,6 +55,16 @@ def _same_dtype(op: str, **tensors: Tensor) -> None:
             raise TypeError(f"{op}: {n} is {t.dtype}, {next(iter(tensors))} is {first}")
 
 
+def _check_like(op: str, name: str, t: Optional[Tensor], shape, dtype: Optional[torch.dtype] = None) -> None:
+    """A gradient or saved result that the kernels read at the sizes of the inputs."""
+    if t is None:
+        return
+    if t.shape != shape:
+        raise ValueError(f"{op}: {name} must be {tuple(shape)}, got {tuple(t.shape)}")
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f"{op}: {name} must be {dtype}, got {t.dtype}")
+
+
 def _check_sizes(op: str, *tensors: Tensor) -> None:
     """The C calls take most sizes as 32-bit numbers."""
     for t in tensors:
@@ -175,6 +185,8 @@ def _qk_norm_rope_bwd_impl(q, k, q_weight, k_weight, cos, sin, positions, eps, g
     device = _require_device(q, k, q_weight, k_weight, cos, sin, positions, grad_q, grad_k)
     _check_qk(q, k, q_weight, k_weight, cos, sin, positions)
     _check_sizes("qk_norm_rope", q, k)
+    _check_like("qk_norm_rope_bwd", "grad_q", grad_q, q.shape)
+    _check_like("qk_norm_rope_bwd", "grad_k", grad_k, k.shape)
     q, k, cos, sin = _rows(q), _rows(k), _table(cos), _table(sin)
     q_weight, k_weight = q_weight.contiguous(), k_weight.contiguous()
     grad_q, grad_k = _rows(grad_q.to(q.dtype)), _rows(grad_k.to(k.dtype))
@@ -313,6 +325,10 @@ def _attention_bwd_impl(q, k, v, out, lse, grad_out, grad_lse, causal, scale, kv
     device = _require_device(q, k, v, out, lse, grad_out, grad_lse, kv_lens, q_start)
     _check_attention(q, k, v, kv_lens, q_start)
     _check_sizes("attention", q, k)
+    _check_like("attention_bwd", "out", out, q.shape, q.dtype)
+    _check_like("attention_bwd", "lse", lse, q.shape[:3], torch.float32)
+    _check_like("attention_bwd", "grad_out", grad_out, q.shape)
+    _check_like("attention_bwd", "grad_lse", grad_lse, q.shape[:3])
     q, k, v, out, grad_out = _chunked(q), _chunked(k), _chunked(v), _chunked(out), _chunked(grad_out.to(q.dtype))
     lse = lse.contiguous()
     grad_lse = None if grad_lse is None else grad_lse.to(torch.float32).contiguous()
@@ -454,6 +470,14 @@ def _embedding_fake(ids, weight, scale, padding_idx):
 
 def _embedding_bwd_impl(ids, grad_out, rows, scale, padding_idx) -> Tensor:
     device = _require_device(ids, grad_out)
+    _index_code("embedding_bwd: ids", ids)
+    dtype_code(grad_out.dtype)
+    if grad_out.dim() == 0 or grad_out.shape[:-1] != ids.shape or grad_out.shape[-1] == 0:
+        raise ValueError(f"embedding_bwd: grad_out must be ({', '.join(map(str, ids.shape))}, hidden), "
+                         f"got {tuple(grad_out.shape)}")
+    if rows < 0 or not -1 <= padding_idx < max(1, rows):
+        raise ValueError(f"embedding_bwd: bad rows {rows} or padding_idx {padding_idx}")
+    _check_sizes("embedding", grad_out)
     hidden = grad_out.shape[-1]
     flat = ids.contiguous()
     g = _table(grad_out.reshape(-1, hidden))
