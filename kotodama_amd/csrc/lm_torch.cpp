@@ -344,7 +344,7 @@ PyObject* py_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
       !take(a[6], true, &c.q_start) || !take(a[7], &c.start_value) || !take(a[8], &want_lse) || !unwatched())
     return none();
   const bool rec = recorded({&c.q, &c.k, &c.v});
-  if (rec && !(no_tangent(c.q) && no_tangent(c.k) && no_tangent(c.v))) return none();
+  if (!(no_tangent(c.q) && no_tangent(c.k) && no_tangent(c.v))) return none();  // refused in Python
   Tensor out, lse;
   bool ok = false;
   {
@@ -370,7 +370,8 @@ PyObject* py_qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
       !take(a[6], true, &c.positions) || !take(a[7], &c.eps) || !unwatched())
     return none();
   const bool rec = recorded({&c.q, &c.k, &c.wq, &c.wk});
-  if (rec && !(no_tangent(c.q) && no_tangent(c.k) && no_tangent(c.wq) && no_tangent(c.wk))) return none();
+  for (const Tensor* t : {&c.q, &c.k, &c.wq, &c.wk, &c.cos, &c.sin})
+    if (!no_tangent(*t)) return none();
   Tensor yq, yk;
   bool ok = false;
   {
@@ -396,7 +397,7 @@ PyObject* py_embedding(PyObject*, PyObject* const* a, Py_ssize_t n) {
       padding < -1 || !unwatched())
     return none();
   const bool rec = recorded({&w});
-  if (rec && !no_tangent(w)) return none();
+  if (!no_tangent(w)) return none();
   bool ok = false;
   {
     pybind11::gil_scoped_release nogil;

@@ -17,7 +17,8 @@ stream, in bf16 or fp32 with fp32 statistics and sums:
 Inputs may have any strides; one whose last dimension is not contiguous, or
 whose rows the attention kernels cannot load in 16-byte pieces, is copied
 first.  As everywhere in this package there is no CPU path: CPU tensors raise.
-Gradients of gradients are not provided.  Results repeat bit for bit: no
+Gradients of gradients and forward-mode derivatives are not provided (the
+latter raise :class:`NotImplementedError`).  Results repeat bit for bit: no
 kernel adds with atomics.
 """
 
@@ -29,6 +30,7 @@ from typing import Optional, Union
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _capi
 from ._native import native
@@ -70,6 +72,15 @@ def _check_sizes(op: str, *tensors: Tensor) -> None:
     for t in tensors:
         if max(t.shape, default=0) >= 1 << 31:
             raise ValueError(f"{op}: a size of {max(t.shape)} is over 2^31")
+
+
+def _no_tangents(op: str, *tensors: Tensor) -> None:
+    """Forward mode has no rule here: a tangent would be lost, as the ops see plain tensors."""
+    if torch.compiler.is_compiling():
+        return
+    for t in tensors:
+        if forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{op}: forward-mode differentiation is not provided")
 
 
 _i64x3 = ctypes.c_int64 * 3
@@ -250,6 +261,7 @@ def qk_norm_rope(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, cos: 
         res = native.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps)
         if res is not None:
             return res
+    _no_tangents("qk_norm_rope", q, k, q_weight, k_weight, cos, sin)
     if torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad):
         raise NotImplementedError("qk_norm_rope: cos and sin have no gradient; detach them")
     if _eager_direct(q, k, q_weight, k_weight, cos, sin, positions):
@@ -424,6 +436,7 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, causal: bool = True, scale: Op
         res = native.attention(q, k, v, causal, scale, kv_lens, start, value, bool(want_lse))
         if res is not None:
             return res
+    _no_tangents("attention", q, k, v)
     if _eager_direct(q, k, v, kv_lens, start):
         out, lse = _attention_impl(q, k, v, causal, scale, kv_lens, start, value, want_lse)
     else:
@@ -537,6 +550,7 @@ def embedding(ids: Tensor, weight: Tensor, scale: float = 1.0, padding_idx: Opti
         out = native.embedding(ids, weight, scale, pad)
         if out is not None:
             return out
+    _no_tangents("embedding", weight)
     if _eager_direct(ids, weight):
         return _embedding_impl(ids, weight, scale, pad)
     _require_device(ids, weight)
