@@ -26,6 +26,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import operator
 from typing import Optional, Union
 
 import torch
@@ -429,7 +430,7 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, causal: bool = True, scale: Op
     if isinstance(q_start, Tensor):
         start = q_start
     elif q_start is not None:
-        value = int(q_start)
+        value = operator.index(q_start)
         if abs(value) > 1 << 40:
             raise ValueError(f"attention: q_start {value} is out of range")
     if not torch.compiler.is_compiling():
@@ -541,7 +542,7 @@ def embedding(ids: Tensor, weight: Tensor, scale: float = 1.0, padding_idx: Opti
     """
     pad = -1
     if padding_idx is not None:
-        pad = int(padding_idx)
+        pad = operator.index(padding_idx)
         rows = weight.shape[0] if weight.dim() == 2 else 0
         if not -rows <= pad < rows:
             raise ValueError(f"embedding: padding_idx {pad} is not a row of the table")
