@@ -35,13 +35,16 @@ def visible(b, tq, tk, causal, kv_lens, q_start):
     return seen
 
 
-def attention(q, k, v, causal=True, scale=None, kv_lens=None, q_start=None, grad_out=None, grad_lse=None):
+def attention(q, k, v, causal=True, scale=None, kv_lens=None, q_start=None, grad_out=None, grad_lse=None,
+              delta_from_p=False):
     """{name: (value, bound)} for out and lse, and dq, dk, dv where ``grad_out`` is given.
 
     The inputs are taken as they are (bf16 or fp32 tensors, any device); the
     bounds are those of a kernel that computes scores and sums in fp32 and
     rounds the probabilities and score gradients to the inputs' type for the
-    products with v, k and q.
+    products with v, k and q.  Such a kernel may read the row sum of do * o off
+    the output, which is rounded; ``delta_from_p``: it forms the sum of p * dp
+    instead, in fp32.
     """
     u = HALF_STEP[q.dtype]
     up = u if q.dtype == torch.bfloat16 else 0.0
@@ -82,6 +85,9 @@ def attention(q, k, v, causal=True, scale=None, kv_lens=None, q_start=None, grad
     gv = g.abs() @ v.abs().transpose(-1, -2)
     go = (g.abs() * out.abs()).sum(-1, keepdim=True)
     err_delta = (g.abs() * err_o).sum(-1, keepdim=True) + (d + 4) * E32 * (go + abs(gl))
+    if delta_from_p:
+        # dp's own error, and the sum's over keys of terms off by p's
+        err_delta = (p * ((d + 4) * E32 * gv + (rp + (tk + 4) * E32) * dp.abs())).sum(-1, keepdim=True) + 4 * E32 * abs(gl)
     err_ds = up * ds.abs() + p * (rp * (dp - delta + gl).abs() + (d + 4) * E32 * gv + err_delta)
 
     def shared(x):
