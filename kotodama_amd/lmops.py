@@ -18,8 +18,9 @@ Inputs may have any strides; one whose last dimension is not contiguous, or
 whose rows the attention kernels cannot load in 16-byte pieces, is copied
 first.  As everywhere in this package there is no CPU path: CPU tensors raise.
 Gradients of gradients and forward-mode derivatives are not provided (the
-latter raise :class:`NotImplementedError`).  Results repeat bit for bit: no
-kernel adds with atomics.
+latter raise :class:`NotImplementedError`).  Results repeat bit for bit: every
+sum is taken in a fixed order (the embedding's sort counts tokens with atomics
+in LDS, whole numbers whose order does not show).
 """
 
 from __future__ import annotations
