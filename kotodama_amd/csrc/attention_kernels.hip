@@ -27,9 +27,13 @@
 // Tiles go from HBM to LDS directly (global_load_lds, 16 bytes per lane), the
 // next one requested before the current one is worked on.  A tile row is held
 // as 16-byte chunks, chunk c of row r at place c ^ g(r) with
-// g = 2 (r % 8) + (r / 8) % 2: 16 rows of one chunk and 4 rows of a chunk pair
-// each fall on distinct banks, so the row reads and the transposed reads of a
-// tile are both free of conflicts.
+// g = 2 (r % 8) + (r / 8) % 2 (rows of 8 chunks: 2 (r % 8 / 2) + (r / 8) % 2): 16
+// rows of one chunk fall on distinct banks, so the row reads of a tile are free
+// of conflicts, and so are fp32's column reads.  bf16's transposed reads are not:
+// 32 lanes read four chunks of each of four rows, and rows r and r + 1 (r even)
+// lie 32 bytes apart there, so that half of their chunks share banks.  Each
+// such read takes two cycles more than it needs: 33, 25 and 28% of the cycles
+// of the LDS in the forward, dq and (dk, dv) at 2 x 4096 tokens, 32/8 heads of 128.
 //
 // Rows beyond a sequence are never read: a tile's row index is clamped to the
 // last row that exists, and what it gives is masked.
