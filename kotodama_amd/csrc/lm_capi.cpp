@@ -156,7 +156,13 @@ AttnPlan attention_plan(int base, int64_t heads, int64_t lines, int64_t kv_slots
   const int64_t waves = heads * ((lines + 31) / 32), full = (int64_t)cus * (base == kAttnDkv ? 16 : 8);
   p.log = waves >= full ? 0 : waves * 2 >= full ? 1 : 2;
   if (base == kAttnFwd && p.log == 2) {
-    // tiles of 128 keys; four at least a part where there are many rows to join
+    // Tiles of 128 keys.  A part of one is short of work but not of time where
+    // few rows join: one token over 1024, 2048 or 4096 keys (8/4 heads) takes
+    // 7.0 + 3.8 us (kernel + join) against 10.7 + 3.8 with four tiles at least a
+    // part, 512 keys 7.1 + 3.9 against 10.2 whole.  With many rows the join
+    // costs more than the split gains: 4 x 512 causal tokens (4/2 heads) 10.7 us
+    // whole against 12.9 + 22.2 in parts of two tiles, 2 x 613 in fp32 (6 heads
+    // of 80) 30.0 against 35.4 + 20.6.  Past 4096 keys both ask for the same.
     const int64_t least = heads * lines <= (int64_t)cus * 4 ? 1 : 4;
     const int64_t most = (kv_slots + 127) / 128 / least, want = (int64_t)cus * kSplitPerCu / (waves > 0 ? waves : 1);
     const int64_t n = want < most ? want : most;
