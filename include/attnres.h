@@ -480,9 +480,11 @@ int attnres_merge_bwd(const void* partial, int64_t num_tokens, int hidden, int p
  * dtype: bf16 or fp32 (all of q, k, v, out); head_dim a multiple of 8 up to
  * 128; scale positive; 16-byte aligned pointers and strides, tokens less than
  * 32 MiB apart; at most 4096 query heads per key head.  lse ((batch, heads, q_len) fp32)
- * may be NULL.  Scores and sums are fp32; the probabilities are rounded to the
- * dtype for the product with v, the result once.  workspace: device memory of
- * attnres_attention_workspace_size bytes (backward 0 or 1).
+ * may be NULL.  Scores, probabilities, statistics and sums are fp32, and the
+ * result is rounded once; with dtype bf16 the probabilities are also rounded, to
+ * bf16, as the operand of their product with v.  fp32 calls round nothing else.
+ * workspace: device memory of attnres_attention_workspace_size bytes (backward
+ * 0 or 1).
  */
 int attnres_attention_workspace_size(int batch, int heads, int kv_heads, int64_t q_len, int64_t kv_slots, int head_dim,
                                      int dtype, int backward, int64_t* bytes);
@@ -495,7 +497,15 @@ int attnres_attention_fwd(const void* q, const int64_t* q_strides, const void* k
 
 /*
  * Its backward: the gradients of q, k and v from dL/dout and dL/dlse (or
- * NULL), the probabilities recomputed from q, k and the forward's lse.  Every
+ * NULL), the probabilities p_ij recomputed from q, k and the forward's lse:
+ *   delta_i = sum_d grad_out_id out_id - grad_lse_i,  dp_ij = grad_out_i . v_j
+ *   ds_ij = p_ij (dp_ij - delta_i)
+ *   grad_q_i = scale sum_j ds_ij k_j,  grad_k_j = scale sum_i ds_ij q_i,
+ *   grad_v_j = sum_i p_ij grad_out_i
+ * all in fp32, gradients rounded once; with dtype bf16 the p and the ds are also
+ * rounded, to bf16, as operands of the last three products.  delta reads `out` as it was
+ * stored, rounded to dtype (with bf16, rows that are worked on together and see
+ * at most 256 keys each take sum_j p_ij dp_ij in fp32 instead).  Every
  * row of grad_q, grad_k and grad_v is written (zeros where nothing is seen);
  * no atomics, so results repeat bit for bit.
  */

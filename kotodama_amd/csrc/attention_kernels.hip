@@ -100,7 +100,12 @@ struct Bf16 {
   }
   static __device__ __forceinline__ Frag zero() { return Frag{u32x4{0, 0, 0, 0}}; }
   static __device__ __forceinline__ Frag load(const char* p) { return Frag{*reinterpret_cast<const u32x4*>(p)}; }
-  // registers 8s .. 8s+7 of a result tile as the B operand of step s (rounded to bf16)
+  // Registers 8s .. 8s+7 of a result tile as the B operand of step s.  Rounded:
+  // probabilities and score gradients are held in fp32 up to here, but the
+  // matrix instructions take both operands in one type, and in fp32 they run at
+  // a sixteenth of bf16's rate.  With this rounding (and delta's,
+  // see attention_bwd_dq) results are off by 2.0e-3 to 2.4e-3 of their norm,
+  // against 1.7e-3 for 32-bit products rounded once at the end.
   static __device__ __forceinline__ Frag from_acc(const f32x16& c, int s) {
     Frag f;
 #pragma unroll
@@ -792,7 +797,8 @@ __device__ __forceinline__ void attention_bwd_dq(const lm_attn_params& P, char* 
   constexpr int NB = RW::kBlocks;
   const int mine = KS == 1 ? 0 : 32 * NB * R.part;  // this wave's keys of a tile
   // sum_d do o = sum_j p dp.  The first is one product a row, but the output it
-  // reads was rounded to bf16; where a row sees few keys that rounding is as
+  // reads was rounded to bf16, the only form the forward stores (an fp32 copy
+  // would be two thirds of its writes); where a row sees few keys that rounding is as
   // large as any other in dq (an output of few values is as large as they
   // are).  Tiles of such rows are walked once more for the second: 1% of the
   // pairs of a sequence of 4096, and dq and dk keep the error of their own

@@ -417,7 +417,11 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, causal: bool = True, scale: Op
 
     Returns the (B, H, Tq, D) result over (B, Tq, H, D) memory, and with
     ``want_lse`` also the fp32 log-sum-exp of each row's scores (B, H, Tq).
-    Differentiable in q, k and v, through both results.  D is a multiple of 8
+    Differentiable in q, k and v, through both results.  Scores, probabilities,
+    sums and statistics are fp32; with bf16 inputs the probabilities and the
+    score gradients are rounded to bf16 for the products with v, k, q and the
+    output's gradient, and the backward reads the rounded output.  fp32 inputs
+    round none of them.  D is a multiple of 8
     up to 128.  A NaN or infinity in a key or value that exists may reach
     every query of its sequence.
     """
