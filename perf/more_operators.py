@@ -62,7 +62,7 @@ def listed() -> list:
              temperature=1.0, dtype=BF16),
         # A serving batch's drafts from a small model.
         dict(name="verify_batch64", kind="verify", batch=64, q_len=8, new="draft", vocab=49152, probs=True,
-             temperature=0.8, dtype=BF16),
+             temperature=0.75, dtype=BF16),
     ]
 
 
@@ -78,7 +78,7 @@ def draw(rng) -> dict:
     if kind == "verify":
         case["new"] = rng.choice(("chunk", "draft"))
         case.update(q_len=rng.randint(1, 9), vocab=_log_int(rng, 200, 130000), probs=rng.random() < 0.7,
-                    temperature=rng.choice((0.0, 0.7, 1.0, 1.3)), dtype=rng.choice((BF16, FP32)))
+                    temperature=rng.choice((0.0, 0.75, 1.0, 1.25)), dtype=rng.choice((BF16, FP32)))
     else:
         case.update(kv_len=_log_int(rng, 1, 65536 if kind != "write" else 4096), page=rng.choice((16, 32, 64, 128)))
         case["q_len"] = 1 if case["new"] == "one" else min(case["kv_len"], _log_int(rng, 1, 2048))
