@@ -574,6 +574,105 @@ int attnres_embedding_bwd(const void* ids, int index_dtype, int64_t num_ids, con
                           int64_t rows, int hidden, int dtype, float scale, int64_t padding_idx, void* grad_weight,
                           void* workspace, int64_t workspace_bytes, void* stream);
 
+/*
+ * ---- Serving from a paged cache ------------------------------------------
+ *
+ * Keys and values lie in pages of page_size rows (a power of two from 16 to 65536):
+ * k_cache and v_cache (pages, kv_heads, page_size, head_dim), element strides
+ * given as (page, head, row).  block_table (seqs, table_width) int32, rows
+ * table_ld apart, names each sequence's pages in order: token t of sequence s is row
+ * t % page_size of page block_table[s][t / page_size], its slot
+ * page * page_size + t % page_size.  New tokens are packed: sequence s has the
+ * tokens q_starts[s] .. q_starts[s + 1] - 1 (seqs + 1 whole numbers, the first
+ * 0); those behind the last sequence are padding.  Lengths and starts
+ * stay on the device; what would lead out of the tensors is taken into them.
+ */
+
+/*
+ * Slots for new tokens.  A sequence holds held[s] tokens in ceil(held / page_size)
+ * pages and adds new_tokens[s].  Free pages are free_pages[0 .. free_count[0] - 1],
+ * taken from the end: a sequence gets the pages it needs where the needs of all
+ * sequences up to it are at most free_count, and else is refused, as is one whose tokens do
+ * not fit its row of the table or the call's `tokens`, or whose lengths are negative or
+ * over 2^30.  Writes the new pages into block_table, and
+ *   slots (tokens,)      each token's slot; -1 for padding and refused sequences
+ *   positions (tokens,)  its place in its sequence; 0 for padding
+ *   q_starts (seqs + 1,) running sums of new_tokens, at most `tokens`
+ *   kv_lens (seqs,)      held + new_tokens, 0 for refused sequences
+ *   free_count_out (1,)  pages that stay free
+ * all int32.  free_count_out is not free_count.  held_dtype, new_dtype: ATTNRES_INDEX_*.
+ */
+int attnres_paged_slots(void* block_table, int64_t table_ld, int seqs, int table_width, const void* held,
+                        int held_dtype, const void* new_tokens, int new_dtype, const void* free_pages, int free_len,
+                        const void* free_count, int page_size, int64_t tokens, void* slots, void* positions,
+                        void* q_starts, void* kv_lens, void* free_count_out, void* stream);
+
+/*
+ * Gives pages back: sequence s, which held held[s] tokens, keeps the first kept[s]
+ * (taken into [0, held]), and the pages behind them are appended to free_pages
+ * (free_len entries; what does not fit is dropped), sequence by sequence, a
+ * sequence's last page first.  Their entries in the table stay, unused.
+ */
+int attnres_paged_release(const void* block_table, int64_t table_ld, int seqs, int table_width, const void* held,
+                          int held_dtype, const void* kept, int kept_dtype, void* free_pages, int free_len,
+                          const void* free_count, int page_size, void* free_count_out, void* stream);
+
+/*
+ * Writes new keys and values (tokens, kv_heads, head_dim), element strides (token, head),
+ * into their slots ((tokens,) slots_dtype, no slot twice).  A slot outside the cache
+ * (-1) is skipped.  dtype bf16 or fp32 of all; head_dim a multiple of 8 up to 128; 16-byte
+ * aligned pointers and strides.
+ */
+int attnres_paged_write(const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                        int64_t tokens, int kv_heads, int head_dim, int dtype, void* k_cache,
+                        const int64_t* k_cache_strides, void* v_cache, const int64_t* v_cache_strides, int64_t pages,
+                        int page_size, const void* slots, int slots_dtype, void* stream);
+
+/*
+ * Attention of the new tokens over their sequences' pages: token i of the n new ones of
+ * a sequence is at position kv_lens[s] - n + i and sees the keys up to it
+ * (none where that is negative).  q and out (tokens, heads, head_dim), element
+ * strides (token, head); query head h reads key head h / (heads / kv_heads).  q_starts may be
+ * NULL: one token per sequence.  Types, rounding, scale and alignment as attnres_attention_fwd.
+ * Rows that see no key, padding among them, are zero with lse ((tokens, heads) fp32 or NULL)
+ * -inf.  Rows of the cache behind a sequence's length are not used, whatever they
+ * hold; a table entry outside the cache, or a NaN or infinity in a key or value that
+ * exists, may make every row of its sequence NaN.  Sums are taken in a fixed order.
+ * workspace: device memory of attnres_paged_attention_workspace_size bytes.
+ */
+int attnres_paged_attention_workspace_size(int64_t tokens, int seqs, int heads, int kv_heads, int head_dim, int dtype,
+                                           int table_width, int page_size, int64_t* bytes);
+int attnres_paged_attention_fwd(const void* q, const int64_t* q_strides, const void* k_cache, const int64_t* k_strides,
+                                const void* v_cache, const int64_t* v_strides, int64_t tokens, int seqs, int heads,
+                                int kv_heads, int head_dim, int dtype, int64_t pages, int page_size,
+                                const void* block_table, int64_t table_ld, int table_width, const void* kv_lens,
+                                int lens_dtype, const void* q_starts, int starts_dtype, float scale, void* out,
+                                const int64_t* out_strides, float* lse, void* workspace, int64_t workspace_bytes,
+                                void* stream);
+
+/*
+ * Drafted tokens against the model's logits.  Sequence s has the rows q_starts[s] ..
+ * q_starts[s + 1] - 1: ids of the last token that stands and of the drafts behind it, and the
+ * logits (rows, vocab) that the model gave for them, rows logits_ld apart.  With
+ * p_r = softmax(logits_r / temperature) and q_r the draft's distribution (draft_probs
+ * (rows, vocab), rows draft_ld apart, or NULL: 1 at the draft), the draft ids[r + 1] stays if
+ * uniforms[r][0] q_r(draft) < p_r(draft).  In place of the first that does not comes a token
+ * from max(p_r - q_r, 0) (from p_r where that is all zero), or, behind
+ * drafts that all stay, one from p_r of the last row: the first j at which the running sum
+ * exceeds uniforms[r][1] times the whole.  temperature 0: p_r is 1 at the largest logit (the lowest index of
+ * several), and draft_probs are not read.
+ * tokens (rows,), of ids' type: row r the token behind ids[r], -1 behind the last.  counts (seqs,)
+ * int32: how many of a sequence's tokens there are, at least 1 where it has rows.  A row with a NaN or
+ * +infinity, or nothing but -infinity, gives no token (-1, not counted).
+ * Tokens are those of the definition: sums are taken in 64 bits where they decide.
+ * vocab up to 2^21.  workspace: device memory of attnres_verify_drafts_workspace_size bytes.
+ */
+int attnres_verify_drafts_workspace_size(int64_t rows, int vocab, int64_t* bytes);
+int attnres_verify_drafts(const void* logits, int64_t logits_ld, int logits_dtype, const void* draft_probs,
+                          int64_t draft_ld, int draft_dtype, int64_t rows, int vocab, const void* ids, int ids_dtype,
+                          const void* q_starts, int starts_dtype, int seqs, const float* uniforms, float temperature,
+                          void* tokens, void* counts, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

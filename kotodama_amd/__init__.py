@@ -13,6 +13,10 @@ Hand-written HIP kernels behind a C ABI (``include/attnres.h``,
 * :func:`kotodama_amd.attention`, :func:`kotodama_amd.qk_norm_rope`,
   :func:`kotodama_amd.embedding` — the language model's own operators around
   the routing, forward and backward (:mod:`kotodama_amd.lmops`)
+* :func:`kotodama_amd.paged_attention`, :func:`kotodama_amd.paged_write`,
+  :func:`kotodama_amd.paged_slots` / :func:`kotodama_amd.paged_release`,
+  :func:`kotodama_amd.verify_drafts` — serving from a paged cache
+  (:class:`kotodama_amd.PagedCache`, :mod:`kotodama_amd.paged`)
 * :mod:`kotodama_amd.checkpoint` — routing weights from trained checkpoints
   (safe loading only)
 """
@@ -21,6 +25,7 @@ from . import ops  # noqa: F401  (registers the attnres_hip ops)
 from .checkpoint import RoutingWeights, load_checkpoint_registry, load_routing_weights
 from .engine import AttnResRouter, BlockArena, forward_attn_res, forward_attn_res_cached
 from .lmops import attention, embedding, qk_norm_rope
+from .paged import PagedCache, PagedSlots, paged_attention, paged_release, paged_slots, paged_write, verify_drafts
 from .routing import block_attn_res_from_list, route_static, route_weights
 from .schedule import AttnResSchedule
 
@@ -28,6 +33,8 @@ __all__ = [
     "AttnResRouter",
     "AttnResSchedule",
     "BlockArena",
+    "PagedCache",
+    "PagedSlots",
     "RoutingWeights",
     "attention",
     "block_attn_res_from_list",
@@ -36,7 +43,12 @@ __all__ = [
     "forward_attn_res_cached",
     "load_checkpoint_registry",
     "load_routing_weights",
+    "paged_attention",
+    "paged_release",
+    "paged_slots",
+    "paged_write",
     "qk_norm_rope",
     "route_static",
     "route_weights",
+    "verify_drafts",
 ]

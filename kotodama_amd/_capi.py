@@ -77,6 +77,13 @@ EXPORTS = (
     "attnres_embedding_fwd",
     "attnres_embedding_workspace_size",
     "attnres_embedding_bwd",
+    "attnres_paged_slots",
+    "attnres_paged_release",
+    "attnres_paged_write",
+    "attnres_paged_attention_workspace_size",
+    "attnres_paged_attention_fwd",
+    "attnres_verify_drafts_workspace_size",
+    "attnres_verify_drafts",
 )
 
 _c_vp = ctypes.c_void_p
@@ -604,6 +611,151 @@ _SIGNATURES = {
         ],
         _c_int,
     ),
+    "attnres_paged_slots": (
+        [
+            _c_vp,  # block_table
+            _c_i64,  # table_ld
+            _c_int,  # seqs
+            _c_int,  # table_width
+            _c_vp,  # held
+            _c_int,  # held_dtype
+            _c_vp,  # new_tokens
+            _c_int,  # new_dtype
+            _c_vp,  # free_pages
+            _c_int,  # free_len
+            _c_vp,  # free_count
+            _c_int,  # page_size
+            _c_i64,  # tokens
+            _c_vp,  # slots
+            _c_vp,  # positions
+            _c_vp,  # q_starts
+            _c_vp,  # kv_lens
+            _c_vp,  # free_count_out
+            _c_vp,  # stream
+        ],
+        _c_int,
+    ),
+    "attnres_paged_release": (
+        [
+            _c_vp,  # block_table
+            _c_i64,  # table_ld
+            _c_int,  # seqs
+            _c_int,  # table_width
+            _c_vp,  # held
+            _c_int,  # held_dtype
+            _c_vp,  # kept
+            _c_int,  # kept_dtype
+            _c_vp,  # free_pages
+            _c_int,  # free_len
+            _c_vp,  # free_count
+            _c_int,  # page_size
+            _c_vp,  # free_count_out
+            _c_vp,  # stream
+        ],
+        _c_int,
+    ),
+    "attnres_paged_write": (
+        [
+            _c_vp,  # k
+            ctypes.POINTER(_c_i64),  # k_strides
+            _c_vp,  # v
+            ctypes.POINTER(_c_i64),  # v_strides
+            _c_i64,  # tokens
+            _c_int,  # kv_heads
+            _c_int,  # head_dim
+            _c_int,  # dtype
+            _c_vp,  # k_cache
+            ctypes.POINTER(_c_i64),  # k_cache_strides
+            _c_vp,  # v_cache
+            ctypes.POINTER(_c_i64),  # v_cache_strides
+            _c_i64,  # pages
+            _c_int,  # page_size
+            _c_vp,  # slots
+            _c_int,  # slots_dtype
+            _c_vp,  # stream
+        ],
+        _c_int,
+    ),
+    "attnres_paged_attention_workspace_size": (
+        [
+            _c_i64,  # tokens
+            _c_int,  # seqs
+            _c_int,  # heads
+            _c_int,  # kv_heads
+            _c_int,  # head_dim
+            _c_int,  # dtype
+            _c_int,  # table_width
+            _c_int,  # page_size
+            ctypes.POINTER(_c_i64),  # bytes
+        ],
+        _c_int,
+    ),
+    "attnres_paged_attention_fwd": (
+        [
+            _c_vp,  # q
+            ctypes.POINTER(_c_i64),  # q_strides
+            _c_vp,  # k_cache
+            ctypes.POINTER(_c_i64),  # k_strides
+            _c_vp,  # v_cache
+            ctypes.POINTER(_c_i64),  # v_strides
+            _c_i64,  # tokens
+            _c_int,  # seqs
+            _c_int,  # heads
+            _c_int,  # kv_heads
+            _c_int,  # head_dim
+            _c_int,  # dtype
+            _c_i64,  # pages
+            _c_int,  # page_size
+            _c_vp,  # block_table
+            _c_i64,  # table_ld
+            _c_int,  # table_width
+            _c_vp,  # kv_lens
+            _c_int,  # lens_dtype
+            _c_vp,  # q_starts
+            _c_int,  # starts_dtype
+            _c_float,  # scale
+            _c_vp,  # out
+            ctypes.POINTER(_c_i64),  # out_strides
+            _c_vp,  # lse
+            _c_vp,  # workspace
+            _c_i64,  # workspace_bytes
+            _c_vp,  # stream
+        ],
+        _c_int,
+    ),
+    "attnres_verify_drafts_workspace_size": (
+        [
+            _c_i64,  # rows
+            _c_int,  # vocab
+            ctypes.POINTER(_c_i64),  # bytes
+        ],
+        _c_int,
+    ),
+    "attnres_verify_drafts": (
+        [
+            _c_vp,  # logits
+            _c_i64,  # logits_ld
+            _c_int,  # logits_dtype
+            _c_vp,  # draft_probs
+            _c_i64,  # draft_ld
+            _c_int,  # draft_dtype
+            _c_i64,  # rows
+            _c_int,  # vocab
+            _c_vp,  # ids
+            _c_int,  # ids_dtype
+            _c_vp,  # q_starts
+            _c_int,  # starts_dtype
+            _c_int,  # seqs
+            _c_vp,  # uniforms
+            _c_float,  # temperature
+            _c_vp,  # tokens
+            _c_vp,  # counts
+            _c_vp,  # workspace
+            _c_i64,  # workspace_bytes
+            _c_vp,  # stream
+        ],
+        _c_int,
+    ),
 }
 
 _lock = threading.Lock()
@@ -783,6 +935,42 @@ def embedding_workspace_size(num_ids: int, rows: int, hidden: int) -> int:
 
 def embedding_bwd(*args) -> None:
     check("attnres_embedding_bwd", lib().attnres_embedding_bwd(*args))
+
+
+def paged_slots(*args) -> None:
+    check("attnres_paged_slots", lib().attnres_paged_slots(*args))
+
+
+def paged_release(*args) -> None:
+    check("attnres_paged_release", lib().attnres_paged_release(*args))
+
+
+def paged_write(*args) -> None:
+    check("attnres_paged_write", lib().attnres_paged_write(*args))
+
+
+def paged_attention_workspace_size(*args) -> int:
+    """Bytes of workspace :func:`paged_attention_fwd` needs on the current device."""
+    out = _c_i64(0)
+    check("attnres_paged_attention_workspace_size",
+          lib().attnres_paged_attention_workspace_size(*args, ctypes.byref(out)))
+    return out.value
+
+
+def paged_attention_fwd(*args) -> None:
+    check("attnres_paged_attention_fwd", lib().attnres_paged_attention_fwd(*args))
+
+
+def verify_drafts_workspace_size(rows: int, vocab: int) -> int:
+    """Bytes of workspace :func:`verify_drafts` needs."""
+    out = _c_i64(0)
+    check("attnres_verify_drafts_workspace_size",
+          lib().attnres_verify_drafts_workspace_size(rows, vocab, ctypes.byref(out)))
+    return out.value
+
+
+def verify_drafts(*args) -> None:
+    check("attnres_verify_drafts", lib().attnres_verify_drafts(*args))
 
 
 def set_kernel_policy(policy: int) -> int:

@@ -2,8 +2,9 @@
 
 ``native.route`` / ``route_list`` / ``merge`` / ``block_step`` and the training
 points' ``step`` / ``bwd_rows`` / ``bwd_defer`` / ``gather_seg``, and the
-language-model operators' ``attention`` / ``qk_norm_rope`` / ``embedding`` launch one
-plain call and return its result, or return None with nothing done for any
+language-model operators' ``attention`` / ``qk_norm_rope`` / ``embedding`` and the serving ones'
+``paged_slots`` / ``paged_release`` / ``paged_write`` / ``paged_attention`` / ``verify_drafts`` launch one
+plain call and return its result (``paged_write``: True), or return None with nothing done for any
 call that is not plain (the caller then takes it through Python).  Loaded on
 first use.  Without the built extension every function returns None and the
 calls take the ctypes path, which reports a missing library; so they do, with
@@ -22,7 +23,8 @@ from pathlib import Path
 NAME = "_attnres_torch" + importlib.machinery.EXTENSION_SUFFIXES[0]
 PATH = Path(__file__).resolve().parent / "lib" / NAME
 FUNCTIONS = ("route", "route_list", "merge", "block_step", "step", "bwd_rows", "bwd_defer", "gather_seg", "attention",
-             "qk_norm_rope", "embedding")
+             "qk_norm_rope", "embedding", "paged_slots", "paged_release", "paged_write", "paged_attention",
+             "verify_drafts")
 
 _lock = threading.Lock()
 

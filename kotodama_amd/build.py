@@ -4,17 +4,17 @@ Steps (all outputs under ``kotodama_amd/lib/``):
 
 1. ``hipcc --genco --offload-arch=gfx950`` compiles ``csrc/attnres_kernels.hip``
    once per code-object part (``-DATTNRES_PART=0..11``, in parallel), and
-   ``csrc/lm_kernels.hip`` and ``csrc/attention_kernels.hip`` into the parts
+   the language-model operators' kernels (``LM_PARTS``) into the parts
    after those (``-DLM_PART``).
 2. ``gcc`` assembles ``csrc/attnres_blob.S``, which ``.incbin``s the parts.
 3. ``hipcc -c -fPIC`` compiles ``csrc/attnres_noalloc.hip`` (the no-alloc
    entry point; its device array needs HIP device code of its own).
-4. ``g++`` links ``csrc/attnres_capi.cpp``, ``csrc/lm_capi.cpp``, the blob and that object into the
+4. ``g++`` links the host sources (``HOST_SOURCES``), the blob and that object into the
    shared library, linked against ROCm's ``libamdhip64.so.7``.  Loaded after ``import torch``,
    the dynamic linker binds that soname to the HIP runtime torch already
    loaded, so streams and device memory are shared with torch.
-5. Where a ROCm torch is importable, ``g++`` compiles ``csrc/attnres_torch.cpp``
-   and ``csrc/lm_torch.cpp`` against its headers into ``_attnres_torch`` (with this Python's extension
+5. Where a ROCm torch is importable, ``g++`` compiles the torch layer's sources (``NATIVE_SOURCES``)
+   against its headers into ``_attnres_torch`` (with this Python's extension
    suffix), the CPython extension through which the eager torch layer calls
    that library.  The library needs no torch and is in place before this step
    can fail; an extension of an earlier build does not stay beside it.
@@ -37,11 +37,13 @@ LIBDIR = PKG / "lib"
 INCLUDE = PKG.parent / "include"
 LIB_NAME = "libattnres_hip.so"
 NATIVE_NAME = "_attnres_torch" + EXTENSION_SUFFIXES[0]  # as _native.py looks it up
-NATIVE_SOURCES = ("attnres_torch.cpp", "lm_torch.cpp")
+NATIVE_SOURCES = ("attnres_torch.cpp", "lm_torch.cpp", "serving_torch.cpp")
 ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 ARCH = "gfx950"
 NUM_PARTS = 12  # of attnres_kernels.hip
-LM_PARTS = {12: "lm_kernels.hip", 13: "attention_kernels.hip", 14: "attention_kernels.hip"}
+LM_PARTS = {12: "lm_kernels.hip", 13: "attention_kernels.hip", 14: "attention_kernels.hip",
+            15: "paged_attention_kernels.hip", 16: "serving_kernels.hip"}
+HOST_SOURCES = ("attnres_capi.cpp", "lm_capi.cpp", "serving_capi.cpp")
 
 # Packed-fp32 VALU ops are disabled for every HIP compile (the kernels are
 # written with scalar fp32 arithmetic).
@@ -142,8 +144,7 @@ def build(verbose: bool = False, out_dir: Path | None = None, defines: tuple = (
                 f"-I{INCLUDE}",
                 f"-I{CSRC}",
                 f"-I{ROCM / 'include'}",
-                str(CSRC / "attnres_capi.cpp"),
-                str(CSRC / "lm_capi.cpp"),
+                *(str(CSRC / src) for src in HOST_SOURCES),
                 str(blob_o),
                 str(noalloc_o),
                 f"-L{ROCM / 'lib'}",

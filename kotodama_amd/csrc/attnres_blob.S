@@ -61,4 +61,12 @@ attnres_hsaco_part13:
     .global attnres_hsaco_part14
 attnres_hsaco_part14:
     .incbin "attnres_gfx950_part14.hsaco"
+    .balign 4096
+    .global attnres_hsaco_part15
+attnres_hsaco_part15:
+    .incbin "attnres_gfx950_part15.hsaco"
+    .balign 4096
+    .global attnres_hsaco_part16
+attnres_hsaco_part16:
+    .incbin "attnres_gfx950_part16.hsaco"
     .section .note.GNU-stack,"",@progbits

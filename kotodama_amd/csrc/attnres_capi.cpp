@@ -39,10 +39,12 @@ extern "C" const unsigned char attnres_hsaco_part11[];
 extern "C" const unsigned char attnres_hsaco_part12[];
 extern "C" const unsigned char attnres_hsaco_part13[];
 extern "C" const unsigned char attnres_hsaco_part14[];
+extern "C" const unsigned char attnres_hsaco_part15[];
+extern "C" const unsigned char attnres_hsaco_part16[];
 
 namespace {
 
-constexpr int kParts = 15;  // 12..14: the language-model operators (lm_capi.cpp)
+constexpr int kParts = 17;  // 12..16: the language-model operators (lm_capi.cpp, serving_capi.cpp)
 constexpr int kMaxDevices = 64;
 constexpr int kMaxThreads = 512;  // __launch_bounds__ of every kernel
 
@@ -127,7 +129,7 @@ struct DeviceState {
   KernelSlot bwd_mqg[2 * 9];     // batched-query backward on the matrix cores: query groups x S
   KernelSlot bwd_defer[4 * 10];  // row-per-wave backward with deferred block gradients: row width x S
   KernelSlot gather_seg[4 * ATTNRES_SEG_MAX_BLOCKS];  // segment sums: row width x blocks
-  KernelSlot lm[ATTNRES_INTERNAL_SLOTS];  // the language-model operators, numbered by lm_capi.cpp
+  KernelSlot lm[ATTNRES_INTERNAL_SLOTS];  // the language-model operators, numbered by lm_capi.cpp and serving_capi.cpp
 };
 
 DeviceState g_dev[kMaxDevices];
@@ -215,7 +217,8 @@ int ensure_loaded(DeviceState** out) {
                                             attnres_hsaco_part3, attnres_hsaco_part4, attnres_hsaco_part5,
                                             attnres_hsaco_part6, attnres_hsaco_part7, attnres_hsaco_part8,
                                             attnres_hsaco_part9, attnres_hsaco_part10, attnres_hsaco_part11,
-                                            attnres_hsaco_part12, attnres_hsaco_part13, attnres_hsaco_part14};
+                                            attnres_hsaco_part12, attnres_hsaco_part13, attnres_hsaco_part14,
+                                            attnres_hsaco_part15, attnres_hsaco_part16};
       // On a failure nothing stays half-loaded: the next call starts over.
       auto unload = [&st](int n) {
         for (int j = 0; j < n; ++j) {

@@ -4,7 +4,7 @@
 
 #include <hip/hip_runtime.h>
 
-#define ATTNRES_INTERNAL_SLOTS 128 /* kernels of lm_capi.cpp */
+#define ATTNRES_INTERNAL_SLOTS 128 /* kernels of lm_capi.cpp and serving_capi.cpp */
 #define ATTNRES_HIDDEN __attribute__((visibility("hidden")))
 
 #ifdef __cplusplus

@@ -749,6 +749,14 @@ PyMethodDef kMethods[] = {
     {"qk_norm_rope", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_qk_norm_rope)), METH_FASTCALL,
      nullptr},
     {"embedding", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_embedding)), METH_FASTCALL, nullptr},
+    {"paged_slots", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_slots)), METH_FASTCALL, nullptr},
+    {"paged_release", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_release)), METH_FASTCALL,
+     nullptr},
+    {"paged_write", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_write)), METH_FASTCALL, nullptr},
+    {"paged_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_attention)), METH_FASTCALL,
+     nullptr},
+    {"verify_drafts", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_verify_drafts)), METH_FASTCALL,
+     nullptr},
     {"block_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_block_step)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

@@ -1,5 +1,5 @@
 // What the sources of the native call path share (attnres_torch.cpp: routing,
-// lm_torch.cpp: the language-model operators).
+// lm_torch.cpp: the language-model operators, serving_torch.cpp: the serving ones).
 #ifndef KOTODAMA_AMD_ATTNRES_TORCH_COMMON_H
 #define KOTODAMA_AMD_ATTNRES_TORCH_COMMON_H
 
@@ -174,6 +174,13 @@ inline PyObject* wrap(const Tensor& t) {
 PyObject* py_attention(PyObject*, PyObject* const* a, Py_ssize_t n);
 PyObject* py_qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n);
 PyObject* py_embedding(PyObject*, PyObject* const* a, Py_ssize_t n);
+
+// The entries of serving_torch.cpp.
+PyObject* py_paged_slots(PyObject*, PyObject* const* a, Py_ssize_t n);
+PyObject* py_paged_release(PyObject*, PyObject* const* a, Py_ssize_t n);
+PyObject* py_paged_write(PyObject*, PyObject* const* a, Py_ssize_t n);
+PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n);
+PyObject* py_verify_drafts(PyObject*, PyObject* const* a, Py_ssize_t n);
 
 }  // namespace attnres_torch
 

@@ -6,12 +6,12 @@
 #include <hip/hip_runtime.h>
 
 #include <cmath>
-#include <cstdarg>
 #include <cstdio>
 #include <cstring>
 
 #include "attnres.h"
 #include "attnres_internal.h"
+#include "lm_host.h"
 #include "lm_params.h"
 
 namespace {
@@ -32,42 +32,12 @@ enum Slot {
   kEmbedSort = kEmbedJoin + 2,
   kSlots
 };
-static_assert(kSlots <= ATTNRES_INTERNAL_SLOTS, "kernel slots");
+static_assert(kSlots <= kServingSlots, "kernel slots");
 
 constexpr int64_t kMaxLen = (int64_t)1 << 30;  // tokens of one sequence
 constexpr int kSplitPerCu = 2;                 // workgroups per CU to split the key axis into
 constexpr int64_t kMaxTokenStride = (int64_t)32 << 20;  // bytes
 constexpr int kMaxGroup = 4096;                // query heads per key head
-
-int fail(int code, const char* fmt, ...) {
-  char buf[400];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof(buf), fmt, ap);
-  va_end(ap);
-  return attnres_internal_fail(code, buf);
-}
-
-bool valid_dtype(int d) { return d == ATTNRES_DTYPE_F32 || d == ATTNRES_DTYPE_BF16; }
-bool valid_index(int d) { return d == ATTNRES_INDEX_I32 || d == ATTNRES_INDEX_I64; }
-int esize(int d) { return d == ATTNRES_DTYPE_BF16 ? 2 : 4; }
-bool aligned(const void* p, int n) { return ((uintptr_t)p & (uintptr_t)(n - 1)) == 0; }
-
-template <typename Params>
-int launch(int slot, int part, const char* name, unsigned gx, unsigned gy, unsigned block, unsigned lds, Params& P,
-           void* stream) {
-  if ((uint64_t)gx * block > UINT32_MAX)  // a launch's threads along one axis
-    return fail(ATTNRES_ERR_UNSUPPORTED, "%s: too many rows for one call", name);
-  hipFunction_t f = nullptr;
-  int cus = 0;
-  int rc = attnres_internal_kernel(slot, part, name, &f, &cus);
-  if (rc != ATTNRES_OK) return rc;
-  size_t sz = sizeof(Params);
-  void* cfg[] = {HIP_LAUNCH_PARAM_BUFFER_POINTER, &P, HIP_LAUNCH_PARAM_BUFFER_SIZE, &sz, HIP_LAUNCH_PARAM_END};
-  hipError_t e = hipModuleLaunchKernel(f, gx, gy, 1, block, 1, 1, lds, (hipStream_t)stream, nullptr, cfg);
-  if (e != hipSuccess) return fail(ATTNRES_ERR_HIP, "hipModuleLaunchKernel(%s) failed: %s", name, hipGetErrorString(e));
-  return ATTNRES_OK;
-}
 
 // A tensor argument's strides; dimensions of one element have none.
 int take_strides(const char* what, const void* p, const int64_t* st, int64_t nb, int64_t nh, int64_t nt, int es,

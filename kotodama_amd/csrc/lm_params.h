@@ -1,6 +1,6 @@
 /*
  * Kernel-argument blocks of the language-model operators (lm_kernels.hip,
- * attention_kernels.hip), shared by the gfx950 code objects and the host
+ * attention_kernels.hip, paged_attention_kernels.hip, serving_kernels.hip), shared by the gfx950 code objects and the host
  * launcher (lm_capi.cpp), as attnres_params.h is for the routing kernels.
  *
  * Plain C types only: included by g++ (host) and by hipcc (device) alike.
@@ -129,5 +129,121 @@ typedef struct lm_embed_params {
   int32_t threads_per_row;
   float scale;
 } lm_embed_params;
+
+/*
+ * Attention of packed new tokens over a paged cache.  Sequence s has the tokens
+ * q_starts[s] .. q_starts[s + 1] - 1 (s, where q_starts is NULL), the last at position
+ * kv_lens[s] - 1; key j is row j % page_size of page table[s][j / page_size].
+ */
+#define LM_PAGED_THREADS (64 * LM_ATTN_WAVES)
+#define LM_PAGED_MIN_PAGE 16 /* rows of a wave's load lie in one page */
+typedef struct lm_paged_params {
+  const void* q;         /* (tokens, heads, dim) */
+  const void* k;         /* (pages, kv_heads, page_size, dim) */
+  const void* v;
+  void* o;               /* (tokens, heads, dim) */
+  float* lse;            /* (tokens, heads) or NULL */
+  float* part;           /* (slots, kv_heads, part_rows, dim): sums of a part of the keys */
+  float* part_ml;        /* (slots, kv_heads, part_rows, 2): their maxima (times log2 e) and sums of weights */
+  const int32_t* table;  /* (seqs, table_width), rows table_ld apart */
+  const void* kv_lens;   /* (seqs,) */
+  const void* q_starts;  /* (seqs + 1,) or NULL */
+  lm_strides sk, sv;     /* page, head, token */
+  int64_t q_t, q_h, o_t, o_h;
+  int64_t table_ld;
+  int32_t tokens;
+  int32_t seqs;
+  int32_t heads;
+  int32_t kv_heads;
+  int32_t pages;
+  int32_t capacity;      /* keys of a table row: table_width * page_size */
+  int32_t shift;         /* log2 of page_size */
+  int32_t dim;
+  int32_t wide;          /* sequences of over 32 rows in tiles of 128 */
+  int32_t target;        /* workgroups to split the key axis for, */
+  int32_t least;         /* least blocks (of 32 keys a wave) of a part */
+  int32_t slots;         /* parts of split tiles that the workspace holds */
+  int32_t part_rows;     /* rows of one */
+  int32_t lens64;
+  int32_t starts64;
+  float scale_log2;
+} lm_paged_params;
+
+/*
+ * Block tables, slot maps and the free list of a paged cache.  A sequence that holds n tokens
+ * has ceil(n / page_size) pages in its row of the table; free[0 .. count - 1] are the pages that
+ * none has, taken from the end.
+ */
+#define LM_SLOTS_THREADS 1024
+typedef struct lm_slots_params {
+  int32_t* table;        /* (seqs, table_width), rows table_ld apart */
+  int32_t* free;         /* (free_len,); slots: read, release: written behind count */
+  const int32_t* count;  /* [0] */
+  const void* held;      /* (seqs,) tokens held before */
+  const void* change;    /* (seqs,) slots: new tokens, release: tokens kept */
+  int32_t* slots;        /* (tokens,) page * page_size + row, or -1 */
+  int32_t* positions;    /* (tokens,) */
+  int32_t* q_starts;     /* (seqs + 1,) */
+  int32_t* kv_lens;      /* (seqs,) tokens held after; 0: refused */
+  int32_t* count_out;    /* [0] */
+  int64_t table_ld;
+  int64_t page_limit;    /* 2^31 / page_size: pages whose slots 32 bits count */
+  int32_t tokens;
+  int32_t seqs;
+  int32_t table_width;
+  int32_t free_len;
+  int32_t shift;         /* log2 of page_size */
+  int32_t held64;
+  int32_t change64;
+} lm_slots_params;
+
+/* Rows of new keys and values into their slots of the cache. */
+typedef struct lm_write_params {
+  const void* k;         /* (tokens, kv_heads, dim) */
+  const void* v;
+  void* k_cache;         /* (pages, kv_heads, page_size, dim) */
+  void* v_cache;
+  const void* slots;     /* (tokens,) */
+  lm_strides sk, sv;     /* bytes: page, head, token */
+  int64_t k_t, k_h, v_t, v_h; /* bytes */
+  int64_t limit;         /* pages * page_size */
+  int32_t tokens;
+  int32_t chunks;        /* 16-byte pieces of a head's row */
+  int32_t per_token;     /* kv_heads * chunks */
+  int32_t shift;
+  int32_t slots64;
+} lm_write_params;
+
+/*
+ * Drafted tokens against the target's logits.  Sequence s has the rows q_starts[s] ..
+ * q_starts[s + 1] - 1; row r's draft is ids[r + 1].
+ */
+#define LM_VERIFY_SLICE 4096      /* logits of a workgroup of the first pass */
+#define LM_VERIFY_PIECE 512       /* logits of a wave's step in the second */
+#define LM_VERIFY_MAX_PIECES 4096
+typedef struct lm_verify_params {
+  const void* logits;       /* (rows, vocab), rows logits_ld apart */
+  const void* draft;        /* (rows, vocab) probabilities or NULL */
+  const void* ids;          /* (rows,) */
+  const void* q_starts;     /* (seqs + 1,) */
+  const float* uniforms;    /* (rows, 2) */
+  void* tokens;             /* (rows,) as ids */
+  int32_t* counts;          /* (seqs,) */
+  double* part_sum;         /* (rows, slices) sums of exp((x - top) / temperature) */
+  float* part_top;          /* (rows, slices) */
+  int32_t* part_at;         /* (rows, slices) where it is first */
+  int64_t logits_ld, draft_ld;
+  int32_t rows;
+  int32_t seqs;
+  int32_t vocab;
+  int32_t slices;
+  int32_t logits_f32, draft_f32;
+  int32_t logits_vec, draft_vec; /* rows load in 16-byte pieces */
+  int32_t ids64;
+  int32_t starts64;
+  int32_t greedy;
+  float inv_temp;
+  double inv_temp64;
+} lm_verify_params;
 
 #endif /* KOTODAMA_AMD_LM_PARAMS_H */
