@@ -583,7 +583,7 @@ int attnres_embedding_bwd(const void* ids, int index_dtype, int64_t num_ids, con
  * table_ld apart, names each sequence's pages in order: token t of sequence s is row
  * t % page_size of page block_table[s][t / page_size], its slot
  * page * page_size + t % page_size.  New tokens are packed: sequence s has the
- * tokens q_starts[s] .. q_starts[s + 1] - 1 (seqs + 1 whole numbers, the first
+ * tokens q_starts[s] .. q_starts[s + 1] - 1 (seqs + 1 whole numbers, rising from
  * 0); those behind the last sequence are padding.  Lengths and starts
  * stay on the device; what would lead out of the tensors is taken into them.
  */

@@ -525,7 +525,7 @@ __device__ __forceinline__ void verify_pick(const lm_verify_params& P, PickShare
       if (d >= 0 && d < P.vocab) {
         const RowStats R = row_stats(P, r0 + i);
         if (P.greedy) {
-          stays = d == R.at;
+          stays = d == R.at && R.sum > 0;  // a NaN is not
         } else {
           const float x = get1(row_of(P.logits, P.logits_ld, r0 + i, P.logits_f32), (int)d, P.logits_f32);
           const double p = exp(((double)x - (double)R.top) * P.inv_temp64) / R.sum;

@@ -32,7 +32,9 @@ eager, which is where this package's kernels run.  With its ``kernels`` the
 embedding, the norms and rotation of queries and keys and the attention run
 on this package's kernels too (:mod:`kotodama_amd.lmops`), compiled around or
 not.  :meth:`LanguageModel.logits` runs the model behind a KV cache (prefill
-and single tokens) through the engine's cached loop and those operators.
+and single tokens) through the engine's cached loop and those operators;
+:meth:`LanguageModel.logits_paged` and :meth:`LanguageModel.step_paged` serve many
+sequences from a paged one (:mod:`kotodama_amd.paged`), prompts in chunks, single tokens and drafts.
 """
 
 from __future__ import annotations
@@ -45,7 +47,7 @@ import torch
 import torch.nn.functional as F
 from torch import Tensor, nn
 
-from . import engine, lmops
+from . import engine, lmops, paged
 
 
 @dataclass(frozen=True)
@@ -144,6 +146,18 @@ def _attention_cached(x: Tensor, an: Tensor, wq: Tensor, wk: Tensor, wv: Tensor,
         k, v = torch.cat((past[0], k), 2), torch.cat((past[1], v), 2)
     o = lmops.attention(q, k, v)
     return F.linear(o.transpose(1, 2).reshape(b, t, heads * head_dim), wo), (k, v)
+
+
+def _attention_paged(x: Tensor, an: Tensor, wq: Tensor, wk: Tensor, wv: Tensor, wo: Tensor, qn: Tensor, kn: Tensor,
+                     cos: Tensor, sin: Tensor, heads: int, kv_heads: int, head_dim: int, eps: float,
+                     layer: paged.PagedLayer) -> Tensor:
+    """The same for the packed new tokens (1, N, hidden) of a step over a paged cache, which it writes."""
+    q, k, v = _project(x, an, wq, wk, wv, heads, kv_heads, head_dim, eps)
+    step = layer.step
+    q, k = lmops.qk_norm_rope(q, k, qn, kn, cos, sin, eps, positions=step.positions)
+    paged.paged_write(k[0].transpose(0, 1), v[0].transpose(0, 1), layer.k, layer.v, step.slots)
+    o = paged.paged_attention(q[0].transpose(0, 1), layer.k, layer.v, layer.block_table, step.kv_lens, step.q_starts)
+    return F.linear(o.reshape(1, x.shape[1], heads * head_dim), wo)
 
 
 def _swiglu(x: Tensor, fn: Tensor, wg: Tensor, wu: Tensor, wd: Tensor, eps: float) -> Tensor:
@@ -249,6 +263,9 @@ class _Attention(nn.Module):
         c = self.c
         args = (x, self.pre_norm.weight, self.wq, self.wk, self.wv, self.wo, self.q_norm.weight, self.k_norm.weight,
                 rope_cos, rope_sin, c.num_attention_heads, c.num_kv_heads, c.head_dim, c.norm_eps)
+        if isinstance(layer_past, paged.PagedLayer):
+            out = _attention_paged(*args, layer_past)
+            return (out, layer_past) if use_cache else out
         if use_cache or layer_past is not None:
             out, kv = _attention_cached(*args, layer_past)
             return (out, kv) if use_cache else out
@@ -365,6 +382,45 @@ class LanguageModel(nn.Module):
         x = lmops.embedding(input_ids, self.embed)
         x, past_kv = engine.forward_attn_res_cached(self, x, None, past_kv)
         return F.linear(_rms(x, self.norm.weight, self.config.norm_eps), self.embed), past_kv
+
+    def new_cache(self, pages: int, sequences: int, page_size: int = 64,
+                  max_tokens: Optional[int] = None) -> paged.PagedCache:
+        """An empty paged cache of the model's layers for ``sequences`` sequences of up to ``max_tokens``, in
+        whole pages (by default as many as its rope tables have rows for, which is the most)."""
+        c = self.config
+        most = self.rope_cos.shape[0]
+        max_tokens = most // page_size * page_size if max_tokens is None else max_tokens
+        if max_tokens > most:
+            raise ValueError(f"{max_tokens} tokens, but the model's rope tables have {most} rows")
+        return paged.PagedCache(c.num_layers, pages, page_size, c.num_kv_heads, c.head_dim, sequences, max_tokens,
+                                self.embed.dtype, self.embed.device)
+
+    @torch.no_grad()
+    def logits_paged(self, input_ids: Tensor, cache: paged.PagedCache, step: paged.PagedSlots,
+                     rows: Optional[Tensor] = None) -> Tensor:
+        """Logits (N, vocabulary) of the packed new tokens ``input_ids`` (N,) of a step that ``cache.extend`` made,
+        or of its ``rows`` only; their keys and values stay in the cache.  Rows of padding and of refused sequences
+        mean nothing."""
+        x = lmops.embedding(input_ids[None], self.embed)
+        x, _ = engine.forward_attn_res_cached(self, x, None, cache.layers(step))
+        x = x[0] if rows is None else x[0, rows]
+        return F.linear(_rms(x, self.norm.weight, self.config.norm_eps), self.embed)
+
+    @torch.no_grad()
+    def step_paged(self, input_ids: Tensor, new: Tensor, cache: paged.PagedCache, uniforms: Tensor,
+                   draft_probs: Optional[Tensor] = None, temperature: float = 1.0) -> tuple[Tensor, Tensor]:
+        """One step of speculative sampling for every sequence: its last token and drafts behind it (``new[b]``
+        tokens in all; 1: no draft; 0: sits out) in, the tokens behind them out.
+
+        Returns :func:`paged.verify_drafts`'s tokens (N,) and counts (B,); the cache keeps what stands.  A refused sequence
+        gets no token and keeps what it had."""
+        held = cache.lens.clone()
+        step = cache.extend(new, input_ids.shape[0])
+        logits = self.logits_paged(input_ids, cache, step)
+        tokens, counts = paged.verify_drafts(logits, input_ids, step.q_starts, uniforms, draft_probs, temperature)
+        counts = torch.where(step.kv_lens > 0, counts, 0)
+        cache.keep(held + counts)
+        return torch.where(step.slots >= 0, tokens, -1), counts
 
 
 def make_batch(c: LMConfig, device, seed: int = 1) -> tuple[Tensor, Tensor]:

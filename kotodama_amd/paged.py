@@ -396,7 +396,7 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Te
     head h reads key head ``h // (H // Hk)``.  Key t of sequence b is row
     ``t % page_size`` of page ``block_table[b, t // page_size]`` ((B, M)
     int32).  ``kv_lens`` ((B,)) is how many keys each sequence has and
-    ``q_starts`` ((B + 1,), from 0) where its new tokens begin among the N,
+    ``q_starts`` ((B + 1,), rising from 0) where its new tokens begin among the N,
     whole numbers on the device; without ``q_starts`` each sequence has one.
     Token i of a sequence's n is at position ``kv_lens - n + i`` and sees the
     keys up to it.  Chunks of prompts, drafts and single tokens may be mixed.
@@ -545,7 +545,7 @@ class PagedCache:
     """Every layer's keys and values in pages, and which sequence holds which.
 
     ``pages`` pages of ``page_size`` tokens serve up to ``sequences`` sequences of up to
-    ``max_tokens`` each.  All state (``block_table``, ``lens``, ``free_pages``,
+    ``max_tokens`` (whole pages) each.  All state (``block_table``, ``lens``, ``free_pages``,
     ``free_count``, the pages) is on the device and changed in place, so that a
     captured step runs on from where the last one ended.
     """
@@ -553,11 +553,12 @@ class PagedCache:
     def __init__(self, layers: int, pages: int, page_size: int, kv_heads: int, head_dim: int, sequences: int,
                  max_tokens: int, dtype: torch.dtype, device) -> None:
         self.page_size = _check_page("PagedCache", page_size)
-        self.max_tokens = max_tokens
+        if max_tokens < page_size or max_tokens % page_size:
+            raise ValueError(f"PagedCache: {max_tokens} tokens are not whole pages of {page_size}")
         shape = (layers, 2, pages, kv_heads, page_size, head_dim)
         self.kv = torch.empty(shape, dtype=dtype, device=device)
         i32 = dict(dtype=torch.int32, device=device)
-        self.block_table = torch.zeros((sequences, -(-max_tokens // page_size)), **i32)
+        self.block_table = torch.zeros((sequences, max_tokens // page_size), **i32)
         self.lens = torch.zeros(sequences, **i32)  # tokens that each sequence holds
         self.free_pages = torch.arange(pages - 1, -1, -1, **i32)
         self.free_count = torch.full((1,), pages, **i32)
