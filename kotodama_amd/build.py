@@ -42,7 +42,7 @@ ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 ARCH = "gfx950"
 NUM_PARTS = 12  # of attnres_kernels.hip
 LM_PARTS = {12: "lm_kernels.hip", 13: "attention_kernels.hip", 14: "attention_kernels.hip",
-            15: "paged_attention_kernels.hip", 16: "serving_kernels.hip"}
+            15: "paged_attention_kernels.hip", 16: "paged_attention_kernels.hip", 17: "serving_kernels.hip"}
 HOST_SOURCES = ("attnres_capi.cpp", "lm_capi.cpp", "serving_capi.cpp")
 
 # Packed-fp32 VALU ops are disabled for every HIP compile (the kernels are

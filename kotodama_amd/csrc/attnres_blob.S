@@ -69,4 +69,8 @@ attnres_hsaco_part15:
     .global attnres_hsaco_part16
 attnres_hsaco_part16:
     .incbin "attnres_gfx950_part16.hsaco"
+    .balign 4096
+    .global attnres_hsaco_part17
+attnres_hsaco_part17:
+    .incbin "attnres_gfx950_part17.hsaco"
     .section .note.GNU-stack,"",@progbits

@@ -41,10 +41,11 @@ extern "C" const unsigned char attnres_hsaco_part13[];
 extern "C" const unsigned char attnres_hsaco_part14[];
 extern "C" const unsigned char attnres_hsaco_part15[];
 extern "C" const unsigned char attnres_hsaco_part16[];
+extern "C" const unsigned char attnres_hsaco_part17[];
 
 namespace {
 
-constexpr int kParts = 17;  // 12..16: the language-model operators (lm_capi.cpp, serving_capi.cpp)
+constexpr int kParts = 18;  // 12..17: the language-model operators (lm_capi.cpp, serving_capi.cpp)
 constexpr int kMaxDevices = 64;
 constexpr int kMaxThreads = 512;  // __launch_bounds__ of every kernel
 
@@ -218,7 +219,7 @@ int ensure_loaded(DeviceState** out) {
                                             attnres_hsaco_part6, attnres_hsaco_part7, attnres_hsaco_part8,
                                             attnres_hsaco_part9, attnres_hsaco_part10, attnres_hsaco_part11,
                                             attnres_hsaco_part12, attnres_hsaco_part13, attnres_hsaco_part14,
-                                            attnres_hsaco_part15, attnres_hsaco_part16};
+                                            attnres_hsaco_part15, attnres_hsaco_part16, attnres_hsaco_part17};
       // On a failure nothing stays half-loaded: the next call starts over.
       auto unload = [&st](int n) {
         for (int j = 0; j < n; ++j) {

@@ -137,6 +137,15 @@ typedef struct lm_embed_params {
  */
 #define LM_PAGED_THREADS (64 * LM_ATTN_WAVES)
 #define LM_PAGED_MIN_PAGE 16 /* rows of a wave's load lie in one page */
+/* A tile of rows whose keys several workgroups shared: their sums lie in the slots first, next, next + step ... */
+typedef struct lm_paged_note {
+  int32_t token;         /* its sequence's first */
+  int32_t row0;          /* its first row */
+  int32_t rows;          /* of the sequence */
+  int32_t head;          /* key head */
+  int32_t parts;         /* under two: nothing to join */
+  int32_t first, next, step;
+} lm_paged_note;
 typedef struct lm_paged_params {
   const void* q;         /* (tokens, heads, dim) */
   const void* k;         /* (pages, kv_heads, page_size, dim) */
@@ -145,6 +154,7 @@ typedef struct lm_paged_params {
   float* lse;            /* (tokens, heads) or NULL */
   float* part;           /* (slots, kv_heads, part_rows, dim): sums of a part of the keys */
   float* part_ml;        /* (slots, kv_heads, part_rows, 2): their maxima (times log2 e) and sums of weights */
+  lm_paged_note* notes;  /* few rows: (target, kv_heads); many: (slots, kv_heads) */
   const int32_t* table;  /* (seqs, table_width), rows table_ld apart */
   const void* kv_lens;   /* (seqs,) */
   const void* q_starts;  /* (seqs + 1,) or NULL */
@@ -159,10 +169,12 @@ typedef struct lm_paged_params {
   int32_t capacity;      /* keys of a table row: table_width * page_size */
   int32_t shift;         /* log2 of page_size */
   int32_t dim;
-  int32_t wide;          /* sequences of over 32 rows in tiles of 128 */
-  int32_t target;        /* workgroups to split the key axis for, */
-  int32_t least;         /* least blocks (of 32 keys a wave) of a part */
-  int32_t slots;         /* parts of split tiles that the workspace holds */
+  int32_t group;         /* heads / kv_heads; a number under 2^31 over it: (umulhi(n, mul) + n) >> shift */
+  uint32_t group_mul;
+  int32_t group_shift;
+  int32_t wide;          /* many rows: sequences of over 32 in tiles of 128 */
+  int32_t target;        /* workgroups (few rows: of a key head) to deal the key blocks out to */
+  int32_t slots;         /* parts of tiles that the workspace holds */
   int32_t part_rows;     /* rows of one */
   int32_t lens64;
   int32_t starts64;

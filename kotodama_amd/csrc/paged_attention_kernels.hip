@@ -9,15 +9,24 @@
 // r % group of its new token r / group.
 //
 // How the work is dealt out.  The host knows how many tokens and sequences a
-// call has, the device how long they are; so the grid is a bound, and every
-// workgroup finds its own work in the lengths: a tile of a sequence's rows and a
-// part of its keys.  Sequences of up to 32 rows (single tokens, drafts) are
-// narrow tiles: four waves share the 32 rows and each works on 32 keys of a tile
-// of 128.  The rows of longer ones are taken 128 at a time, each wave 32 of
-// them over all keys, where the call has rows enough to fill the card so
-// (`wide`), else 32 at a time as well.  Tiles of more keys than their
-// share (all blocks over `target` workgroups) are split, and
-// paged_join adds the parts in order, so that results repeat bit for bit.
+// call has, the device how long they are; so the grid is fixed or a bound, and every
+// workgroup finds its own work in the lengths.  Sequences of up to 32 rows (single
+// tokens, drafts) are narrow tiles: four waves share the 32 rows and each works
+// on 32 keys of a block of 128.
+//
+// Calls of few rows (paged_stream): all tiles are narrow.  The blocks of all
+// sequences' tiles lie one after another, and each of a key head's workgroups (two on
+// every CU, over all heads) takes an equal stretch of them, whatever
+// sequences it leads through.
+//
+// Calls with rows enough to fill the card 128 at a time (paged_tiles): the rows of
+// longer sequences are taken so, each wave 32 of them over all keys, a workgroup
+// a tile, the longest of a sequence first.  Tiles of more keys than their share (all blocks
+// over `target` workgroups) are split, narrow ones beside them too.
+//
+// What a workgroup has of a tile that others share goes to the workspace, with a
+// note of its parts, and paged_join adds them in order, so that
+// results repeat bit for bit.
 //
 // Keys are found through the table: a wave-wide load covers at most 8 rows,
 // which lie in one page, so the page's address is uniform and a lane's
@@ -33,50 +42,67 @@ constexpr int kThreads = LM_PAGED_THREADS;
 
 // ---------------------------------------------------------------- schedule --
 
-// One sequence's share of the call: its tokens, keys, tiles of rows and parts of their keys.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// Element i of 32- or 64-bit whole numbers, taken into [0, most]; without a branch: the
+// compiler makes one for each otherwise, and the schedule is a chain of such reads.
+__device__ __forceinline__ int taken(const void* p, int i, int is64, int most) {
+  const int32_t* w = (const int32_t*)p + ((int64_t)i << is64);
+  const int lo = w[0], up = w[is64], hi = is64 ? up : lo >> 31;
+  return hi < 0 ? 0 : hi > 0 || (uint32_t)lo > (uint32_t)most ? most : lo;
+}
+
+// One sequence's share of the call: its tokens, keys and tiles of rows.
 struct Share {
   int first, count;  // new tokens
   int kv_len;
-  int rows, tiles, splits;
+  int rows, tiles;
   bool narrow;
-  int per;  // key tiles of a part
 };
 
 // The sequences' sizes are taken into what the call has, so that no length
 // leads out of its tensors.  Behind the last sequence (s == seqs): the tokens that
 // belong to none, as a sequence without keys.
-__device__ __forceinline__ Share share_of(const lm_paged_params& P, int s, int group) {
+__device__ __forceinline__ Share share_of(const lm_paged_params& P, int s) {
   Share a;
-  int64_t lo, hi;
-  if (P.q_starts == nullptr) {
-    lo = s;
-    hi = s < P.seqs ? s + 1 : P.tokens;
-  } else {
-    lo = s == 0 ? 0 : index_at(P.q_starts, s, P.starts64);
-    hi = s < P.seqs ? index_at(P.q_starts, s + 1, P.starts64) : P.tokens;
+  const int in = s < P.seqs ? s : P.seqs - 1;  // where the last is read in place of none
+  int lo = s, hi = s + 1;
+  if (P.q_starts != nullptr) {
+    lo = s == 0 ? 0 : taken(P.q_starts, s, P.starts64, P.tokens);
+    hi = taken(P.q_starts, in + 1, P.starts64, P.tokens);
   }
-  lo = lo < 0 ? 0 : lo > P.tokens ? P.tokens : lo;
-  hi = hi < lo ? lo : hi > P.tokens ? P.tokens : hi;
-  int64_t n = s < P.seqs ? index_at(P.kv_lens, s, P.lens64) : 0;
-  n = n < 0 ? 0 : n > P.capacity ? P.capacity : n;
-  a.first = (int)lo;
-  a.count = (int)(hi - lo);
-  a.kv_len = (int)n;
-  a.rows = a.count * group;
+  hi = s < P.seqs ? hi : P.tokens;
+  a.first = lo;
+  a.count = hi > lo ? hi - lo : 0;
+  a.kv_len = 0;
+  if (P.seqs > 0) a.kv_len = taken(P.kv_lens, in, P.lens64, P.capacity);
+  a.kv_len = s < P.seqs ? a.kv_len : 0;
+  a.rows = a.count * P.group;
   a.narrow = !P.wide || a.rows <= 32;
   a.tiles = a.narrow ? (a.rows + 31) >> 5 : (a.rows + 127) >> 7;
-  a.splits = a.per = 0;
   return a;
 }
-// A tile's work: blocks of 32 keys that a wave works on.
-__device__ __forceinline__ int blocks_of(const Share& a) {
-  return a.narrow ? (a.kv_len + 127) >> 7 : ((a.kv_len + 63) >> 6) * 2;
+
+// A sequence's own token of row r, rows a group for each (r under 2^31).
+__device__ __forceinline__ int query_of(const lm_paged_params& P, int r) {
+  return (int)((__umulhi((uint32_t)r, P.group_mul) + (uint32_t)r) >> P.group_shift);
 }
-__device__ __forceinline__ void split(Share& a, int most) {
-  a.per = a.narrow ? most : (most + 1) >> 1;
-  const int n = a.narrow ? (a.kv_len + 127) >> 7 : (a.kv_len + 63) >> 6;
-  a.splits = n <= a.per ? 1 : (n + a.per - 1) / a.per;
+
+// The launch's arguments, read anew: values that the code before holds on to would
+// crowd a loop's scalar registers.
+typedef const __attribute__((address_space(4))) lm_paged_params* ParamsPtr;
+__device__ __forceinline__ const lm_paged_params& anew() {
+  ParamsPtr p = (ParamsPtr)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const lm_paged_params*)p;
 }
+
+// What a workgroup takes of a tile: its key blocks t0 .. t1-1 (of 128 keys, in a wide tile 64).
+struct Piece {
+  Share a;
+  int seq, tile, t0, t1;
+  int slot;  // where its sums go in the workspace; -1: it has all keys, and writes the result
+};
 
 struct Shared {
   float sum[LM_ATTN_WAVES];
@@ -84,9 +110,37 @@ struct Shared {
   int upto[kThreads][2];
 };
 
-// Sum of a float over the workgroup (all threads get it); whole numbers under 2^24 or nearly so.
+// Inclusive sums of N numbers over the workgroup's threads into S.upto.
+template <int N>
+__device__ __forceinline__ void scan_all(int (&v)[N], Shared& S) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int x = __shfl_up(v[i], m);
+      v[i] += lane >= m ? x : 0;
+    }
+  __syncthreads();  // what was there has been read
+  if (lane == 63) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) S.scan[wave][i] = v[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+#pragma unroll
+    for (int w = 0; w < LM_ATTN_WAVES - 1; ++w) v[i] += w < wave ? S.scan[w][i] : 0;
+    S.upto[threadIdx.x][i] = v[i];
+  }
+  __syncthreads();
+}
+
+// Sum over the workgroup, to every thread, in a fixed order.
 __device__ __forceinline__ float sum_all(float v, Shared& S) {
+#pragma unroll
   for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
+  __syncthreads();
   if ((threadIdx.x & 63) == 0) S.sum[threadIdx.x >> 6] = v;
   __syncthreads();
   float t = 0.f;
@@ -95,270 +149,434 @@ __device__ __forceinline__ float sum_all(float v, Shared& S) {
   return t;
 }
 
-// Inclusive sums of two numbers over the workgroup's threads into S.upto.
-__device__ __forceinline__ void scan_all(int a, int b, Shared& S) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// The thread whose inclusive sum is the first over `at`, which is under the last.
+__device__ __forceinline__ int find_upto(const Shared& S, int at) {
+  int lo = 0;
 #pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const int x = __shfl_up(a, m), y = __shfl_up(b, m);
-    a += lane >= m ? x : 0;
-    b += lane >= m ? y : 0;
-  }
-  if (lane == 63) {
-    S.scan[wave][0] = a;
-    S.scan[wave][1] = b;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < LM_ATTN_WAVES - 1; ++i) {
-    a += i < wave ? S.scan[i][0] : 0;
-    b += i < wave ? S.scan[i][1] : 0;
-  }
-  S.upto[threadIdx.x][0] = a;
-  S.upto[threadIdx.x][1] = b;
-  __syncthreads();
+  for (int step = kThreads / 2; step > 0; step >>= 1)
+    if (S.upto[lo + step - 1][0] <= at) lo += step;
+  return uniform(lo);
 }
 
-// The blocks of 32 keys that a part may have: an equal share for `target` workgroups.
-// (A float's rounding moves the share by a part in 2^24; every workgroup of
-// both launches finds the same.)
-__device__ __forceinline__ int most_blocks(const lm_paged_params& P, int group, Shared& S) {
-  float work = 0.f;
-  for (int s = threadIdx.x; s < P.seqs; s += kThreads) {
-    const Share a = share_of(P, s, group);
-    work += (float)a.tiles * (float)blocks_of(a);
-  }
-  work = sum_all(work, S) * (float)P.kv_heads / (float)P.target;
-  const int n = work < 1e9f ? (int)__builtin_ceilf(work) : 1 << 30;
-  return n < P.least ? P.least : n;
-}
-
-// A workgroup's work.
-struct Job {
-  Share a;
-  int seq, tile, part;
-  int slot;  // where a split tile's parts begin
-};
-
-// Finds part `w` of the call's (all sequences' parts one after another).
-__device__ __forceinline__ bool find_job(const lm_paged_params& P, int w, int group, Shared& S, Job& J) {
-  const int most = most_blocks(P, group, S);
-  int parts = 0, slots = 0;  // before this stretch of sequences
-  for (int base = 0; base <= P.seqs; base += kThreads) {
-    const int s = base + (int)threadIdx.x;
-    int mine = 0, held = 0;
-    if (s <= P.seqs) {
-      Share a = share_of(P, s, group);
-      split(a, most);
-      mine = a.tiles * a.splits;
-      held = a.splits > 1 ? mine : 0;
-    }
-    scan_all(mine, held, S);
-    const int total = S.upto[kThreads - 1][0];
-    if (w - parts < total) {
-      int lo = 0;  // the first sequence whose parts end behind w
-#pragma unroll
-      for (int step = kThreads / 2; step > 0; step >>= 1)
-        if (S.upto[lo + step - 1][0] <= w - parts) lo += step;
-      const int before = lo > 0 ? S.upto[lo - 1][0] : 0;
-      J.seq = __builtin_amdgcn_readfirstlane(base + lo);
-      J.a = share_of(P, J.seq, group);
-      split(J.a, most);
-      const int i = __builtin_amdgcn_readfirstlane(w - parts - before);
-      const int rank = i / J.a.splits;
-      J.part = i - rank * J.a.splits;
-      J.tile = J.a.tiles - 1 - rank;  // the longest first
-      J.slot = __builtin_amdgcn_readfirstlane(slots + (lo > 0 ? S.upto[lo - 1][1] : 0)) + rank * J.a.splits;
-      return true;
-    }
-    parts += total;
-    slots += S.upto[kThreads - 1][1];
-    __syncthreads();
-  }
-  return false;
+// A tile whose keys several workgroups share, for the join; whole tiles have none (parts 0).
+__device__ __forceinline__ void write_note(const lm_paged_params& P, int at, const Share& a, int row0, int head,
+                                           int parts, int first, int next, int step) {
+  lm_paged_note n;
+  n.token = a.first;
+  n.row0 = row0;
+  n.rows = a.rows;
+  n.head = head;
+  n.parts = parts;
+  n.first = first;
+  n.next = next;
+  n.step = step;
+  P.notes[at] = n;
 }
 
 // ------------------------------------------------------------------- pages --
 
-// A sequence's pages, as one wave reads them.
-struct Pages {
-  const int32_t* table;
-  int shift, pages, last;  // last: the last key that exists
-  bool bad;                // an entry outside the cache was met
-
-  // The pages of 64 rows from `row`: lane i holds that of row + i (of the last row behind it).
-  __device__ __forceinline__ int of(int row, int lane) const {
-    const int r = row + lane;
-    return table[(r < last ? r : last) >> shift];
-  }
-  // Entries as they may be read.
-  __device__ __forceinline__ int checked(int page) {
-    const bool out = (uint32_t)page >= (uint32_t)pages;
-    bad = bad || __any(out);
-    return out ? 0 : page;
+// Where a head's rows lie: its first page's, and the bytes from page to page and row to row.
+struct Rows {
+  const char* base;
+  uint32_t page_bytes, row_bytes;
+  __device__ __forceinline__ Rows(const void* p, const lm_strides& st, int kvh, int es)
+      : base((const char*)p + (int64_t)kvh * st.h * es), page_bytes((uint32_t)(st.b * es)),
+        row_bytes((uint32_t)(st.t * es)) {}
+  __device__ __forceinline__ const char* at(uint32_t page, uint32_t row) const {
+    return base + (uint64_t)page * page_bytes + row * row_bytes;  // a page's rows span under 2^31 bytes
   }
 };
 
-// Requests the R rows of tile KT from key `row0` (a multiple of 32) into `lds`, as
-// KT::request does for contiguous keys.  `page`: Pages::of(row0).
+// A sequence's pages as one wave reads them, and its keys and values by them.
+// Everything here is uniform, and is kept in scalar registers by reading the table
+// through the scalar cache: with the lanes' own addresses, or pages
+// handed on by v_readlane, the wide tiles' vector unit, which is what they wait for
+// next to the matrix cores, had 18% more to do (2048 tokens behind 14336, 32/8 heads of 128: 575 against 510 us).
 template <typename KT>
-__device__ __forceinline__ void request_paged(char* lds, const char* src, const lm_strides& st, int es, int row0, int last,
-                                              int shift, int page, int chunks, int wave, int lane) {
-  constexpr int kPerWave = 64 / KT::kChunks;  // rows of a wave's load
-  static_assert(kPerWave <= LM_PAGED_MIN_PAGE, "in one page");
-  constexpr int kWaves = KT::kRound / kPerWave;
-  const int mask = (1 << shift) - 1;
-  const int64_t page_bytes = st.b * es;
-  const uint32_t row_bytes = (uint32_t)(st.t * es);
-  const int mine = lane / KT::kChunks;
+struct Keys {
+  static constexpr int kPerWave = 64 / KT::kChunks;  // rows of a wave's load
+  static_assert(kPerWave <= LM_PAGED_MIN_PAGE && LM_PAGED_MIN_PAGE == 16, "in one page");
+  static constexpr int kWaves = KT::kRound / kPerWave;
+  static constexpr int kLog = KT::kRows == 64 ? 6 : 5;
+  // Pages that a wave asks for in a tile: of each round's first row, or of each 16 rows.
+  static constexpr bool kByRound = KT::kRound >= 16;
+  static constexpr int kPages = kByRound ? KT::kRounds : KT::kRows / 16;
+
+  const __attribute__((address_space(4))) int32_t* table;
+  Rows k, v;
+  int shift, pages, last;  // last: the last key that exists
+  int chunks, wave;
+  bool one;                // a tile lies in one page
+  bool bad;                // an entry outside the cache was met
+  int page[kPages];        // of the tile that is requested next
+
+  __device__ __forceinline__ Keys(const lm_paged_params& P, const Piece& J, int kvh, int es, int wave_)
+      : table((const __attribute__((address_space(4))) int32_t*)(P.table + (int64_t)J.seq * P.table_ld)),
+        k(P.k, P.sk, kvh, es), v(P.v, P.sv, kvh, es), shift(P.shift), pages(P.pages), last(J.a.kv_len - 1),
+        chunks(P.dim * es / 16), wave(wave_), one(P.shift >= kLog), bad(false) {}
+
+  // Reads the pages of the tile from key `row0` on (a multiple of 32); of the last key's behind it.
+  __device__ __forceinline__ void find(int row0) {
+    auto of = [&](int j) {
+      const int r = row0 + (kByRound ? j * KT::kRound + wave * kPerWave : 16 * j);
+      return table[(r < last ? r : last) >> shift];
+    };
+    page[0] = of(0);
+    if (one) {
 #pragma unroll
-  for (int i = 0; i < KT::kRounds; ++i) {
-    const int first = i * KT::kRound + wave * kPerWave;
-    const int p = __builtin_amdgcn_readlane(page, first);
-    const char* base = src + (int64_t)p * page_bytes;
-    const int row = row0 + first;
-    char* to = lds + (i * kWaves + wave) * 1024;
-    const uint32_t chunk = KT::chunk_offset(i, wave, lane, chunks);
-    if (row + kPerWave - 1 <= last) {
-      KT::load_lds(to, base + (uint64_t)((uint32_t)(row & mask)) * row_bytes, (uint32_t)mine * row_bytes + chunk);
-    } else {  // rows behind the last repeat it
-      const int r = row + mine < last ? row + mine : last;
-      KT::load_lds(to, base, (uint32_t)(r & mask) * row_bytes + chunk);
+      for (int j = 1; j < kPages; ++j) page[j] = page[0];
+    } else {
+#pragma unroll
+      for (int j = 1; j < kPages; ++j) page[j] = of(j);
     }
   }
+  __device__ __forceinline__ uint32_t checked(int p) {
+    const bool out = (uint32_t)p >= (uint32_t)pages;
+    bad = bad || out;
+    return out ? 0 : (uint32_t)p;
+  }
+
+  // Requests that tile, as KT::request does for contiguous keys.
+  __device__ __forceinline__ void request(char* kl, char* vl, int row0, int lane) {
+    const uint32_t mask = (1u << shift) - 1;
+    const int mine = lane / KT::kChunks;
+    const uint32_t ko = (uint32_t)mine * k.row_bytes, vo = (uint32_t)mine * v.row_bytes;
+    auto load = [&](int i, const char* kb, const char* vb, uint32_t kr, uint32_t vr) {
+      const uint32_t c = KT::chunk_offset(i, wave, lane, chunks);
+      KT::load_lds(kl + (i * kWaves + wave) * 1024, kb, kr + c);
+      KT::load_lds(vl + (i * kWaves + wave) * 1024, vb, vr + c);
+    };
+    if (row0 + KT::kRows - 1 <= last) {
+      if (one) {
+        const uint32_t p = checked(page[0]), r = ((uint32_t)row0 & mask) + (uint32_t)(wave * kPerWave);
+        const char *kb = k.at(p, r), *vb = v.at(p, r);
+#pragma unroll
+        for (int i = 0; i < KT::kRounds; ++i) {
+          load(i, kb, vb, ko, vo);
+          kb += KT::kRound * k.row_bytes;
+          vb += KT::kRound * v.row_bytes;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < KT::kRounds; ++i) {
+          const uint32_t p = checked(page[kByRound ? i : i * KT::kRound / 16]);
+          const uint32_t r = (uint32_t)(row0 + i * KT::kRound + wave * kPerWave) & mask;
+          load(i, k.at(p, r), v.at(p, r), ko, vo);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < KT::kRounds; ++i) {  // rows behind the last repeat it
+        const uint32_t p = checked(page[kByRound ? i : i * KT::kRound / 16]);
+        const int r = row0 + i * KT::kRound + wave * kPerWave + mine;
+        const uint32_t in = (uint32_t)(r < last ? r : last) & mask;
+        load(i, k.at(p, 0), v.at(p, 0), in * k.row_bytes, in * v.row_bytes);
+      }
+    }
+  }
+};
+
+// ------------------------------------------------------------------- tiles --
+
+// A row of a tile: which it is, and the keys it sees.
+struct Row {
+  int row, query, head, lim;
+  bool exists;
+  __device__ __forceinline__ Row(const lm_paged_params& P, const Share& a, int r, int kvh) {
+    row = r;
+    query = query_of(P, r);
+    head = kvh * P.group + (r - query * P.group);
+    exists = r < a.rows;
+    lim = a.kv_len == 0 ? 0 : a.kv_len - a.count + query + 1;
+  }
+};
+// The keys that row r sees, if any.
+__device__ __forceinline__ int sees(const lm_paged_params& P, const Share& a, int r) {
+  return a.kv_len == 0 ? 0 : a.kv_len - a.count + query_of(P, r) + 1;
 }
 
-// ----------------------------------------------------------------- forward --
+template <typename T>
+__device__ __forceinline__ const char* q_row(const lm_paged_params& P, const Share& a, const Row& R) {
+  return (const char*)P.q + ((int64_t)(a.first + R.query) * P.q_t + (int64_t)R.head * P.q_h) * T::kBytes;
+}
+template <typename T>
+__device__ __forceinline__ char* o_row(const lm_paged_params& P, const Share& a, const Row& R) {
+  return (char*)P.o + ((int64_t)(a.first + R.query) * P.o_t + (int64_t)R.head * P.o_h) * T::kBytes;
+}
+__device__ __forceinline__ float lse_of(float m, float l) {
+  return l == 0.f ? kNegInf : (m + __builtin_amdgcn_logf(l)) * kLn2;
+}
 
-// KS 4: a narrow tile, KS 1: a wide one.
-template <typename T, int DP, int DC, int KS>
-__device__ __forceinline__ void paged_rows(const lm_paged_params& P, const Job& J, int kvh, int group, char* lds,
-                                           float* ml, int* flag) {
-  constexpr int kKeys = KS == 4 ? 128 : 64;  // keys of a tile
-  constexpr int NB = kKeys / 32 / KS;        // 32-key blocks of a wave in it
-  using KT = Tile<T, DP, kKeys>;
-  const int lane = threadIdx.x & 63, h = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int part = wave % KS;
-  const int g0 = J.tile * (32 * LM_ATTN_WAVES / KS), r0 = g0 + wave / KS * 32;
-  const int start = J.a.kv_len - J.a.count;  // position of token 0
-  const int row = r0 + (lane & 31), query = row / group;
-  const int head = kvh * group + (row - query * group);
-  const bool exists = row < J.a.rows;
-  const int lim = J.a.kv_len == 0 ? 0 : start + query + 1;  // keys this row sees, if any
-  // the keys that the wave's rows see: the most, and what all see (rows that are not there are not stored)
-  auto sees = [&](int r) { return J.a.kv_len == 0 ? 0 : start + r / group + 1; };
-  auto end = [&](int r) { return r < J.a.rows ? r : J.a.rows; };
-  const int most = __builtin_amdgcn_readfirstlane(r0 < J.a.rows ? sees(end(r0 + 32) - 1) : 0);
-  const int all = __builtin_amdgcn_readfirstlane(sees(r0));
-  const int any = __builtin_amdgcn_readfirstlane(sees(end(g0 + 32 * LM_ATTN_WAVES / KS) - 1));
-  const int tiles = any <= 0 ? 0 : (any + kKeys - 1) / kKeys;
-  const int t0 = J.part * J.a.per, t1 = tiles < t0 + J.a.per ? tiles : t0 + J.a.per;
+// The workgroup's LDS, in four arrays of their own: the compiler lets a read of one pass a
+// load into another that is under way; where both are in one array it waits for the
+// load, and a wide tile's next block is no longer on its way while it works on one.
+#define LDS_ARRAYS LM_LDS char *a, LM_LDS char *b, LM_LDS char *c, LM_LDS char *d
+template <typename T, int DP>
+constexpr int kLdsBytes = Tile<T, DP, 64>::kBytes;  // of each
+__device__ __forceinline__ char* lds_of(int wave, LDS_ARRAYS) {
+  LM_LDS char* lo = wave == 0 ? a : b;
+  LM_LDS char* hi = wave == 2 ? c : d;
+  return (char*)(wave < 2 ? lo : hi);
+}
+
+// 32 rows, four waves: each works on its own 32 keys of a block of 128, loads them itself
+// and waits for no other; in the end every wave adds all four's sums of its 32 columns.
+// ml: 4 x 128 floats.
+template <typename T, int DP, int DC>
+__device__ __forceinline__ void narrow_tile(const Piece& J, int kvh, LDS_ARRAYS, float* ml) {
+  using KT = Tile<T, DP, 32, 1>;
+  const lm_paged_params& P = anew();
+  const int lane = threadIdx.x & 63, h = lane >> 5, wave = uniform(threadIdx.x >> 6);
+  const int r0 = J.tile * 32;
+  const Row R(P, J.a, r0 + (lane & 31), kvh);
+  // rows that are not there are not stored
+  const int most = uniform(sees(P, J.a, (r0 + 32 < J.a.rows ? r0 + 32 : J.a.rows) - 1));
+  const int all = uniform(sees(P, J.a, r0));
+  const int own = 32 * wave;
+  const int end = most < J.t1 * 128 ? most : J.t1 * 128;  // of the keys
 
   typename T::Frag qf[DC / 16];
-  load_rows<T, DC>(qf, (const char*)P.q + ((int64_t)(J.a.first + query) * P.q_t + (int64_t)head * P.q_h) * T::kBytes,
-                   P.dim, h, exists);
+  load_rows<T, DC>(qf, q_row<T>(P, J.a, R), P.dim, h, R.exists);
   f32x16 acc[DC / 32];
 #pragma unroll
   for (int i = 0; i < DC / 32; ++i) acc[i] = zero16();
   float m = kNegInf, l = 0.f;
   const int row_at = KT::row_at(lane), col_at = KT::col_at(lane);
-  const int chunks = P.dim * T::kBytes / 16;
-  const char* kp = (const char*)P.k + (int64_t)kvh * P.sk.h * T::kBytes;
-  const char* vp = (const char*)P.v + (int64_t)kvh * P.sv.h * T::kBytes;
-  Pages pg;
-  pg.table = P.table + (int64_t)J.seq * P.table_ld;
-  pg.shift = P.shift;
-  pg.pages = P.pages;
-  pg.last = J.a.kv_len - 1;
-  pg.bad = false;
-
-  if constexpr (KS == 4) {
-    // each wave reads only its own 32 keys of a tile, so it loads them itself and waits for no other
-    using MT = typename KT::Mine;
-    const int own = 32 * wave;
-    char* kc = lds;
-    char* vc = lds + KT::kBytes;
-    int page = t0 < t1 && t0 * kKeys + own < most ? pg.of(t0 * kKeys + own, lane) : 0;
-    for (int t = t0; t < t1 && t * kKeys + own < most; ++t) {
-      const int key0 = t * kKeys + own;
-      int ln = lane;  // opaque: offsets formed anew for each tile instead of held in registers
-      asm volatile("" : "+v"(ln));
-      const int now = pg.checked(page);
-      page = t + 1 < t1 ? pg.of(key0 + kKeys, ln) : 0;
-      request_paged<MT>(kc + own * KT::kRowBytes, kp, P.sk, T::kBytes, key0, pg.last, pg.shift, now, chunks, 0, ln);
-      request_paged<MT>(vc + own * KT::kRowBytes, vp, P.sv, T::kBytes, key0, pg.last, pg.shift, now, chunks, 0, ln);
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      attend<T, KT, DC, NB>(kc, vc, own, key0, all, lim, qf, acc, m, l, P.scale_log2, row_at, col_at, lane, h);
+  Keys<KT> keys(P, J, kvh, T::kBytes, 0);
+  char* kc = lds_of(wave, a, b, c, d);
+  char* vc = kc + KT::kBytes;
+  int key0 = J.t0 * 128 + own;
+  if (key0 < end) keys.find(key0);
+  for (; key0 < end; key0 += 128) {
+    int ln = lane;  // opaque: offsets formed anew for each block instead of held in registers
+    asm volatile("" : "+v"(ln));
+    keys.request(kc, vc, key0, ln);
+    if (key0 + 128 < end) keys.find(key0 + 128);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    attend<T, KT, DC, 1>(kc, vc, 0, key0, all, R.lim, qf, acc, m, l, P.scale_log2, row_at, col_at, lane, h);
+  }
+  l += other_half(l);
+  if (keys.bad) l = __builtin_nanf("");
+  static_assert(64 * DC / 2 * 4 <= kLdsBytes<T, DP>, "a wave's sums in its array");
+  put<DC>(reinterpret_cast<float*>(kc), acc, lane);
+  ml[wave * 128 + lane] = m;
+  ml[wave * 128 + 64 + lane] = l;
+  __syncthreads();
+  m = kNegInf;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) m = fmaxf(m, ml[w * 128 + lane]);
+  float fade[4];
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float om = ml[w * 128 + lane];
+    fade[w] = om == kNegInf ? 0.f : exp2_fast(om - m);
+    l = __builtin_fmaf(ml[w * 128 + 64 + lane], fade[w], l);  // a NaN stays one
+  }
+  if (wave < DC / 32 && R.exists) {
+    float sum[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      sum[i] = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) sum[i] = __builtin_fmaf(reinterpret_cast<const float*>(lds_of(w, a, b, c, d))[(wave * 16 + i) * 64 + lane], fade[w], sum[i]);
     }
-  } else {
-    // the waves share the tiles: the next is requested before one is worked on, its pages read a tile before that
-    char* kb[2] = {lds, lds + 2 * KT::kBytes};
-    char* vb[2] = {lds + KT::kBytes, lds + 3 * KT::kBytes};
-    int page = 0;
-    auto request = [&](int t, char* k, char* v) {
-      const int now = pg.checked(page);
-      request_paged<KT>(k, kp, P.sk, T::kBytes, t * kKeys, pg.last, pg.shift, now, chunks, wave, lane);
-      request_paged<KT>(v, vp, P.sv, T::kBytes, t * kKeys, pg.last, pg.shift, now, chunks, wave, lane);
-      if (t + 1 < t1) page = pg.of((t + 1) * kKeys, lane);
-    };
-    auto arrived = [] {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
-    };
-    auto step = [&](int t, const char* kc, const char* vc) {
-      if (t * kKeys >= most) return;
-      attend<T, KT, DC, NB>(kc, vc, 0, t * kKeys, all, lim, qf, acc, m, l, P.scale_log2, row_at, col_at, lane, h);
-    };
-    if (t0 < t1) {
-      page = pg.of(t0 * kKeys, lane);
-      request(t0, kb[0], vb[0]);
+    const lm_paged_params& P = anew();
+    const bool whole = J.slot < 0;
+    const int64_t at = (int64_t)J.slot * P.part_rows + (R.row - r0);
+    const float scale = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;  // a NaN stays one
+    char* to = o_row<T>(P, J.a, R);
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      const int d = 32 * wave + 8 * a + 4 * h;
+      if (d >= P.dim) continue;
+      if (whole)
+        store4<T>(to + d * T::kBytes, sum[4 * a] * scale, sum[4 * a + 1] * scale, sum[4 * a + 2] * scale,
+                  sum[4 * a + 3] * scale);
+      else
+        store4<F32>(reinterpret_cast<char*>(P.part + at * P.dim + d), sum[4 * a], sum[4 * a + 1], sum[4 * a + 2],
+                    sum[4 * a + 3]);
     }
-    for (int t = t0; t < t1; t += 2) {
-      arrived();
-      if (t + 1 < t1) request(t + 1, kb[1], vb[1]);
-      step(t, kb[0], vb[0]);
-      if (t + 1 < t1) {
-        arrived();
-        if (t + 2 < t1) request(t + 2, kb[0], vb[0]);
-        step(t + 1, kb[1], vb[1]);
+    if (wave == 0 && h == 0) {
+      if (!whole) {
+        P.part_ml[at * 2] = m;
+        P.part_ml[at * 2 + 1] = l;
+      } else if (P.lse != nullptr) {
+        P.lse[(int64_t)(J.a.first + R.query) * P.heads + R.head] = lse_of(m, l);
       }
     }
   }
-  // a page outside the cache that any wave met
-  if (pg.bad && lane == 0) *flag = 1;
-  l += other_half(l);
-  if constexpr (KS == 4) {
-    join_waves<DC, KS>(reinterpret_cast<float*>(lds), ml, part, acc, m, l, lane);
-    if (part != 0) return;
-  } else {
+}
+
+// 128 rows, each wave 32 of them over all keys: the waves share the blocks of 64, the next
+// requested before one is worked on, its pages read a block before that.
+template <typename T, int DP, int DC>
+__device__ __forceinline__ void wide_tile(const Piece& J, int kvh, LDS_ARRAYS, int* flag) {
+  using KT = Tile<T, DP, 64>;
+  const lm_paged_params& P = anew();
+  const int lane = threadIdx.x & 63, h = lane >> 5, wave = uniform(threadIdx.x >> 6);
+  const int g0 = J.tile * 128, r0 = g0 + wave * 32;
+  const Row R(P, J.a, r0 + (lane & 31), kvh);
+  auto last_of = [&](int r) { return (r < J.a.rows ? r : J.a.rows) - 1; };
+  const int most = uniform(r0 < J.a.rows ? sees(P, J.a, last_of(r0 + 32)) : 0);
+  const int all = uniform(sees(P, J.a, r0));
+  const int any = uniform(sees(P, J.a, last_of(g0 + 128)));
+  const int t1 = any < J.t1 * 64 ? (any + 63) >> 6 : J.t1;  // no less than 0
+
+  typename T::Frag qf[DC / 16];
+  load_rows<T, DC>(qf, q_row<T>(P, J.a, R), P.dim, h, R.exists);
+  f32x16 acc[DC / 32];
+#pragma unroll
+  for (int i = 0; i < DC / 32; ++i) acc[i] = zero16();
+  float m = kNegInf, l = 0.f;
+  const int row_at = KT::row_at(lane), col_at = KT::col_at(lane);
+  Keys<KT> keys(P, J, kvh, T::kBytes, wave);
+  auto request = [&](int t, char* k, char* v) {
+    keys.request(k, v, t * 64, lane);
+    if (t + 1 < t1) keys.find((t + 1) * 64);
+  };
+  auto arrived = [] {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
+  };
+  auto step = [&](int t, const char* kc, const char* vc) {
+    if (t * 64 >= most) return;
+    attend<T, KT, DC, 2>(kc, vc, 0, t * 64, all, R.lim, qf, acc, m, l, P.scale_log2, row_at, col_at, lane, h);
+  };
+  if (J.t0 < t1) {
+    keys.find(J.t0 * 64);
+    request(J.t0, (char*)a, (char*)b);
   }
+  for (int t = J.t0; t < t1; t += 2) {
+    arrived();
+    if (t + 1 < t1) request(t + 1, (char*)c, (char*)d);
+    step(t, (char*)a, (char*)b);
+    if (t + 1 < t1) {
+      arrived();
+      if (t + 2 < t1) request(t + 2, (char*)a, (char*)b);
+      step(t + 1, (char*)c, (char*)d);
+    }
+  }
+  // a page outside the cache that any wave met
+  if (keys.bad && lane == 0) *flag = 1;
+  __syncthreads();
+  l += other_half(l);
   if (*flag != 0) l = __builtin_nanf("");
-  if (!exists) return;
-  if (J.a.splits > 1) {
-    if (J.slot + J.part >= P.slots) return;
-    const int64_t at = ((int64_t)(J.slot + J.part) * P.kv_heads + kvh) * P.part_rows + (row - g0);
-    if (l != 0.f) store_rows<F32, DC>(reinterpret_cast<char*>(P.part + at * P.dim), acc, 1.f, P.dim, h);
+  if (!R.exists) return;
+  const lm_paged_params& E = anew();
+  if (J.slot >= 0) {
+    const int64_t at = (int64_t)J.slot * E.part_rows + (R.row - g0);
+    store_rows<F32, DC>(reinterpret_cast<char*>(E.part + at * E.dim), acc, 1.f, E.dim, h);
     if (h == 0) {
-      P.part_ml[at * 2] = m;
-      P.part_ml[at * 2 + 1] = l;
+      E.part_ml[at * 2] = m;
+      E.part_ml[at * 2 + 1] = l;
     }
     return;
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;  // a NaN stays one
-  const int64_t token = J.a.first + query;
-  store_rows<T, DC>((char*)P.o + (token * P.o_t + (int64_t)head * P.o_h) * T::kBytes, acc, inv, P.dim, h);
-  if (P.lse != nullptr && h == 0)
-    P.lse[token * P.heads + head] = l == 0.f ? kNegInf : (m + __builtin_amdgcn_logf(l)) * kLn2;
+  store_rows<T, DC>(o_row<T>(E, J.a, R), acc, l == 0.f ? 0.f : 1.f / l, E.dim, h);
+  if (E.lse != nullptr && h == 0) E.lse[(int64_t)(J.a.first + R.query) * E.heads + R.head] = lse_of(m, l);
 }
 
-template <typename T, int DP, int DC, bool WIDE>
-__device__ __forceinline__ void paged_attention(const lm_paged_params& P, char* lds, float* ml, int* flag, Shared& S) {
+// ------------------------------------------------------------- few rows --
+
+// Blocks of a sequence's tiles; a tile without keys has one, as it is written too.
+__device__ __forceinline__ int tile_blocks(const Share& a) { return a.kv_len > 128 ? (a.kv_len + 127) >> 7 : 1; }
+
+template <typename T, int DP, int DC>
+__device__ __forceinline__ void paged_stream(const lm_paged_params& P, LDS_ARRAYS, float* ml, Shared& S) {
+  const int kvh = (int)blockIdx.x % P.kv_heads, w = (int)blockIdx.x / P.kv_heads;
+  auto blocks_at = [&](int s) {
+    const Share a = share_of(P, s < P.seqs ? s : P.seqs);
+    return s > P.seqs ? 0 : a.tiles * tile_blocks(a);
+  };
+  // all blocks (under 2^31: the host sees to it), and this workgroup's stretch of them
+  int before = 0, base = 0;
+  int v[1] = {blocks_at((int)threadIdx.x)};
+  scan_all<1>(v, S);
+  int total = S.upto[kThreads - 1][0];
+  if (P.seqs >= kThreads) {
+    for (base = kThreads; base <= P.seqs; base += kThreads) {
+      v[0] = blocks_at(base + (int)threadIdx.x);
+      scan_all<1>(v, S);
+      total += S.upto[kThreads - 1][0];
+    }
+  }
+  const int each = (int)(((int64_t)total + P.target - 1) / P.target);
+  const int64_t begin = (int64_t)w * each;
+  int at = begin < total ? (int)begin : total;
+  const int end = total - at > each ? at + each : total;
+  const int note = w * P.kv_heads + kvh;          // this workgroup's note, and its slot of a tile that it begins
+  const int cont = P.target * P.kv_heads + note;  // of one that it goes on with
+  bool noted = false;
+  if (at < end) {
+    // the sequence in which the stretch begins
+    if (P.seqs >= kThreads) {
+      for (base = 0;; base += kThreads) {
+        v[0] = blocks_at(base + (int)threadIdx.x);
+        scan_all<1>(v, S);
+        if (at - before < S.upto[kThreads - 1][0]) break;
+        before += S.upto[kThreads - 1][0];
+      }
+    }
+    const int lo = find_upto(S, at - before);
+    if (lo > 0) before += S.upto[lo - 1][0];
+    Piece J;
+    J.seq = base + lo;
+    J.a = share_of(P, J.seq);
+    int n = tile_blocks(J.a);
+    J.tile = uniform((at - before) / n);
+    J.t0 = uniform(at - before - J.tile * n);
+    for (;;) {
+      const int left = end - at;
+      const bool ends = n - J.t0 <= left;  // with this tile's last block
+      J.t1 = uniform(ends ? n : J.t0 + left);
+      J.slot = J.t0 > 0 ? cont : ends ? -1 : note;
+      if (J.t0 == 0 && !ends) {
+        noted = true;
+        if (threadIdx.x == 0)
+          write_note(P, note, J.a, J.tile * 32, kvh, 1 + (n - J.t1 + each - 1) / each, note, cont + P.kv_heads,
+                     P.kv_heads);
+      }
+      narrow_tile<T, DP, DC>(J, kvh, a, b, c, d, ml);
+      at += J.t1 - J.t0;
+      if (at >= end) break;
+      J.t0 = 0;
+      if (++J.tile >= J.a.tiles) {
+        J.tile = 0;
+        do {  // there is one: blocks are left
+          J.a = share_of(P, ++J.seq);
+        } while (J.a.tiles == 0);
+        n = tile_blocks(J.a);
+      }
+      __syncthreads();  // the sums have been read
+    }
+  }
+  if (!noted && threadIdx.x == 0) P.notes[note].parts = 0;
+}
+
+// ------------------------------------------------------------ many rows --
+
+// A tile's work: blocks of 32 keys that a wave works on.
+__device__ __forceinline__ int blocks_of(const Share& a) {
+  return a.narrow ? (a.kv_len + 127) >> 7 : ((a.kv_len + 63) >> 6) * 2;
+}
+// Its parts of at most `most` such blocks, and the key blocks of one.
+struct Split {
+  int n, parts, per;
+  __device__ __forceinline__ Split(const Share& a, int most) {
+    per = a.narrow ? most : (most + 1) >> 1;
+    n = a.narrow ? (a.kv_len + 127) >> 7 : (a.kv_len + 63) >> 6;
+    parts = n <= per ? 1 : (n + per - 1) / per;
+  }
+};
+
+template <typename T, int DP, int DC>
+__device__ __forceinline__ void paged_tiles(const lm_paged_params& P, LDS_ARRAYS, float* ml, int* flag, Shared& S) {
   // Workgroups go to the eight XCDs in turn, each with an L2 of its own: where the key heads
   // divide by eight, each XCD takes an eighth of them, so that the tiles of a sequence's rows find
   // a head's keys in one L2.
   int w = (int)blockIdx.x, kvh;
+  const int all = (int)gridDim.x / P.kv_heads;  // workgroups of a head
   if ((P.kv_heads & 7) == 0) {
     const int hx = P.kv_heads >> 3, x = w & 7;
     w >>= 3;
@@ -370,110 +588,137 @@ __device__ __forceinline__ void paged_attention(const lm_paged_params& P, char* 
     kvh = w - p * P.kv_heads;
     w = p;
   }
-  const int group = P.heads / P.kv_heads;
   if (threadIdx.x == 0) *flag = 0;
-  Job J;
-  if (!find_job(P, w, group, S, J)) return;
-  if (!WIDE || J.a.narrow)
-    paged_rows<T, DP, DC, 4>(P, J, kvh, group, lds, ml, flag);
+  // the most blocks of a part: an equal share for `target` workgroups (a float's rounding moves
+  // it by a part in 2^24; every workgroup finds the same)
+  float work = 0.f;
+  for (int s = threadIdx.x; s < P.seqs; s += kThreads) {
+    const Share a = share_of(P, s);
+    work += (float)a.tiles * (float)blocks_of(a);
+  }
+  work = sum_all(work, S) * (float)P.kv_heads / (float)P.target;
+  const int most = uniform(work < 1.f ? 1 : work > 6e7f ? 1 << 26 : (int)__builtin_ceilf(work));
+  // the sequence of part w, all sequences' parts one after another, and the slots in front of its
+  int parts = 0, slots = 0, base = 0;
+  bool found = false;
+  for (; base <= P.seqs; base += kThreads) {
+    const int s = base + (int)threadIdx.x;
+    const Share a = share_of(P, s < P.seqs ? s : P.seqs);
+    const Split sp(a, most);
+    int v[2];
+    v[0] = s <= P.seqs ? a.tiles * sp.parts : 0;
+    v[1] = sp.parts > 1 ? v[0] : 0;
+    scan_all<2>(v, S);
+    const int n = S.upto[kThreads - 1][0];
+    found = w - parts < n;
+    if (found) break;
+    parts += n;
+    slots += S.upto[kThreads - 1][1];
+  }
+  if (!found) {
+    // no part is left: the workgroups behind them clear the notes of the slots that none has
+    for (int64_t i = slots + (w - parts) + (int64_t)threadIdx.x * (all - parts); i < P.slots;
+         i += (int64_t)kThreads * (all - parts))
+      P.notes[i * P.kv_heads + kvh].parts = 0;
+    return;
+  }
+  const int lo = find_upto(S, w - parts);
+  Piece J;
+  J.seq = base + lo;
+  J.a = share_of(P, J.seq);
+  const Split sp(J.a, most);
+  const int i = uniform(w - parts - (lo > 0 ? S.upto[lo - 1][0] : 0));
+  const int rank = i / sp.parts, part = i - rank * sp.parts;
+  J.tile = uniform(J.a.tiles - 1 - rank);  // the longest first
+  J.t0 = uniform(part * sp.per);
+  J.t1 = uniform(J.t0 + sp.per < sp.n ? J.t0 + sp.per : sp.n);
+  J.slot = -1;
+  if (sp.parts > 1) {
+    const int first = uniform(slots + (lo > 0 ? S.upto[lo - 1][1] : 0) + rank * sp.parts);
+    if (first + sp.parts > P.slots) return;  // starts that do not rise
+    J.slot = (first + part) * P.kv_heads + kvh;
+    if (threadIdx.x == 0)
+      write_note(P, J.slot, J.a, J.tile * (J.a.narrow ? 32 : 128), kvh, part == 0 ? sp.parts : 0, J.slot,
+                 J.slot + P.kv_heads, P.kv_heads);
+  }
+  if (J.a.narrow)
+    narrow_tile<T, DP, DC>(J, kvh, a, b, c, d, ml);
   else
-    paged_rows<T, DP, DC, 1>(P, J, kvh, group, lds, ml, flag);
+    wide_tile<T, DP, DC>(J, kvh, a, b, c, d, flag);
 }
 
 // -------------------------------------------------------------------- join --
 
-// Joins the parts of the split tiles: eight lane groups of 32 (four columns a lane)
-// take a row's parts in turn, or, where a row has fewer than eight, several
-// rows.  A workgroup walks over the rows of the split sequences.
+// Joins the parts of a tile that workgroups shared (blockIdx.x: its note).  Eight lane groups
+// of 32, four columns a lane, take a row's parts in turn, or, where it has
+// fewer than eight, several rows.  A row's maxima and sums are requested together with its
+// first parts, so that up to 64 parts are one round trip.
 template <typename T>
-__device__ __forceinline__ void paged_join(const lm_paged_params& P, Shared& S, f32x4* red) {
-  const int group = P.heads / P.kv_heads;
-  const int most = most_blocks(P, group, S);
-  const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
-  const int d = 4 * lane;
-  int items = 0, slots = 0;  // before this stretch of sequences
-  auto side_by_side = [](int splits) { return splits <= 2 ? 2 : splits <= 4 ? 4 : 8; };  // parts at a time
-  for (int base = 0; base < P.seqs; base += kThreads) {
-    const int s = base + (int)threadIdx.x;
-    int mine = 0, held = 0;
-    if (s < P.seqs) {
-      Share a = share_of(P, s, group);
-      split(a, most);
-      if (a.splits > 1) {
-        const int each = 8 / side_by_side(a.splits);  // rows at a time
-        mine = (a.rows + each - 1) / each * P.kv_heads;
-        held = a.tiles * a.splits;
-      }
+__device__ __forceinline__ void paged_join(const lm_paged_params& P, f32x4* red) {
+  const lm_paged_note N = P.notes[blockIdx.x];
+  if (N.parts < 2) return;
+  // starts that do not rise can leave a note unwritten: what leads out of the call is none
+  const int64_t slots = (int64_t)P.slots * P.kv_heads;
+  if (N.first < 0 || N.first >= slots || N.next < 0 || N.step < 0 || N.next + (N.parts - 2) * (int64_t)N.step >= slots ||
+      N.token < 0 || N.row0 < 0 || N.head < 0 || N.head >= P.kv_heads ||
+      (int64_t)N.token * P.group + N.rows > (int64_t)P.tokens * P.group)
+    return;
+  const int lane = threadIdx.x & 31, g = threadIdx.x >> 5, d = 4 * lane;
+  const int pp = N.parts <= 2 ? 2 : N.parts <= 4 ? 4 : 8, each = 8 / pp;  // parts and rows side by side
+  const int phase = g % pp;
+  const int left = N.rows - N.row0, rows = left < P.part_rows ? left : P.part_rows;
+  auto line = [&](int p, int r) {
+    return (int64_t)(p == 0 ? N.first : N.next + (int64_t)(p - 1) * N.step) * P.part_rows + r;
+  };
+  constexpr int U = 8;
+  for (int r0 = (int)blockIdx.y * each; r0 < rows; r0 += (int)gridDim.y * each) {
+    const int r = r0 + g / pp;
+    const bool live = r < rows;
+    const int rr = live ? r : r0;
+    f32x4 v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int p = phase + pp * u < N.parts ? phase + pp * u : phase < N.parts ? phase : 0;
+      v[u] = *reinterpret_cast<const f32x4*>(P.part + line(p, rr) * P.dim + (d < P.dim ? d : 0));
     }
-    scan_all(mine, held, S);
-    const int total = S.upto[kThreads - 1][0];
-    // this workgroup's items of the stretch: those of all, counted from the first stretch on, that fall to it
-    int i = ((int)blockIdx.x - items % (int)gridDim.x + (int)gridDim.x) % (int)gridDim.x;
-    for (; i < total; i += gridDim.x) {
-      int lo = 0;
+    // the common maximum and the sum: 32 lanes over the parts
+    float m = kNegInf, l = 0.f;
+    for (int p = lane; p < N.parts; p += 32) m = fmaxf(m, P.part_ml[line(p, rr) * 2]);
 #pragma unroll
-      for (int step = kThreads / 2; step > 0; step >>= 1)
-        if (S.upto[lo + step - 1][0] <= i) lo += step;
-      Share a = share_of(P, base + lo, group);
-      split(a, most);
-      const int j = i - (lo > 0 ? S.upto[lo - 1][0] : 0);
-      const int first = slots + (lo > 0 ? S.upto[lo - 1][1] : 0);
-      const int pp = side_by_side(a.splits), each = 8 / pp;
-      const int kvh = j % P.kv_heads;
-      const int row = j / P.kv_heads * each + g / pp, phase = g % pp;
-      const int size = a.narrow ? 32 : 128, tile = row / size;
-      const int slot = first + (a.tiles - 1 - tile) * a.splits;
-      const bool live = row < a.rows && slot + a.splits <= P.slots;
-      const int64_t step = (int64_t)P.kv_heads * P.part_rows;
-      const int64_t at = live ? ((int64_t)slot * P.kv_heads + kvh) * P.part_rows + (row - tile * size) : 0;
-      // the common maximum and the sum: 32 lanes over the parts
-      float m = kNegInf, l = 0.f;
-      if (live) {
-        for (int p = lane; p < a.splits; p += 32) m = fmaxf(m, P.part_ml[(at + p * step) * 2]);
-      }
-#pragma unroll
-      for (int x = 1; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
-      if (live) {
-        for (int p = lane; p < a.splits; p += 32) {
-          const float pm = P.part_ml[(at + p * step) * 2], pl = P.part_ml[(at + p * step) * 2 + 1];
-          l += pm == kNegInf ? pl : pl * exp2_fast(pm - m);  // no keys: zero, or the NaN of a bad page
-        }
-      }
-#pragma unroll
-      for (int x = 1; x < 32; x <<= 1) l += __shfl_xor(l, x);
-      f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-      if (live && d < P.dim) {
-#pragma unroll 4
-        for (int p = phase; p < a.splits; p += pp) {
-          const float pm = P.part_ml[(at + p * step) * 2], pl = P.part_ml[(at + p * step) * 2 + 1];
-          const f32x4 v = *reinterpret_cast<const f32x4*>(P.part + (at + p * step) * P.dim + d);
-          const float w = exp2_fast(pm - m);
-          if (pl != 0.f && pm != kNegInf) {  // a part without keys has written none
-#pragma unroll
-            for (int c = 0; c < 4; ++c) sum[c] = __builtin_fmaf(v[c], w, sum[c]);
-          }
-        }
-      }
-      red[threadIdx.x] = sum;
-      __syncthreads();
-      if (phase == 0 && live && d < P.dim) {
-        for (int p = 1; p < pp; ++p) {
-          const f32x4 o = red[threadIdx.x + 32 * p];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) sum[c] += o[c];
-        }
-        const int query = row / group, head = kvh * group + (row - query * group);
-        const int64_t token = a.first + query;
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        store4<T>((char*)P.o + (token * P.o_t + (int64_t)head * P.o_h + d) * T::kBytes, sum[0] * inv, sum[1] * inv,
-                  sum[2] * inv, sum[3] * inv);
-        if (P.lse != nullptr && d == 0)
-          P.lse[token * P.heads + head] = l == 0.f ? kNegInf : (m + __builtin_amdgcn_logf(l)) * kLn2;
-      }
-      __syncthreads();
+    for (int x = 1; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
+    auto weight = [&](float pm) { return pm == kNegInf ? 0.f : exp2_fast(pm - m); };
+    for (int p = lane; p < N.parts; p += 32) {
+      const int64_t at = line(p, rr) * 2;
+      l = __builtin_fmaf(P.part_ml[at + 1], weight(P.part_ml[at]), l);  // a NaN stays one
     }
-    items += total;
-    slots += S.upto[kThreads - 1][1];
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) l += __shfl_xor(l, x);
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    auto take = [&](int p, const f32x4& x) {
+      const float w = weight(P.part_ml[line(p, rr) * 2]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) sum[c] = __builtin_fmaf(x[c], w, sum[c]);
+    };
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (phase + pp * u < N.parts) take(phase + pp * u, v[u]);
+    for (int p = phase + pp * U; p < N.parts; p += pp)
+      take(p, *reinterpret_cast<const f32x4*>(P.part + line(p, rr) * P.dim + (d < P.dim ? d : 0)));
+    red[threadIdx.x] = sum;
+    __syncthreads();
+    if (phase == 0 && live && d < P.dim) {
+      for (int p = 1; p < pp; ++p) {
+        const f32x4 o = red[threadIdx.x + 32 * p];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) sum[c] += o[c];
+      }
+      const int row = N.row0 + r, query = query_of(P, row), head = N.head * P.group + (row - query * P.group);
+      const int64_t token = N.token + query;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      store4<T>((char*)P.o + (token * P.o_t + (int64_t)head * P.o_h + d) * T::kBytes, sum[0] * inv, sum[1] * inv,
+                sum[2] * inv, sum[3] * inv);
+      if (P.lse != nullptr && d == 0) P.lse[token * P.heads + head] = lse_of(m, l);
+    }
     __syncthreads();
   }
 }
@@ -481,24 +726,30 @@ __device__ __forceinline__ void paged_join(const lm_paged_params& P, Shared& S, 
 }  // namespace
 
 // DP: elements of a tile's row in LDS; DC: columns worked on, the head size rounded up to 32.
-#define LM_PAGED_KERNEL(NAME, T, DP, DC, WIDE, WPE)                                                              \
+#define LM_PAGED_LDS(T, DP)                                                                                      \
+  __shared__ __align__(16) char a[kLdsBytes<T, DP>];                                                           \
+  __shared__ __align__(16) char b[kLdsBytes<T, DP>];                                                           \
+  __shared__ __align__(16) char c[kLdsBytes<T, DP>];                                                           \
+  __shared__ __align__(16) char d[kLdsBytes<T, DP>];                                                           \
+  __shared__ float ml[512];                                                                                      \
+  __shared__ Shared S;
+#define LM_PAGED(NAME, T, DP, DC, WPE)                                                                           \
   extern "C" __global__ void __launch_bounds__(LM_PAGED_THREADS) __attribute__((amdgpu_waves_per_eu(WPE)))      \
-      attnres_paged_attention_##NAME(lm_paged_params P) {                                                        \
-    __shared__ __align__(16) char lds[2 * Tile<T, DP, 128>::kBytes];                                             \
-    __shared__ float ml[128];                                                                                    \
+      attnres_paged_stream_##NAME##_d##DC(lm_paged_params P) {                                                   \
+    LM_PAGED_LDS(T, DP)                                                                                          \
+    paged_stream<T, DP, DC>(P, (LM_LDS char*)a, (LM_LDS char*)b, (LM_LDS char*)c, (LM_LDS char*)d, ml, S);       \
+  }                                                                                                              \
+  extern "C" __global__ void __launch_bounds__(LM_PAGED_THREADS) __attribute__((amdgpu_waves_per_eu(WPE)))      \
+      attnres_paged_tiles_##NAME##_d##DC(lm_paged_params P) {                                                    \
+    LM_PAGED_LDS(T, DP)                                                                                          \
     __shared__ int flag;                                                                                         \
-    __shared__ Shared S;                                                                                         \
-    paged_attention<T, DP, DC, WIDE>(P, lds, ml, &flag, S);                                                      \
+    paged_tiles<T, DP, DC>(P, (LM_LDS char*)a, (LM_LDS char*)b, (LM_LDS char*)c, (LM_LDS char*)d, ml, &flag, S); \
   }
 #define LM_PAGED_JOIN(NAME, T)                                                                                   \
   extern "C" __global__ void __launch_bounds__(LM_PAGED_THREADS) attnres_paged_join_##NAME(lm_paged_params P) {  \
-    __shared__ Shared S;                                                                                         \
     __shared__ f32x4 red[LM_PAGED_THREADS];                                                                      \
-    paged_join<T>(P, S, red);                                                                                    \
+    paged_join<T>(P, red);                                                                                       \
   }
-#define LM_PAGED(NAME, T, DP, DC, WPE)                     \
-  LM_PAGED_KERNEL(NAME##_d##DC##_n, T, DP, DC, false, WPE) \
-  LM_PAGED_KERNEL(NAME##_d##DC##_w, T, DP, DC, true, WPE)
 
 #if LM_PART == 15
 LM_PAGED_JOIN(bf16, Bf16)
@@ -506,6 +757,8 @@ LM_PAGED(bf16, Bf16, 64, 32, 2)
 LM_PAGED(bf16, Bf16, 64, 64, 2)
 LM_PAGED(bf16, Bf16, 128, 96, 2)
 LM_PAGED(bf16, Bf16, 128, 128, 2)
+#endif
+#if LM_PART == 16
 LM_PAGED_JOIN(f32, F32)
 LM_PAGED(f32, F32, 64, 32, 1)
 LM_PAGED(f32, F32, 64, 64, 1)

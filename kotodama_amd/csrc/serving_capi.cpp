@@ -17,9 +17,9 @@
 namespace {
 
 // Code-object parts and kernel slots.
-constexpr int kPagedPart = 15, kServingPart = 16;
+constexpr int kPagedBf16Part = 15, kPagedF32Part = 16, kServingPart = 17;
 enum Slot {
-  kPagedAttn = kServingSlots,   // + 8 * (fp32) + 2 * ((head_dim - 1) / 32) + (wide)
+  kPagedAttn = kServingSlots,   // + 8 * (fp32) + 4 * (many rows) + (head_dim - 1) / 32
   kPagedJoin = kPagedAttn + 16, // + (fp32)
   kPagedSlots = kPagedJoin + 2,
   kPagedRelease,
@@ -34,8 +34,8 @@ constexpr int64_t kMaxTokens = (int64_t)1 << 30;  // of one sequence, and new on
 constexpr int kMaxPage = 1 << 16;                 // rows
 constexpr int kMaxGroup = 4096;                   // query heads per key head
 constexpr int kMaxSeqs = 1 << 20;
-constexpr int kSplitPerCu = 2;  // workgroups per CU to split the key axis for
-constexpr int kWideWaves = 8;   // waves of 32 rows per CU that need no split: the rows of chunks are taken 128 at a time
+constexpr int kSplitPerCu = 2;  // workgroups per CU to deal the key blocks out to
+constexpr int kWideWaves = 8;   // waves of 32 rows per CU that fill the card: chunks' rows are taken 128 at a time
 constexpr int kMaxVocab = LM_VERIFY_PIECE * LM_VERIFY_MAX_PIECES;
 
 int index_size(int code) { return code == ATTNRES_INDEX_I64 ? 8 : 4; }
@@ -70,8 +70,9 @@ int take_cache(const char* what, const void* p, const int64_t* st, int64_t pages
   if (!aligned(p, 16) || out->b % m || out->h % m || out->t % m)
     return fail(ATTNRES_ERR_ALIGN, "%s: pointer and strides must be multiples of 16 bytes", what);
   if (out->b < 0 || out->h < 0 || out->t < 0) return fail(ATTNRES_ERR_ARG, "%s: a stride is negative", what);
-  if (out->t > INT32_MAX / es / page_size)
-    return fail(ATTNRES_ERR_UNSUPPORTED, "%s: a head's rows of a page span 2^31 bytes", what);
+  if (out->t > INT32_MAX / es / page_size || out->b > INT32_MAX / es)
+    return fail(ATTNRES_ERR_UNSUPPORTED, "%s: a head's rows of a page span 2^31 bytes, or its pages lie so far apart",
+                what);
   return ATTNRES_OK;
 }
 
@@ -101,9 +102,10 @@ int check_rows(const char* op, int64_t tokens, int kv_heads, int head_dim, int d
 
 // What the launches and the workspace of a call go by.
 struct PagedPlan {
-  int wide = 0, target = 0, least = 1, slots = 0, part_rows = 0;
-  int64_t grid = 0;  // workgroups per key head
-  int64_t ml = 0, bytes = 0;
+  bool wide = false, split = false;
+  int target = 0, part_rows = 0;
+  int64_t slots = 0, grid = 0, notes = 0;  // of all key heads
+  int64_t at_ml = 0, at_notes = 0, bytes = 0;
 };
 
 int paged_plan(int64_t tokens, int seqs, int heads, int kv_heads, int head_dim, int64_t capacity, PagedPlan* p) {
@@ -112,19 +114,29 @@ int paged_plan(int64_t tokens, int seqs, int heads, int kv_heads, int head_dim, 
   if (rc != ATTNRES_OK) return rc;
   const int64_t rows = tokens * (heads / kv_heads);
   p->wide = rows / 32 * kv_heads >= (int64_t)cus * kWideWaves;
-  p->target = cus * kSplitPerCu;
-  // tiles: every sequence may end inside one; the rows behind the last sequence are one more
-  const int64_t tiles = rows / (p->wide ? 128 : 32) + seqs + 1;
-  const int64_t most = p->wide ? (capacity + 31) / 32 + 1 : (capacity + 127) / 128;  // blocks of a tile
-  const bool split = most > p->least;
-  const int64_t share = (p->target + kv_heads - 1) / kv_heads;
-  // a split tile's parts are under twice its blocks over the share of one; their sum is under twice the target
-  p->slots = split ? (int)(2 * share + 8) : 0;
-  p->part_rows = p->wide ? 128 : rows < 32 ? (int)rows : 32;
-  p->grid = tiles + (split ? share + 8 : 0);
-  const int64_t lines = (int64_t)p->slots * kv_heads * p->part_rows;
-  p->ml = lines * head_dim * 4;
-  p->bytes = p->ml + lines * 8;
+  p->split = capacity > 128;  // tiles of one block of keys are whole
+  if (p->wide) {
+    p->target = cus * kSplitPerCu;
+    // tiles: every sequence may end inside one; the rows behind the last sequence are one more
+    const int64_t tiles = rows / 128 + seqs + 1, share = (p->target + kv_heads - 1) / kv_heads;
+    // a split tile's parts are under twice its blocks over a part's most, and all those blocks at most the target's share
+    p->slots = p->split ? (2 * share + 8) * kv_heads : 0;
+    p->grid = (tiles + (p->split ? share + 8 : 0)) * kv_heads;
+    p->notes = p->slots;
+    p->part_rows = 128;
+  } else {
+    if ((rows / 32 + seqs + 1) * ((capacity + 127) / 128) > INT32_MAX)
+      return fail(ATTNRES_ERR_UNSUPPORTED, "paged_attention: too many keys for one call");
+    p->target = cus * kSplitPerCu / kv_heads > 0 ? cus * kSplitPerCu / kv_heads : 1;
+    p->grid = (int64_t)p->target * kv_heads;
+    p->slots = p->split ? 2 * p->grid : 0;  // each workgroup goes on with a tile and begins one
+    p->notes = p->grid;
+    p->part_rows = rows < 32 ? (int)rows : 32;
+  }
+  const int64_t lines = p->slots * p->part_rows;
+  p->at_ml = lines * head_dim * 4;
+  p->at_notes = p->at_ml + (lines * 8 + 15) / 16 * 16;
+  p->bytes = p->at_notes + p->notes * (int64_t)sizeof(lm_paged_note);
   return ATTNRES_OK;
 }
 
@@ -324,7 +336,8 @@ int attnres_paged_attention_fwd(const void* q, const int64_t* q_strides, const v
   P.o = out;
   P.lse = lse;
   P.part = static_cast<float*>(workspace);
-  P.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan.ml);
+  P.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan.at_ml);
+  P.notes = reinterpret_cast<lm_paged_note*>(static_cast<char*>(workspace) + plan.at_notes);
   P.table = static_cast<const int32_t*>(block_table);
   P.table_ld = table_ld;
   P.kv_lens = kv_lens;
@@ -338,27 +351,26 @@ int attnres_paged_attention_fwd(const void* q, const int64_t* q_strides, const v
   P.pages = (int32_t)pages;
   P.capacity = (int32_t)capacity;
   P.dim = head_dim;
+  P.group = heads / kv_heads;
+  while ((1 << P.group_shift) < P.group) ++P.group_shift;
+  P.group_mul =
+      (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << P.group_shift) - (uint64_t)P.group)) / (uint64_t)P.group + 1);
   P.wide = plan.wide;
   P.target = plan.target;
-  P.least = plan.least;
-  P.slots = plan.slots;
+  P.slots = (int32_t)(plan.slots / kv_heads);
   P.part_rows = plan.part_rows;
   P.scale_log2 = scale * 1.44269504088896340736f;
-  const int64_t grid = plan.grid * kv_heads;
-  if (grid > INT32_MAX - 8) return fail(ATTNRES_ERR_UNSUPPORTED, "paged_attention: too many rows for one call");
+  if (plan.grid > INT32_MAX) return fail(ATTNRES_ERR_UNSUPPORTED, "paged_attention: too many rows for one call");
   const bool f32 = dtype == ATTNRES_DTYPE_F32;
-  const int blocks = (head_dim - 1) / 32;
+  const int blocks = (head_dim - 1) / 32, part = f32 ? kPagedF32Part : kPagedBf16Part;
   char name[64];
-  snprintf(name, sizeof(name), "attnres_paged_attention_%s_d%d_%s", f32 ? "f32" : "bf16", 32 * (blocks + 1),
-           plan.wide ? "w" : "n");
-  rc = launch(kPagedAttn + (f32 ? 8 : 0) + 2 * blocks + plan.wide, kPagedPart, name, (unsigned)grid, 1,
+  snprintf(name, sizeof(name), "attnres_paged_%s_%s_d%d", plan.wide ? "tiles" : "stream", f32 ? "f32" : "bf16",
+           32 * (blocks + 1));
+  rc = launch(kPagedAttn + (f32 ? 8 : 0) + (plan.wide ? 4 : 0) + blocks, part, name, (unsigned)plan.grid, 1,
               LM_PAGED_THREADS, 0, P, stream);
-  if (rc != ATTNRES_OK || plan.slots == 0) return rc;
-  const int64_t lines = tokens * heads;
-  int cus = 0;
-  if ((rc = attnres_internal_num_cus(&cus)) != ATTNRES_OK) return rc;
-  return launch(kPagedJoin + (f32 ? 1 : 0), kPagedPart, f32 ? "attnres_paged_join_f32" : "attnres_paged_join_bf16",
-                (unsigned)(lines < 8 * cus ? lines : 8 * cus), 1, LM_PAGED_THREADS, 0, P, stream);
+  if (rc != ATTNRES_OK || !plan.split) return rc;
+  return launch(kPagedJoin + (f32 ? 1 : 0), part, f32 ? "attnres_paged_join_f32" : "attnres_paged_join_bf16",
+                (unsigned)plan.notes, plan.part_rows < 8 ? plan.part_rows : 8, LM_PAGED_THREADS, 0, P, stream);
 }
 
 int attnres_verify_drafts_workspace_size(int64_t rows, int vocab, int64_t* bytes) {

@@ -259,8 +259,8 @@ def _check_cache_memory(op: str, k_cache: Tensor, v_cache: Tensor) -> None:
     for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
         if t.numel() and not _aligned(t):
             raise ValueError(f"{op}: {name} must lie in 16-byte pieces, got strides {t.stride()}")
-        if t.numel() and t.stride(2) * t.shape[2] * t.element_size() >= 1 << 31:
-            raise ValueError(f"{op}: {name}: a head's rows of a page span 2^31 bytes")
+        if t.numel() and max(t.stride(2) * t.shape[2], t.stride(0)) * t.element_size() >= 1 << 31:
+            raise ValueError(f"{op}: {name}: a head's rows of a page span 2^31 bytes, or its pages lie so far apart")
 
 
 def _check_write(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, slots: Tensor) -> None:
