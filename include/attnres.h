@@ -667,7 +667,7 @@ int attnres_paged_attention_fwd(const void* q, const int64_t* q_strides, const v
  * Tokens are those of the definition: sums are taken in 64 bits where they decide.
  * vocab up to 2^21.  workspace: device memory of attnres_verify_drafts_workspace_size bytes.
  */
-int attnres_verify_drafts_workspace_size(int64_t rows, int vocab, int64_t* bytes);
+int attnres_verify_drafts_workspace_size(int64_t rows, int seqs, int vocab, int64_t* bytes);
 int attnres_verify_drafts(const void* logits, int64_t logits_ld, int logits_dtype, const void* draft_probs,
                           int64_t draft_ld, int draft_dtype, int64_t rows, int vocab, const void* ids, int ids_dtype,
                           const void* q_starts, int starts_dtype, int seqs, const float* uniforms, float temperature,

@@ -726,6 +726,7 @@ _SIGNATURES = {
     "attnres_verify_drafts_workspace_size": (
         [
             _c_i64,  # rows
+            _c_int,  # seqs
             _c_int,  # vocab
             ctypes.POINTER(_c_i64),  # bytes
         ],
@@ -961,11 +962,11 @@ def paged_attention_fwd(*args) -> None:
     check("attnres_paged_attention_fwd", lib().attnres_paged_attention_fwd(*args))
 
 
-def verify_drafts_workspace_size(rows: int, vocab: int) -> int:
+def verify_drafts_workspace_size(rows: int, seqs: int, vocab: int) -> int:
     """Bytes of workspace :func:`verify_drafts` needs."""
     out = _c_i64(0)
     check("attnres_verify_drafts_workspace_size",
-          lib().attnres_verify_drafts_workspace_size(rows, vocab, ctypes.byref(out)))
+          lib().attnres_verify_drafts_workspace_size(rows, seqs, vocab, ctypes.byref(out)))
     return out.value
 
 

@@ -230,9 +230,15 @@ typedef struct lm_write_params {
  * Drafted tokens against the target's logits.  Sequence s has the rows q_starts[s] ..
  * q_starts[s + 1] - 1; row r's draft is ids[r + 1].
  */
-#define LM_VERIFY_SLICE 4096      /* logits of a workgroup of the first pass */
-#define LM_VERIFY_PIECE 512       /* logits of a wave's step in the second */
-#define LM_VERIFY_MAX_PIECES 4096
+#define LM_VERIFY_PART 2048  /* logits of a wave of the first launch, */
+#define LM_VERIFY_SLICE 4096 /* of a workgroup of the second, */
+#define LM_VERIFY_PIECE 512  /* and of a wave's step there */
+/* What a sequence's token is taken from: the row behind the drafts that stay, its largest logit and its sum. */
+typedef struct lm_verify_choice {
+  double sum;
+  float top;
+  int32_t accepted;
+} lm_verify_choice;
 typedef struct lm_verify_params {
   const void* logits;       /* (rows, vocab), rows logits_ld apart */
   const void* draft;        /* (rows, vocab) probabilities or NULL */
@@ -241,21 +247,23 @@ typedef struct lm_verify_params {
   const float* uniforms;    /* (rows, 2) */
   void* tokens;             /* (rows,) as ids */
   int32_t* counts;          /* (seqs,) */
-  double* part_sum;         /* (rows, slices) sums of exp((x - top) / temperature) */
-  float* part_top;          /* (rows, slices) */
-  int32_t* part_at;         /* (rows, slices) where it is first */
+  double* part_sum;         /* (rows, parts) sums of exp((x - top) / temperature) */
+  float* part_top;          /* (rows, parts) */
+  int32_t* part_at;         /* (rows, parts) where it is first, greedily */
+  double* piece_sum;        /* (seqs, slices, pieces, 2): of the weights, and of the exponentials */
+  lm_verify_choice* chosen; /* (seqs,) */
   int64_t logits_ld, draft_ld;
   int32_t rows;
   int32_t seqs;
   int32_t vocab;
-  int32_t slices;
+  int32_t parts;            /* of a row, a wave each */
+  int32_t slices;           /* of a row, a workgroup each */
   int32_t logits_f32, draft_f32;
   int32_t logits_vec, draft_vec; /* rows load in 16-byte pieces */
   int32_t ids64;
   int32_t starts64;
   int32_t greedy;
-  float inv_temp;
-  double inv_temp64;
+  double scale_log2;        /* log2(e) / temperature */
 } lm_verify_params;
 
 #endif /* KOTODAMA_AMD_LM_PARAMS_H */

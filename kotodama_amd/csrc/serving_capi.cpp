@@ -25,6 +25,7 @@ enum Slot {
   kPagedRelease,
   kPagedWrite,
   kVerifyRows,
+  kVerifyPieces,
   kVerifyPick,
   kEnd
 };
@@ -36,7 +37,7 @@ constexpr int kMaxGroup = 4096;                   // query heads per key head
 constexpr int kMaxSeqs = 1 << 20;
 constexpr int kSplitPerCu = 2;  // workgroups per CU to deal the key blocks out to
 constexpr int kWideWaves = 8;   // waves of 32 rows per CU that fill the card: chunks' rows are taken 128 at a time
-constexpr int kMaxVocab = LM_VERIFY_PIECE * LM_VERIFY_MAX_PIECES;
+constexpr int kMaxVocab = 1 << 21;
 
 int index_size(int code) { return code == ATTNRES_INDEX_I64 ? 8 : 4; }
 
@@ -190,6 +191,25 @@ int fill_slots(const char* op, lm_slots_params* P, void* table, int64_t table_ld
   P->free_len = free_len;
   P->page_limit = ((int64_t)1 << 31) >> P->shift;
   return ATTNRES_OK;
+}
+
+// ---------------------------------------------------------------- verify --
+
+struct VerifyPlan {
+  int64_t parts, slices, at_pieces, at_chosen, at_top, at_at, bytes;
+};
+
+VerifyPlan verify_plan(int64_t rows, int64_t seqs, int vocab) {
+  VerifyPlan p;
+  p.parts = (vocab + LM_VERIFY_PART - 1) / LM_VERIFY_PART;
+  p.slices = (vocab + LM_VERIFY_SLICE - 1) / LM_VERIFY_SLICE;
+  const int64_t n = rows * p.parts;
+  p.at_pieces = n * 8;
+  p.at_chosen = p.at_pieces + seqs * p.slices * (LM_VERIFY_SLICE / LM_VERIFY_PIECE) * 16;
+  p.at_top = p.at_chosen + seqs * (int64_t)sizeof(lm_verify_choice);
+  p.at_at = p.at_top + n * 4;
+  p.bytes = p.at_at + n * 4;
+  return p;
 }
 
 // Workgroups for so many tokens or pages: every one scans all lengths, so few.
@@ -373,11 +393,12 @@ int attnres_paged_attention_fwd(const void* q, const int64_t* q_strides, const v
                 (unsigned)plan.notes, plan.part_rows < 8 ? plan.part_rows : 8, LM_PAGED_THREADS, 0, P, stream);
 }
 
-int attnres_verify_drafts_workspace_size(int64_t rows, int vocab, int64_t* bytes) {
-  if (bytes == nullptr || rows < 0 || vocab < 1) return fail(ATTNRES_ERR_ARG, "verify_drafts: bad sizes or bytes");
-  if (vocab > kMaxVocab || rows > (1 << 24))
-    return fail(ATTNRES_ERR_UNSUPPORTED, "verify_drafts: a vocabulary over 2^21, or over 2^24 rows");
-  *bytes = rows * ((vocab + LM_VERIFY_SLICE - 1) / LM_VERIFY_SLICE) * 16;
+int attnres_verify_drafts_workspace_size(int64_t rows, int seqs, int vocab, int64_t* bytes) {
+  if (bytes == nullptr || rows < 0 || vocab < 1 || seqs < 0)
+    return fail(ATTNRES_ERR_ARG, "verify_drafts: bad sizes or bytes");
+  if (vocab > kMaxVocab || rows > (1 << 24) || seqs > kMaxSeqs)
+    return fail(ATTNRES_ERR_UNSUPPORTED, "verify_drafts: a vocabulary over 2^21, over 2^24 rows or 2^20 sequences");
+  *bytes = verify_plan(rows, seqs, vocab).bytes;
   return ATTNRES_OK;
 }
 
@@ -386,12 +407,10 @@ int attnres_verify_drafts(const void* logits, int64_t logits_ld, int logits_dtyp
                           const void* q_starts, int starts_dtype, int seqs, const float* uniforms, float temperature,
                           void* tokens, void* counts, void* workspace, int64_t workspace_bytes, void* stream) {
   int64_t need = 0;
-  int rc = attnres_verify_drafts_workspace_size(rows, vocab, &need);
+  int rc = attnres_verify_drafts_workspace_size(rows, seqs, vocab, &need);
   if (rc != ATTNRES_OK) return rc;
   if (!valid_dtype(logits_dtype) || (draft_probs != nullptr && !valid_dtype(draft_dtype)))
     return fail(ATTNRES_ERR_ARG, "verify_drafts: bad dtype");
-  if (seqs < 0) return fail(ATTNRES_ERR_ARG, "verify_drafts: bad seqs");
-  if (seqs > kMaxSeqs) return fail(ATTNRES_ERR_UNSUPPORTED, "verify_drafts: over 2^20 sequences");
   if (!(temperature >= 0) || !std::isfinite(temperature) || (temperature > 0 && temperature < 1e-6f))
     return fail(ATTNRES_ERR_ARG, "verify_drafts: temperature is not 0 or from 1e-6 up");
   if ((rc = check_index("verify_drafts: ids", ids, ids_dtype, rows > 0)) != ATTNRES_OK ||
@@ -430,21 +449,31 @@ int attnres_verify_drafts(const void* logits, int64_t logits_ld, int logits_dtyp
   P.rows = (int32_t)rows;
   P.seqs = seqs;
   P.vocab = vocab;
-  P.slices = (vocab + LM_VERIFY_SLICE - 1) / LM_VERIFY_SLICE;
+  const VerifyPlan plan = verify_plan(rows, seqs, vocab);
+  P.parts = (int32_t)plan.parts;
+  P.slices = (int32_t)plan.slices;
   P.greedy = temperature == 0;
-  P.inv_temp64 = temperature == 0 ? 1.0 : 1.0 / (double)temperature;
-  P.inv_temp = (float)P.inv_temp64;
+  P.scale_log2 = temperature == 0 ? 1.0 : 1.44269504088896340736 / (double)temperature;
   char* ws = static_cast<char*>(workspace);
-  const int64_t n = rows * P.slices;
   P.part_sum = reinterpret_cast<double*>(ws);
-  P.part_top = reinterpret_cast<float*>(ws + n * 8);
-  P.part_at = reinterpret_cast<int32_t*>(ws + n * 12);
+  P.piece_sum = reinterpret_cast<double*>(ws + plan.at_pieces);
+  P.part_top = reinterpret_cast<float*>(ws + plan.at_top);
+  P.part_at = reinterpret_cast<int32_t*>(ws + plan.at_at);
+  P.chosen = reinterpret_cast<lm_verify_choice*>(ws + plan.at_chosen);
+  if (rows * plan.parts > INT32_MAX - 4 || seqs * plan.slices > INT32_MAX)
+    return fail(ATTNRES_ERR_UNSUPPORTED, "verify_drafts: too many rows for one call");
   if (rows > 0) {
-    if (n > INT32_MAX) return fail(ATTNRES_ERR_UNSUPPORTED, "verify_drafts: too many rows for one call");
-    rc = launch(kVerifyRows, kServingPart, "attnres_verify_rows", (unsigned)n, 1, 256, 0, P, stream);
+    rc = launch(kVerifyRows, kServingPart, "attnres_verify_rows", (unsigned)((rows * plan.parts + 3) / 4), 1, 256, 0, P,
+                stream);
     if (rc != ATTNRES_OK) return rc;
   }
-  return launch(kVerifyPick, kServingPart, "attnres_verify_pick", (unsigned)seqs + 1, 1, 1024, 0, P, stream);
+  if (seqs == 0) return ATTNRES_OK;
+  if (rows > 0 && !P.greedy) {
+    rc = launch(kVerifyPieces, kServingPart, "attnres_verify_pieces", (unsigned)(seqs * plan.slices), 1, 256, 0, P,
+                stream);
+    if (rc != ATTNRES_OK) return rc;
+  }
+  return launch(kVerifyPick, kServingPart, "attnres_verify_pick", (unsigned)seqs, 1, P.greedy ? 256 : 64, 0, P, stream);
 }
 
 }  // extern "C"

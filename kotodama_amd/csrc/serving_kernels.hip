@@ -206,14 +206,24 @@ __device__ __forceinline__ void paged_write(const lm_write_params& P) {
 // Without draft probabilities q is 1 at the draft; greedily (temperature 0) p is 1 at the
 // largest logit, the lowest index where several are.
 //
-// Which token a number falls to depends on sums over the whole vocabulary
-// next to a border, so the chosen row's are taken in 64 bits.  For the drafts' test one
-// probability each is enough: 32-bit exponentials, whose sum errs by
-// under 1e-5, and a row nearer to its border than that is summed again in 64 bits.
+// Which token a number falls to depends on sums over the whole vocabulary next to
+// a border, of which there are as many as tokens: in 32 bits one choice in some
+// hundreds would be another's.  So exponentials and sums are taken in 64.  Three launches:
+//   rows   a wave per 2048 logits of each row: the largest, and the sum of exponentials
+//          against it
+//   pieces a workgroup per 4096 of the one row of each sequence that a token is taken
+//          from (every one finds the first draft that falls for itself): the weights'
+//          sum of each 512
+//   pick   a wave per sequence: the piece, then the token in it
+// (The last workgroup of a sequence to arrive could pick: one launch less, but the fence that
+// shows it the others' sums writes back an L2 each time, 73 us more for 64 sequences.)
+// Bound by the first launch: reading the logits once, and 64-bit arithmetic on them after
+// that (one round of workgroups fills the card, so that one does not hide the other);
+// for few rows by the launches' latencies.  64 sequences of up to 8 drafts, vocabulary
+// 49152, bf16: XX us.
 
 constexpr int kVerifyThreads = 256;
-constexpr int kPickThreads = 1024;
-constexpr int kPickWaves = kPickThreads / 64;
+constexpr int kSide = kVerifyThreads / 16;  // drafts side by side
 constexpr float kNegInf = -__builtin_inff();
 
 // Eight consecutive values of a row from column j on (j a multiple of 8); `fill` behind its end.
@@ -260,6 +270,25 @@ __device__ __forceinline__ N wave_sum(N v) {
   return v;
 }
 
+// 2^t for t <= 0, to 1e-15 of itself: the polynomial that meets 2^f at the eleven Chebyshev points of
+// [-1/2, 1/2].  Under 2^-1080 it is zero, and a NaN is taken for that.
+__device__ __forceinline__ double exp2_neg(double t) {
+  t = fmax(t, -1080.0);
+  const double n = __builtin_rint(t), f = t - n;
+  double p = 7.07258594926922339e-09;
+  p = __builtin_fma(p, f, 1.02086902999583060e-07);
+  p = __builtin_fma(p, f, 1.32154425879216893e-06);
+  p = __builtin_fma(p, f, 1.52526572602008367e-05);
+  p = __builtin_fma(p, f, 1.54035304417360499e-04);
+  p = __builtin_fma(p, f, 1.33335582301649744e-03);
+  p = __builtin_fma(p, f, 9.61812910760688825e-03);
+  p = __builtin_fma(p, f, 5.55041086644477225e-02);
+  p = __builtin_fma(p, f, 2.40226506959100972e-01);
+  p = __builtin_fma(p, f, 6.93147180559949949e-01);
+  p = __builtin_fma(p, f, 1.0);
+  return __builtin_ldexp(p, (int)n);
+}
+
 // (top, at) of the larger value, the lower index where both are the same.
 __device__ __forceinline__ void larger(float& top, int& at, float t, int a) {
   const bool take = t > top || (t == top && a < at);
@@ -273,303 +302,326 @@ __device__ __forceinline__ int start_at(const lm_verify_params& P, int s) {
   return v < 0 ? 0 : v > P.rows ? P.rows : (int)v;
 }
 
-// First pass: of LM_VERIFY_SLICE logits the largest, where it is first, and the sum of exponentials against it.
-__device__ __forceinline__ void verify_rows(const lm_verify_params& P, float* tops, int* ats, double* sums) {
-  const int r = blockIdx.x / P.slices, slice = blockIdx.x - r * P.slices;
-  if (r >= start_at(P, P.seqs)) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const char* row = row_of(P.logits, P.logits_ld, r, P.logits_f32);
-  constexpr int U = LM_VERIFY_SLICE / (8 * kVerifyThreads);
-  const int first = slice * LM_VERIFY_SLICE;
-  float v[U][8];
-  float top = kNegInf;
-  int at = P.vocab;
-  bool odd = false;  // a NaN
+__device__ __forceinline__ void put_token(const lm_verify_params& P, int64_t r, int64_t token) {
+  if (P.ids64)
+    ((int64_t*)P.tokens)[r] = token;
+  else
+    ((int32_t*)P.tokens)[r] = (int32_t)token;
+}
+
+// N x 8 values of a row, from column j on and every `step` further; `fill` behind its end.
+template <int N>
+__device__ __forceinline__ void get_columns(const void* row, int j, int step, int n, int f32, int vec, float fill,
+                                            float (&v)[N][8]) {
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int j = first + 8 * (u * kVerifyThreads + (int)threadIdx.x);
-    if (j < P.vocab) {
-      get8(row, j, P.vocab, P.logits_f32, P.logits_vec, kNegInf, v[u]);
+  for (int u = 0; u < N; ++u) {
+    if (j + u * step < n) {
+      get8(row, j + u * step, n, f32, vec, fill, v[u]);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[u][i] = kNegInf;
+      for (int i = 0; i < 8; ++i) v[u][i] = fill;
     }
   }
+}
+
+// A wave's part of a row, 2048 logits: the largest and the sum of exponentials against it, a NaN
+// where one is among them or the largest is infinite, zero where all are minus infinity.  Greedily
+// where the largest is first, and one in place of the sum.  (Waves go their own ways: with the
+// largest of a workgroup's 4096, two barriers and every row's place of the largest it took
+// 19 us where it takes 16.)
+constexpr int kPartEach = LM_VERIFY_PART / (8 * 64);
+__device__ __forceinline__ void verify_rows(const lm_verify_params& P) {
+  const int id = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * (kVerifyThreads / 64) + (threadIdx.x >> 6)));
+  const int r = id / P.parts, part = id - r * P.parts;
+  if (r >= P.rows) return;
+  const int lane = threadIdx.x & 63;
+  if (r >= start_at(P, P.seqs)) {  // behind the last sequence
+    if (part == 0 && lane == 0) put_token(P, r, -1);
+    return;
+  }
+  const int base = part * LM_VERIFY_PART + 8 * lane;
+  float v[kPartEach][8];
+  get_columns(row_of(P.logits, P.logits_ld, r, P.logits_f32), base, 512, P.vocab, P.logits_f32, P.logits_vec, kNegInf,
+              v);
+  float top = kNegInf;
+  bool odd = false;  // a NaN
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int j = first + 8 * (u * kVerifyThreads + (int)threadIdx.x);
+  for (int u = 0; u < kPartEach; ++u)
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       odd = odd || v[u][i] != v[u][i];
-      if (v[u][i] > top) {
-        top = v[u][i];
-        at = j + i;
-      }
+      top = fmaxf(top, v[u][i]);
     }
+  int at = P.vocab;
+  if (P.greedy) {
+#pragma unroll
+    for (int u = kPartEach - 1; u >= 0; --u)
+#pragma unroll
+      for (int i = 7; i >= 0; --i) at = v[u][i] == top ? base + 512 * u + i : at;
+    at = top == kNegInf ? P.vocab : at;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) larger(top, at, __shfl_xor(top, m), __shfl_xor(at, m));
+  } else {
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
   }
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) larger(top, at, __shfl_xor(top, m), __shfl_xor(at, m));
-  if (lane == 0) {
-    tops[wave] = top;
-    ats[wave] = at;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kVerifyThreads / 64; ++w) larger(top, at, tops[w], ats[w]);
-  const float ref = top == kNegInf ? 0.f : top;
-  const float k = P.inv_temp * 1.44269504088896340736f;
-  float part = 0.f;
-#pragma unroll
-  for (int u = 0; u < U; ++u)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) part += __builtin_amdgcn_exp2f((v[u][i] - ref) * k);
-  double sum = wave_sum((double)(odd ? __builtin_nanf("") : part));
-  if (lane == 0) sums[wave] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) {
+  odd = __any(odd) || top == __builtin_inff();
+  double sum = top == kNegInf ? 0.0 : 1.0;
+  if (!P.greedy && top != kNegInf && !odd) {
     sum = 0;
-    for (int w = 0; w < kVerifyThreads / 64; ++w) sum += sums[w];
-    const int64_t o = (int64_t)r * P.slices + slice;
-    P.part_top[o] = top;
-    P.part_at[o] = at;
-    P.part_sum[o] = sum;
+#pragma unroll
+    for (int u = 0; u < kPartEach; ++u)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += exp2_neg(((double)v[u][i] - (double)top) * P.scale_log2);
+    sum = wave_sum(sum);
+  }
+  if (lane == 0) {
+    P.part_top[id] = top;
+    P.part_at[id] = at;
+    P.part_sum[id] = odd ? (double)__builtin_nanf("") : sum;
   }
 }
 
-struct PickShared {
-  double sums[kPickWaves];
-  double pieces[LM_VERIFY_MAX_PIECES];
-  int first, token;
-};
-
-// Sum over the workgroup, to every thread, in a fixed order.
-__device__ __forceinline__ double block_sum(double v, PickShared& S) {
-  v = wave_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) S.sums[threadIdx.x >> 6] = v;
-  __syncthreads();
-  double t = 0;
-#pragma unroll
-  for (int i = 0; i < kPickWaves; ++i) t += S.sums[i];
-  return t;
-}
-
-// The sum of a row's exponentials against `top`, in 64 bits.
-__device__ __forceinline__ double row_sum(const lm_verify_params& P, const char* row, float top, PickShared& S) {
-  double t = 0;
-  for (int j = 8 * (int)threadIdx.x; j < P.vocab; j += 8 * kPickThreads) {
-    float v[8];
-    get8(row, j, P.vocab, P.logits_f32, P.logits_vec, kNegInf, v);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) t += exp(((double)v[i] - (double)top) * P.inv_temp64);
-  }
-  return block_sum(t, S);
-}
-
-// A wave's 512 values from `j0`: each lane's eight weights.
-__device__ __forceinline__ void weights8(const lm_verify_params& P, const char* row, const char* draft, int gone, int j,
-                                         float top, double inv, double (&w)[8]) {
-  float v[8], q[8];
-  get8(row, j, P.vocab, P.logits_f32, P.logits_vec, kNegInf, v);
-  if (draft != nullptr) get8(draft, j, P.vocab, P.draft_f32, P.draft_vec, 0.f, q);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    double p = exp(((double)v[i] - (double)top) * P.inv_temp64) * inv;
-    if (draft != nullptr) {
-      p -= (double)q[i];
-      p = p < 0 ? 0 : p;  // a NaN stays one
-    }
-    w[i] = j + i == gone ? 0 : p;
-  }
-}
-
-// A token from the row's weights by the number u; -1 where they have no sum, none where it is zero.
-constexpr int kNoWeight = -2;
-__device__ __forceinline__ int sample(const lm_verify_params& P, const char* row, const char* draft, int gone, float top,
-                                      double inv, double u, PickShared& S) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int pieces = (P.vocab + LM_VERIFY_PIECE - 1) / LM_VERIFY_PIECE;
-  for (int p = wave; p < pieces; p += kPickWaves) {
-    const int j = p * LM_VERIFY_PIECE + 8 * lane;
-    double t = 0;
-    if (j < P.vocab) {
-      double w[8];
-      weights8(P, row, draft, gone, j, top, inv, w);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) t += w[i];
-    }
-    t = wave_sum(t);
-    if (lane == 0) S.pieces[p] = t;
-  }
-  __syncthreads();
-  if (wave == 0) {
-    // every lane a stretch of pieces
-    const int each = (pieces + 63) / 64;
-    double mine = 0;
-    for (int i = 0; i < each; ++i) {
-      const int p = lane * each + i;
-      if (p < pieces) mine += S.pieces[p];
-    }
-    double upto = mine;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-      const double x = __shfl_up(upto, m);
-      upto += lane >= m ? x : 0;
-    }
-    const double total = __shfl(upto, 63);
-    const double goal = u * total;
-    int token = !(total >= 0) || total > 1e300 ? -1 : total == 0 ? kNoWeight : -3;
-    if (token == -3) {
-      // the last lane with a weight takes what rounding leaves over
-      const uint64_t heavy = __ballot(mine > 0), over = __ballot(mine > 0 && upto > goal);
-      const int who = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(heavy);
-      double sum = __shfl(upto - mine, who);
-      int piece = -1;
-      double at = sum;
-      for (int i = 0; i < each; ++i) {  // every lane the same
-        const int p = who * each + i;
-        const double w = p < pieces ? S.pieces[p] : 0;
-        if (w > 0) {
-          piece = p;
-          at = sum;
-          if (sum + w > goal) break;
-        }
-        sum += w;
-      }
-      double w[8];
-      const int j = piece * LM_VERIFY_PIECE + 8 * lane;
-      double own = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = 0;
-      if (j < P.vocab) weights8(P, row, draft, gone, j, top, inv, w);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) own += w[i];
-      double end = own;
-#pragma unroll
-      for (int m = 1; m < 64; m <<= 1) {
-        const double x = __shfl_up(end, m);
-        end += lane >= m ? x : 0;
-      }
-      const uint64_t some = __ballot(own > 0), past = __ballot(own > 0 && at + end > goal);
-      const int lane2 = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
-      double run = at + (end - own);
-      int mineTok = -1;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const bool before = mineTok < 0 || run <= goal;  // not past the goal yet
-        if (w[i] > 0 && before) mineTok = j + i;
-        run += w[i];
-      }
-      token = __shfl(mineTok, lane2);
-    }
-    if (lane == 0) S.token = token;
-  }
-  __syncthreads();
-  const int t = S.token;
-  __syncthreads();
-  return t;
-}
-
-// A row's largest logit, where it is first, and the sum of its exponentials (the first pass's), to every lane.
+// A row's largest logit, where it is first, and its sum of exponentials, by 16 lanes side by side.
 struct RowStats {
   float top;
   int at;
   double sum;
 };
 __device__ __forceinline__ RowStats row_stats(const lm_verify_params& P, int64_t r) {
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 15;
+  const int64_t o = r * P.parts;
   RowStats R = {kNegInf, P.vocab, 0};
-  for (int i = lane; i < P.slices; i += 64) larger(R.top, R.at, P.part_top[r * P.slices + i], P.part_at[r * P.slices + i]);
+  for (int i = lane; i < P.parts; i += 16) larger(R.top, R.at, P.part_top[o + i], P.part_at[o + i]);
 #pragma unroll
-  for (int m = 1; m < 64; m <<= 1) larger(R.top, R.at, __shfl_xor(R.top, m), __shfl_xor(R.at, m));
-  for (int i = lane; i < P.slices; i += 64) {
-    const float t = P.part_top[r * P.slices + i];
-    const double sum = P.part_sum[r * P.slices + i];
-    R.sum += t == kNegInf ? sum : sum * exp(((double)t - (double)R.top) * P.inv_temp64);  // of none: zero, or a NaN
+  for (int m = 1; m < 16; m <<= 1) larger(R.top, R.at, __shfl_xor(R.top, m), __shfl_xor(R.at, m));
+  for (int i = lane; i < P.parts; i += 16) {
+    const float t = P.part_top[o + i];
+    // (of a part without a logit: zero, or a NaN)
+    R.sum = __builtin_fma(P.part_sum[o + i], t == kNegInf ? 1.0 : exp2_neg(((double)t - (double)R.top) * P.scale_log2),
+                          R.sum);
   }
-  R.sum = wave_sum(R.sum);
+#pragma unroll
+  for (int m = 1; m < 16; m <<= 1) R.sum += __shfl_xor(R.sum, m);
   return R;
 }
 
-// Second pass: a workgroup per sequence, and one for the rows behind the last.
-__device__ __forceinline__ void verify_pick(const lm_verify_params& P, PickShared& S) {
-  const int tid = threadIdx.x, wave = tid >> 6, s = blockIdx.x;
-  auto put = [&](int r, int64_t token) {
-    if (P.ids64)
-      ((int64_t*)P.tokens)[r] = token;
-    else
-      ((int32_t*)P.tokens)[r] = (int32_t)token;
-  };
-  const int r0 = start_at(P, s);
-  if (s == P.seqs) {
-    for (int64_t r = r0 + tid; r < P.rows; r += kPickThreads) put((int)r, -1);
-    return;
-  }
-  const int next = start_at(P, s + 1), drafts = next - r0 - 1;
-  if (drafts < 0) {
-    if (tid == 0) P.counts[s] = 0;
-    return;
-  }
-  auto draft_of = [&](int i) { return index_at(P.ids, r0 + i + 1, P.ids64); };
-  auto weight_of = [&](int i, int64_t d) {  // the draft's own probability
-    return P.draft == nullptr ? 1.0 : (double)get1(row_of(P.draft, P.draft_ld, r0 + i, P.draft_f32), (int)d, P.draft_f32);
-  };
-  // the first draft that does not stay
-  int from = 0, a = drafts;
-  while (from < drafts) {
-    if (tid == 0) S.first = 2 * drafts;
-    __syncthreads();
-    for (int i = from + wave; i < drafts; i += kPickWaves) {
-      const int64_t d = draft_of(i);
-      bool stays = false, near = false;
-      if (d >= 0 && d < P.vocab) {
-        const RowStats R = row_stats(P, r0 + i);
-        if (P.greedy) {
-          stays = d == R.at && R.sum > 0;  // a NaN is not
-        } else {
-          const float x = get1(row_of(P.logits, P.logits_ld, r0 + i, P.logits_f32), (int)d, P.logits_f32);
-          const double p = exp(((double)x - (double)R.top) * P.inv_temp64) / R.sum;
-          const double need = (double)P.uniforms[2 * (int64_t)(r0 + i)] * weight_of(i, d);
-          stays = need < p;
-          near = fabs(need - p) <= 1e-4 * p;
-        }
+__device__ __forceinline__ int64_t draft_of(const lm_verify_params& P, int r) {
+  return index_at(P.ids, (int64_t)r + 1, P.ids64);
+}
+
+struct PickShared {
+  RowStats stats[kSide];
+  int first;
+};
+
+// How many of a sequence's drafts (rows from r0 on) stay, and the statistics of the row behind them, by the whole
+// workgroup, 16 lanes a row.
+__device__ __forceinline__ int accepted(const lm_verify_params& P, int r0, int drafts, RowStats* R, PickShared& S) {
+  if (threadIdx.x == 0) S.first = drafts;
+  __syncthreads();
+  int base = 0;
+  for (;; base += kSide) {
+    const int i = base + (int)threadIdx.x / 16;
+    if (i <= drafts) {
+      // what the draft is compared by is requested with the statistics
+      const int64_t d = i < drafts ? draft_of(P, r0 + i) : -1;
+      const bool names = d >= 0 && d < P.vocab;
+      float x = 0.f, q = 1.f, u = 0.f;
+      if (names && !P.greedy) {
+        x = get1(row_of(P.logits, P.logits_ld, r0 + i, P.logits_f32), (int)d, P.logits_f32);
+        if (P.draft != nullptr) q = get1(row_of(P.draft, P.draft_ld, r0 + i, P.draft_f32), (int)d, P.draft_f32);
+        u = P.uniforms[2 * (int64_t)(r0 + i)];
       }
-      if (!stays || near) {
-        if ((tid & 63) == 0) atomicMin(&S.first, 2 * i + (near ? 1 : 0));
-        break;
+      const RowStats mine = row_stats(P, r0 + i);
+      bool stays = false;
+      if (names)
+        stays = P.greedy ? d == mine.at && mine.sum > 0  // a NaN is not
+                         : (double)u * (double)q <
+                               exp2_neg(((double)x - (double)mine.top) * P.scale_log2) / mine.sum;
+      if ((threadIdx.x & 15) == 0) {
+        S.stats[threadIdx.x / 16] = mine;
+        if (!stays) atomicMin(&S.first, i);
       }
     }
     __syncthreads();
-    const int found = S.first;
-    __syncthreads();
-    a = found >> 1;
-    if (a == drafts || (found & 1) == 0) break;
-    const char* row = row_of(P.logits, P.logits_ld, r0 + a, P.logits_f32);
-    const RowStats R = row_stats(P, r0 + a);
-    const double sum = row_sum(P, row, R.top, S);
-    const int64_t d = draft_of(a);
-    const double p = exp(((double)get1(row, (int)d, P.logits_f32) - (double)R.top) * P.inv_temp64) / sum;
-    if (!((double)P.uniforms[2 * (int64_t)(r0 + a)] * weight_of(a, d) < p)) break;
-    from = a + 1;
-    a = drafts;
+    if (S.first < base + kSide) break;  // at the latest behind the last draft
+    __syncthreads();                    // the statistics have been passed over
   }
-  // the token in its place, or the one behind them all
-  const RowStats R = row_stats(P, r0 + a);
-  const char* row = row_of(P.logits, P.logits_ld, r0 + a, P.logits_f32);
-  int token;
+  *R = S.stats[S.first - base];
+  return S.first;
+}
+
+// The weights that a token of row r is taken by: those of p - q times the row's sum of exponentials,
+// or of p where `draft` is NULL, without the column `gone`.
+struct Weights {
+  const char *row, *draft;
+  int gone;
+  double top, sum;
+};
+__device__ __forceinline__ Weights weights_of(const lm_verify_params& P, int r, bool swapped, const RowStats& R) {
+  Weights W;
+  W.row = row_of(P.logits, P.logits_ld, r, P.logits_f32);
+  W.draft = swapped && P.draft != nullptr ? row_of(P.draft, P.draft_ld, r, P.draft_f32) : nullptr;
+  W.gone = -1;
+  if (swapped && P.draft == nullptr) {
+    const int64_t d = draft_of(P, r);
+    W.gone = d >= 0 && d < P.vocab ? (int)d : -1;
+  }
+  W.top = (double)R.top;
+  W.sum = R.sum;
+  return W;
+}
+// e: the exponentials, w: the weights, of eight columns from j on
+__device__ __forceinline__ void weights8(const lm_verify_params& P, const Weights& W, int j, const float (&v)[8],
+                                         const float (&q)[8], double (&e)[8], double (&w)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    e[i] = exp2_neg(((double)v[i] - W.top) * P.scale_log2);
+    w[i] = W.draft != nullptr ? fmax(__builtin_fma(-W.sum, (double)q[i], e[i]), 0.0) : e[i];
+    w[i] = j + i == W.gone ? 0.0 : w[i];
+  }
+}
+
+constexpr int kPieces = LM_VERIFY_SLICE / LM_VERIFY_PIECE;  // of a workgroup
+static_assert(LM_VERIFY_PIECE == 8 * 64, "a piece is a wave's values");
+
+// A stretch of the row that a sequence's token is taken from: its pieces' sums.
+__device__ __forceinline__ void verify_pieces(const lm_verify_params& P, PickShared& S) {
+  const int s = blockIdx.x / P.slices, slice = blockIdx.x - s * P.slices;
+  const int r0 = start_at(P, s), drafts = start_at(P, s + 1) - r0 - 1;
+  if (drafts < 0) return;
+  RowStats R;
+  const int a = accepted(P, r0, drafts, &R, S);
+  if (slice == 0 && threadIdx.x == 0) {
+    P.chosen[s].sum = R.sum;
+    P.chosen[s].top = R.top;
+    P.chosen[s].accepted = a;
+  }
+  const Weights W = weights_of(P, r0 + a, a < drafts, R);
+  constexpr int kEach = LM_VERIFY_SLICE / (8 * kVerifyThreads);
+  const int j = slice * LM_VERIFY_SLICE + 8 * (int)threadIdx.x;
+  float v[kEach][8], q[kEach][8];
+  get_columns(W.row, j, 8 * kVerifyThreads, P.vocab, P.logits_f32, P.logits_vec, kNegInf, v);
+  if (W.draft != nullptr) get_columns(W.draft, j, 8 * kVerifyThreads, P.vocab, P.draft_f32, P.draft_vec, 0.f, q);
+  double* pieces = P.piece_sum + 2 * (int64_t)s * P.slices * kPieces;
+#pragma unroll
+  for (int u = 0; u < kEach; ++u) {
+    double e[8], w[8], se = 0, sw = 0;
+    weights8(P, W, j + u * 8 * kVerifyThreads, v[u], q[u], e, w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      se += e[i];
+      sw += w[i];
+    }
+    se = wave_sum(se);
+    sw = wave_sum(sw);
+    const int piece = slice * kPieces + u * (kVerifyThreads / 64) + (threadIdx.x >> 6);
+    if ((threadIdx.x & 63) == 0) {
+      pieces[2 * piece] = sw;
+      pieces[2 * piece + 1] = se;
+    }
+  }
+}
+
+// A token by the number u from a sequence's pieces (which: their weights, or 1 their exponentials), by one wave; -1
+// where they sum to nothing.
+__device__ __forceinline__ int sample(const lm_verify_params& P, Weights W, const double* pieces, int which, double u) {
+  const int lane = threadIdx.x & 63, n = P.slices * kPieces;
+  if (which == 1) {
+    W.draft = nullptr;
+    W.gone = -1;
+  }
+  // every lane a stretch of pieces
+  const int each = (n + 63) / 64;
+  double mine = 0;
+  for (int i = 0; i < each; ++i) {
+    const int p = lane * each + i;
+    if (p < n) mine += pieces[2 * p + which];
+  }
+  double upto = mine;
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    const double x = __shfl_up(upto, m);
+    upto += lane >= m ? x : 0;
+  }
+  const double goal = u * __shfl(upto, 63);
+  // the first lane over the goal; what rounding leaves over is for the last with a weight
+  const uint64_t heavy = __ballot(mine > 0), over = __ballot(mine > 0 && upto > goal);
+  if (heavy == 0) return -1;
+  const int who = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(heavy);
+  double sum = __shfl(upto - mine, who), at = sum;
+  int piece = -1;
+  for (int i = 0; i < each; ++i) {  // every lane the same
+    const int p = who * each + i;
+    const double w = p < n ? pieces[2 * p + which] : 0;
+    if (w > 0) {
+      piece = p;
+      at = sum;
+      if (sum + w > goal) break;
+    }
+    sum += w;
+  }
+  const int j = piece * LM_VERIFY_PIECE + 8 * lane;
+  double e[8], w[8], own = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = 0;
+  if (j < P.vocab) {
+    float v[8], q[8];
+    get8(W.row, j, P.vocab, P.logits_f32, P.logits_vec, kNegInf, v);
+    if (W.draft != nullptr) get8(W.draft, j, P.vocab, P.draft_f32, P.draft_vec, 0.f, q);
+    weights8(P, W, j, v, q, e, w);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) own += w[i];
+  double end = own;
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    const double x = __shfl_up(end, m);
+    end += lane >= m ? x : 0;
+  }
+  const uint64_t some = __ballot(own > 0), past = __ballot(own > 0 && at + end > goal);
+  if (some == 0) return -1;
+  const int in = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
+  double run = at + (end - own);
+  int token = -1;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (w[i] > 0 && (token < 0 || run <= goal)) token = j + i;  // the sum in front is not over the goal yet
+    run += w[i];
+  }
+  return __shfl(token, in);
+}
+
+// The tokens of a sequence, by one wave; greedily by a workgroup, from the rows alone.
+__device__ __forceinline__ void verify_pick(const lm_verify_params& P, PickShared& S) {
+  const int s = blockIdx.x;
+  const int r0 = start_at(P, s), drafts = start_at(P, s + 1) - r0 - 1;
+  if (drafts < 0) {
+    if (threadIdx.x == 0) P.counts[s] = 0;
+    return;
+  }
+  RowStats R;
+  int a, token = -1;
   if (P.greedy) {
+    a = accepted(P, r0, drafts, &R, S);
     token = R.sum > 0 ? R.at : -1;  // a NaN is not
   } else {
-    const double inv = 1.0 / row_sum(P, row, R.top, S), u = (double)P.uniforms[2 * (int64_t)(r0 + a) + 1];
-    const bool swapped = a < drafts;
-    const char* draft = swapped && P.draft != nullptr ? row_of(P.draft, P.draft_ld, r0 + a, P.draft_f32) : nullptr;
-    const int64_t d = swapped ? draft_of(a) : -1;
-    const int gone = swapped && P.draft == nullptr && d >= 0 && d < P.vocab ? (int)d : -1;
-    token = sample(P, row, draft, gone, R.top, inv, u, S);
-    if (token == kNoWeight) token = sample(P, row, nullptr, -1, R.top, inv, u, S);
+    const lm_verify_choice C = P.chosen[s];
+    a = C.accepted;
+    R.top = C.top;
+    R.sum = C.sum;
+    if (R.sum > 0) {
+      const Weights W = weights_of(P, r0 + a, a < drafts, R);
+      const double goal = (double)P.uniforms[2 * (int64_t)(r0 + a) + 1];
+      const double* pieces = P.piece_sum + 2 * (int64_t)s * P.slices * kPieces;
+      token = sample(P, W, pieces, 0, goal);
+      if (token < 0) token = sample(P, W, pieces, 1, goal);  // of p - q nothing is left
+    }
   }
-  for (int i = tid; i <= drafts; i += kPickThreads) put(r0 + i, i < a ? draft_of(i) : i == a ? token : -1);
-  if (tid == 0) P.counts[s] = token < 0 ? a : a + 1;
+  for (int i = threadIdx.x; i <= drafts; i += blockDim.x)
+    put_token(P, r0 + i, i < a ? draft_of(P, r0 + i) : i == a ? token : -1);
+  if (threadIdx.x == 0) P.counts[s] = token < 0 ? a : a + 1;
 }
 
 }  // namespace
@@ -583,13 +635,13 @@ extern "C" __global__ void __launch_bounds__(LM_SLOTS_THREADS) attnres_paged_rel
   paged_release(P, S);
 }
 extern "C" __global__ void __launch_bounds__(256) attnres_paged_write(lm_write_params P) { paged_write(P); }
-extern "C" __global__ void __launch_bounds__(kVerifyThreads) attnres_verify_rows(lm_verify_params P) {
-  __shared__ float tops[kVerifyThreads / 64];
-  __shared__ int ats[kVerifyThreads / 64];
-  __shared__ double sums[kVerifyThreads / 64];
-  verify_rows(P, tops, ats, sums);
+extern "C" __global__ void __launch_bounds__(kVerifyThreads) attnres_verify_rows(lm_verify_params P) { verify_rows(P); }
+extern "C" __global__ void __launch_bounds__(kVerifyThreads) attnres_verify_pieces(lm_verify_params P) {
+  __shared__ PickShared S;
+  verify_pieces(P, S);
 }
-extern "C" __global__ void __launch_bounds__(kPickThreads) attnres_verify_pick(lm_verify_params P) {
+// 64 threads, or kVerifyThreads greedily
+extern "C" __global__ void __launch_bounds__(kVerifyThreads) attnres_verify_pick(lm_verify_params P) {
   __shared__ PickShared S;
   verify_pick(P, S);
 }

@@ -234,7 +234,7 @@ PyObject* py_verify_drafts(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t rows = logits.size(0), seqs = q_starts.size(0) - 1;
     int64_t bytes = 0;
     const OnDevice on(logits);
-    if (attnres_verify_drafts_workspace_size(rows, (int)logits.size(1), &bytes) == ATTNRES_OK) {
+    if (attnres_verify_drafts_workspace_size(rows, (int)seqs, (int)logits.size(1), &bytes) == ATTNRES_OK) {
       tokens = empty({rows}, ids.scalar_type(), logits.device());
       counts = ints(seqs, logits);
       const Tensor ws = workspace(bytes, logits.device());

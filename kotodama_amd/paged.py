@@ -472,8 +472,8 @@ def _verify_drafts_impl(logits, ids, q_starts, uniforms, draft_probs, temperatur
         draft_probs = _table(draft_probs)
         draft_args = (draft_probs.data_ptr(), draft_probs.stride(0), dtype_code(draft_probs.dtype))
     with _DeviceStream(device) as stream:
-        nbytes = _capi.verify_drafts_workspace_size(n, v)
-        ws = torch.empty(max(1, nbytes // 8), device=device, dtype=torch.float64)
+        nbytes = _capi.verify_drafts_workspace_size(n, q_starts.shape[0] - 1, v)
+        ws = _workspace(nbytes, device)
         _capi.verify_drafts(logits.data_ptr(), logits.stride(0), dtype_code(logits.dtype), *draft_args, n, v,
                             ids.data_ptr(), ids_code, q_starts.data_ptr(), starts_code, q_starts.shape[0] - 1,
                             uniforms.data_ptr(), float(temperature), tokens.data_ptr(), counts.data_ptr(),
