@@ -17,7 +17,8 @@
 // Calls of few rows (paged_stream): all tiles are narrow.  The blocks of all
 // sequences' tiles lie one after another, and each of a key head's workgroups (two on
 // every CU, over all heads) takes an equal stretch of them, whatever
-// sequences it leads through.
+// sequences it leads through; or, where no row of the table holds many blocks, a workgroup
+// takes a whole tile.
 //
 // Calls with rows enough to fill the card 128 at a time (paged_tiles): the rows of
 // longer sequences are taken so, each wave 32 of them over all keys, a workgroup
@@ -108,6 +109,8 @@ struct Shared {
   float sum[LM_ATTN_WAVES];
   int scan[LM_ATTN_WAVES][2];
   int upto[kThreads][2];
+  Share share;
+  int seq, before;
 };
 
 // Inclusive sums of N numbers over the workgroup's threads into S.upto.
@@ -479,27 +482,29 @@ __device__ __forceinline__ void wide_tile(const Piece& J, int kvh, LDS_ARRAYS, i
 
 // ------------------------------------------------------------- few rows --
 
-// Blocks of a sequence's tiles; a tile without keys has one, as it is written too.
-__device__ __forceinline__ int tile_blocks(const Share& a) { return a.kv_len > 128 ? (a.kv_len + 127) >> 7 : 1; }
+// Key blocks of a tile.
+__device__ __forceinline__ int tile_blocks(const Share& a) { return (a.kv_len + 127) >> 7; }
+// And what it counts for in the stretches: one where tiles are not split, and where it has no keys, as it is
+// written too.
+__device__ __forceinline__ int tile_units(const lm_paged_params& P, const Share& a) {
+  return P.slots > 0 && a.kv_len > 128 ? tile_blocks(a) : 1;
+}
 
 template <typename T, int DP, int DC>
 __device__ __forceinline__ void paged_stream(const lm_paged_params& P, LDS_ARRAYS, float* ml, Shared& S) {
   const int kvh = (int)blockIdx.x % P.kv_heads, w = (int)blockIdx.x / P.kv_heads;
-  auto blocks_at = [&](int s) {
-    const Share a = share_of(P, s < P.seqs ? s : P.seqs);
-    return s > P.seqs ? 0 : a.tiles * tile_blocks(a);
-  };
-  // all blocks (under 2^31: the host sees to it), and this workgroup's stretch of them
-  int before = 0, base = 0;
-  int v[1] = {blocks_at((int)threadIdx.x)};
+  auto share = [&](int s) { return share_of(P, s < P.seqs ? s : P.seqs); };
+  auto units = [&](const Share& x, int s) { return s > P.seqs ? 0 : x.tiles * tile_units(P, x); };
+  // all units (under 2^31: the host sees to it), and this workgroup's stretch of them
+  Share mine = share((int)threadIdx.x);
+  int v[1] = {units(mine, (int)threadIdx.x)};
+  int own = v[0];
   scan_all<1>(v, S);
   int total = S.upto[kThreads - 1][0];
-  if (P.seqs >= kThreads) {
-    for (base = kThreads; base <= P.seqs; base += kThreads) {
-      v[0] = blocks_at(base + (int)threadIdx.x);
-      scan_all<1>(v, S);
-      total += S.upto[kThreads - 1][0];
-    }
+  for (int base = kThreads; base <= P.seqs; base += kThreads) {
+    v[0] = units(share(base + (int)threadIdx.x), base + (int)threadIdx.x);
+    scan_all<1>(v, S);
+    total += S.upto[kThreads - 1][0];
   }
   const int each = (int)(((int64_t)total + P.target - 1) / P.target);
   const int64_t begin = (int64_t)w * each;
@@ -509,27 +514,35 @@ __device__ __forceinline__ void paged_stream(const lm_paged_params& P, LDS_ARRAY
   const int cont = P.target * P.kv_heads + note;  // of one that it goes on with
   bool noted = false;
   if (at < end) {
-    // the sequence in which the stretch begins
+    // the sequence in which the stretch begins: its thread hands it on
+    int before = 0, base = 0;
     if (P.seqs >= kThreads) {
-      for (base = 0;; base += kThreads) {
-        v[0] = blocks_at(base + (int)threadIdx.x);
+      for (;; base += kThreads) {
+        mine = share(base + (int)threadIdx.x);
+        v[0] = own = units(mine, base + (int)threadIdx.x);
         scan_all<1>(v, S);
         if (at - before < S.upto[kThreads - 1][0]) break;
         before += S.upto[kThreads - 1][0];
       }
     }
-    const int lo = find_upto(S, at - before);
-    if (lo > 0) before += S.upto[lo - 1][0];
+    if (at - before < v[0] && at - before >= v[0] - own) {
+      S.share = mine;
+      S.seq = base + (int)threadIdx.x;
+      S.before = before + v[0] - own;
+    }
+    __syncthreads();
     Piece J;
-    J.seq = base + lo;
-    J.a = share_of(P, J.seq);
-    int n = tile_blocks(J.a);
+    J.a = S.share;
+    J.seq = uniform(S.seq);
+    before = uniform(S.before);
+    int n = tile_units(P, J.a);
     J.tile = uniform((at - before) / n);
     J.t0 = uniform(at - before - J.tile * n);
     for (;;) {
       const int left = end - at;
       const bool ends = n - J.t0 <= left;  // with this tile's last block
-      J.t1 = uniform(ends ? n : J.t0 + left);
+      const int taken = ends ? n - J.t0 : left;
+      J.t1 = uniform(ends ? tile_blocks(J.a) : J.t0 + left);
       J.slot = J.t0 > 0 ? cont : ends ? -1 : note;
       if (J.t0 == 0 && !ends) {
         noted = true;
@@ -538,20 +551,20 @@ __device__ __forceinline__ void paged_stream(const lm_paged_params& P, LDS_ARRAY
                      P.kv_heads);
       }
       narrow_tile<T, DP, DC>(J, kvh, a, b, c, d, ml);
-      at += J.t1 - J.t0;
+      at += taken;
       if (at >= end) break;
       J.t0 = 0;
       if (++J.tile >= J.a.tiles) {
         J.tile = 0;
-        do {  // there is one: blocks are left
+        do {  // there is one: units are left
           J.a = share_of(P, ++J.seq);
         } while (J.a.tiles == 0);
-        n = tile_blocks(J.a);
+        n = tile_units(P, J.a);
       }
       __syncthreads();  // the sums have been read
     }
   }
-  if (!noted && threadIdx.x == 0) P.notes[note].parts = 0;
+  if (!noted && P.slots > 0 && threadIdx.x == 0) P.notes[note].parts = 0;
 }
 
 // ------------------------------------------------------------ many rows --
