@@ -35,7 +35,6 @@ constexpr int64_t kMaxTokens = (int64_t)1 << 30;  // of one sequence, and new on
 constexpr int kMaxPage = 1 << 16;                 // rows
 constexpr int kMaxGroup = 4096;                   // query heads per key head
 constexpr int kMaxSeqs = 1 << 20;
-constexpr int kSplitPerCu = 2;  // workgroups per CU to deal the key blocks out to
 // Keys that one workgroup takes of a tile without splitting it: a block of 128 costs it some 1.2 us, the
 // launch that joins parts 4 to 5 (one token over 512 keys, 32/8 heads of 128: 11.7 us whole, 8.2 + 4.2 in
 // parts; over 1024 keys 17.2 and 8.0 + 5.1).
@@ -113,15 +112,20 @@ struct PagedPlan {
   int64_t at_ml = 0, at_notes = 0, bytes = 0;
 };
 
-int paged_plan(int64_t tokens, int seqs, int heads, int kv_heads, int head_dim, int64_t capacity, PagedPlan* p) {
+int paged_plan(int64_t tokens, int seqs, int heads, int kv_heads, int head_dim, int dtype, int64_t capacity,
+               PagedPlan* p) {
   int cus = 0;
   const int rc = attnres_internal_num_cus(&cus);
   if (rc != ATTNRES_OK) return rc;
   const int64_t rows = tokens * (heads / kv_heads);
+  // Workgroups to deal out to: two a CU, or one where the LDS has no room for two (64 ragged fp32 sequences of
+  // up to 2048 keys, 8/4 heads of 128: 90 us, 97 with two rounds of them).  Heads of up to 64 in bf16 have room
+  // for four, but shorter stretches cost more than they hide (64 sequences of up to 4096 keys: 39 us against 34).
+  const int64_t at_once = (int64_t)cus * (head_dim > 64 && dtype == ATTNRES_DTYPE_F32 ? 1 : 2);
   p->wide = rows / 32 * kv_heads >= (int64_t)cus * kWideWaves;
   p->split = capacity > kWholeKeys;
   if (p->wide) {
-    p->target = cus * kSplitPerCu;
+    p->target = (int)at_once;
     // tiles: every sequence may end inside one; the rows behind the last sequence are one more
     const int64_t tiles = rows / 128 + seqs + 1, share = (p->target + kv_heads - 1) / kv_heads;
     // a split tile's parts are under twice its blocks over a part's most, and all those blocks at most the target's share
@@ -133,7 +137,7 @@ int paged_plan(int64_t tokens, int seqs, int heads, int kv_heads, int head_dim, 
     if ((rows / 32 + seqs + 1) * ((capacity + 127) / 128) > INT32_MAX)
       return fail(ATTNRES_ERR_UNSUPPORTED, "paged_attention: too many keys for one call");
     const int64_t tiles = rows / 32 + seqs + 1;
-    p->target = !p->split ? (int)tiles : cus * kSplitPerCu / kv_heads > 0 ? cus * kSplitPerCu / kv_heads : 1;
+    p->target = !p->split ? (int)tiles : at_once > kv_heads ? (int)(at_once / kv_heads) : 1;
     p->grid = (int64_t)p->target * kv_heads;
     p->slots = p->split ? 2 * p->grid : 0;  // each workgroup goes on with a tile and begins one
     p->notes = p->split ? p->grid : 0;
@@ -310,7 +314,7 @@ int attnres_paged_attention_workspace_size(int64_t tokens, int seqs, int heads, 
   int rc = check_attention(tokens, seqs, heads, kv_heads, head_dim, dtype, table_width, page_size, &shift);
   if (rc != ATTNRES_OK) return rc;
   PagedPlan plan;
-  rc = paged_plan(tokens, seqs, heads, kv_heads, head_dim, (int64_t)table_width * page_size, &plan);
+  rc = paged_plan(tokens, seqs, heads, kv_heads, head_dim, dtype, (int64_t)table_width * page_size, &plan);
   *bytes = plan.bytes;
   return rc;
 }
@@ -350,7 +354,8 @@ int attnres_paged_attention_fwd(const void* q, const int64_t* q_strides, const v
     return rc;
   const int64_t capacity = pages == 0 ? 0 : (int64_t)table_width * page_size;
   PagedPlan plan;
-  if ((rc = paged_plan(tokens, seqs, heads, kv_heads, head_dim, (int64_t)table_width * page_size, &plan)) != ATTNRES_OK)
+  if ((rc = paged_plan(tokens, seqs, heads, kv_heads, head_dim, dtype, (int64_t)table_width * page_size, &plan)) !=
+      ATTNRES_OK)
     return rc;
   if (plan.bytes > 0 && (workspace == nullptr || workspace_bytes < plan.bytes))
     return fail(ATTNRES_ERR_ARG, "paged_attention: workspace of %lld bytes needed", (long long)plan.bytes);
@@ -395,8 +400,10 @@ int attnres_paged_attention_fwd(const void* q, const int64_t* q_strides, const v
   rc = launch(kPagedAttn + (f32 ? 8 : 0) + (plan.wide ? 4 : 0) + blocks, part, name, (unsigned)plan.grid, 1,
               LM_PAGED_THREADS, 0, P, stream);
   if (rc != ATTNRES_OK || !plan.split) return rc;
+  // workgroups of a note, over its rows (11 sequences, one of 301 new tokens, fp32: 6.4 us with 16, 10.8 with 4)
+  const int lines = plan.wide ? 8 : plan.part_rows < 16 ? plan.part_rows : 16;
   return launch(kPagedJoin + (f32 ? 1 : 0), part, f32 ? "attnres_paged_join_f32" : "attnres_paged_join_bf16",
-                (unsigned)plan.notes, plan.part_rows < 8 ? plan.part_rows : 8, LM_PAGED_THREADS, 0, P, stream);
+                (unsigned)plan.notes, (unsigned)lines, LM_PAGED_THREADS, 0, P, stream);
 }
 
 int attnres_verify_drafts_workspace_size(int64_t rows, int seqs, int vocab, int64_t* bytes) {
