@@ -113,6 +113,10 @@ struct Shared {
   int seq, before;
 };
 
+// Sums of numbers that are not negative stop at the largest: starts that do not rise name rows many times over, and
+// a sum that wrapped would lead out of the sequences.
+__device__ __forceinline__ int add_sat(int a, int b) { return __builtin_elementwise_add_sat(a, b); }
+
 // Inclusive sums of N numbers over the workgroup's threads into S.upto.
 template <int N>
 __device__ __forceinline__ void scan_all(int (&v)[N], Shared& S) {
@@ -122,7 +126,7 @@ __device__ __forceinline__ void scan_all(int (&v)[N], Shared& S) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int x = __shfl_up(v[i], m);
-      v[i] += lane >= m ? x : 0;
+      v[i] = add_sat(v[i], lane >= m ? x : 0);
     }
   __syncthreads();  // what was there has been read
   if (lane == 63) {
@@ -133,7 +137,7 @@ __device__ __forceinline__ void scan_all(int (&v)[N], Shared& S) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
 #pragma unroll
-    for (int w = 0; w < LM_ATTN_WAVES - 1; ++w) v[i] += w < wave ? S.scan[w][i] : 0;
+    for (int w = 0; w < LM_ATTN_WAVES - 1; ++w) v[i] = add_sat(v[i], w < wave ? S.scan[w][i] : 0);
     S.upto[threadIdx.x][i] = v[i];
   }
   __syncthreads();
@@ -382,7 +386,9 @@ __device__ __forceinline__ void narrow_tile(const Piece& J, int kvh, LDS_ARRAYS,
     for (int i = 0; i < 16; ++i) {
       sum[i] = 0.f;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) sum[i] = __builtin_fmaf(reinterpret_cast<const float*>(lds_of(w, a, b, c, d))[(wave * 16 + i) * 64 + lane], fade[w], sum[i]);
+      for (int w = 0; w < 4; ++w)
+        sum[i] = __builtin_fmaf(reinterpret_cast<const float*>(lds_of(w, a, b, c, d))[(wave * 16 + i) * 64 + lane],
+                                fade[w], sum[i]);
     }
     const lm_paged_params& P = anew();
     const bool whole = J.slot < 0;
@@ -495,16 +501,15 @@ __device__ __forceinline__ void paged_stream(const lm_paged_params& P, LDS_ARRAY
   const int kvh = (int)blockIdx.x % P.kv_heads, w = (int)blockIdx.x / P.kv_heads;
   auto share = [&](int s) { return share_of(P, s < P.seqs ? s : P.seqs); };
   auto units = [&](const Share& x, int s) { return s > P.seqs ? 0 : x.tiles * tile_units(P, x); };
-  // all units (under 2^31: the host sees to it), and this workgroup's stretch of them
+  // all units (under 2^31 where starts rise: the host sees to it), and this workgroup's stretch of them
   Share mine = share((int)threadIdx.x);
   int v[1] = {units(mine, (int)threadIdx.x)};
-  int own = v[0];
   scan_all<1>(v, S);
   int total = S.upto[kThreads - 1][0];
   for (int base = kThreads; base <= P.seqs; base += kThreads) {
     v[0] = units(share(base + (int)threadIdx.x), base + (int)threadIdx.x);
     scan_all<1>(v, S);
-    total += S.upto[kThreads - 1][0];
+    total = add_sat(total, S.upto[kThreads - 1][0]);
   }
   const int each = (int)(((int64_t)total + P.target - 1) / P.target);
   const int64_t begin = (int64_t)w * each;
@@ -519,16 +524,17 @@ __device__ __forceinline__ void paged_stream(const lm_paged_params& P, LDS_ARRAY
     if (P.seqs >= kThreads) {
       for (;; base += kThreads) {
         mine = share(base + (int)threadIdx.x);
-        v[0] = own = units(mine, base + (int)threadIdx.x);
+        v[0] = units(mine, base + (int)threadIdx.x);
         scan_all<1>(v, S);
         if (at - before < S.upto[kThreads - 1][0]) break;
         before += S.upto[kThreads - 1][0];
       }
     }
-    if (at - before < v[0] && at - before >= v[0] - own) {
+    const int front = threadIdx.x > 0 ? S.upto[threadIdx.x - 1][0] : 0;
+    if (at - before < v[0] && at - before >= front) {
       S.share = mine;
       S.seq = base + (int)threadIdx.x;
-      S.before = before + v[0] - own;
+      S.before = before + front;
     }
     __syncthreads();
     Piece J;
@@ -625,12 +631,12 @@ __device__ __forceinline__ void paged_tiles(const lm_paged_params& P, LDS_ARRAYS
     const int n = S.upto[kThreads - 1][0];
     found = w - parts < n;
     if (found) break;
-    parts += n;
-    slots += S.upto[kThreads - 1][1];
+    parts = add_sat(parts, n);
+    slots = add_sat(slots, S.upto[kThreads - 1][1]);
   }
   if (!found) {
     // no part is left: the workgroups behind them clear the notes of the slots that none has
-    for (int64_t i = slots + (w - parts) + (int64_t)threadIdx.x * (all - parts); i < P.slots;
+    for (int64_t i = (int64_t)slots + (w - parts) + (int64_t)threadIdx.x * (all - parts); i < P.slots;
          i += (int64_t)kThreads * (all - parts))
       P.notes[i * P.kv_heads + kvh].parts = 0;
     return;
@@ -647,8 +653,8 @@ __device__ __forceinline__ void paged_tiles(const lm_paged_params& P, LDS_ARRAYS
   J.t1 = uniform(J.t0 + sp.per < sp.n ? J.t0 + sp.per : sp.n);
   J.slot = -1;
   if (sp.parts > 1) {
-    const int first = uniform(slots + (lo > 0 ? S.upto[lo - 1][1] : 0) + rank * sp.parts);
-    if (first + sp.parts > P.slots) return;  // starts that do not rise
+    const int first = uniform(add_sat(add_sat(slots, lo > 0 ? S.upto[lo - 1][1] : 0), rank * sp.parts));
+    if (first > P.slots - sp.parts) return;  // starts that do not rise
     J.slot = (first + part) * P.kv_heads + kvh;
     if (threadIdx.x == 0)
       write_note(P, J.slot, J.a, J.tile * (J.a.narrow ? 32 : 128), kvh, part == 0 ? sp.parts : 0, J.slot,
