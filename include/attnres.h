@@ -593,14 +593,14 @@ int attnres_embedding_bwd(const void* ids, int index_dtype, int64_t num_ids, con
  * pages and adds new_tokens[s].  Free pages are free_pages[0 .. free_count[0] - 1],
  * taken from the end: a sequence gets the pages it needs where the needs of all
  * sequences up to it are at most free_count, and else is refused, as is one whose tokens do
- * not fit its row of the table or the call's `tokens`, or whose lengths are negative or
- * over 2^30.  Writes the new pages into block_table, and
+ * not fit its row of the table, or end behind the call's `tokens` (as all behind it do), or
+ * whose lengths are negative or over 2^30.  Writes the new pages into block_table, and
  *   slots (tokens,)      each token's slot; -1 for padding and refused sequences
  *   positions (tokens,)  its place in its sequence; 0 for padding
  *   q_starts (seqs + 1,) running sums of new_tokens, at most `tokens`
  *   kv_lens (seqs,)      held + new_tokens, 0 for refused sequences
  *   free_count_out (1,)  pages that stay free
- * all int32.  free_count_out is not free_count.  held_dtype, new_dtype: ATTNRES_INDEX_*.
+ * all int32.  No result shares memory with an input.  held_dtype, new_dtype: ATTNRES_INDEX_*.
  */
 int attnres_paged_slots(void* block_table, int64_t table_ld, int seqs, int table_width, const void* held,
                         int held_dtype, const void* new_tokens, int new_dtype, const void* free_pages, int free_len,
@@ -611,7 +611,8 @@ int attnres_paged_slots(void* block_table, int64_t table_ld, int seqs, int table
  * Gives pages back: sequence s, which held held[s] tokens, keeps the first kept[s]
  * (taken into [0, held]), and the pages behind them are appended to free_pages
  * (free_len entries; what does not fit is dropped), sequence by sequence, a
- * sequence's last page first.  Their entries in the table stay, unused.
+ * sequence's last page first.  Their entries in the table stay, unused.  free_count_out is not
+ * free_count.
  */
 int attnres_paged_release(const void* block_table, int64_t table_ld, int seqs, int table_width, const void* held,
                           int held_dtype, const void* kept, int kept_dtype, void* free_pages, int free_len,
@@ -620,7 +621,7 @@ int attnres_paged_release(const void* block_table, int64_t table_ld, int seqs, i
 /*
  * Writes new keys and values (tokens, kv_heads, head_dim), element strides (token, head),
  * into their slots ((tokens,) slots_dtype, no slot twice).  A slot outside the cache
- * (-1) is skipped.  dtype bf16 or fp32 of all; head_dim a multiple of 8 up to 128; 16-byte
+ * (-1) is skipped.  No stride of a cache is 0 where it has more than one.  dtype bf16 or fp32 of all; head_dim a multiple of 8 up to 128; 16-byte
  * aligned pointers and strides.
  */
 int attnres_paged_write(const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,

@@ -128,7 +128,8 @@ int paged_plan(int64_t tokens, int seqs, int heads, int kv_heads, int head_dim, 
     p->target = (int)at_once;
     // tiles: every sequence may end inside one; the rows behind the last sequence are one more
     const int64_t tiles = rows / 128 + seqs + 1, share = (p->target + kv_heads - 1) / kv_heads;
-    // a split tile's parts are under twice its blocks over a part's most, and all those blocks at most the target's share
+    // a split tile's parts are under twice its blocks over a part's most, and all those blocks at most the target's
+    // share
     p->slots = p->split ? (2 * share + 8) * kv_heads : 0;
     p->grid = (tiles + (p->split ? share + 8 : 0)) * kv_heads;
     p->notes = p->slots;
@@ -291,6 +292,9 @@ int attnres_paged_write(const void* k, const int64_t* k_strides, const void* v, 
       (rc = take_cache("paged_write: v_cache", v_cache, v_cache_strides, pages, kv_heads, page_size, es, &P.sv)) !=
           ATTNRES_OK)
     return rc;
+  for (const lm_strides* c : {&P.sk, &P.sv})
+    if ((pages > 1 && c->b == 0) || (kv_heads > 1 && c->h == 0) || c->t == 0)
+      return fail(ATTNRES_ERR_ARG, "paged_write: rows of the cache lie on one another (a stride is 0)");
   for (int64_t* st : {&P.k_t, &P.k_h, &P.v_t, &P.v_h, &P.sk.b, &P.sk.h, &P.sk.t, &P.sv.b, &P.sv.h, &P.sv.t}) *st *= es;
   P.k = k;
   P.v = v;

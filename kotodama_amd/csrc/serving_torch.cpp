@@ -9,8 +9,8 @@ namespace {
 
 // Whole numbers on the tensors' device, one contiguous dimension of n.
 bool lengths(const Tensor& t, const Tensor& ref, int64_t n) {
-  return dense(t) && (t.scalar_type() == at::kInt || t.scalar_type() == at::kLong) && t.get_device() == ref.get_device() &&
-         t.dim() == 1 && t.size(0) == n && t.is_contiguous();
+  return dense(t) && (t.scalar_type() == at::kInt || t.scalar_type() == at::kLong) &&
+         t.get_device() == ref.get_device() && t.dim() == 1 && t.size(0) == n && t.is_contiguous();
 }
 int index_code(const Tensor& t) {
   return t.defined() && t.scalar_type() == at::kLong ? ATTNRES_INDEX_I64 : ATTNRES_INDEX_I32;
@@ -215,6 +215,7 @@ PyObject* py_verify_drafts(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return none();
   for (const Tensor* t : {&logits, &uniforms, &draft})
     if (!no_tangent(*t)) return none();
+  if (temperature != 0 && !(temperature >= 1e-6 && temperature < 1e38)) return none();  // before it is rounded to fp32
   auto rows_ok = [](const Tensor& t) {
     return dense(t) && dtype_ok(t.scalar_type()) && t.dim() == 2 && t.size(1) > 0 && t.size(1) <= INT32_MAX &&
            (t.stride(1) == 1 || t.size(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1));

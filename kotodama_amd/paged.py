@@ -162,8 +162,8 @@ def paged_slots(block_table: Tensor, held: Tensor, new: Tensor, free_pages: Tens
     written into it.  They come from the end of ``free_pages[:free_count]``, in the
     sequences' order: a sequence gets all it needs where the needs of the
     sequences up to it are at most ``free_count`` pages, and is refused
-    otherwise, as is one whose tokens do not fit its row of the table or the
-    ``num_tokens`` of the packed batch, or whose lengths are negative or over 2^30.  ``num_tokens`` (a
+    otherwise, as is one whose tokens do not fit its row of the table, or end behind the
+    ``num_tokens`` of the packed batch (as all behind it do), or whose lengths are negative or over 2^30.  ``num_tokens`` (a
     number on the host) may be more than the sum of ``new``: the rows behind
     are padding.  ``held`` and ``new`` are (B,) whole numbers on the device,
     ``page_size`` a power of two from 16 to 65536.
@@ -254,13 +254,15 @@ def _check_cache(op: str, k_cache: Tensor, v_cache: Tensor) -> None:
     _check_sizes(op, k_cache)
 
 
-def _check_cache_memory(op: str, k_cache: Tensor, v_cache: Tensor) -> None:
+def _check_cache_memory(op: str, k_cache: Tensor, v_cache: Tensor, written: bool = False) -> None:
     # a cache is written in place and read by its pages: not copied
     for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
         if t.numel() and not _aligned(t):
             raise ValueError(f"{op}: {name} must lie in 16-byte pieces, got strides {t.stride()}")
         if t.numel() and max(t.stride(2) * t.shape[2], t.stride(0)) * t.element_size() >= 1 << 31:
             raise ValueError(f"{op}: {name}: a head's rows of a page span 2^31 bytes, or its pages lie so far apart")
+        if written and t.numel() and any(t.stride(i) == 0 for i in range(3) if t.shape[i] > 1):
+            raise ValueError(f"{op}: rows of {name} lie on one another, got strides {t.stride()}")
 
 
 def _check_write(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, slots: Tensor) -> None:
@@ -280,7 +282,7 @@ def _cache_strides(t: Tensor):
 def _paged_write_impl(k, v, k_cache, v_cache, slots) -> None:
     device = _require_device(k, v, k_cache, v_cache, slots)
     _check_write(k, v, k_cache, v_cache, slots)
-    _check_cache_memory("paged_write", k_cache, v_cache)
+    _check_cache_memory("paged_write", k_cache, v_cache, written=True)
     k, v = _pieces(k), _pieces(v)
     slots, code = _lengths(slots)
     n, hk, d = k.shape

@@ -162,7 +162,8 @@ def _caches(g, pages, hk, page, d, dtype, layout="pages"):
 
 @pytest.mark.parametrize("dtype", [BF, FP], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("layout", ["pages", "tokens", "apart"])
-@pytest.mark.parametrize("n,hk,page,d", [(0, 1, 16, 8), (1, 1, 16, 8), (7, 3, 32, 72), (301, 8, 64, 128), (3000, 2, 16, 64)])
+@pytest.mark.parametrize("n,hk,page,d", [(0, 1, 16, 8), (1, 1, 16, 8), (7, 3, 32, 72), (301, 8, 64, 128),
+                                         (3000, 2, 16, 64)])
 def test_write(n, hk, page, d, layout, dtype):
     g = _gen(n + d)
     pages = n // page + 3
@@ -199,6 +200,18 @@ def test_write_of_unaligned_rows():
     slots = torch.arange(20, 29, device=DEV)
     kotodama_amd.paged_write(k, v, kc, vc, slots)
     assert torch.equal(kc[1, :, 4:13], k.transpose(0, 1)) and torch.equal(vc[1, :, 4:13], v.transpose(0, 1))
+
+
+def test_write_refuses_caches_whose_rows_lie_on_one_another():
+    x = torch.zeros(5, 2, 64, dtype=BF, device=DEV)
+    cache = torch.zeros(3, 2, 16, 64, dtype=BF, device=DEV)
+    for over in (cache[:1].expand(3, -1, -1, -1), cache[:, :1].expand(-1, 2, -1, -1), cache[:, :, :1].expand(-1, -1, 16, -1)):
+        for kc, vc in ((over, cache), (cache, over)):
+            with pytest.raises(ValueError, match="on one another"):
+                kotodama_amd.paged_write(x, x, kc, vc, torch.arange(5, device=DEV))
+    one = cache[:1].as_strided((1, 2, 16, 64), (0, 1024, 64, 1))  # one page: no other lies on it
+    kotodama_amd.paged_write(x + 1, x + 2, one, cache[1:2], torch.arange(5, device=DEV))
+    assert (cache[0, :, :5] == 1).all() and (cache[1, :, :5] == 2).all()
 
 
 # ------------------------------------------------------------- attention --
@@ -280,6 +293,27 @@ def test_single_tokens_over_a_split_cache(dtype, lens, h, hk, d):
 ])
 def test_many_rows(dtype, new, lens, h, hk, page, d, pad):
     _attention(sum(new), new, lens, h, hk, page, d, dtype, pad)
+
+
+@DTYPES
+def test_many_rows_of_many_sequences(dtype):
+    # more sequences than a workgroup's threads, the long ones in the second stretch of them, and split
+    new = [1] * 280 + [2100] + [3] * 40
+    lens = [1 + 7 * i for i in range(280)] + [6000] + [3 + 100 * i for i in range(40)]
+    _attention(17, new, lens, 32, 8, 64, 64, dtype, 5)
+
+
+def test_starts_that_fall():
+    # rows named many times over: whatever they then hold, nothing leads out of the call
+    for n, h, hk in ((4, 4, 2), (2100, 32, 8)):
+        lens = [700 + i for i in range(40)] + [700] * 260
+        q, kc, vc, table, kv_lens, _ = _batch(19, [0] * 300, lens, h, hk, 64, 64, BF, pad=n + 9)
+        print(f"paged_attention, falling starts: {n} tokens", flush=True)
+        starts = [0] + [n, 0] * 150
+        out = kotodama_amd.paged_attention(q, kc, vc, table, kv_lens, _ints(starts))
+        assert out[0].isfinite().all()
+        want = kotodama_amd.paged_attention(q, kc, vc, table, kv_lens, _ints([0] * 301))
+        assert not want.any()  # the next call finds nothing of it
 
 
 @DTYPES
@@ -455,6 +489,14 @@ def test_verify_at_the_edges():
     _verify(none, ids, starts, u, q, 0.0)
 
 
+def test_verify_refuses_temperatures_before_rounding_them():
+    logits, ids, starts, u, probs = _drafts(_gen(23), [3, 2], 50)
+    for t in (1e-300, 1e-7, 9e-7, -1e-300, 2e38, 1e300, math.inf, math.nan):
+        with pytest.raises(ValueError, match="temperature"):
+            kotodama_amd.verify_drafts(logits, ids, _ints(starts), u, probs, t)
+    _verify(logits, ids, starts, u, probs, 2.0**-19)
+
+
 def test_verify_takes_the_lowest_of_equal_logits():
     g = _gen(5)
     logits = torch.randint(0, 3, (6, 9000), generator=g, device=DEV).to(BF)
@@ -620,7 +662,8 @@ def test_ops_are_registered_soundly(op):
         "slots": (paged.paged_slots_op, (table, _ints([37, 68]), _ints([3, 2]), free, count, 16, 5)),
         "release": (paged.paged_release_op, (table.clamp(min=0), lens, _ints([3, 2]), free, count, 16)),
         "write": (paged.paged_write_op, (q[:, :2], q[:, 2:], kc, vc, torch.arange(5, device=DEV))),
-        "attention": (paged.paged_attention_op, (q, kc.nan_to_num(), vc.nan_to_num(), table, lens, _ints(starts), 0.125)),
+        "attention": (paged.paged_attention_op, (q, kc.nan_to_num(), vc.nan_to_num(), table, lens, _ints(starts),
+                                                 0.125)),
         "verify": (paged.verify_drafts_op, (logits, ids, _ints(vs), u, probs, 1.0)),
     }[op]
     torch.library.opcheck(fn, args, test_utils=("test_schema", "test_faketensor"))

@@ -155,7 +155,7 @@ def test_derivatives_are_refused():
         with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU path"):
             call(leaf, logits)
         with forward_ad.dual_level(), torch.no_grad(), pytest.raises(NotImplementedError, match="forward"):
-            call(forward_ad.make_dual(leaf.detach(), leaf.detach()), forward_ad.make_dual(logits.detach(), logits.detach()))
+            call(*(forward_ad.make_dual(t.detach(), t.detach()) for t in (leaf, logits)))
 
 
 def _st(*v):
@@ -197,7 +197,8 @@ def test_write_abi_refusals():
     assert write(n=0) == _capi.OK  # nothing to do: returns before any HIP call
     assert write(pages=0) == _capi.OK
     for kw in (dict(k=None), dict(n=-1), dict(hk=0), dict(dt=7), dict(kc=None), dict(pages=-1), dict(slots=None),
-               dict(sd=5), dict(cst=(2048, -1024, 64))):
+               dict(sd=5), dict(cst=(2048, -1024, 64)), dict(cst=(0, 1024, 64)), dict(cst=(2048, 0, 64)),
+               dict(cst=(2048, 1024, 0))):
         assert write(**kw) == _capi.ERR_ARG, kw
     for kw in (dict(d=4), dict(d=68), dict(d=136), dict(page=8), dict(page=48), dict(cst=(2048, 1024, 1 << 28)),
                dict(hk=(1 << 14) + 1), dict(n=1 << 31)):
