@@ -1,7 +1,7 @@
 /*
- * Kernel-argument blocks of the language-model operators (lm_kernels.hip,
- * attention_kernels.hip, paged_attention_kernels.hip, serving_kernels.hip), shared by the gfx950 code objects and the host
- * launcher (lm_capi.cpp), as attnres_params.h is for the routing kernels.
+ * Kernel-argument blocks of the language-model operators (lm_kernels.hip, attention_kernels.hip,
+ * paged_attention_kernels.hip, serving_kernels.hip), shared by the gfx950 code objects and the
+ * host launchers (lm_capi.cpp, serving_capi.cpp), as attnres_params.h is for the routing kernels.
  *
  * Plain C types only: included by g++ (host) and by hipcc (device) alike.
  */
@@ -173,6 +173,7 @@ typedef struct lm_paged_params {
   uint32_t group_mul;
   int32_t group_shift;
   int32_t wide;          /* many rows: sequences of over 32 in tiles of 128 */
+  int32_t turn;          /* many rows: a head's parts from this one on go the shortest first; 0: none */
   int32_t target;        /* workgroups (few rows: of a key head) to deal the key blocks out to */
   int32_t slots;         /* parts of tiles that the workspace holds */
   int32_t part_rows;     /* rows of one */

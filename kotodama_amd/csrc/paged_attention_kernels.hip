@@ -648,7 +648,10 @@ __device__ __forceinline__ void paged_tiles(const lm_paged_params& P, LDS_ARRAYS
   const Split sp(J.a, most);
   const int i = uniform(w - parts - (lo > 0 ? S.upto[lo - 1][0] : 0));
   const int rank = i / sp.parts, part = i - rank * sp.parts;
-  J.tile = uniform(J.a.tiles - 1 - rank);  // the longest first
+  // The longest first; where all tiles run at once, those that share a CU with them the shortest first (prompts from
+  // their start: 4 of 2048, 8/4 heads of 128, 61 us, all longest first 70; one of 8192, 190 and 208).
+  const int early = P.turn > 0 && sp.parts == 1 ? P.turn - (w - i) : J.a.tiles;  // of this sequence
+  J.tile = uniform(rank < early || early >= J.a.tiles ? J.a.tiles - 1 - rank : rank - (early > 0 ? early : 0));
   J.t0 = uniform(part * sp.per);
   J.t1 = uniform(J.t0 + sp.per < sp.n ? J.t0 + sp.per : sp.n);
   J.slot = -1;
@@ -678,8 +681,8 @@ __device__ __forceinline__ void paged_join(const lm_paged_params& P, f32x4* red)
   if (N.parts < 2) return;
   // starts that do not rise can leave a note unwritten: what leads out of the call is none
   const int64_t slots = (int64_t)P.slots * P.kv_heads;
-  if (N.first < 0 || N.first >= slots || N.next < 0 || N.step < 0 || N.next + (N.parts - 2) * (int64_t)N.step >= slots ||
-      N.token < 0 || N.row0 < 0 || N.head < 0 || N.head >= P.kv_heads ||
+  if (N.first < 0 || N.first >= slots || N.next < 0 || N.step < 0 ||
+      N.next + (N.parts - 2) * (int64_t)N.step >= slots || N.token < 0 || N.row0 < 0 || N.head < 0 || N.head >= P.kv_heads ||
       (int64_t)N.token * P.group + N.rows > (int64_t)P.tokens * P.group)
     return;
   const int lane = threadIdx.x & 31, g = threadIdx.x >> 5, d = 4 * lane;

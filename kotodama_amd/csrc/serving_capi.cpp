@@ -107,7 +107,7 @@ int check_rows(const char* op, int64_t tokens, int kv_heads, int head_dim, int d
 // What the launches and the workspace of a call go by.
 struct PagedPlan {
   bool wide = false, split = false;
-  int target = 0, part_rows = 0;
+  int target = 0, part_rows = 0, turn = 0;
   int64_t slots = 0, grid = 0, notes = 0;  // of all key heads
   int64_t at_ml = 0, at_notes = 0, bytes = 0;
 };
@@ -126,6 +126,8 @@ int paged_plan(int64_t tokens, int seqs, int heads, int kv_heads, int head_dim, 
   p->split = capacity > kWholeKeys;
   if (p->wide) {
     p->target = (int)at_once;
+    // where all tiles run at once, workgroups as many apart as there are CUs share one
+    if (rows / 128 * kv_heads <= at_once && at_once > cus) p->turn = cus / kv_heads;
     // tiles: every sequence may end inside one; the rows behind the last sequence are one more
     const int64_t tiles = rows / 128 + seqs + 1, share = (p->target + kv_heads - 1) / kv_heads;
     // a split tile's parts are under twice its blocks over a part's most, and all those blocks at most the target's
@@ -391,6 +393,7 @@ int attnres_paged_attention_fwd(const void* q, const int64_t* q_strides, const v
   P.group_mul =
       (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << P.group_shift) - (uint64_t)P.group)) / (uint64_t)P.group + 1);
   P.wide = plan.wide;
+  P.turn = plan.turn;
   P.target = plan.target;
   P.slots = (int32_t)(plan.slots / kv_heads);
   P.part_rows = plan.part_rows;

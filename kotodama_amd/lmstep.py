@@ -412,8 +412,8 @@ class LanguageModel(nn.Module):
         """One step of speculative sampling for every sequence: its last token and drafts behind it (``new[b]``
         tokens in all; 1: no draft; 0: sits out) in, the tokens behind them out.
 
-        Returns :func:`paged.verify_drafts`'s tokens (N,) and counts (B,); the cache keeps what stands.  A refused sequence
-        gets no token and keeps what it had."""
+        Returns :func:`paged.verify_drafts`'s tokens (N,) and counts (B,); the cache keeps what stands.  A refused
+        sequence gets no token and keeps what it had."""
         held = cache.lens.clone()
         step = cache.extend(new, input_ids.shape[0])
         logits = self.logits_paged(input_ids, cache, step)

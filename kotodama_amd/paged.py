@@ -163,8 +163,8 @@ def paged_slots(block_table: Tensor, held: Tensor, new: Tensor, free_pages: Tens
     sequences' order: a sequence gets all it needs where the needs of the
     sequences up to it are at most ``free_count`` pages, and is refused
     otherwise, as is one whose tokens do not fit its row of the table, or end behind the
-    ``num_tokens`` of the packed batch (as all behind it do), or whose lengths are negative or over 2^30.  ``num_tokens`` (a
-    number on the host) may be more than the sum of ``new``: the rows behind
+    ``num_tokens`` of the packed batch (as all behind it do), or whose lengths are
+    negative or over 2^30.  ``num_tokens`` (a number on the host) may be more than the sum of ``new``: the rows behind
     are padding.  ``held`` and ``new`` are (B,) whole numbers on the device,
     ``page_size`` a power of two from 16 to 65536.
 

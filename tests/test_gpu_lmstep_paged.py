@@ -117,3 +117,36 @@ def test_a_refused_sequence_keeps_what_it_has():
     cache.keep(_ints([0, 16]))
     tokens, counts = model.step_paged(ids[:3], _ints([1, 2]), cache, u[:3])
     assert counts.tolist()[0] == 1 and counts.tolist()[1] >= 1
+
+
+def test_a_captured_step_serves_like_the_eager_one():
+    c, model, g = _model(seq=64)
+    caches = [model.new_cache(pages=14, sequences=3, page_size=16) for _ in range(2)]
+    prompt = torch.randint(0, 1000, (20,), generator=g, device=DEV)
+    for cache in caches:
+        model.logits_paged(prompt, cache, cache.extend(_ints([9, 4, 7]), 20))
+    n = 8
+    ids, new = torch.zeros(n, dtype=torch.int64, device=DEV), _ints([0, 0, 0])
+    u, probs = torch.zeros((n, 2), device=DEV), torch.full((n, 1000), 1e-3, device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        model.step_paged(ids, new, caches[0], u, probs)  # nothing new: loads what it calls
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = model.step_paged(ids, new, caches[0], u, probs)
+    for i, some in enumerate(([1, 3, 2], [4, 0, 4], [1, 1, 1], [0, 0, 0], [2, 5, 1], [3, 4, 3])):  # the last: over n
+        ids.copy_(torch.randint(0, 1000, (n,), generator=g, device=DEV))
+        new.copy_(_ints(some))
+        u.copy_(torch.rand((n, 2), generator=g, device=DEV))
+        u[:, 0].mul_(0.01)  # so that drafts stay
+        graph.replay()
+        torch.cuda.synchronize()
+        want = model.step_paged(ids, new, caches[1], u, probs)
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), i
+        assert [m > 0 for m in got[1].tolist()] == [k > 0 and (i < 5 or b < 2) for b, k in enumerate(some)]
+        for name in ("lens", "free_count", "free_pages", "block_table"):
+            assert torch.equal(getattr(caches[0], name), getattr(caches[1], name)), (i, name)

@@ -205,7 +205,8 @@ def test_write_of_unaligned_rows():
 def test_write_refuses_caches_whose_rows_lie_on_one_another():
     x = torch.zeros(5, 2, 64, dtype=BF, device=DEV)
     cache = torch.zeros(3, 2, 16, 64, dtype=BF, device=DEV)
-    for over in (cache[:1].expand(3, -1, -1, -1), cache[:, :1].expand(-1, 2, -1, -1), cache[:, :, :1].expand(-1, -1, 16, -1)):
+    for over in (cache[:1].expand(3, -1, -1, -1), cache[:, :1].expand(-1, 2, -1, -1),
+                 cache[:, :, :1].expand(-1, -1, 16, -1)):
         for kc, vc in ((over, cache), (cache, over)):
             with pytest.raises(ValueError, match="on one another"):
                 kotodama_amd.paged_write(x, x, kc, vc, torch.arange(5, device=DEV))
@@ -224,7 +225,8 @@ def _batch(seed, new, lens, h, hk, page, d, dtype, pad=0, layout="pages", index=
     pages = sum(-(-n // page) for n in lens) + extra
     kc, vc = _caches(g, pages, hk, page, d, dtype, layout)
     order = torch.randperm(pages, generator=g, device=DEV).tolist()
-    table = torch.full((len(lens), m), -(2**31), dtype=torch.int32, device=DEV)  # entries behind the length are not read
+    # entries behind the length are not read
+    table = torch.full((len(lens), m), -(2**31), dtype=torch.int32, device=DEV)
     used = torch.zeros(pages, page, dtype=torch.bool, device=DEV)
     for b, n in enumerate(lens):
         mine = [order.pop() for _ in range(-(-n // page))]
@@ -290,6 +292,7 @@ def test_single_tokens_over_a_split_cache(dtype, lens, h, hk, d):
     ([2050, 1, 1, 9], [2050, 700, 1, 3000], 32, 8, 64, 128, 3),  # chunks of 128 rows a tile beside single tokens
     ([700, 0, 1400, 8], [900, 0, 1400, 8], 16, 16, 16, 64, 200),
     ([3000], [9000], 8, 8, 32, 72, 0),  # few tiles, long: split
+    ([1300, 1000, 30], [1300, 1000, 30], 32, 8, 64, 64, 0),  # all tiles at once, none split
 ])
 def test_many_rows(dtype, new, lens, h, hk, page, d, pad):
     _attention(sum(new), new, lens, h, hk, page, d, dtype, pad)
@@ -626,6 +629,63 @@ def test_another_stream():
     torch.cuda.synchronize()
     for o, t, c in got:
         assert torch.equal(o, want) and torch.equal(t, tokens) and torch.equal(c, counts)
+
+
+def test_two_graphs_at_once():
+    # split attention and verification, each graph with a workspace of its own, replayed on two streams together
+    q, kc, vc, table, lens, starts = _batch(73, [2] * 30, [2000 + 50 * i for i in range(30)], 8, 2, 16, 64, BF)
+    g = _gen(74)
+    logits, ids, vs, u, probs = _drafts(g, [5] * 30, 9001)
+    s, v = _ints(starts), _ints(vs)
+    sides = [(q.clone(), logits.clone(), u.clone()) for _ in range(2)]
+
+    def call(x):
+        return (*kotodama_amd.paged_attention(x[0], kc, vc, table, lens, s, want_lse=True),
+                *kotodama_amd.verify_drafts(x[1], ids, v, x[2], probs))
+
+    want = call(sides[0])
+    torch.cuda.synchronize()
+    graphs, results, streams = [], [], [torch.cuda.Stream() for _ in range(2)]
+    for x in sides:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            results.append(call(x))
+        graphs.append(graph)
+    for i in range(4):
+        for x in sides:
+            for t in x:
+                t.copy_(torch.rand(t.shape, generator=g, device=DEV) if t.shape[-1] == 2 else
+                        _randn(g, *t.shape, dtype=t.dtype))
+        want = [call(x) for x in sides]
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(results, want):
+            assert all(torch.equal(x, y) for x, y in zip(a, b)), i
+
+
+def test_under_inference_mode():
+    with torch.inference_mode():
+        cache = kotodama_amd.PagedCache(1, 9, 16, 2, 64, 2, 64, BF, DEV)
+        g = _gen(75)
+        q, k, v = (_randn(g, 40, h, 64) for h in (4, 2, 2))
+        for native in (True, False):
+            step = cache.extend(_ints([20, 17]), 40)
+            layer = cache.layers(step)[0]
+            if native:
+                kotodama_amd.paged_write(k, v, layer.k, layer.v, step.slots)
+                out = kotodama_amd.paged_attention(q, layer.k, layer.v, cache.block_table, step.kv_lens, step.q_starts)
+            else:
+                paged._paged_write_impl(k, v, layer.k, layer.v, step.slots)
+                again, _ = paged._paged_attention_impl(q, layer.k, layer.v, cache.block_table, step.kv_lens,
+                                                       step.q_starts, 1 / 8)
+                assert torch.equal(out, again)
+            assert step.kv_lens.tolist() == [20, 17]
+            cache.keep(_ints([0, 0]))
+    want, bound = PO.attention(q, layer.k, layer.v, cache.block_table, [20, 17], [0, 20, 37])[0]
+    assert ((out.double() - want).abs() <= bound).all()
 
 
 def test_compiled_calls():

@@ -191,8 +191,8 @@ def test_slots_abi_refusals():
 def test_write_abi_refusals():
     def write(k=FAKE, st=(128, 64), n=5, hk=2, d=64, dt=BF, kc=FAKE, cst=(2048, 1024, 64), pages=3, page=16,
               slots=FAKE, sd=0):
-        return _capi.lib().attnres_paged_write(k, _st(*st), FAKE, _st(*st), n, hk, d, dt, kc, _st(*cst), FAKE, _st(*cst),
-                                               pages, page, slots, sd, None)
+        return _capi.lib().attnres_paged_write(k, _st(*st), FAKE, _st(*st), n, hk, d, dt, kc, _st(*cst), FAKE,
+                                               _st(*cst), pages, page, slots, sd, None)
 
     assert write(n=0) == _capi.OK  # nothing to do: returns before any HIP call
     assert write(pages=0) == _capi.OK
@@ -212,8 +212,8 @@ def test_attention_abi_refusals():
     def fwd(q=FAKE, qst=(256, 64), kc=FAKE, cst=(2048, 1024, 64), n=5, seqs=2, h=4, hk=2, d=64, dt=BF, pages=3, page=16,
             table=FAKE, ld=4, width=4, lens=FAKE, ld_=0, starts=FAKE, scale=0.1, out=FAKE, lse=None):
         return _capi.lib().attnres_paged_attention_fwd(
-            q, _st(*qst), kc, _st(*cst), FAKE, _st(*cst), n, seqs, h, hk, d, dt, pages, page, table, ld, width, lens, ld_,
-            starts, 0, scale, out, _st(*qst), lse, None, 0, None)
+            q, _st(*qst), kc, _st(*cst), FAKE, _st(*cst), n, seqs, h, hk, d, dt, pages, page, table, ld, width, lens,
+            ld_, starts, 0, scale, out, _st(*qst), lse, None, 0, None)
 
     assert fwd(n=0) == _capi.OK
     for kw in (dict(n=-1), dict(seqs=-1), dict(h=3), dict(hk=0), dict(h=0), dict(dt=9), dict(width=-1), dict(q=None),
@@ -233,8 +233,8 @@ def test_attention_abi_refusals():
 def test_verify_abi_refusals():
     def verify(logits=FAKE, ld=9, ldt=BF, q=None, qdt=BF, rows=5, vocab=9, ids=FAKE, idt=1, starts=FAKE, seqs=2, u=FAKE,
                t=1.0, out=FAKE, counts=FAKE, ws=FAKE, nbytes=1 << 20):
-        return _capi.lib().attnres_verify_drafts(logits, ld, ldt, q, ld, qdt, rows, vocab, ids, idt, starts, 0, seqs, u, t,
-                                                 out, counts, ws, nbytes, None)
+        return _capi.lib().attnres_verify_drafts(logits, ld, ldt, q, ld, qdt, rows, vocab, ids, idt, starts, 0, seqs, u,
+                                                 t, out, counts, ws, nbytes, None)
 
     assert verify(rows=0, seqs=0) == _capi.OK
     for kw in (dict(logits=None), dict(ld=8), dict(ldt=4), dict(q=FAKE, qdt=4), dict(rows=-1), dict(vocab=0),
