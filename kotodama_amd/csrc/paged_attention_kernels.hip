@@ -22,8 +22,8 @@
 //
 // Calls with rows enough to fill the card 128 at a time (paged_tiles): the rows of
 // longer sequences are taken so, each wave 32 of them over all keys, a workgroup
-// a tile, the longest of a sequence first.  Tiles of more keys than their share (all blocks
-// over `target` workgroups) are split, narrow ones beside them too.
+// a tile, the longest of a sequence first.  Where they are too few or too unequal for the card, long tiles are
+// split, narrow ones beside them too (part_blocks).
 //
 // What a workgroup has of a tile that others share goes to the workspace, with a
 // note of its parts, and paged_join adds them in order, so that
@@ -107,6 +107,8 @@ struct Piece {
 
 struct Shared {
   float sum[LM_ATTN_WAVES];
+  float most[LM_ATTN_WAVES];
+  float cost[8];
   int scan[LM_ATTN_WAVES][2];
   int upto[kThreads][2];
   Share share;
@@ -143,17 +145,27 @@ __device__ __forceinline__ void scan_all(int (&v)[N], Shared& S) {
   __syncthreads();
 }
 
-// Sum over the workgroup, to every thread, in a fixed order.
-__device__ __forceinline__ float sum_all(float v, Shared& S) {
+__device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) S.sum[threadIdx.x >> 6] = v;
-  __syncthreads();
-  float t = 0.f;
+  return v;
+}
+// Sum of `v` and largest of `t` over the workgroup, to every thread, in a fixed order.
+__device__ __forceinline__ void sum_and_most(float& v, float& t, Shared& S) {
+  v = wave_sum(v);
 #pragma unroll
-  for (int i = 0; i < LM_ATTN_WAVES; ++i) t += S.sum[i];
-  return t;
+  for (int m = 1; m < 64; m <<= 1) t = fmaxf(t, __shfl_xor(t, m));
+  if ((threadIdx.x & 63) == 0) {
+    S.sum[threadIdx.x >> 6] = v;
+    S.most[threadIdx.x >> 6] = t;
+  }
+  __syncthreads();
+  v = t = 0.f;
+#pragma unroll
+  for (int i = 0; i < LM_ATTN_WAVES; ++i) {
+    v += S.sum[i];
+    t = fmaxf(t, S.most[i]);
+  }
 }
 
 // The thread whose inclusive sum is the first over `at`, which is under the last.
@@ -589,6 +601,60 @@ struct Split {
   }
 };
 
+// The most blocks of a part.  Tried are the longest tile's, halves, thirds .. sevenths of them, and an equal share
+// for `target` workgroups; of those whose parts the launch has room for (whole tiles always are) the one
+// whose last workgroup should end first: rounds of the longest part, or all work and a part
+// behind it; a workgroup that has its CU for itself takes 0.6 of the time.  A part costs some 8 blocks'
+// time to begin and end, the join as much.  Every workgroup comes to the same.  (With the equal share
+// alone, tiles a little fewer than workgroups were all cut in unequal halves: 1536 tokens behind 14848, 32/8 heads of 128,
+// 632 us where it takes 440; 3 prompts of 2048, 8/4 heads, 125 and 58.)
+constexpr int kCuts = 8;
+constexpr float kPartCost = 8.f, kAlone = 0.6f;
+template <bool TWO>  // workgroups of a CU
+__device__ __forceinline__ int part_blocks(const lm_paged_params& P, int all, Shared& S) {
+  float work = 0.f, top = 0.f;
+  for (int s = threadIdx.x; s < P.seqs; s += kThreads) {
+    const Share a = share_of(P, s);
+    const float n = a.tiles > 0 ? (float)blocks_of(a) : 0.f;
+    work += (float)a.tiles * n;
+    top = fmaxf(top, n);
+  }
+  sum_and_most(work, top, S);
+  const float target = (float)P.target, heads = (float)P.kv_heads, each = work * heads / target;
+  const int longest = uniform(top < 1.f ? 1 : top < 0x1p24f ? (int)top : (int)top + 4);  // (a float's rounding)
+  if (P.slots == 0 || each >= 8.f * top) return longest;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  auto cut = [&](int j) {
+    const float c = __builtin_ceilf(j + 1 < kCuts ? top / (float)(j + 1) : each);
+    return uniform(c < 1.f ? 1 : c < top ? (int)c : longest);
+  };
+#pragma unroll
+  for (int u = 0; u < kCuts / LM_ATTN_WAVES; ++u) {  // each wave its own
+    const int j = wave * (kCuts / LM_ATTN_WAVES) + u, most = cut(j);
+    float parts = 0.f, shared = 0.f;
+    for (int s = lane; s <= P.seqs; s += 64) {  // the rows behind the last too: whole tiles
+      const Share a = share_of(P, s);
+      const Split sp(a, most);
+      const float n = (float)a.tiles * (float)sp.parts;
+      parts += n;
+      shared += sp.parts > 1 ? n : 0.f;
+    }
+    parts = wave_sum(parts);
+    shared = wave_sum(shared);
+    const float n = parts * heads, part = (float)most + kPartCost;
+    float cost = fminf(__builtin_ceilf(n / target) * part, each + part);
+    if (TWO && 2.f * n <= target) cost = kAlone * part;
+    cost += shared > 0.f ? kPartCost : 0.f;
+    const bool room = shared == 0.f || (shared <= (float)P.slots && parts <= (float)all);
+    if (lane == 0) S.cost[j] = room ? cost : __builtin_inff();
+  }
+  __syncthreads();
+  int best = 0;
+#pragma unroll
+  for (int j = 1; j < kCuts; ++j) best = S.cost[j] < S.cost[best] ? j : best;
+  return cut(uniform(best));
+}
+
 template <typename T, int DP, int DC>
 __device__ __forceinline__ void paged_tiles(const lm_paged_params& P, LDS_ARRAYS, float* ml, int* flag, Shared& S) {
   // Workgroups go to the eight XCDs in turn, each with an L2 of its own: where the key heads
@@ -608,15 +674,7 @@ __device__ __forceinline__ void paged_tiles(const lm_paged_params& P, LDS_ARRAYS
     w = p;
   }
   if (threadIdx.x == 0) *flag = 0;
-  // the most blocks of a part: an equal share for `target` workgroups (a float's rounding moves
-  // it by a part in 2^24; every workgroup finds the same)
-  float work = 0.f;
-  for (int s = threadIdx.x; s < P.seqs; s += kThreads) {
-    const Share a = share_of(P, s);
-    work += (float)a.tiles * (float)blocks_of(a);
-  }
-  work = sum_all(work, S) * (float)P.kv_heads / (float)P.target;
-  const int most = uniform(work < 1.f ? 1 : work > 6e7f ? 1 << 26 : (int)__builtin_ceilf(work));
+  const int most = part_blocks<!(T::kBytes == 4 && DC > 64)>(P, all, S);
   // the sequence of part w, all sequences' parts one after another, and the slots in front of its
   int parts = 0, slots = 0, base = 0;
   bool found = false;

@@ -39,7 +39,10 @@ constexpr int kMaxSeqs = 1 << 20;
 // launch that joins parts 4 to 5 (one token over 512 keys, 32/8 heads of 128: 11.7 us whole, 8.2 + 4.2 in
 // parts; over 1024 keys 17.2 and 8.0 + 5.1).
 constexpr int64_t kWholeKeys = 512;
-constexpr int kWideWaves = 8;   // waves of 32 rows per CU that fill the card: chunks' rows are taken 128 at a time
+// Waves of 32 rows per CU from which rows are taken 128 at a time; twice as many where a CU has room for one
+// workgroup.  (bf16, heads of 128: 2 prompts of 2048, 8/4 heads, 54 us, 32 at a time 67; 1100 tokens, 32/8 heads,
+// 38 and 59; half as many rows: 55 and 34, 18 and 14.  fp32: 1100 behind 7092, 32/8 heads, 1770 and 1490.)
+constexpr int kWideWaves = 4;
 constexpr int kMaxVocab = 1 << 21;
 
 int index_size(int code) { return code == ATTNRES_INDEX_I64 ? 8 : 4; }
@@ -122,7 +125,7 @@ int paged_plan(int64_t tokens, int seqs, int heads, int kv_heads, int head_dim, 
   // up to 2048 keys, 8/4 heads of 128: 90 us, 97 with two rounds of them).  Heads of up to 64 in bf16 have room
   // for four, but shorter stretches cost more than they hide (64 sequences of up to 4096 keys: 39 us against 34).
   const int64_t at_once = (int64_t)cus * (head_dim > 64 && dtype == ATTNRES_DTYPE_F32 ? 1 : 2);
-  p->wide = rows / 32 * kv_heads >= (int64_t)cus * kWideWaves;
+  p->wide = rows / 32 * kv_heads >= (int64_t)cus * (at_once > cus ? kWideWaves : 2 * kWideWaves);
   p->split = capacity > kWholeKeys;
   if (p->wide) {
     p->target = (int)at_once;

@@ -292,7 +292,8 @@ def test_single_tokens_over_a_split_cache(dtype, lens, h, hk, d):
     ([2050, 1, 1, 9], [2050, 700, 1, 3000], 32, 8, 64, 128, 3),  # chunks of 128 rows a tile beside single tokens
     ([700, 0, 1400, 8], [900, 0, 1400, 8], 16, 16, 16, 64, 200),
     ([3000], [9000], 8, 8, 32, 72, 0),  # few tiles, long: split
-    ([1300, 1000, 30], [1300, 1000, 30], 32, 8, 64, 64, 0),  # all tiles at once, none split
+    ([1300, 700, 30], [1300, 700, 30], 32, 8, 64, 64, 0),  # all tiles at once, none split
+    ([1040], [16000], 32, 8, 64, 64, 0),  # halves
 ])
 def test_many_rows(dtype, new, lens, h, hk, page, d, pad):
     _attention(sum(new), new, lens, h, hk, page, d, dtype, pad)
