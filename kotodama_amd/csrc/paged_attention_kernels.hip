@@ -606,8 +606,8 @@ struct Split {
 // whose last workgroup should end first: rounds of the longest part, or all work and a part
 // behind it; a workgroup that has its CU for itself takes 0.6 of the time.  A part costs some 8 blocks'
 // time to begin and end, the join as much.  Every workgroup comes to the same.  (With the equal share
-// alone, tiles a little fewer than workgroups were all cut in unequal halves: 1536 tokens behind 14848, 32/8 heads of 128,
-// 632 us where it takes 440; 3 prompts of 2048, 8/4 heads, 125 and 58.)
+// alone, tiles a little fewer than workgroups were all cut in unequal halves: 1536 tokens behind
+// 14848, 32/8 heads of 128, 632 us where it takes 440; 3 prompts of 2048, 8/4 heads, 125 and 58.)
 constexpr int kCuts = 8;
 constexpr float kPartCost = 8.f, kAlone = 0.6f;
 template <bool TWO>  // workgroups of a CU
@@ -740,8 +740,8 @@ __device__ __forceinline__ void paged_join(const lm_paged_params& P, f32x4* red)
   // starts that do not rise can leave a note unwritten: what leads out of the call is none
   const int64_t slots = (int64_t)P.slots * P.kv_heads;
   if (N.first < 0 || N.first >= slots || N.next < 0 || N.step < 0 ||
-      N.next + (N.parts - 2) * (int64_t)N.step >= slots || N.token < 0 || N.row0 < 0 || N.head < 0 || N.head >= P.kv_heads ||
-      (int64_t)N.token * P.group + N.rows > (int64_t)P.tokens * P.group)
+      N.next + (N.parts - 2) * (int64_t)N.step >= slots || N.token < 0 || N.row0 < 0 || N.head < 0 ||
+      N.head >= P.kv_heads || (int64_t)N.token * P.group + N.rows > (int64_t)P.tokens * P.group)
     return;
   const int lane = threadIdx.x & 31, g = threadIdx.x >> 5, d = 4 * lane;
   const int pp = N.parts <= 2 ? 2 : N.parts <= 4 ? 4 : 8, each = 8 / pp;  // parts and rows side by side
