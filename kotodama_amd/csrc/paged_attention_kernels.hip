@@ -605,11 +605,12 @@ struct Split {
 // for `target` workgroups; of those whose parts the launch has room for (whole tiles always are) the one
 // whose last workgroup should end first: rounds of the longest part, or all work and a part
 // behind it; a workgroup that has its CU for itself takes 0.6 of the time.  A part costs some 8 blocks'
-// time to begin and end, the join as much.  Every workgroup comes to the same.  (With the equal share
-// alone, tiles a little fewer than workgroups were all cut in unequal halves: 1536 tokens behind
-// 14848, 32/8 heads of 128, 632 us where it takes 440; 3 prompts of 2048, 8/4 heads, 125 and 58.)
+// time to begin and end, the join as much and 24 where it reads `target` parts' sums (2 prompts of 2048,
+// 8/4 heads of 128: 55 us whole, 83 in halves; 1024 behind 15360, 32/8 heads: 309 in halves).  Every workgroup
+// comes to the same.  (With the equal share alone, tiles a little fewer than workgroups were all cut in unequal
+// halves: 1536 tokens behind 14848, 632 us where it takes 440; 3 prompts of 2048, 125 and 58.)
 constexpr int kCuts = 8;
-constexpr float kPartCost = 8.f, kAlone = 0.6f;
+constexpr float kPartCost = 8.f, kAlone = 0.6f, kJoinCost = 24.f;
 template <bool TWO>  // workgroups of a CU
 __device__ __forceinline__ int part_blocks(const lm_paged_params& P, int all, Shared& S) {
   float work = 0.f, top = 0.f;
@@ -644,7 +645,7 @@ __device__ __forceinline__ int part_blocks(const lm_paged_params& P, int all, Sh
     const float n = parts * heads, part = (float)most + kPartCost;
     float cost = fminf(__builtin_ceilf(n / target) * part, each + part);
     if (TWO && 2.f * n <= target) cost = kAlone * part;
-    cost += shared > 0.f ? kPartCost : 0.f;
+    cost += shared > 0.f ? kPartCost + kJoinCost * shared * heads / target : 0.f;
     const bool room = shared == 0.f || (shared <= (float)P.slots && parts <= (float)all);
     if (lane == 0) S.cost[j] = room ? cost : __builtin_inff();
   }
