@@ -36,6 +36,7 @@
 // the cache is read as page 0 and makes the rows that are worked on with it NaN.
 
 #include "attention_tiles.h"
+#include "paged_schedule.h"
 
 namespace {
 
@@ -53,14 +54,6 @@ __device__ __forceinline__ int taken(const void* p, int i, int is64, int most) {
   return hi < 0 ? 0 : hi > 0 || (uint32_t)lo > (uint32_t)most ? most : lo;
 }
 
-// One sequence's share of the call: its tokens, keys and tiles of rows.
-struct Share {
-  int first, count;  // new tokens
-  int kv_len;
-  int rows, tiles;
-  bool narrow;
-};
-
 // The sequences' sizes are taken into what the call has, so that no length
 // leads out of its tensors.  Behind the last sequence (s == seqs): the tokens that
 // belong to none, as a sequence without keys.
@@ -73,14 +66,9 @@ __device__ __forceinline__ Share share_of(const lm_paged_params& P, int s) {
     hi = taken(P.q_starts, in + 1, P.starts64, P.tokens);
   }
   hi = s < P.seqs ? hi : P.tokens;
-  a.first = lo;
-  a.count = hi > lo ? hi - lo : 0;
-  a.kv_len = 0;
-  if (P.seqs > 0) a.kv_len = taken(P.kv_lens, in, P.lens64, P.capacity);
-  a.kv_len = s < P.seqs ? a.kv_len : 0;
-  a.rows = a.count * P.group;
-  a.narrow = !P.wide || a.rows <= 32;
-  a.tiles = a.narrow ? (a.rows + 31) >> 5 : (a.rows + 127) >> 7;
+  int kv_len = 0;
+  if (P.seqs > 0) kv_len = taken(P.kv_lens, in, P.lens64, P.capacity);
+  a.set(lo, hi, s < P.seqs ? kv_len : 0, P.group, P.wide != 0);
   return a;
 }
 
@@ -587,30 +575,7 @@ __device__ __forceinline__ void paged_stream(const lm_paged_params& P, LDS_ARRAY
 
 // ------------------------------------------------------------ many rows --
 
-// A tile's work: blocks of 32 keys that a wave works on.
-__device__ __forceinline__ int blocks_of(const Share& a) {
-  return a.narrow ? (a.kv_len + 127) >> 7 : ((a.kv_len + 63) >> 6) * 2;
-}
-// Its parts of at most `most` such blocks, and the key blocks of one.
-struct Split {
-  int n, parts, per;
-  __device__ __forceinline__ Split(const Share& a, int most) {
-    per = a.narrow ? most : (most + 1) >> 1;
-    n = a.narrow ? (a.kv_len + 127) >> 7 : (a.kv_len + 63) >> 6;
-    parts = n <= per ? 1 : (n + per - 1) / per;
-  }
-};
-
-// The most blocks of a part.  Tried are the longest tile's, halves, thirds .. sevenths of them, and an equal share
-// for `target` workgroups; of those whose parts the launch has room for (whole tiles always are) the one
-// whose last workgroup should end first: rounds of the longest part, or all work and a part
-// behind it; a workgroup that has its CU for itself takes 0.6 of the time.  A part costs some 8 blocks'
-// time to begin and end, the join as much and 24 where it reads `target` parts' sums (2 prompts of 2048,
-// 8/4 heads of 128: 55 us whole, 83 in halves; 1024 behind 15360, 32/8 heads: 309 in halves).  Every workgroup
-// comes to the same.  (With the equal share alone, tiles a little fewer than workgroups were all cut in unequal
-// halves: 1536 tokens behind 14848, 632 us where it takes 440; 3 prompts of 2048, 125 and 58.)
-constexpr int kCuts = 8;
-constexpr float kPartCost = 8.f, kAlone = 0.6f, kJoinCost = 24.f;
+// The cut (Cuts) of the call's tiles.
 template <bool TWO>  // workgroups of a CU
 __device__ __forceinline__ int part_blocks(const lm_paged_params& P, int all, Shared& S) {
   float work = 0.f, top = 0.f;
@@ -621,17 +586,12 @@ __device__ __forceinline__ int part_blocks(const lm_paged_params& P, int all, Sh
     top = fmaxf(top, n);
   }
   sum_and_most(work, top, S);
-  const float target = (float)P.target, heads = (float)P.kv_heads, each = work * heads / target;
-  const int longest = uniform(top < 1.f ? 1 : top < 0x1p24f ? (int)top : (int)top + 4);  // (a float's rounding)
-  if (P.slots == 0 || each >= 8.f * top) return longest;
+  const Cuts C(work, top, P.target, P.kv_heads);
+  if (P.slots == 0 || C.many()) return uniform(C.longest);
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  auto cut = [&](int j) {
-    const float c = __builtin_ceilf(j + 1 < kCuts ? top / (float)(j + 1) : each);
-    return uniform(c < 1.f ? 1 : c < top ? (int)c : longest);
-  };
 #pragma unroll
   for (int u = 0; u < kCuts / LM_ATTN_WAVES; ++u) {  // each wave its own
-    const int j = wave * (kCuts / LM_ATTN_WAVES) + u, most = cut(j);
+    const int j = wave * (kCuts / LM_ATTN_WAVES) + u, most = uniform(C.most(j));
     float parts = 0.f, shared = 0.f;
     for (int s = lane; s <= P.seqs; s += 64) {  // the rows behind the last too: whole tiles
       const Share a = share_of(P, s);
@@ -642,18 +602,13 @@ __device__ __forceinline__ int part_blocks(const lm_paged_params& P, int all, Sh
     }
     parts = wave_sum(parts);
     shared = wave_sum(shared);
-    const float n = parts * heads, part = (float)most + kPartCost;
-    float cost = fminf(__builtin_ceilf(n / target) * part, each + part);
-    if (TWO && 2.f * n <= target) cost = kAlone * part;
-    cost += shared > 0.f ? kPartCost + kJoinCost * shared * heads / target : 0.f;
-    const bool room = shared == 0.f || (shared <= (float)P.slots && parts <= (float)all);
-    if (lane == 0) S.cost[j] = room ? cost : __builtin_inff();
+    if (lane == 0) S.cost[j] = C.cost(most, parts, shared, TWO, P.slots, all);
   }
   __syncthreads();
   int best = 0;
 #pragma unroll
   for (int j = 1; j < kCuts; ++j) best = S.cost[j] < S.cost[best] ? j : best;
-  return cut(uniform(best));
+  return uniform(C.most(best));
 }
 
 template <typename T, int DP, int DC>

@@ -13,6 +13,7 @@
 #include "attnres_internal.h"
 #include "lm_host.h"
 #include "lm_params.h"
+#include "paged_schedule.h"
 
 namespace {
 
@@ -35,14 +36,6 @@ constexpr int64_t kMaxTokens = (int64_t)1 << 30;  // of one sequence, and new on
 constexpr int kMaxPage = 1 << 16;                 // rows
 constexpr int kMaxGroup = 4096;                   // query heads per key head
 constexpr int kMaxSeqs = 1 << 20;
-// Keys that one workgroup takes of a tile without splitting it: a block of 128 costs it some 1.2 us, the
-// launch that joins parts 4 to 5 (one token over 512 keys, 32/8 heads of 128: 11.7 us whole, 8.2 + 4.2 in
-// parts; over 1024 keys 17.2 and 8.0 + 5.1).
-constexpr int64_t kWholeKeys = 512;
-// Waves of 32 rows per CU from which rows are taken 128 at a time; twice as many where a CU has room for one
-// workgroup.  (bf16, heads of 128: 2 prompts of 2048, 8/4 heads, 54 us, 32 at a time 67; 1100 tokens, 32/8 heads,
-// 38 and 59; half as many rows: 55 and 34, 18 and 14.  fp32: 1100 behind 7092, 32/8 heads, 1770 and 1490.)
-constexpr int kWideWaves = 4;
 constexpr int kMaxVocab = 1 << 21;
 
 int index_size(int code) { return code == ATTNRES_INDEX_I64 ? 8 : 4; }
@@ -107,52 +100,13 @@ int check_rows(const char* op, int64_t tokens, int kv_heads, int head_dim, int d
 
 // ------------------------------------------------------------- attention --
 
-// What the launches and the workspace of a call go by.
-struct PagedPlan {
-  bool wide = false, split = false;
-  int target = 0, part_rows = 0, turn = 0;
-  int64_t slots = 0, grid = 0, notes = 0;  // of all key heads
-  int64_t at_ml = 0, at_notes = 0, bytes = 0;
-};
-
-int paged_plan(int64_t tokens, int seqs, int heads, int kv_heads, int head_dim, int dtype, int64_t capacity,
-               PagedPlan* p) {
+int plan_attention(int64_t tokens, int seqs, int heads, int kv_heads, int head_dim, int dtype, int64_t capacity,
+                   PagedPlan* p) {
   int cus = 0;
   const int rc = attnres_internal_num_cus(&cus);
   if (rc != ATTNRES_OK) return rc;
-  const int64_t rows = tokens * (heads / kv_heads);
-  // Workgroups to deal out to: two a CU, or one where the LDS has no room for two (64 ragged fp32 sequences of
-  // up to 2048 keys, 8/4 heads of 128: 90 us, 97 with two rounds of them).  Heads of up to 64 in bf16 have room
-  // for four, but shorter stretches cost more than they hide (64 sequences of up to 4096 keys: 39 us against 34).
-  const int64_t at_once = (int64_t)cus * (head_dim > 64 && dtype == ATTNRES_DTYPE_F32 ? 1 : 2);
-  p->wide = rows / 32 * kv_heads >= (int64_t)cus * (at_once > cus ? kWideWaves : 2 * kWideWaves);
-  p->split = capacity > kWholeKeys;
-  if (p->wide) {
-    p->target = (int)at_once;
-    // where all tiles run at once, workgroups as many apart as there are CUs share one
-    if (rows / 128 * kv_heads <= at_once && at_once > cus) p->turn = cus / kv_heads;
-    // tiles: every sequence may end inside one; the rows behind the last sequence are one more
-    const int64_t tiles = rows / 128 + seqs + 1, share = (p->target + kv_heads - 1) / kv_heads;
-    // a split tile's parts are under twice its blocks over a part's most, and all those blocks at most the target's
-    // share
-    p->slots = p->split ? (2 * share + 8) * kv_heads : 0;
-    p->grid = (tiles + (p->split ? share + 8 : 0)) * kv_heads;
-    p->notes = p->slots;
-    p->part_rows = 128;
-  } else {
-    if ((rows / 32 + seqs + 1) * ((capacity + 127) / 128) > INT32_MAX)
-      return fail(ATTNRES_ERR_UNSUPPORTED, "paged_attention: too many keys for one call");
-    const int64_t tiles = rows / 32 + seqs + 1;
-    p->target = !p->split ? (int)tiles : at_once > kv_heads ? (int)(at_once / kv_heads) : 1;
-    p->grid = (int64_t)p->target * kv_heads;
-    p->slots = p->split ? 2 * p->grid : 0;  // each workgroup goes on with a tile and begins one
-    p->notes = p->split ? p->grid : 0;
-    p->part_rows = rows < 32 ? (int)rows : 32;
-  }
-  const int64_t lines = p->slots * p->part_rows;
-  p->at_ml = lines * head_dim * 4;
-  p->at_notes = p->at_ml + (lines * 8 + 15) / 16 * 16;
-  p->bytes = p->at_notes + p->notes * (int64_t)sizeof(lm_paged_note);
+  if (!paged_plan(cus, tokens, seqs, heads, kv_heads, head_dim, dtype == ATTNRES_DTYPE_F32, capacity, p))
+    return fail(ATTNRES_ERR_UNSUPPORTED, "paged_attention: too many keys for one call");
   return ATTNRES_OK;
 }
 
@@ -323,7 +277,7 @@ int attnres_paged_attention_workspace_size(int64_t tokens, int seqs, int heads, 
   int rc = check_attention(tokens, seqs, heads, kv_heads, head_dim, dtype, table_width, page_size, &shift);
   if (rc != ATTNRES_OK) return rc;
   PagedPlan plan;
-  rc = paged_plan(tokens, seqs, heads, kv_heads, head_dim, dtype, (int64_t)table_width * page_size, &plan);
+  rc = plan_attention(tokens, seqs, heads, kv_heads, head_dim, dtype, (int64_t)table_width * page_size, &plan);
   *bytes = plan.bytes;
   return rc;
 }
@@ -363,7 +317,7 @@ int attnres_paged_attention_fwd(const void* q, const int64_t* q_strides, const v
     return rc;
   const int64_t capacity = pages == 0 ? 0 : (int64_t)table_width * page_size;
   PagedPlan plan;
-  if ((rc = paged_plan(tokens, seqs, heads, kv_heads, head_dim, dtype, (int64_t)table_width * page_size, &plan)) !=
+  if ((rc = plan_attention(tokens, seqs, heads, kv_heads, head_dim, dtype, (int64_t)table_width * page_size, &plan)) !=
       ATTNRES_OK)
     return rc;
   if (plan.bytes > 0 && (workspace == nullptr || workspace_bytes < plan.bytes))
