@@ -96,7 +96,7 @@ struct Piece {
 struct Shared {
   float sum[LM_ATTN_WAVES];
   float most[LM_ATTN_WAVES];
-  float cost[8];
+  float cost[kCuts], shared[kCuts];
   int scan[LM_ATTN_WAVES][2];
   int upto[kThreads][2];
   Share share;
@@ -575,9 +575,9 @@ __device__ __forceinline__ void paged_stream(const lm_paged_params& P, LDS_ARRAY
 
 // ------------------------------------------------------------ many rows --
 
-// The cut (Cuts) of the call's tiles.
+// The cut (Cuts) of the call's tiles.  `used`: how many parts of split tiles a head has with it.
 template <bool TWO>  // workgroups of a CU
-__device__ __forceinline__ int part_blocks(const lm_paged_params& P, int all, Shared& S) {
+__device__ __forceinline__ int part_blocks(const lm_paged_params& P, int all, int* used, Shared& S) {
   float work = 0.f, top = 0.f;
   for (int s = threadIdx.x; s < P.seqs; s += kThreads) {
     const Share a = share_of(P, s);
@@ -587,6 +587,7 @@ __device__ __forceinline__ int part_blocks(const lm_paged_params& P, int all, Sh
   }
   sum_and_most(work, top, S);
   const Cuts C(work, top, P.target, P.kv_heads);
+  *used = 0;
   if (P.slots == 0 || C.many()) return uniform(C.longest);
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
 #pragma unroll
@@ -602,12 +603,16 @@ __device__ __forceinline__ int part_blocks(const lm_paged_params& P, int all, Sh
     }
     parts = wave_sum(parts);
     shared = wave_sum(shared);
-    if (lane == 0) S.cost[j] = C.cost(most, parts, shared, TWO, P.slots, all);
+    if (lane == 0) {
+      S.cost[j] = C.cost(most, parts, shared, TWO, P.slots, all);
+      S.shared[j] = shared;
+    }
   }
   __syncthreads();
   int best = 0;
 #pragma unroll
   for (int j = 1; j < kCuts; ++j) best = S.cost[j] < S.cost[best] ? j : best;
+  *used = uniform((int)S.shared[best]);
   return uniform(C.most(best));
 }
 
@@ -630,7 +635,10 @@ __device__ __forceinline__ void paged_tiles(const lm_paged_params& P, LDS_ARRAYS
     w = p;
   }
   if (threadIdx.x == 0) *flag = 0;
-  const int most = part_blocks<!(T::kBytes == 4 && DC > 64)>(P, all, S);
+  int used;
+  const int most = part_blocks<!(T::kBytes == 4 && DC > 64)>(P, all, &used, S);
+  if (threadIdx.x == 0)
+    for_unused_notes(w, all, used, P.slots, [&](int i) { P.notes[(int64_t)i * P.kv_heads + kvh].parts = 0; });
   // the sequence of part w, all sequences' parts one after another, and the slots in front of its
   int parts = 0, slots = 0, base = 0;
   bool found = false;
@@ -648,13 +656,7 @@ __device__ __forceinline__ void paged_tiles(const lm_paged_params& P, LDS_ARRAYS
     parts = add_sat(parts, n);
     slots = add_sat(slots, S.upto[kThreads - 1][1]);
   }
-  if (!found) {
-    // no part is left: the workgroups behind them clear the notes of the slots that none has
-    for (int64_t i = (int64_t)slots + (w - parts) + (int64_t)threadIdx.x * (all - parts); i < P.slots;
-         i += (int64_t)kThreads * (all - parts))
-      P.notes[i * P.kv_heads + kvh].parts = 0;
-    return;
-  }
+  if (!found) return;
   const int lo = find_upto(S, w - parts);
   Piece J;
   J.seq = base + lo;
@@ -671,7 +673,7 @@ __device__ __forceinline__ void paged_tiles(const lm_paged_params& P, LDS_ARRAYS
   J.slot = -1;
   if (sp.parts > 1) {
     const int first = uniform(add_sat(add_sat(slots, lo > 0 ? S.upto[lo - 1][1] : 0), rank * sp.parts));
-    if (first > P.slots - sp.parts) return;  // starts that do not rise
+    if (first > P.slots - sp.parts) return;  // lengths that change under the launch
     J.slot = (first + part) * P.kv_heads + kvh;
     if (threadIdx.x == 0)
       write_note(P, J.slot, J.a, J.tile * (J.a.narrow ? 32 : 128), kvh, part == 0 ? sp.parts : 0, J.slot,
@@ -693,9 +695,9 @@ template <typename T>
 __device__ __forceinline__ void paged_join(const lm_paged_params& P, f32x4* red) {
   const lm_paged_note N = P.notes[blockIdx.x];
   if (N.parts < 2) return;
-  // starts that do not rise can leave a note unwritten: what leads out of the call is none
+  // lengths that change under the launch can leave a note unwritten: what leads out of the call is none
   const int64_t slots = (int64_t)P.slots * P.kv_heads;
-  if (N.first < 0 || N.first >= slots || N.next < 0 || N.step < 0 ||
+  if (N.first < 0 || N.first >= slots || N.next < 0 || N.step < 1 ||
       N.next + (N.parts - 2) * (int64_t)N.step >= slots || N.token < 0 || N.row0 < 0 || N.head < 0 ||
       N.head >= P.kv_heads || (int64_t)N.token * P.group + N.rows > (int64_t)P.tokens * P.group)
     return;

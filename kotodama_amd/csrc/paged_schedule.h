@@ -142,6 +142,14 @@ struct Cuts {
   }
 };
 
+// Of the notes of a head's slots, its parts write the first `used`.  The others are cleared, or the join would take up
+// what an earlier call has left there: by all of the head's workgroups in turn, as a cut may leave none without a
+// part.
+template <typename F>
+LM_BOTH void for_unused_notes(int w, int all, int used, int slots, F clear) {
+  for (int i = used + w; i < slots; i += all) clear(i);
+}
+
 }  // namespace
 
 #endif  // KOTODAMA_AMD_PAGED_SCHEDULE_H
