@@ -621,7 +621,8 @@ int attnres_paged_release(const void* block_table, int64_t table_ld, int seqs, i
 /*
  * Writes new keys and values (tokens, kv_heads, head_dim), element strides (token, head),
  * into their slots ((tokens,) slots_dtype, no slot twice).  A slot outside the cache
- * (-1) is skipped.  No stride of a cache is 0 where it has more than one.  dtype bf16 or fp32 of all;
+ * (-1) is skipped.  A cache's strides each lead past all that its smaller ones reach, so that no two of
+ * its rows lie on one another, and k_cache, v_cache, k and v share no memory.  dtype bf16 or fp32 of all;
  * head_dim a multiple of 8 up to 128; 16-byte aligned pointers and strides.
  */
 int attnres_paged_write(const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,

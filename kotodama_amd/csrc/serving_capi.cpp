@@ -5,6 +5,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
 #include <cstring>
@@ -74,6 +75,21 @@ int take_cache(const char* what, const void* p, const int64_t* st, int64_t pages
     return fail(ATTNRES_ERR_UNSUPPORTED, "%s: a head's rows of a page span 2^31 bytes, or its pages lie so far apart",
                 what);
   return ATTNRES_OK;
+}
+
+// No two rows of a cache lie on one another: strides that each lead past all that the smaller ones reach.
+bool rows_apart(const lm_strides& st, int64_t pages, int kv_heads, int page_size, int head_dim) {
+  struct Axis {
+    int64_t stride, size;
+  } a[3] = {{st.b, pages}, {st.h, kv_heads}, {st.t, page_size}};
+  std::sort(a, a + 3, [](const Axis& x, const Axis& y) { return x.stride < y.stride; });
+  __int128 reach = head_dim - 1;
+  for (const Axis& x : a) {
+    if (x.size <= 1) continue;
+    if (x.stride <= reach) return false;
+    reach += (__int128)x.stride * (x.size - 1);
+  }
+  return true;
 }
 
 // A (tokens, heads, head_dim) tensor's strides (token, head).
@@ -252,8 +268,9 @@ int attnres_paged_write(const void* k, const int64_t* k_strides, const void* v, 
           ATTNRES_OK)
     return rc;
   for (const lm_strides* c : {&P.sk, &P.sv})
-    if ((pages > 1 && c->b == 0) || (kv_heads > 1 && c->h == 0) || c->t == 0)
-      return fail(ATTNRES_ERR_ARG, "paged_write: rows of the cache lie on one another (a stride is 0)");
+    if (!rows_apart(*c, pages, kv_heads, page_size, head_dim))
+      return fail(ATTNRES_ERR_ARG, "paged_write: rows of the cache may lie on one another: a stride does not lead past "
+                                   "what the smaller ones reach");
   for (int64_t* st : {&P.k_t, &P.k_h, &P.v_t, &P.v_h, &P.sk.b, &P.sk.h, &P.sk.t, &P.sv.b, &P.sv.h, &P.sv.t}) *st *= es;
   P.k = k;
   P.v = v;

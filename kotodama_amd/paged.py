@@ -254,6 +254,16 @@ def _check_cache(op: str, k_cache: Tensor, v_cache: Tensor) -> None:
     _check_sizes(op, k_cache)
 
 
+def _rows_apart(t: Tensor) -> bool:
+    """Strides that each lead past all that the smaller ones reach: no two elements lie on one another."""
+    reach = 0
+    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1):
+        if stride <= reach:
+            return False
+        reach += stride * (size - 1)
+    return True
+
+
 def _check_cache_memory(op: str, k_cache: Tensor, v_cache: Tensor, written: bool = False) -> None:
     # a cache is written in place and read by its pages: not copied
     for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
@@ -261,7 +271,7 @@ def _check_cache_memory(op: str, k_cache: Tensor, v_cache: Tensor, written: bool
             raise ValueError(f"{op}: {name} must lie in 16-byte pieces, got strides {t.stride()}")
         if t.numel() and max(t.stride(2) * t.shape[2], t.stride(0)) * t.element_size() >= 1 << 31:
             raise ValueError(f"{op}: {name}: a head's rows of a page span 2^31 bytes, or its pages lie so far apart")
-        if written and t.numel() and any(t.stride(i) == 0 for i in range(3) if t.shape[i] > 1):
+        if written and t.numel() and not _rows_apart(t):
             raise ValueError(f"{op}: rows of {name} lie on one another, got strides {t.stride()}")
 
 
@@ -310,7 +320,10 @@ def paged_write(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, slots: T
     them) are ``page * page_size + row``; one outside the cache (-1: padding,
     a refused sequence) is skipped.  No slot may be named twice: which of its
     tokens a row then holds, and whether whole, is not said.  ``k`` and ``v``
-    may have any strides, the caches any whose rows lie in 16-byte pieces.
+    may have any strides, the caches any whose rows lie in 16-byte pieces and that each lead past all that
+    the smaller ones reach: rows that lie on one another, as in an overlapping view, are refused.  The
+    host does not see it where ``k_cache`` and ``v_cache`` share rows, or a cache shares memory
+    with ``k`` or ``v``: what stands there afterwards is not said either.
     """
     if not torch.compiler.is_compiling() and native.paged_write(k, v, k_cache, v_cache, slots):
         return
