@@ -269,7 +269,8 @@ def _check_cache_memory(op: str, k_cache: Tensor, v_cache: Tensor, written: bool
     for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
         if t.numel() and not _aligned(t):
             raise ValueError(f"{op}: {name} must lie in 16-byte pieces, got strides {t.stride()}")
-        if t.numel() and max(t.stride(2) * t.shape[2], t.stride(0)) * t.element_size() >= 1 << 31:
+        apart = t.stride(0) if t.shape[0] > 1 else 0
+        if t.numel() and max(t.stride(2) * t.shape[2], apart) * t.element_size() >= 1 << 31:
             raise ValueError(f"{op}: {name}: a head's rows of a page span 2^31 bytes, or its pages lie so far apart")
         if written and t.numel() and not _rows_apart(t):
             raise ValueError(f"{op}: rows of {name} lie on one another, got strides {t.stride()}")

@@ -70,6 +70,18 @@ def test_rows_apart_are_taken(shape, strides):
     paged._check_cache_memory("paged_write", cache, cache, written=True)
 
 
+def test_one_page_has_no_page_stride():
+    # as the C entry has it: how far apart pages lie matters where there are two
+    far = torch.zeros(2048, dtype=torch.bfloat16).as_strided((1, 2, 16, 64), (1 << 31, 1024, 64, 1))
+    paged._check_cache_memory("paged_attention", far, far)
+    paged._check_cache_memory("paged_write", far, far, written=True)
+    two = torch.empty((0,), dtype=torch.bfloat16).as_strided((0, 2, 16, 64), (1 << 31, 1024, 64, 1))
+    paged._check_cache_memory("paged_write", two, two, written=True)
+    far = torch.empty(1, dtype=torch.bfloat16, device="meta").as_strided((2, 2, 16, 64), (1 << 31, 1024, 64, 1))
+    with pytest.raises(ValueError, match="so far apart"):
+        paged._check_cache_memory("paged_attention", far, far)
+
+
 def test_against_every_element():
     # what is taken has no two elements in one place
     for shape in ((2, 2, 16, 8), (3, 1, 16, 8), (2, 3, 16, 8)):
