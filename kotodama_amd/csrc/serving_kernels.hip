@@ -297,10 +297,20 @@ __device__ __forceinline__ void larger(float& top, int& at, float t, int a) {
   at = take ? a : at;
 }
 
-// The tokens' rows lie in the call: starts are taken into it.
+// The tokens' rows lie in the call: starts are taken into it.  Without a branch, so that several are requested
+// together.
 __device__ __forceinline__ int start_at(const lm_verify_params& P, int s) {
-  const int64_t v = s == 0 ? 0 : index_at(P.q_starts, s, P.starts64);
-  return v < 0 ? 0 : v > P.rows ? P.rows : (int)v;
+  const int32_t* w = (const int32_t*)P.q_starts + ((int64_t)s << P.starts64);
+  const int lo = w[0], up = w[P.starts64], hi = P.starts64 ? up : lo >> 31;
+  const int v = hi < 0 ? 0 : hi > 0 || (uint32_t)lo > (uint32_t)P.rows ? P.rows : lo;
+  return s == 0 ? 0 : v;
+}
+
+// How many drafts sequence s has, from row r0 on; under 0: it has no row.  Rows from the last start on are padding,
+// of which the first launch leaves nothing: where starts fall, no sequence reads there.
+__device__ __forceinline__ int drafts_of(const lm_verify_params& P, int s, int r0) {
+  const int end = start_at(P, s + 1), last = start_at(P, P.seqs);
+  return (end < last ? end : last) - r0 - 1;
 }
 
 __device__ __forceinline__ void put_token(const lm_verify_params& P, int64_t r, int64_t token) {
@@ -490,7 +500,7 @@ static_assert(LM_VERIFY_PIECE == 8 * 64, "a piece is a wave's values");
 // A stretch of the row that a sequence's token is taken from: its pieces' sums.
 __device__ __forceinline__ void verify_pieces(const lm_verify_params& P, PickShared& S) {
   const int s = blockIdx.x / P.slices, slice = blockIdx.x - s * P.slices;
-  const int r0 = start_at(P, s), drafts = start_at(P, s + 1) - r0 - 1;
+  const int r0 = start_at(P, s), drafts = drafts_of(P, s, r0);
   if (drafts < 0) return;
   RowStats R;
   const int a = accepted(P, r0, drafts, &R, S);
@@ -597,7 +607,7 @@ __device__ __forceinline__ int sample(const lm_verify_params& P, Weights W, cons
 // The tokens of a sequence, by one wave; greedily by a workgroup, from the rows alone.
 __device__ __forceinline__ void verify_pick(const lm_verify_params& P, PickShared& S) {
   const int s = blockIdx.x;
-  const int r0 = start_at(P, s), drafts = start_at(P, s + 1) - r0 - 1;
+  const int r0 = start_at(P, s), drafts = drafts_of(P, s, r0);
   if (drafts < 0) {
     if (threadIdx.x == 0) P.counts[s] = 0;
     return;

@@ -512,8 +512,8 @@ def verify_drafts(logits: Tensor, ids: Tensor, q_starts: Tensor, uniforms: Tenso
                   draft_probs: Optional[Tensor] = None, temperature: float = 1.0) -> tuple[Tensor, Tensor]:
     """Which drafted tokens stay, and the token behind them: speculative sampling's rule.
 
-    Sequence b's rows ``q_starts[b] .. q_starts[b + 1] - 1`` are the packed
-    input of a model's step: ``ids`` its last token and the drafts behind it,
+    Sequence b's rows ``q_starts[b] .. q_starts[b + 1] - 1`` (whole numbers rising from 0, the rows from the
+    last on padding) are the packed input of a model's step: ``ids`` its last token and the drafts behind it,
     ``logits`` (N, V) the model's for each.  With p = softmax(logits /
     temperature) of row r and q the distribution that the draft ``ids[r + 1]``
     was drawn from (``draft_probs[r]``; none given: the draft is certain), the
