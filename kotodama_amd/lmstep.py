@@ -33,8 +33,9 @@ embedding, the norms and rotation of queries and keys and the attention run
 on this package's kernels too (:mod:`kotodama_amd.lmops`), compiled around or
 not.  :meth:`LanguageModel.logits` runs the model behind a KV cache (prefill
 and single tokens) through the engine's cached loop and those operators;
-:meth:`LanguageModel.logits_paged` and :meth:`LanguageModel.step_paged` serve many
-sequences from a paged one (:mod:`kotodama_amd.paged`), prompts in chunks, single tokens and drafts.
+:meth:`LanguageModel.logits_paged` serves many sequences from a paged one
+(:mod:`kotodama_amd.paged`), prompts in chunks, single tokens and drafts, and
+:meth:`LanguageModel.step_paged` is its step where all have single tokens or drafts.
 """
 
 from __future__ import annotations
@@ -413,7 +414,13 @@ class LanguageModel(nn.Module):
         tokens in all; 1: no draft; 0: sits out) in, the tokens behind them out.
 
         Returns :func:`paged.verify_drafts`'s tokens (N,) and counts (B,); the cache keeps what stands.  A refused
-        sequence gets no token and keeps what it had."""
+        sequence gets no token and keeps what it had.
+
+        A chunk of a prompt does not belong here: every row behind a sequence's first is taken for a draft, so it
+        would be cut, without an error, at the first token that the model would not have drawn.  A step with one
+        among its sequences is ``cache.extend``, :meth:`logits_paged` with the ``rows`` that a token is taken from
+        (of a chunk its last), :func:`paged.verify_drafts` of those rows with starts of their own, and
+        ``cache.keep`` of what stands: held, the rows left out, and the counts."""
         held = cache.lens.clone()
         step = cache.extend(new, input_ids.shape[0])
         logits = self.logits_paged(input_ids, cache, step)

@@ -13,7 +13,7 @@ ROOT = Path(__file__).resolve().parent.parent
 
 def test_the_guides_loop_gives_a_refused_sequence_nothing():
     text = (ROOT / "INTEGRATION.md").read_text()
-    blocks = [b for b in re.findall(r"```python\n(.*?)```", text, re.S) if "verify_drafts(" in b]
+    blocks = [b for b in re.findall(r"```python\n(.*?)```", text, re.S) if "cache.extend(" in b]
     assert len(blocks) == 1
     lines = blocks[0].splitlines()
     extend = next(i for i, s in enumerate(lines) if "cache.extend(" in s)
