@@ -430,7 +430,7 @@ __device__ __forceinline__ void wide_tile(const Piece& J, int kvh, LDS_ARRAYS, i
   const int most = uniform(r0 < J.a.rows ? sees(P, J.a, last_of(r0 + 32)) : 0);
   const int all = uniform(sees(P, J.a, r0));
   const int any = uniform(sees(P, J.a, last_of(g0 + 128)));
-  const int t1 = any < J.t1 * 64 ? (any + 63) >> 6 : J.t1;  // no less than 0
+  const int t1 = any < J.t1 * 64 ? (any + 63) >> 6 : J.t1;  // 0 or less where no row sees a key: the loop is empty
 
   typename T::Frag qf[DC / 16];
   load_rows<T, DC>(qf, q_row<T>(P, J.a, R), P.dim, h, R.exists);

@@ -96,7 +96,9 @@ struct Share {
   }
 };
 
-// A tile's work: blocks of 32 keys that a wave works on.
+// A tile's work: blocks of 32 keys that a wave works on, as if its rows saw all keys of the sequence.  (A chunk's
+// do but for the chunk itself; tiles of a prompt from its start work on half of them on the average, and count for
+// twice their time in the cut.)
 LM_BOTH int blocks_of(const Share& a) { return a.narrow ? (a.kv_len + 127) >> 7 : ((a.kv_len + 63) >> 6) * 2; }
 
 // Its parts of at most `most` such blocks, and the key blocks of one.

@@ -23,7 +23,8 @@ __device__ __forceinline__ int64_t index_at(const void* p, int64_t i, int is64) 
 // thousand at most, in L2) and takes its share of the tokens, so that one
 // launch does and no workgroup waits for another.  Tokens find their sequence by a
 // search over 1024 ends in LDS.  Bound by latency: the lengths, their
-// sums and the pages, each waiting for the one before.
+// sums and the pages, each waiting for the one before.  The sums are 1024 threads' in 64 bits,
+// over 16 waves, however few sequences there are.
 
 constexpr int kSlotWaves = LM_SLOTS_THREADS / 64;
 constexpr int kMaxTokens = 1 << 30;  // of one sequence
