@@ -29,7 +29,8 @@ extern "C" int paged_notes(int cus, int64_t tokens, int seqs, int heads, int kv_
   std::vector<Share> a(seqs + 1);
   float work = 0.f, top = 0.f;
   for (int s = 0; s <= seqs; ++s) {  // the last: the rows behind all sequences
-    const int lo = s == 0 ? 0 : clamped(starts[s], tokens), hi = s < seqs ? clamped(starts[s + 1], tokens) : (int)tokens;
+    const int lo = s == 0 ? 0 : clamped(starts[s], tokens);
+    const int hi = s < seqs ? clamped(starts[s + 1], tokens) : (int)tokens;
     a[s].set(lo, hi, s < seqs ? clamped(lens[s], capacity) : 0, heads / kv_heads, true);
     if (s == seqs) continue;
     const float n = a[s].tiles > 0 ? (float)blocks_of(a[s]) : 0.f;

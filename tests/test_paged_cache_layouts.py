@@ -18,9 +18,8 @@ def _write(shape, strides):
     pages, hk, page, d = shape
     st = (ctypes.c_int64 * 3)(*strides)
     kst = (ctypes.c_int64 * 2)(hk * d, d)
-    lib = _capi.lib()
-    return lib.attnres_paged_write(FAKE, kst, FAKE, kst, 1 << 30, hk, d, _capi.DTYPE_BF16, FAKE, st, FAKE, st, pages, page,
-                                   FAKE, 0, None)
+    return _capi.lib().attnres_paged_write(FAKE, kst, FAKE, kst, 1 << 30, hk, d, _capi.DTYPE_BF16, FAKE, st, FAKE, st,
+                                           pages, page, FAKE, 0, None)
 
 
 def _view(shape, strides):
@@ -43,7 +42,7 @@ APART = [
     ((3, 2, 16, 64), (2048, 1024, 64)),
     ((3, 2, 16, 64), (2048, 64, 128)),  # tokens outside heads
     ((3, 2, 16, 64), (4096, 64, 256)),  # keys and values side by side
-    ((3, 2, 16, 64), (1024, 3072, 64)),  # heads outside pages
+    ((5, 2, 16, 64), (1024, 5120, 64)),  # heads outside pages
     ((3, 2, 16, 64), (2304, 1152, 72)),
     ((1, 2, 16, 64), (0, 1024, 64)),  # one page: no other lies on it
     ((3, 1, 16, 64), (1024, 0, 64)),
